@@ -54,7 +54,7 @@ EXTRA = {
 # gdn_chunk.hip and gemm_f32.hip load through builtins; they are held to the
 # same for speed, their loops filling the register file to a few registers.
 NO_SCRATCH = {"attn_pp.hip", "attn_pp64.hip", "attn_wide.hip", "gdn_chunk.hip", "gemm.hip", "gemm_f32.hip",
-              "splade_decoder.hip"}
+              "splade_decoder.hip", "tile_nt.hip", "tile_nn.hip", "tile_tn.hip"}
 RESOURCE_REMARKS = ["-Rpass-analysis=kernel-resource-usage", "-fno-caret-diagnostics"]
 # The same sources are also compiled to a device assembly listing, which
 # asmcheck.py walks for instructions that name a register an inline-asm

@@ -17,8 +17,7 @@
 #include <type_traits>
 #include <vector>
 
-#include "inl_common.hpp"
-#include "lanes.hpp"
+#include "norm_rope.hpp"
 
 namespace inl {
 
@@ -50,114 +49,6 @@ struct NormRopeParams {
   int32_t round_norm;
 };
 
-__device__ __forceinline__ float round_bf16(float v) { return (float)(bf16)v; }
-
-template <typename TI>
-__device__ __forceinline__ void load8(const char* p, float (&v)[8]) {
-  if constexpr (sizeof(TI) == 2) {
-    u32x4 w = *reinterpret_cast<const u32x4*>(p);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[2 * j] = __builtin_bit_cast(float, w[j] << 16);
-      v[2 * j + 1] = __builtin_bit_cast(float, w[j] & 0xffff0000u);
-    }
-  } else {
-    f32x4 a = *reinterpret_cast<const f32x4*>(p);
-    f32x4 b = *reinterpret_cast<const f32x4*>(p + 16);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
-  }
-}
-
-// A lane's 8 input values kept as loaded (bf16: one 16-byte vector, f32:
-// two) until the head step that uses them, so that the HB heads in flight
-// cost half the registers in bf16.
-struct Raw8 {
-  u32x4 a, b;
-};
-template <typename TI>
-__device__ __forceinline__ void load_raw(const char* p, Raw8& r) {
-  r.a = *reinterpret_cast<const u32x4*>(p);
-  if constexpr (sizeof(TI) != 2) r.b = *reinterpret_cast<const u32x4*>(p + 16);
-}
-template <typename TI>
-__device__ __forceinline__ void unpack8(const Raw8& r, float (&v)[8]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t a = r.a[j];
-    if constexpr (sizeof(TI) == 2) {
-      v[2 * j] = __builtin_bit_cast(float, a << 16);
-      v[2 * j + 1] = __builtin_bit_cast(float, a & 0xffff0000u);
-    } else {
-      const uint32_t b = r.b[j];
-      v[j] = __builtin_bit_cast(float, a);
-      v[4 + j] = __builtin_bit_cast(float, b);
-    }
-  }
-}
-
-template <typename TO>
-__device__ __forceinline__ void store8(char* p, const float (&v)[8]) {
-  if constexpr (sizeof(TO) == 2) {
-    bf16x8 o;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = (bf16)v[j];
-    *reinterpret_cast<bf16x8*>(p) = o;
-  } else {
-    f32x4 a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
-    *reinterpret_cast<f32x4*>(p) = a;
-    *reinterpret_cast<f32x4*>(p + 16) = b;
-  }
-}
-
-// out[e] = in[e] of lane (lane ^ m), for m a power of two below 64
-// (uniform): one switch for the 8 values. Called with every lane of the
-// wave active (a DPP read of a lane outside exec returns 0).
-__device__ __forceinline__ void xor_lanes8(const float (&in)[8], float (&out)[8], int m, int lane) {
-  switch (m) {
-    case 1:
-#pragma unroll
-      for (int e = 0; e < 8; ++e) out[e] = dpp<0xB1>(in[e]);      // quad_perm [1, 0, 3, 2]
-      break;
-    case 2:
-#pragma unroll
-      for (int e = 0; e < 8; ++e) out[e] = dpp<0x4E>(in[e]);      // quad_perm [2, 3, 0, 1]
-      break;
-    case 4: {
-      const bool hi = lane & 4;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float down = dpp<0x114>(in[e]);   // row_shr:4: lane i - 4
-        const float up = dpp<0x104>(in[e]);     // row_shl:4: lane i + 4
-        out[e] = hi ? down : up;
-      }
-      break;
-    }
-    case 8:
-#pragma unroll
-      for (int e = 0; e < 8; ++e) out[e] = dpp<0x128>(in[e]);     // row_ror:8
-      break;
-    case 16: {
-      const bool odd = lane & 16;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float a = in[e], b = in[e];   // a: rows (0, 0, 2, 2), b: rows (1, 1, 3, 3)
-        asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
-        out[e] = odd ? a : b;
-      }
-      break;
-    }
-    default: {
-      const bool upper = lane & 32;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float a = in[e], b = in[e];   // a: halves (0, 0), b: halves (1, 1)
-        asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
-        out[e] = upper ? a : b;
-      }
-    }
-  }
-}
 // A group of G = head_dim / 8 lanes owns one token: each lane holds 8
 // elements of a head row. The token's norm weights, table row and the lane's
 // cos/sin columns are loaded once per group of HB (4, 5 or 8) heads of the token
@@ -205,7 +96,8 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeParams p) {
   if (p.norm && p.w2 && hfirst + HB > p.w2_heads && hfirst < p.w3_heads) load_raw<TI>(p.w2 + 8 * j * (int)sizeof(TI), w2r);
 
   // rope geometry: `mode` 0 = none for this lane, 1 = pairs (e, e + 4) inside
-  // the lane (rotary_dim 8), 2 = half-split with the partner lane
+  // the lane (rotary_dim 8), 2 = half-split with the partner lane, 3 = adjacent
+  // pairs (2i, 2i + 1) inside the lane
   int mode = 0, partner = lane;
   bool first = true;
   float c[8], sn[8];
@@ -220,6 +112,8 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeParams p) {
   bool xor_partner = false;
   if (p.rotary_dim == 8 && p.sections == 1) {
     mode = j == 0 ? 1 : 0;
+  } else if (p.sections == INL_ROPE_INTERLEAVED) {
+    mode = 8 * j < p.rotary_dim ? 3 : 0;
   } else if (p.rotary_dim > 0) {
     if (p.sections == 2) {
       sec_lanes = G >> 1;
@@ -247,6 +141,12 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeParams p) {
       const f32x4 s4 = *reinterpret_cast<const f32x4*>(p.sin + posc * 4);
 #pragma unroll
       for (int e = 0; e < 4; ++e) { tc[e] = c4[e]; ts[e] = s4[e]; tc[e + 4] = 1.f; ts[e + 4] = 0.f; }
+    } else if (p.sections == INL_ROPE_INTERLEAVED) {
+      const int64_t at = posc * (p.rotary_dim >> 1) + (mode ? 4 * j : 0);
+      const f32x4 c4 = *reinterpret_cast<const f32x4*>(p.cos + at);
+      const f32x4 s4 = *reinterpret_cast<const f32x4*>(p.sin + at);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { tc[e] = c4[e >> 1]; ts[e] = s4[e >> 1]; }
     } else {
       const int half_lanes = sec_lanes >> 1;
       const int width = half_lanes * 8;              // table columns
@@ -302,7 +202,15 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeParams p) {
           v[0][e + 4] = b * c[e] + a * sn[e];
         }
       }
-      if (p.rotary_dim > 0 && !(p.rotary_dim == 8 && p.sections == 1)) {
+      if (mode == 3 && rot) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float a = v[0][e], b = v[0][e + 1];
+          v[0][e] = a * c[e] - b * sn[e];
+          v[0][e + 1] = b * c[e] + a * sn[e];
+        }
+      }
+      if (p.rotary_dim > 0 && p.sections != INL_ROPE_INTERLEAVED && !(p.rotary_dim == 8 && p.sections == 1)) {
         float pv[8];
         if (xor_partner)
           xor_lanes8(v[0], pv, half_lanes, lane);
@@ -328,13 +236,8 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeParams p) {
 
 namespace inl {
 
-// inl_norm_rope_fwd with per-head ranges: heads [0, w2_heads) normalised
-// with weight, [w2_heads, w3_heads) with weight2, the rest without a weight;
-// heads from rope_heads on are not rotated.
-int norm_rope_launch_ex(const inl_norm_rope_desc* d, const void* x, void* y, const void* weight,
-                        const void* weight2, int32_t w2_heads, int32_t w3_heads, int32_t rope_heads,
-                        const int32_t* rows, const float* cos, const float* sin, const float* cos2,
-                        const float* sin2, void* stream) {
+int norm_rope_check(const inl_norm_rope_desc* d, const int32_t* rows, const float* cos, const float* sin,
+                    const float* cos2, const float* sin2) {
   if (!d) return fail(INL_E_INVALID, "norm_rope: desc is NULL");
   if (!dtype_ok(d->dtype) || !dtype_ok(d->out_dtype))
     return fail(INL_E_INVALID, "norm_rope: dtype must be INL_F32 or INL_BF16");
@@ -353,12 +256,28 @@ int norm_rope_launch_ex(const inl_norm_rope_desc* d, const void* x, void* y, con
       if (d->rotary_dim != hd || hd % 32)
         return fail(INL_E_UNSUPPORTED, "norm_rope: axial rope needs rotary_dim == head_dim, a multiple of 32");
       if (!cos2 || !sin2) return fail(INL_E_INVALID, "norm_rope: axial rope needs cos2/sin2");
+    } else if (d->sections == INL_ROPE_INTERLEAVED) {
+      if (d->rotary_dim > hd || d->rotary_dim % 8)
+        return fail(INL_E_UNSUPPORTED, "norm_rope: rotary_dim must be a multiple of 8, <= head_dim");
     } else {
-      return fail(INL_E_INVALID, "norm_rope: sections must be 1 or 2");
+      return fail(INL_E_INVALID, "norm_rope: sections must be 1, 2 or 3");
     }
     if (!rows || !cos || !sin || d->table_rows <= 0)
       return fail(INL_E_INVALID, "norm_rope: rope needs rows, cos, sin and table_rows > 0");
   }
+  return INL_OK;
+}
+
+// inl_norm_rope_fwd with per-head ranges: heads [0, w2_heads) normalised
+// with weight, [w2_heads, w3_heads) with weight2, the rest without a weight;
+// heads from rope_heads on are not rotated.
+int norm_rope_launch_ex(const inl_norm_rope_desc* d, const void* x, void* y, const void* weight,
+                        const void* weight2, int32_t w2_heads, int32_t w3_heads, int32_t rope_heads,
+                        const int32_t* rows, const float* cos, const float* sin, const float* cos2,
+                        const float* sin2, void* stream) {
+  int rc = norm_rope_check(d, rows, cos, sin, cos2, sin2);
+  if (rc) return rc;
+  const int hd = d->head_dim;
   const int64_t xs = d->x_row_stride ? d->x_row_stride : (int64_t)d->heads * hd;
   const int64_t ys = d->y_row_stride ? d->y_row_stride : (int64_t)d->heads * hd;
   if (xs < (int64_t)d->heads * hd || ys < (int64_t)d->heads * hd || (xs * dtype_size(d->dtype)) % 16 ||

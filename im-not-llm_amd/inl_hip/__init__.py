@@ -1099,3 +1099,11 @@ def unit_lower_inverse(a, *, stream=None):
     out = torch.empty_like(a)
     _check(_gdn_inverse(a.shape[0], a.shape[1], a.data_ptr(), out.data_ptr(), _stream_ptr(stream)))
     return out
+
+
+# ---------------------------------------------------------------------------
+# Layer and head ops with their gradients (include/inl_train.h)
+# ---------------------------------------------------------------------------
+
+from .train import (ROPE_AXIAL, ROPE_HALF, ROPE_INTERLEAVED, dense, dense_bwd, gated_ffn,  # noqa: E402,F401
+                    gated_ffn_bwd, norm_rope_qk_bwd, softmax_xent, softmax_xent_bwd)

@@ -199,8 +199,11 @@ int inl_attn_kernel_name(const inl_attn_desc* desc, const char** name);
  *          sections == 2 (axial): each half of the head is rotated by its
  *          own half-split, the first half with cos/sin, the second with
  *          cos2/sin2, tables indexed by rows[token] (per-token tables).
+ *          sections == 3 (INL_ROPE_INTERLEAVED): the first rotary_dim features
+ *          are rotated in adjacent pairs (2i, 2i + 1) with column i of the
+ *          cos/sin row rows[token]; the rest pass through.
  *          rotary_dim == 0 skips the rope.
- * Tables are f32 `[table_rows, rotary_dim / 2]` (sections 1) or
+ * Tables are f32 `[table_rows, rotary_dim / 2]` (sections 1 and 3) or
  * `[table_rows, head_dim / 4]` (sections 2). A row index outside
  * [0, table_rows) yields NaN for that token instead of an out-of-range read.
  * round_tables = 1 rounds table values to bf16 (the reference stores tables
@@ -208,6 +211,9 @@ int inl_attn_kernel_name(const inl_attn_desc* desc, const char** name);
  * output dtype before the rotation (the reference materialises it).
  * In-place operation (y == x, same strides) is allowed.
  * --------------------------------------------------------------------- */
+#define INL_ROPE_HALF 1
+#define INL_ROPE_AXIAL 2
+#define INL_ROPE_INTERLEAVED 3
 typedef struct inl_norm_rope_desc {
   int64_t n_tokens;
   int32_t heads;
@@ -218,8 +224,8 @@ typedef struct inl_norm_rope_desc {
   int32_t out_dtype;              /* y dtype */
   int32_t norm;                   /* 1 = apply the RMSNorm */
   float eps;
-  int32_t rotary_dim;             /* 0 = no rope; sections 1: 8 or a multiple of 16 <= head_dim */
-  int32_t sections;               /* 1 = half-split, 2 = axial */
+  int32_t rotary_dim;             /* 0 = no rope; sections 1: 8 or a multiple of 16 <= head_dim; sections 3: a multiple of 8 */
+  int32_t sections;               /* INL_ROPE_*: 1 = half-split, 2 = axial, 3 = adjacent pairs */
   int32_t table_rows;
   int32_t round_tables;
   int32_t round_norm;
