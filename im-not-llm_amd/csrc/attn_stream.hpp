@@ -42,6 +42,15 @@ __device__ __forceinline__ void dma_b128(i32x4 rsrc, uint32_t lds, uint32_t voff
                :: "v"(voff), "s"(rsrc), "{m0}"(lds) : "memory");
 }
 
+// The same at voff + soff (soff uniform): the sum is made in a register of the
+// load's own, so that a kernel with many offsets need not keep them all; it
+// stands where the wait between a write of M0 and the load has to be.
+__device__ __forceinline__ void dma_b128_at(i32x4 rsrc, uint32_t lds, uint32_t voff, uint32_t soff) {
+  uint32_t at;
+  asm volatile("v_add_u32_e32 %0, %3, %1\n\tbuffer_load_dwordx4 %0, %2, 0 offen lds"
+               : "=&v"(at) : "v"(voff), "s"(rsrc), "s"(soff), "{m0}"(lds) : "memory");
+}
+
 // LDS access at an integer byte address: with a per-lane base register and a
 // compile-time offset the offset lands in the instruction's offset field.
 template <typename T>

@@ -287,9 +287,9 @@ struct DensePlan {
 int dense_plan(const inl_dense_desc& d, DensePlan* p, int* cus) {
   int rc = device_cus(cus);
   if (rc) return rc;
-  p->y = tile_plan(d.m, d.n, d.k, false, MAX_SPLITS, *cus);
-  p->dx = tile_plan(d.m, d.k, d.n, false, MAX_SPLITS, *cus);
-  p->dw = tile_plan(d.n, d.k, d.m, false, MAX_SPLITS, *cus);
+  p->y = tile_plan(d.m, d.n, d.k, 0, false, MAX_SPLITS, *cus);
+  p->dx = tile_plan(d.m, d.k, d.n, 1, false, MAX_SPLITS, *cus);
+  p->dw = tile_plan(d.n, d.k, d.m, 2, false, MAX_SPLITS, *cus);
   return INL_OK;
 }
 

@@ -35,12 +35,12 @@ struct FfnPlan {
 int ffn_plan(const inl_gated_ffn_desc& d, FfnPlan* p) {
   int rc = device_cus(&p->cus);
   if (rc) return rc;
-  p->h = tile_plan(d.m, d.inner, d.hidden, true, MAX_SPLITS, p->cus);
-  p->y = tile_plan(d.m, d.hidden, d.inner, false, MAX_SPLITS, p->cus);
-  p->dh = tile_plan(d.m, d.inner, d.hidden, false, MAX_SPLITS, p->cus);
-  p->dwd = tile_plan(d.hidden, d.inner, d.m, false, MAX_SPLITS, p->cus);
-  p->dx = tile_plan(d.m, d.hidden, 2 * d.inner, false, MAX_SPLITS, p->cus);
-  p->dwgu = tile_plan(2 * d.inner, d.hidden, d.m, false, MAX_SPLITS, p->cus);
+  p->h = tile_plan(d.m, d.inner, d.hidden, 0, true, MAX_SPLITS, p->cus);
+  p->y = tile_plan(d.m, d.hidden, d.inner, 0, false, MAX_SPLITS, p->cus);
+  p->dh = tile_plan(d.m, d.inner, d.hidden, 1, false, MAX_SPLITS, p->cus);
+  p->dwd = tile_plan(d.hidden, d.inner, d.m, 2, false, MAX_SPLITS, p->cus);
+  p->dx = tile_plan(d.m, d.hidden, 2 * d.inner, 1, false, MAX_SPLITS, p->cus);
+  p->dwgu = tile_plan(2 * d.inner, d.hidden, d.m, 2, false, MAX_SPLITS, p->cus);
   return INL_OK;
 }
 

@@ -11,11 +11,16 @@
 // operands are read with ds_read_b64_tr_b16, which hands lane j of 16 the four
 // k values of column j.
 //
-// Pipeline: 8 or 4 waves, each WNB x WMB blocks of v_mfma_f32_32x32x16_bf16; a
-// ring of 32-wide k slices in LDS filled by direct loads; operands read one
-// 16-wide k step ahead. A workgroup is persistent: its units (tile, k range)
-// form one stream of stages, so the next unit's first loads are in flight
-// while a unit's epilogue runs.
+// Pipeline: 8 or 4 waves, each WNB x WMB blocks of v_mfma_f32_16x16x32_bf16; a
+// ring of 64-wide k slices in LDS (128-byte rows: whole cache lines) filled by direct
+// loads, operands read a phase ahead (see the k loop). A workgroup is persistent: its
+// units (tile, k range) form one stream of stages, so the next unit's first loads
+// are in flight while a unit's epilogue runs.
+//
+// The 16 x 16 x 32 instruction and not 32 x 32 x 16: both run at the same rate, but a large
+// product is bound by the card's power, and on values that toggle (normal
+// random bf16) a loop of the former alone held 2,022 TFLOP/s and of the latter 1,748
+// (on zeros 2,448 and 2,329).
 //
 // Units: a tile's k range may be cut into `splits` parts of `kper` stages
 // (EPI_PART writes f32 partial tiles, a second kernel adds them in order), so
@@ -42,7 +47,7 @@ enum TileEpi {
   EPI_LINEAR = 1,    // y = act(alpha c + bias) + beta res; pre = alpha c + bias
   EPI_GATED = 2,     // w = n gate rows then n up rows: y = act(gate) * up; pre = gate, up
   EPI_DGATED = 3,    // c = dh, pre = [g u]: y = [dh u act'(g), dh act(g)]
-  EPI_XENT = 4,      // scores alpha c + bias: row maxima and sums of exponentials per 32 WNB columns
+  EPI_XENT = 4,      // scores alpha c + bias: row maxima and sums of exponentials per 16 WNB columns
   EPI_DXENT = 5,     // y = dl (softmax - onehot)
 };
 
@@ -77,7 +82,9 @@ struct TileParams {
   int32_t kper;             // stages per unit
 };
 
-constexpr int TG_BK = 32;
+constexpr int TG_BK = 64;      // k per LDS stage
+constexpr int TG_KS = TG_BK / 32;   // MFMA k steps of it
+constexpr int TG_ROW = TG_BK * 2;
 constexpr int TG_STG = 4096;   // per-wave epilogue staging: 32 rows x 128 bytes
 constexpr int TG_XCDS = 8;
 constexpr int TG_GROUP = 8;
@@ -86,23 +93,28 @@ template <int NWN_, int NWM_, int WNB_, int WMB_, int STAGES_, int WPC_>
 struct TileShape {
   static constexpr int NWN = NWN_, NWM = NWM_, WNB = WNB_, WMB = WMB_;
   static constexpr int NW = NWN * NWM;
-  static constexpr int BN = NWN * WNB * 32, BM = NWM * WMB * 32;
+  static constexpr int BN = NWN * WNB * 16, BM = NWM * WMB * 16;
   static constexpr int STAGES = STAGES_, WPC = WPC_;
-  static constexpr int W = BN * 64, X = BM * 64;
+  static constexpr int W = BN * TG_ROW, X = BM * TG_ROW;
   static constexpr int STAGE = W + X;
-  static constexpr int PER_WAVE = STAGE / 1024 / NW;
-  static constexpr int W_PER_WAVE = W / 1024 / NW;
+  // Direct loads of 1 KiB per wave and stage. With four or more w blocks per wave
+  // a stage's w comes in H = 2 halves (each wave's lower and upper blocks).
+  static constexpr int H = WNB >= 4 ? 2 : 1;
+  static constexpr int WH = WNB / H;
+  static constexpr int PX = X / 1024 / NW, PW = W / 1024 / NW / H;
+  static constexpr int PER_WAVE = PX + H * PW;
   static constexpr int RING = STAGES * STAGE;
   static constexpr int LDS = RING + NW * TG_STG;
-  static_assert((STAGE / 1024) % NW == 0 && (W / 1024) % NW == 0, "the direct loads split evenly over the waves");
-  static_assert(NW % 2 == 0, "w blocks of one wave share its parity (EPI_GATED)");
-  static_assert(STAGES >= 2 && (STAGES - 1) * PER_WAVE <= 63, "vmcnt range");
+  static_assert(X % (1024 * NW) == 0 && W % (1024 * NW * H) == 0, "the direct loads split evenly over the waves");
+  static_assert(NW % 4 == 0, "w blocks of one wave are all gate or all up rows (EPI_GATED)");
+  static_assert(H == 1 || (WH * 2 == NW && STAGES == 2), "a half is the waves' next blocks");
+  static_assert((STAGES - 1) * PER_WAVE <= 63, "vmcnt range");
 };
 // 0: 256 x 256, one workgroup of 8 waves per CU. 1: 128 x 128, two of 4 waves
 // per CU. 2: 64 x 64, for outputs that would leave most of the chip idle.
 template <int SH>
-using TileShapeOf = std::conditional_t<SH == 0, TileShape<2, 4, 4, 2, 3, 1>,
-                    std::conditional_t<SH == 1, TileShape<2, 2, 2, 2, 4, 2>, TileShape<2, 2, 1, 1, 6, 2>>>;
+using TileShapeOf = std::conditional_t<SH == 0, TileShape<2, 4, 8, 4, 2, 1>,
+                    std::conditional_t<SH == 1, TileShape<2, 2, 4, 4, 2, 2>, TileShape<2, 2, 2, 2, 3, 2>>>;
 constexpr int TG_SHAPES = 3;
 
 struct TilePlan {
@@ -110,9 +122,9 @@ struct TilePlan {
   int splits;
   int32_t kper;
 };
-// The shape and k split with the least estimated time. `gated`: w has 2n rows.
-// max_splits 1 keeps every tile in one unit.
-TilePlan tile_plan(int64_t m, int64_t n, int64_t k, bool gated, int max_splits, int cus);
+// The shape and k split with the least estimated time. by_cols: operands stored by
+// columns (0 to 2); `gated`: w has 2n rows. max_splits 1 keeps every tile in one unit.
+TilePlan tile_plan(int64_t m, int64_t n, int64_t k, int by_cols, bool gated, int max_splits, int cus);
 
 // f32 partials of a plan (0 for one split).
 inline size_t tile_part_bytes(const TilePlan& t, int64_t m, int64_t n) {
@@ -122,17 +134,17 @@ inline size_t tile_part_bytes(const TilePlan& t, int64_t m, int64_t n) {
 namespace {
 
 // 16-byte chunk c of stored row r of an operand stage, R = rows of m or n per
-// tile. OP_ROWS: 64-byte rows, the 16 rows of one ds_read_b128 pass cover all
-// banks. OP_COLS: 2 R-byte rows, the 4 rows x 64 bytes that 32 lanes of a
+// tile. OP_ROWS: 128-byte rows, the 16 rows of one ds_read_b128 pass cover all
+// banks. OP_COLS: 2 R-byte rows, the 8 rows x 32 bytes that 32 lanes of a
 // transposed read touch cover all banks.
 template <int L, int R>
 __device__ __forceinline__ int tg_swz(int r, int c) {
-  if constexpr (L == OP_ROWS) return c ^ ((r >> 2) & 3);
-  if constexpr (R >= 128) return c ^ ((r & 3) << 2);
-  return c ^ (((r >> 1) & 1) << 2);
+  if constexpr (L == OP_ROWS) return c ^ ((r >> 1) & 7);
+  if constexpr (R >= 128) return c ^ ((r & 3) << 2) ^ (((r >> 3) & 1) << 1);
+  return c ^ (((r >> 1) & 1) << 2) ^ (((r >> 3) & 1) << 1);
 }
 template <int L, int R>
-constexpr int tg_chunks() { return L == OP_ROWS ? 4 : R / 8; }
+constexpr int tg_chunks() { return L == OP_ROWS ? TG_ROW / 16 : R / 8; }
 
 template <int SH, int LX, int LW, int EPI, bool OUT16, bool RES>
 __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) void tile_gemm_kernel(TileParams p) {
@@ -155,7 +167,7 @@ __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) voi
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = wave / C::NWM, wm = wave % C::NWM;
-  const int l32 = lane & 31, hf = lane >> 5;
+  const int l16 = lane & 15, quad = lane >> 4;
 
   // ---- units ----
   struct Unit {
@@ -177,96 +189,156 @@ __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) voi
   };
 
   // ---- loads ----
-  // Per-lane byte offsets of this wave's 1 KiB blocks {wave, wave + NW, ...} of
-  // a stage (w first). The chunk of a lane is the same in all blocks of an
-  // OP_ROWS operand.
-  uint32_t goff[PER_WAVE];
-#pragma unroll
-  for (int i = 0; i < PER_WAVE; ++i) {
-    const bool is_w = i < C::W_PER_WAVE;
-    const int blk = wave + NW * i - (is_w ? 0 : C::W / 1024);
-    const int cpr = is_w ? tg_chunks<LW, BN>() : tg_chunks<LX, BM>();
-    const int b = EPI == EPI_GATED && is_w ? blk >> 1 : blk;   // 16 gate (even) or up (odd) rows
-    const int at = b * 64 + lane, r = at / cpr, cp = at % cpr;
-    const int c = is_w ? tg_swz<LW, BN>(r, cp) : tg_swz<LX, BM>(r, cp);
-    goff[i] = (uint32_t)r * (uint32_t)(is_w ? p.ws_b : p.xs_b) + c * 16;
+  // Per-lane byte offset of this wave's first 1 KiB block of x and of w; the
+  // following blocks are uniform steps away (added at each load: eight offsets
+  // held in registers would not fit beside the operands).
+  // OP_ROWS: LDS row r of an operand is its row r; a half of w is every other
+  // block. OP_COLS: [64 k][columns]; w's halves are tiles of their own, each
+  // with the half's columns of both waves along n.
+  constexpr int NWH = BN / C::H;   // columns of an OP_COLS half of w
+  uint32_t xo, wo;
+  {
+    constexpr int cpr = tg_chunks<LX, BM>();
+    const int at = wave * 64 + lane, r = at / cpr;
+    xo = (uint32_t)r * (uint32_t)p.xs_b + tg_swz<LX, BM>(r, at % cpr) * 16;
   }
-  const int my_chunk = (lane & 3) ^ ((lane >> 4) & 3);   // k chunk of an OP_ROWS load
+  {
+    constexpr int cpr = tg_chunks<LW, NWH>();
+    const int at = wave * 64 + lane;
+    int r = at / cpr;
+    int c = tg_swz<LW, NWH>(r, at % cpr);
+    if (LW == OP_COLS) c = c / (C::WH * 2) * (WNB * 2) + c % (C::WH * 2);   // chunk of 8 columns
+    // EPI_GATED: LDS rows are 16 gate rows, then their 16 up rows, and so on
+    if (EPI == EPI_GATED) r = (r >> 5) * 16 + (r & 15);
+    wo = (uint32_t)r * (uint32_t)p.ws_b + c * 16;
+  }
+  const uint32_t xstep = (LX == OP_ROWS ? NW * 8 : NW * 64 / tg_chunks<LX, BM>()) * (uint32_t)p.xs_b;
+  const uint32_t wstep = (LW == OP_COLS ? NW * 64 / tg_chunks<LW, NWH>() : EPI == EPI_GATED ? NW * 4 : NW * 8) * (uint32_t)p.ws_b;
 
   // Descriptors start at a unit's first row and at the stage's k, so that no
   // offset exceeds 31 bits; rows past the end read as zero, and so does k past
-  // the end: OP_COLS by the range, OP_ROWS by an offset out of it.
-  int ld_j = 0, ld_ks = 0, ld_end = 0, ld_slot = 0;
-  const char* xp = nullptr;
-  const char* wp = nullptr;
-  uint32_t x_rows = 0, w_rows = 0;   // rows (OP_ROWS) or columns (OP_COLS) of this unit
+  // the end: OP_COLS by the range, OP_ROWS by an offset out of it. They, the
+  // offsets and the LDS base are kept from stage to stage and only moved on: the
+  // scalar instructions of a stage's loads stand in line with its products.
+  const int tail = p.k - (kst - 1) * TG_BK;   // k of the last stage
+  const uint32_t xnext = LX == OP_ROWS ? TG_ROW : TG_BK * (uint32_t)p.xs_b;
+  const uint32_t wnext = LW == OP_ROWS ? TG_ROW : TG_BK * (uint32_t)p.ws_b;
+  int ld_j = 0, ld_ks = 0, ld_end = 0;
+  i32x4 xrs, wrs;
+  uint32_t x_bytes = 0, w_bytes = 0, x_cut = 0, w_cut = 0;   // ranges, and by how much the last stage's are shorter
+  // (whole 16-byte chunks: an odd row end lies inside its padded row)
+  auto range = [&](int L, uint32_t rows, int64_t stride, int ks) __attribute__((always_inline)) {
+    return L == OP_ROWS ? (rows - 1) * (uint32_t)stride + (uint32_t)((ks + 7) & ~7) * 2
+                        : (uint32_t)(ks - 1) * (uint32_t)stride + ((rows + 7) & ~7u) * 2;
+  };
+  auto ld_tail = [&]() __attribute__((always_inline)) {
+    x_bytes -= x_cut;
+    w_bytes -= w_cut;
+    if (LX == OP_ROWS || LW == OP_ROWS) {
+      // (the lane's chunk anew: this is rare, and a register less in the loop)
+      const int l = (int)opaque((uint32_t)lane);
+      const int chunk = (l & 7) ^ ((wave * 4 + (l >> 4)) & 7);
+      const uint32_t kill = chunk * 8 >= tail ? 0x80000000u : 0u;
+      if (LX == OP_ROWS) xo |= kill;
+      if (LW == OP_ROWS) wo |= kill;
+    }
+  };
   auto ld_unit = [&]() __attribute__((always_inline)) {
     const Unit q = unit_of(ld_j);
     ld_ks = q.s * p.kper;
     ld_end = min(ld_ks + p.kper, kst);
     const int64_t k0 = (int64_t)ld_ks * TG_BK;
     const int64_t r0 = (int64_t)q.mt * BM;
-    x_rows = (uint32_t)min((int64_t)BM, p.m - r0);
-    xp = p.x + (LX == OP_ROWS ? r0 * p.xs_b + k0 * 2 : k0 * p.xs_b + r0 * 2);
+    // (a 64-bit minimum is vector code)
+    const uint32_t x_rows = (uint32_t)__builtin_amdgcn_readfirstlane((int)min((int64_t)BM, p.m - r0));
     const int c0 = q.nt * BNO;
-    w_rows = (uint32_t)min(BNO, p.n - c0);
-    const int64_t c1 = EPI == EPI_GATED && (wave & 1) ? (int64_t)p.n + c0 : (int64_t)c0;
-    wp = p.w + (LW == OP_ROWS ? c1 * p.ws_b + k0 * 2 : k0 * p.ws_b + c1 * 2);
+    const uint32_t w_rows = (uint32_t)min(BNO, p.n - c0);
+    const int64_t c1 = EPI == EPI_GATED && (wave & 2) ? (int64_t)p.n + c0 : (int64_t)c0;
+    const uint32_t xr = range(LX, x_rows, p.xs_b, TG_BK), wr = range(LW, w_rows, p.ws_b, TG_BK);
+    x_bytes = xr;
+    w_bytes = wr;
+    x_cut = (uint32_t)__builtin_amdgcn_readfirstlane((int)(xr - range(LX, x_rows, p.xs_b, tail)));
+    w_cut = (uint32_t)__builtin_amdgcn_readfirstlane((int)(wr - range(LW, w_rows, p.ws_b, tail)));
+    xrs = pp_rsrc_words(p.x + (LX == OP_ROWS ? r0 * p.xs_b + k0 * 2 : k0 * p.xs_b + r0 * 2), xr);
+    wrs = pp_rsrc_words(p.w + (LW == OP_ROWS ? c1 * p.ws_b + k0 * 2 : k0 * p.ws_b + c1 * 2), wr);
+    xo &= 0x7fffffffu;
+    wo &= 0x7fffffffu;
+    if (ld_ks + 1 == kst) ld_tail();
+    xrs[2] = (int)x_bytes;
+    wrs[2] = (int)w_bytes;
   };
-  auto range = [&](int L, uint32_t rows, int64_t stride, int left) __attribute__((always_inline)) {
-    // (whole 16-byte chunks: an odd row end lies inside its padded row)
-    return L == OP_ROWS ? (uint32_t)((rows - 1) * stride) + (uint32_t)((left + 7) & ~7) * 2
-                        : (uint32_t)((min(left, TG_BK) - 1) * stride) + ((rows + 7) & ~7u) * 2;
+  auto move_on = [&](i32x4& rs, uint32_t by) __attribute__((always_inline)) {
+    const uint64_t at = (((uint64_t)(uint32_t)rs[1] << 32) | (uint32_t)rs[0]) + by;
+    rs[0] = (int)(uint32_t)at;
+    rs[1] = (int)(uint32_t)(at >> 32);
   };
-  const i32x4 none = pp_rsrc_words(p.x, 0);
-  auto issue = [&]() __attribute__((always_inline)) {
-    const uint32_t st = lds0 + (uint32_t)ld_slot * STAGE;
-    if (++ld_slot == STAGES) ld_slot = 0;
-    if (ld_j < my_units) {
-      const int left = p.k - ld_ks * TG_BK;   // k from this stage on
-      const i32x4 xrs = pp_rsrc_words(xp, range(LX, x_rows, p.xs_b, left));
-      const i32x4 wrs = pp_rsrc_words(wp, range(LW, w_rows, p.ws_b, left));
-      uint32_t kill = 0;
-      if ((LX == OP_ROWS || LW == OP_ROWS) && left < TG_BK) kill = my_chunk * 8 >= left ? 0x80000000u : 0u;
-#pragma unroll
-      for (int i = 0; i < PER_WAVE; ++i) {
-        const bool is_w = i < C::W_PER_WAVE;
-        const bool rows = (is_w ? LW : LX) == OP_ROWS;
-        dma_b128(is_w ? wrs : xrs, st + (wave + NW * i) * 1024, rows ? goff[i] | kill : goff[i]);
-      }
-      xp += LX == OP_ROWS ? TG_BK * 2 : TG_BK * p.xs_b;
-      wp += LW == OP_ROWS ? TG_BK * 2 : TG_BK * p.ws_b;
-      if (++ld_ks == ld_end) {
-        if (++ld_j < my_units) ld_unit();
-      }
-    } else {   // past the last stage: zeros, so that every stage counts the same loads
-#pragma unroll
-      for (int i = 0; i < PER_WAVE; ++i) dma_b128(none, st + (wave + NW * i) * 1024, goff[i]);
+  // Loads of the cursor's stage in two parts: x with the first half of w (h = 0),
+  // then the other half, then move the cursor on (end). Past the last stage:
+  // zeros, so that every stage counts the same loads.
+  uint32_t ld_at = lds0 + (uint32_t)wave * 1024, ld_slot = 0;
+  auto load = [&](int h, int i) __attribute__((always_inline)) {
+    if (h == 0 && i < C::PX) {
+      dma_b128_at(xrs, ld_at + C::W + NW * 1024 * i, xo, i * xstep);
+      return;
     }
+    if (h == 0) i -= C::PX;
+    const uint32_t half = LW == OP_ROWS ? h * wstep : h * C::WH * 32;
+    const int blk = LW == OP_ROWS ? NW * (C::H * i + h) : h * (NWH / 8) + NW * i;
+    dma_b128_at(wrs, ld_at + blk * 1024, wo, half + i * (LW == OP_ROWS ? C::H * wstep : wstep));
+  };
+  auto end = [&](int h) __attribute__((always_inline)) {
+    if (h + 1 < C::H) return;
+    ld_slot = ld_slot + 1 == STAGES ? 0 : ld_slot + 1;
+    ld_at = lds0 + (uint32_t)wave * 1024 + ld_slot * STAGE;
+    move_on(xrs, xnext);
+    move_on(wrs, wnext);
+    if (++ld_ks >= ld_end) {   // (past the last unit, too)
+      if (++ld_j < my_units) {
+        ld_unit();
+      } else {
+        x_bytes = w_bytes = 0;
+      }
+    } else if (ld_ks + 1 == kst) {
+      ld_tail();
+    }
+    // (set apart from the branches: a choice between whole descriptors is made in
+    // vector registers)
+    xrs[2] = (int)x_bytes;
+    wrs[2] = (int)w_bytes;
+    asm volatile("" : "+s"(xrs), "+s"(wrs));
+  };
+  constexpr int L0 = C::PX + C::PW, L1 = C::H == 2 ? C::PW : 0;   // loads of the two parts
+  auto issue = [&](int h) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < (h ? L1 : L0); ++i) load(h, i);
+    end(h);
   };
 
-  // ---- fragments: w rows (wn WNB + a) 32 + l32, x rows (wm WMB + b) 32 + l32, k = 16 ks + 8 hf .. + 7 ----
+  // ---- fragments: w rows (wn WNB + a) 16 + l16, x rows (wm WMB + b) 16 + l16, k = 32 ks + 8 quad .. + 7 ----
+  // OP_ROWS: blocks are 16 rows apart, a multiple of the swizzle's period, so a
+  // block is a constant offset from the first. OP_COLS: so is a k step; of x, blocks
+  // 2 and 3 are 0 and 1 with chunk bit 2 the other way (two registers less).
   auto frag_addr = [&](int L, int R, int blk, int ks) __attribute__((always_inline)) {
     if (L == OP_ROWS) {
-      const int r = blk * 32 + l32, c = 2 * ks + hf;
-      return (uint32_t)(r * 64 + ((c ^ ((r >> 2) & 3)) << 4));
+      const int r = blk * 16 + l16, c = 4 * ks + quad;
+      return (uint32_t)(r * TG_ROW + ((c ^ ((r >> 1) & 7)) << 4));
     }
-    const int a16 = lane & 15, e = a16 >> 2;
-    const int col = blk * 32 + (lane & 16) + 4 * (a16 & 3);
-    const int sw = R >= 128 ? e << 2 : (e >> 1) << 2;
-    return (uint32_t)((16 * ks + 8 * hf + e) * (2 * R) + (((col >> 3) ^ sw) << 4) + (a16 & 1) * 8);
+    // lane 4 e + j of 16 addresses columns 4 j .. + 3 of k row e and receives
+    // column 4 e + j of k rows 0 .. 3; a second read takes rows 4 .. 7
+    const int e = l16 >> 2, r = 8 * quad + e;
+    const int c = blk * 2 + ((l16 & 3) >> 1);
+    const int sw = (R >= 128 ? e << 2 : (e >> 1) << 2) ^ ((quad & 1) << 1);
+    return (uint32_t)(r * (2 * R) + ((c ^ sw) << 4) + (l16 & 1) * 8);
   };
-  // OP_COLS: the second k step is a constant offset from the first
-  uint32_t fa[WNB][LW == OP_ROWS ? 2 : 1], fb[WMB][LX == OP_ROWS ? 2 : 1];
+  constexpr int NFA = LW == OP_ROWS ? TG_KS : C::WH, NFB = 2;
+  static_assert(TG_KS == 2 && (WMB == 2 || WMB == 4), "two address registers for x");
+  uint32_t fa[NFA], fb[NFB];
 #pragma unroll
-  for (int ks = 0; ks < 2; ++ks) {
+  for (int i = 0; i < NFA; ++i)
+    fa[i] = opaque(lds0 + (LW == OP_ROWS ? frag_addr(LW, BN, wn * WNB, i) : frag_addr(LW, NWH, wn * C::WH + i, 0)));
 #pragma unroll
-    for (int a = 0; a < WNB; ++a)
-      if (LW == OP_ROWS || ks == 0) fa[a][ks] = opaque(lds0 + frag_addr(LW, BN, wn * WNB + a, ks));
-#pragma unroll
-    for (int b = 0; b < WMB; ++b)
-      if (LX == OP_ROWS || ks == 0) fb[b][ks] = opaque(lds0 + C::W + frag_addr(LX, BM, wm * WMB + b, ks));
-  }
+  for (int i = 0; i < NFB; ++i)
+    fb[i] = opaque(lds0 + C::W + (LX == OP_ROWS ? frag_addr(LX, BM, wm * WMB, i) : frag_addr(LX, BM, wm * WMB + i, 0)));
   auto tr_read = [&](uint32_t at, int pitch) __attribute__((always_inline)) {
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(size_t)at);
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -274,65 +346,68 @@ __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) voi
     const u32x2 l = __builtin_bit_cast(u32x2, lo), h = __builtin_bit_cast(u32x2, hi);
     return (u32x4){l[0], l[1], h[0], h[1]};
   };
+  // (the addresses move from slot to slot, so that what is left is a constant
+  // offset of the read)
+  int rd_slot = 0;
+  auto rd_next = [&]() __attribute__((always_inline)) {
+    const bool wrap = ++rd_slot == STAGES;
+    if (wrap) rd_slot = 0;
+    const uint32_t by = wrap ? (uint32_t)-(int)((STAGES - 1) * STAGE) : (uint32_t)STAGE;
+#pragma unroll
+    for (uint32_t& a : fa) a = opaque(a + by);
+#pragma unroll
+    for (uint32_t& b : fb) b = opaque(b + by);
+  };
+  auto read_w = [&](int h, int i, int ks) __attribute__((always_inline)) {
+    if constexpr (LW == OP_ROWS) return lds_load<u32x4>(fa[ks] + (h * C::WH + i) * 16 * TG_ROW);
+    else return tr_read(fa[i] + h * (C::W / C::H) + ks * 32 * 2 * NWH, 2 * NWH);
+  };
+  auto read_x = [&](int b, int ks) __attribute__((always_inline)) {
+    if constexpr (LX == OP_ROWS) return lds_load<u32x4>(fb[ks] + b * 16 * TG_ROW);
+    else return tr_read((b < 2 ? fb[b] : opaque(fb[b & 1]) ^ 64u) + ks * 32 * 2 * BM, 2 * BM);
+  };
 
-  f32x16 acc[WNB][WMB];
-  const f32x16 zero = {};
+  f32x4 acc[WNB][WMB];
+  const f32x4 zero = {};
 #pragma unroll
   for (int a = 0; a < WNB; ++a)
 #pragma unroll
     for (int b = 0; b < WMB; ++b) acc[a][b] = zero;
 
-  struct Half {
-    u32x4 a[WNB], b[WMB];
-  };
-  int rd_slot = 0;
-  auto read_half = [&](int ks, Half& f) __attribute__((always_inline)) {
-    const uint32_t so = (uint32_t)rd_slot * STAGE;
-#pragma unroll
-    for (int a = 0; a < WNB; ++a) {
-      if constexpr (LW == OP_ROWS) f.a[a] = lds_load<u32x4>(fa[a][ks] + so);
-      else f.a[a] = tr_read(fa[a][0] + so + ks * 16 * 2 * BN, 2 * BN);
-    }
-#pragma unroll
-    for (int b = 0; b < WMB; ++b) {
-      if constexpr (LX == OP_ROWS) f.b[b] = lds_load<u32x4>(fb[b][ks] + so);
-      else f.b[b] = tr_read(fb[b][0] + so + ks * 16 * 2 * BM, 2 * BM);
-    }
-  };
-  auto mfmas = [&](const Half& f) __attribute__((always_inline)) {
-#pragma unroll
-    for (int a = 0; a < WNB; ++a)
-#pragma unroll
-      for (int b = 0; b < WMB; ++b)
-        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f.a[a]),
-                                                            __builtin_bit_cast(bf16x8, f.b[b]), acc[a][b], 0, 0, 0);
+  auto mfma = [&](int a, int b, const u32x4& w, const u32x4& x) __attribute__((always_inline)) {
+    acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, x),
+                                                        acc[a][b], 0, 0, 0);
   };
 
-  // ---- epilogue: acc[a][b][4 g + e] is row (wm WMB + b) 32 + l32, w row (wn WNB + a) 32 + 8 g + 4 hf + e ----
-  // Staging of one wave: 32 rows x 128 bytes, 16-byte chunk c of row r at
+  // ---- epilogue: acc[a][b][e] is row (wm WMB + b) 16 + l16, w row (wn WNB + a) 16 + 4 quad + e ----
+  // Staging of one wave: 32 rows (two x blocks) x 128 bytes, 16-byte chunk c of row r at
   // r * 128 + ((c ^ ((r >> 1) & 7)) << 4); 64 bf16 columns, or 32 f32 ones where
   // the value still meets memory (RES, EPI_DGATED) or is stored in f32.
   const uint32_t stg = lds0 + C::RING + (uint32_t)wave * TG_STG;
+  // (the lane anew for each tile: what an epilogue derives from it would otherwise
+  // be kept in registers through the k loop)
+  int el = lane;
   auto stg_at = [&](int r, int c) __attribute__((always_inline)) {
     return stg + (uint32_t)r * 128 + (((uint32_t)c ^ (((uint32_t)r >> 1) & 7)) << 4);
   };
-  auto put16 = [&](int c, f32x4 v) __attribute__((always_inline)) {
+  // 4 values of row r, columns c .. + 3
+  auto put16 = [&](int r, int c, f32x4 v) __attribute__((always_inline)) {
     const f32x2 lo = {v[0], v[1]}, hi = {v[2], v[3]};
     const u32x2 q = {__builtin_bit_cast(uint32_t, __builtin_convertvector(lo, bf16x2)),
                      __builtin_bit_cast(uint32_t, __builtin_convertvector(hi, bf16x2))};
-    lds_store<u32x2>(stg_at(l32, c >> 3) + ((c & 7) << 1), q);
+    lds_store<u32x2>(stg_at(r, c >> 3) + ((c & 7) << 1), q);
   };
-  auto put32 = [&](int c, f32x4 v) __attribute__((always_inline)) {
-    lds_store<u32x4>(stg_at(l32, c >> 2), __builtin_bit_cast(u32x4, v));
+  auto put32 = [&](int r, int c, f32x4 v) __attribute__((always_inline)) {
+    lds_store<u32x4>(stg_at(r, c >> 2), __builtin_bit_cast(u32x4, v));
   };
   // The staged rows row0 .. + 31, columns col0 .. + width, to bf16 rows at dst
   auto flush16 = [&](char* dst, int64_t stride, int64_t row0, int64_t col0, int width, int64_t end)
       __attribute__((always_inline)) {
-    const int c = lane & 7;
+    const int c = el & 7;
     const int64_t col = col0 + c * 8;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int r = (lane >> 3) + 8 * j;
+      const int r = (el >> 3) + 8 * j;
       const u32x4 v = lds_load<u32x4>(stg_at(r, c));
       const int64_t row = row0 + r;
       if (row < p.m && col < end && c * 8 < width) *reinterpret_cast<u32x4*>(dst + (row * stride + col) * 2) = v;
@@ -340,11 +415,11 @@ __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) voi
   };
   // The same from f32 staging, with what the value meets in memory
   auto flush32 = [&](char* dst, int64_t row0, int col0, int width) __attribute__((always_inline)) {
-    const int c = lane & 7;
+    const int c = el & 7;
     const int col = col0 + c * 4;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int r = (lane >> 3) + 8 * j;
+      const int r = (el >> 3) + 8 * j;
       f32x4 t = __builtin_bit_cast(f32x4, lds_load<u32x4>(stg_at(r, c)));
       const int64_t row = row0 + r;
       if (row < p.m && col < p.n && c * 4 < width) {
@@ -389,181 +464,179 @@ __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) voi
   constexpr bool STG16 = EPI == EPI_GATED || EPI == EPI_DXENT || (EPI == EPI_LINEAR && OUT16 && !RES);
 
   auto tile_end = [&](const Unit& q) __attribute__((always_inline)) {
+    el = (int)opaque((uint32_t)lane);
     const int ncol0 = q.nt * BNO;
+    const int er = el & 15, ec = 4 * (el >> 4);   // this lane's row and first column of a block
 #pragma unroll
-    for (int b = 0; b < WMB; ++b) {
-      const int64_t row0 = (int64_t)q.mt * BM + (wm * WMB + b) * 32;
+    for (int b0 = 0; b0 < WMB; b0 += 2) {
+      const int64_t row0 = (int64_t)q.mt * BM + (wm * WMB + b0) * 16;
       if constexpr (EPI == EPI_GATED) {
-        // block wn WNB + a: 16 gate rows and their 16 up rows, output columns 16 (wn WNB + a) ..
-        constexpr int PER = WNB < 4 ? WNB : 4;
+        // blocks 2 i and 2 i + 1: 16 gate rows and their up rows, output columns 16 (wn WNB / 2 + i) ..
+        constexpr int NG = WNB / 2;
+        const int col = ncol0 + wn * NG * 16;
+        if (p.pre) {
 #pragma unroll
-        for (int a0 = 0; a0 < WNB; a0 += PER) {
-          const int col = ncol0 + (wn * WNB + a0) * 16;
-          if (p.pre) {
+          for (int part = 0; part < 2; ++part) {
 #pragma unroll
-            for (int part = 0; part < 2; ++part) {
+            for (int i = 0; i < NG; ++i)
 #pragma unroll
-              for (int a = a0; a < a0 + PER; ++a)
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                  f32x4 v;
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) v[e] = acc[a][b][4 * (g + 2 * part) + e];
-                  put16((a - a0) * 16 + 8 * g + 4 * hf, v);
-                }
-              flush16(p.pre + (part ? (int64_t)p.n * 2 : 0), p.ps, row0, col, PER * 16, p.n);
-            }
+              for (int b = 0; b < 2; ++b) put16(b * 16 + er, i * 16 + ec, acc[2 * i + part][b0 + b]);
+            flush16(p.pre + (part ? (int64_t)p.n * 2 : 0), p.ps, row0, col, NG * 16, p.n);
           }
-#pragma unroll
-          for (int a = a0; a < a0 + PER; ++a)
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              f32x4 v;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) v[e] = acc[a][b][4 * g + e];
-              v = act_apply4(p.act, v);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) v[e] *= acc[a][b][4 * (g + 2) + e];
-              put16((a - a0) * 16 + 8 * g + 4 * hf, v);
-            }
-          flush16(p.y, p.ys, row0, col, PER * 16, p.n);
         }
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            f32x4 v = act_apply4(p.act, acc[2 * i][b0 + b]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] *= acc[2 * i + 1][b0 + b][e];
+            put16(b * 16 + er, i * 16 + ec, v);
+          }
+        flush16(p.y, p.ys, row0, col, NG * 16, p.n);
       } else if constexpr (EPI == EPI_XENT || EPI == EPI_DXENT) {
-        const int64_t row = row0 + l32;
-        const bool in = row < p.m;
-        const int colb = ncol0 + wn * WNB * 32 + 4 * hf;   // this lane's first column
-        const int t = in ? p.target[row] : p.ignore;
-        const int tc = t == p.ignore ? -1 : t - p.col0;    // the target's column, if it is in [0, n)
+        const int colb = ncol0 + wn * WNB * 16 + ec;   // this lane's first column
+        const bool whole = ncol0 + BN <= p.n;
         // Scores in place of the products, columns past n -inf. (One block of
         // columns at a time: with all bias loads in flight at once the 256 x 256
         // shape spills.)
-        const bool whole = ncol0 + BN <= p.n;
 #pragma unroll
         for (int a = 0; a < WNB; ++a) {
+          f32x4 bv = zero;
           if (p.bias) {
-            f32x4 bv[4];
-            if (whole) {   // (uniform)
-#pragma unroll
-              for (int g = 0; g < 4; ++g) bv[g] = *reinterpret_cast<const f32x4*>(p.bias + colb + a * 32 + 8 * g);
+            if (whole) {
+              bv = *reinterpret_cast<const f32x4*>(p.bias + colb + a * 16);
             } else {
 #pragma unroll
-              for (int g = 0; g < 4; ++g)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) bv[g][e] = p.bias[min(colb + a * 32 + 8 * g + e, p.n - 1)];
+              for (int e = 0; e < 4; ++e) bv[e] = p.bias[min(colb + a * 16 + e, p.n - 1)];
             }
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[a][b][4 * g + e] = __builtin_fmaf(p.alpha, acc[a][b][4 * g + e], bv[g][e]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[a][b][e] *= p.alpha;
           }
-          if (!whole) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
+          for (int b = b0; b < b0 + 2; ++b)
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (colb + a * 32 + 8 * g + e >= p.n) acc[a][b][4 * g + e] = -INFINITY;
-          }
+            for (int e = 0; e < 4; ++e) {
+              float s = __builtin_fmaf(p.alpha, acc[a][b][e], bv[e]);
+              if (!whole && colb + a * 16 + e >= p.n) s = -INFINITY;
+              acc[a][b][e] = s;
+            }
           __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (EPI == EPI_XENT) {
-          if (__any(tc >= colb && tc < colb + WNB * 32)) {
+#pragma unroll
+          for (int b = b0; b < b0 + 2; ++b) {
+            const int64_t row = row0 + (b - b0) * 16 + er;
+            const bool in = row < p.m;
+            const int t = in ? p.target[row] : p.ignore;
+            const int tc = t == p.ignore ? -1 : t - p.col0;   // the target's column, if it is in [0, n)
+            if (__any(tc >= colb - ec && tc < colb - ec + WNB * 16)) {
+#pragma unroll
+              for (int a = 0; a < WNB; ++a)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (in && tc == colb + a * 16 + e && tc < p.n) p.at[row] = acc[a][b][e];
+            }
+            float top = -INFINITY;
 #pragma unroll
             for (int a = 0; a < WNB; ++a)
 #pragma unroll
-              for (int g = 0; g < 4; ++g)
+              for (int e = 0; e < 4; ++e) top = fmaxf(top, acc[a][b][e]);
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float base = top == -INFINITY ? 0.f : top;
+            float sum = 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (in && tc == colb + a * 32 + 8 * g + e && tc < p.n) p.at[row] = acc[a][b][4 * g + e];
+            for (int a = 0; a < WNB; ++a)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f((acc[a][b][e] - base) * 1.44269504088896f);
+            sum += __shfl_xor(sum, 16, 64);
+            sum += __shfl_xor(sum, 32, 64);
+            if (in && el < 16) p.part[(int64_t)(q.nt * C::NWN + wn) * p.m + row] = make_float2(top, sum);
           }
-          float top = -INFINITY;
-#pragma unroll
-          for (int a = 0; a < WNB; ++a)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) top = fmaxf(top, acc[a][b][e]);
-          top = fmaxf(top, __shfl_xor(top, 32, 64));
-          const float base = top == -INFINITY ? 0.f : top;
-          float sum = 0.f;
-#pragma unroll
-          for (int a = 0; a < WNB; ++a) {
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f((acc[a][b][e] - base) * 1.44269504088896f);
-          }
-          sum += __shfl_xor(sum, 32, 64);
-          if (in && hf == 0) p.part[(int64_t)(q.nt * C::NWN + wn) * p.m + row] = make_float2(top, sum);
         } else {
-          const float lse = in ? p.lse[row] : 0.f;
-          const float f = in && t != p.ignore ? p.dl[row] : 0.f;
-          // (an ignored row is zeros whatever its scores are)
-          const bool live = f != 0.f || f != f;
+          float lse[2], f[2];
+          int tc[2];
+          bool live[2];   // (an ignored row is zeros whatever its scores are)
 #pragma unroll
-          for (int a0 = 0; a0 < WNB; a0 += (WNB < 2 ? 1 : 2)) {
-            constexpr int PER = WNB < 2 ? 1 : 2;
+          for (int b = 0; b < 2; ++b) {
+            const int64_t row = row0 + b * 16 + er;
+            const bool in = row < p.m;
+            const int t = in ? p.target[row] : p.ignore;
+            tc[b] = t == p.ignore ? -1 : t - p.col0;
+            lse[b] = in ? p.lse[row] : 0.f;
+            f[b] = t != p.ignore ? p.dl[row] : 0.f;
+            live[b] = f[b] != 0.f || f[b] != f[b];
+          }
+          constexpr int PER = WNB < 4 ? WNB : 4;
+#pragma unroll
+          for (int a0 = 0; a0 < WNB; a0 += PER) {
 #pragma unroll
             for (int a = a0; a < a0 + PER; ++a)
 #pragma unroll
-              for (int g = 0; g < 4; ++g) {
-                __builtin_amdgcn_sched_barrier(0);
-                const int col = colb + a * 32 + 8 * g;
+              for (int b = 0; b < 2; ++b) {
                 f32x4 v;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                  float pr = __builtin_amdgcn_exp2f((acc[a][b][4 * g + e] - lse) * 1.44269504088896f);
-                  if (col + e == tc) pr -= 1.f;
-                  v[e] = live && (whole || col + e < p.n) ? pr * f : 0.f;
+                  const int col = colb + a * 16 + e;
+                  float pr = __builtin_amdgcn_exp2f((acc[a][b0 + b][e] - lse[b]) * 1.44269504088896f);
+                  if (col == tc[b]) pr -= 1.f;
+                  v[e] = live[b] && (whole || col < p.n) ? pr * f[b] : 0.f;
                 }
-                put16((a - a0) * 32 + 8 * g + 4 * hf, v);
+                put16(b * 16 + er, (a - a0) * 16 + ec, v);
+                __builtin_amdgcn_sched_barrier(0);
               }
-            flush16(p.y, p.ys, row0, ncol0 + (wn * WNB + a0) * 32, PER * 32, p.n_store);
+            flush16(p.y, p.ys, row0, ncol0 + (wn * WNB + a0) * 16, PER * 16, p.n_store);
           }
         }
       } else {
         constexpr int COLS = STG16 ? 64 : 32;
-        constexpr int PER = COLS / 32 < WNB ? COLS / 32 : WNB;
+        constexpr int PER = COLS / 16 < WNB ? COLS / 16 : WNB;
         char* dst = EPI == EPI_PART ? p.y + (int64_t)q.s * p.m * p.n * 4 : p.y;
 #pragma unroll
         for (int a0 = 0; a0 < WNB; a0 += PER) {
-          const int col0 = ncol0 + (wn * WNB + a0) * 32;
-          f32x4 z[PER * 4];
+          const int col0 = ncol0 + (wn * WNB + a0) * 16;
+          f32x4 z[PER][2];
 #pragma unroll
           for (int a = 0; a < PER; ++a)
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
+            for (int b = 0; b < 2; ++b)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                z[a * 4 + g][e] = EPI == EPI_LINEAR ? p.alpha * acc[a0 + a][b][4 * g + e] : acc[a0 + a][b][4 * g + e];
+                z[a][b][e] = EPI == EPI_LINEAR ? p.alpha * acc[a0 + a][b0 + b][e] : acc[a0 + a][b0 + b][e];
           if constexpr (EPI == EPI_LINEAR) {
             if (p.bias) {
 #pragma unroll
-              for (int i = 0; i < PER * 4; ++i) {
-                const int col = min(col0 + i * 8 + 4 * hf, p.n - 4);
-                const f32x4 bv = *reinterpret_cast<const f32x4*>(p.bias + col);
+              for (int a = 0; a < PER; ++a) {
+                const f32x4 bv = *reinterpret_cast<const f32x4*>(p.bias + min(col0 + a * 16 + ec, p.n - 4));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) z[i][e] += bv[e];
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) z[a][b][e] += bv[e];
               }
             }
             if (p.pre) {
 #pragma unroll
-              for (int i = 0; i < PER * 4; ++i) put16(i * 8 + 4 * hf, z[i]);
-              flush16(p.pre, p.ps, row0, col0, PER * 32, p.n);
+              for (int a = 0; a < PER; ++a)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) put16(b * 16 + er, a * 16 + ec, z[a][b]);
+              flush16(p.pre, p.ps, row0, col0, PER * 16, p.n);
             }
             if (p.act != ACT_NONE) {
 #pragma unroll
-              for (int i = 0; i < PER * 4; ++i) z[i] = act_apply4(p.act, z[i]);
+              for (int a = 0; a < PER; ++a)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) z[a][b] = act_apply4(p.act, z[a][b]);
             }
           }
-          if constexpr (STG16) {
 #pragma unroll
-            for (int i = 0; i < PER * 4; ++i) put16(i * 8 + 4 * hf, z[i]);
-            flush16(dst, p.ys, row0, col0, PER * 32, p.n);
-          } else {
+          for (int a = 0; a < PER; ++a)
 #pragma unroll
-            for (int i = 0; i < PER * 4; ++i) put32(i * 8 + 4 * hf, z[i]);
-            flush32(dst, row0, col0, PER * 32);
-          }
+            for (int b = 0; b < 2; ++b) {
+              if constexpr (STG16) put16(b * 16 + er, a * 16 + ec, z[a][b]);
+              else put32(b * 16 + er, a * 16 + ec, z[a][b]);
+            }
+          if constexpr (STG16) flush16(dst, p.ys, row0, col0, PER * 16, p.n);
+          else flush32(dst, row0, col0, PER * 16);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
@@ -573,35 +646,126 @@ __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) voi
       for (int b = 0; b < WMB; ++b) acc[a][b] = zero;
   };
 
-  // The cross entropy epilogues need the registers of the next unit's first
-  // operands: they are read after it.
-  constexpr bool LATE = EPI == EPI_XENT || EPI == EPI_DXENT;
-  // One iteration per stage: read its second k step while the first one's
-  // MFMAs run; wait for the next stage (vmcnt) and for every wave to have read
-  // this one (barrier), refill its slot, and read the next stage's first step
-  // while the second step's MFMAs run.
   ld_unit();
-  Half h0, h1;
-#pragma unroll
-  for (int i = 0; i < STAGES; ++i) issue();
-  asm volatile("s_waitcnt vmcnt(%0)" :: "n"((STAGES - 1) * PER_WAVE) : "memory");
-  lds_barrier();
-  read_half(0, h0);
-  for (int j = 0; j < my_units; ++j) {
-    const Unit q = unit_of(j);
-    const int stages = min(p.kper, kst - q.s * p.kper);
-    for (int s = 0; s < stages; ++s) {
-      read_half(1, h1);
-      mfmas(h0);
-      asm volatile("s_waitcnt vmcnt(%0)" :: "n"((STAGES - 2) * PER_WAVE) : "memory");
+  u32x4 fx[TG_KS][WMB], fw[C::H][TG_KS][C::WH];   // operands of a stage
+  if constexpr (C::H == 2) {
+    // Two phases per stage, the products of the lower and of the upper w blocks.
+    // The operands of a phase are read from LDS in the one before: during phase A the
+    // upper w blocks of its stage, during phase B x and the lower w blocks of the
+    // next (x into the registers that the step's products have just read). So
+    // x and the lower half of a slot are free one phase into its stage, the upper half two, and
+    // their refills have three of the four phases of a two-slot ring to arrive.
+    auto boundary = [&]() __attribute__((always_inline)) {
+      // every wave's loads of what the next phase reads have landed, and its
+      // reads of what is refilled now are done
+      asm volatile("s_waitcnt vmcnt(%0)" :: "n"(C::PER_WAVE) : "memory");
       lds_barrier();
-      issue();
-      if (++rd_slot == STAGES) rd_slot = 0;
-      if (!LATE || s + 1 < stages) read_half(0, h0);
-      mfmas(h1);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto read_first = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int ks = 0; ks < TG_KS; ++ks) {
+#pragma unroll
+        for (int i = 0; i < C::WH; ++i) fw[0][ks][i] = read_w(0, i, ks);
+#pragma unroll
+        for (int b = 0; b < WMB; ++b) fx[ks][b] = read_x(b, ks);
+      }
+    };
+    // The products of a phase (h: lower or upper w blocks), each followed by a read or a
+    // refill at most: a product keeps its matrix core busy for four issue slots of
+    // the wave, which hide that many instructions and not a dozen at once. With the
+    // reads and refills in groups a stage of 4,096 rows of zeros took 1.11 us, so 1.02.
+    // AHEAD: read the other w blocks, and in phase B x, for the next phase.
+    auto phase = [&](auto hc, auto ahead) __attribute__((always_inline)) {
+      constexpr int h = decltype(hc)::value;
+      constexpr bool AHEAD = decltype(ahead)::value;
+      constexpr int L = h ? L1 : L0;
+      constexpr int NP = TG_KS * WMB * C::WH;            // products
+      constexpr int XR = h && AHEAD ? WMB * TG_KS : 0;   // x reads, one behind each block's last product of a step
+#pragma unroll
+      for (int t = 0; t < NP; ++t) {
+        const int ks = t / (WMB * C::WH), b = t / C::WH % WMB, i = t % C::WH;
+        mfma(h * C::WH + i, b, fw[h][ks][i], fx[ks][b]);
+        if constexpr (XR > 0) {
+          if (i == C::WH - 1) fx[ks][b] = read_x(b, ks);
+        }
+        // w reads of a k step in the first half of the step's products: the registers
+        // of the steps before are free by then
+        if constexpr (AHEAD) {
+          const int u = t % (WMB * C::WH);
+          const int r = u % 2 == 1 && u / 2 < C::WH ? ks * C::WH + u / 2 : -1;
+          if (r >= 0) fw[1 - h][r / C::WH][r % C::WH] = read_w(1 - h, r % C::WH, r / C::WH);
+        }
+        // refills: spread over the rest
+        {
+          constexpr int first = h == 0 ? 2 : NP / 2 + 2, step = h == 0 ? (NP - 4) / L0 : NP / 8;
+          if ((t - first) >= 0 && (t - first) % step == 0 && (t - first) / step < L) load(h, (t - first) / step);
+          static_assert(first + (L > 0 ? L - 1 : 0) * step < NP, "every refill of a phase has a place");
+          if (t == NP - 3) {
+            if (h == 0 && AHEAD) rd_next();
+            end(h);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    const std::integral_constant<int, 0> A{};
+    const std::integral_constant<int, 1> B{};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      issue(0);
+      issue(1);
     }
-    tile_end(q);
-    if (LATE) read_half(0, h0);
+    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(C::PER_WAVE + C::PW) : "memory");
+    lds_barrier();
+    for (int j = 0; j < my_units; ++j) {
+      const Unit q = unit_of(j);
+      const int stages = min(p.kper, kst - q.s * p.kper);
+      read_first();
+      for (int s = 1; s < stages; ++s) {
+        boundary();
+        phase(A, std::true_type{});
+        boundary();
+        phase(B, std::true_type{});
+      }
+      // the last stage reads nothing past itself: the epilogue needs the registers
+      boundary();
+      phase(A, std::true_type{});
+      boundary();
+      phase(B, std::false_type{});
+      tile_end(q);
+    }
+  } else {
+    // Small tiles: whole stages, STAGES - 1 of them in flight.
+    auto read_stage = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int ks = 0; ks < TG_KS; ++ks) {
+#pragma unroll
+        for (int i = 0; i < C::WH; ++i) fw[0][ks][i] = read_w(0, i, ks);
+#pragma unroll
+        for (int b = 0; b < WMB; ++b) fx[ks][b] = read_x(b, ks);
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) issue(0);
+    for (int j = 0; j < my_units; ++j) {
+      const Unit q = unit_of(j);
+      const int stages = min(p.kper, kst - q.s * p.kper);
+      for (int s = 0; s < stages; ++s) {
+        asm volatile("s_waitcnt vmcnt(%0)" :: "n"((STAGES - 2) * C::PER_WAVE) : "memory");
+        lds_barrier();   // this stage is in LDS, and every wave has read the one before
+        issue(0);        // ... whose slot this refills
+        read_stage();
+        rd_next();
+#pragma unroll
+        for (int ks = 0; ks < TG_KS; ++ks)
+#pragma unroll
+          for (int i = 0; i < C::WH; ++i)
+#pragma unroll
+            for (int b = 0; b < WMB; ++b) mfma(i, b, fw[0][ks][i], fx[ks][b]);
+      }
+      tile_end(q);
+    }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the dummy loads past the end
 }

@@ -122,14 +122,25 @@ int tile_tn_linear(TileParams p, const TilePlan& plan, bool out_bf16, float* par
                   : tile_launch<OP_COLS, OP_COLS, EPI_LINEAR, false, false>(p, plan, cus, stream);
 }
 
-TilePlan tile_plan(int64_t m, int64_t n, int64_t k, bool gated, int max_splits, int cus) {
+// Estimated us of a launch: `start`, then the units of the fullest CU one after
+// another, each kper stages and `drain`. A stage of the largest shape is slower on a
+// full chip than on a few CUs (the clock goes down under load), 1.05 to 1.42 us.
+// Fitted to x . w^T in bf16, us of the shapes 0 / 1 / 2, one split:
+//   (1,024 rows, 1,024 outputs, k 8,192): 141 / 60 / 35    (8,192, 1,024, 1,024): 29 / 21 / 34
+//   (8,192, 1,024, 2,048): 45 / 35 / 58                    (12,000, 768, 768): 24 / 24 / 29
+//   (20,011, 768, 768): 27 / 30 / 46                       (16,384, 2,304, 768): 63 / 60 / 103
+//   (16,384, 4,096, 1,024): 114 / 137 / 226                (2,048, 4,096, 1,024): 29 / 21 / 34
+// Joining s splits: a launch, and the partials written and read.
+// An operand by columns costs two reads per fragment, which the smaller shapes
+// feel: `cols` us a stage more for each.
+TilePlan tile_plan(int64_t m, int64_t n, int64_t k, int by_cols, bool gated, int max_splits, int cus) {
   struct Cost {
     int bn, bm;
-    float stage, drain, start;   // us
+    float stage, full, drain, start, cols;
   };
-  static const Cost costs[TG_SHAPES] = {{TileShapeOf<0>::BN, TileShapeOf<0>::BM, 0.56f, 9.f, 2.f},
-                                        {TileShapeOf<1>::BN, TileShapeOf<1>::BM, 0.25f, 2.2f, 2.9f},
-                                        {TileShapeOf<2>::BN, TileShapeOf<2>::BM, 0.13f, 0.5f, 3.7f}};
+  static const Cost costs[TG_SHAPES] = {{TileShapeOf<0>::BN, TileShapeOf<0>::BM, 1.05f, 1.42f, 4.5f, 4.f, 0.f},
+                                        {TileShapeOf<1>::BN, TileShapeOf<1>::BM, 0.44f, 0.47f, 1.f, 4.5f, 0.045f},
+                                        {TileShapeOf<2>::BN, TileShapeOf<2>::BM, 0.25f, 0.21f, 0.4f, 3.5f, 0.02f}};
   const int64_t kst = std::max<int64_t>(1, (k + TG_BK - 1) / TG_BK);
   TilePlan best{0, 1, (int32_t)kst};
   float least = -1.f;
@@ -137,13 +148,14 @@ TilePlan tile_plan(int64_t m, int64_t n, int64_t k, bool gated, int max_splits, 
     const Cost& c = costs[i];
     const int64_t bno = gated ? c.bn / 2 : c.bn;
     const int64_t tiles = ((m + c.bm - 1) / c.bm) * ((n + bno - 1) / bno);
-    for (int s = 1; s <= max_splits && s <= kst; s = s < 4 ? s + 1 : s + s / 4) {
+    for (int s = 1; s <= max_splits && s <= kst; ++s) {
       const int64_t kper = (kst + s - 1) / s;
-      const int64_t used = (kst + kper - 1) / kper;   // splits that have work
-      if (used != s) continue;
-      float t = c.start + (float)((tiles * s + cus - 1) / cus) * ((float)kper * c.stage + c.drain);
-      // joining: the partials written and read at some 3.5 TB/s, and a launch
-      if (s > 1) t += 3.f + (float)m * (float)n * (gated ? 2.f : 1.f) * 8.f * (float)s / 3.5e6f;
+      if ((kst + kper - 1) / kper != s) continue;   // a split would have no work
+      const int64_t units = tiles * s;
+      const float fill = std::min(1.f, (float)units / (float)cus);
+      const float stage = c.stage + fill * (c.full - c.stage) + (float)by_cols * c.cols;
+      float t = c.start + (float)((units + cus - 1) / cus) * ((float)kper * stage + c.drain);
+      if (s > 1) t += 3.f + (float)m * (float)n * (gated ? 2.f : 1.f) * 8.f * (float)s / 7e6f;
       if (least < 0.f || t < least) {
         least = t;
         best = {i, s, (int32_t)kper};

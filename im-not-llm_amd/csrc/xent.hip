@@ -79,10 +79,10 @@ __global__ __launch_bounds__(256) void xent_dloss_kernel(const float* dl, const 
 
 constexpr int MAX_SPLITS = 32;
 
-// Vocabulary entries per piece: g of a piece is some 64 MiB, so that dw and dx
+// Vocabulary entries per piece: g of a piece is some 128 MiB, so that dw and dx
 // read it from the 256 MB Infinity Cache, in whole 256-column tiles.
 int64_t piece_cols(int64_t m, int64_t vocab) {
-  int64_t p = ((int64_t)1 << 25) / std::max<int64_t>(m, 1);
+  int64_t p = ((int64_t)1 << 26) / std::max<int64_t>(m, 1);
   p = std::min(std::max<int64_t>(p, 4096), vocab);
   return (p + 255) / 256 * 256;
 }
@@ -96,11 +96,11 @@ struct XentPlan {
 int xent_plan(const inl_softmax_xent_desc& d, XentPlan* p) {
   int rc = device_cus(&p->cus);
   if (rc) return rc;
-  p->s = tile_plan(d.m, d.vocab, d.hidden, false, 1, p->cus);
+  p->s = tile_plan(d.m, d.vocab, d.hidden, 0, false, 1, p->cus);
   p->piece = piece_cols(d.m, d.vocab);
-  p->g = tile_plan(d.m, p->piece, d.hidden, false, 1, p->cus);
-  p->dw = tile_plan(std::min(p->piece, d.vocab), d.hidden, d.m, false, MAX_SPLITS, p->cus);
-  p->dx = tile_plan(d.m, d.hidden, p->piece, false, MAX_SPLITS, p->cus);
+  p->g = tile_plan(d.m, p->piece, d.hidden, 0, false, 1, p->cus);
+  p->dw = tile_plan(std::min(p->piece, d.vocab), d.hidden, d.m, 2, false, MAX_SPLITS, p->cus);
+  p->dx = tile_plan(d.m, d.hidden, p->piece, 1, false, MAX_SPLITS, p->cus);
   return INL_OK;
 }
 
