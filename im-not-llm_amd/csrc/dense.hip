@@ -284,10 +284,14 @@ struct DensePlan {
   }
 };
 
-int dense_plan(const inl_dense_desc& d, DensePlan* p, int* cus) {
+int dense_plan(const inl_dense_desc& d, bool backward, DensePlan* p, int* cus) {
+  if (!backward && d.m <= FEW_DENSE_ROWS) return INL_OK;
   int rc = device_cus(cus);
   if (rc) return rc;
-  p->y = tile_plan(d.m, d.n, d.k, 0, false, MAX_SPLITS, *cus);
+  if (!backward) {
+    p->y = tile_plan(d.m, d.n, d.k, 0, false, MAX_SPLITS, *cus);
+    return INL_OK;
+  }
   p->dx = tile_plan(d.m, d.k, d.n, 1, false, MAX_SPLITS, *cus);
   p->dw = tile_plan(d.n, d.k, d.m, 2, false, MAX_SPLITS, *cus);
   return INL_OK;
@@ -304,7 +308,7 @@ extern "C" int inl_dense_workspace_size(const inl_dense_desc* d, int32_t backwar
   if (rc) return rc;
   DensePlan plan;
   int cus = 0;
-  if ((rc = dense_plan(*d, &plan, &cus))) return rc;
+  if ((rc = dense_plan(*d, backward != 0, &plan, &cus))) return rc;
   *bytes = plan.need(*d, backward != 0);
   return INL_OK;
 }
@@ -324,7 +328,7 @@ extern "C" int inl_dense_fwd(const inl_dense_desc* d, const void* x, const void*
   if ((uintptr_t)bias & 15) return fail(INL_E_INVALID, "dense: bias must be 16-byte aligned");
   DensePlan plan;
   int cus = 0;
-  if ((rc = dense_plan(*d, &plan, &cus))) return rc;
+  if ((rc = dense_plan(*d, false, &plan, &cus))) return rc;
   if ((rc = check_workspace("dense", ws, ws_bytes, plan.need(*d, false)))) return rc;
   TileParams p{};
   p.x = (const char*)x;
@@ -371,7 +375,7 @@ extern "C" int inl_dense_bwd(const inl_dense_desc* d, const void* dy, const void
   if (acts && (rc = check_rows("dense: pre", pre, d->n, s.pre, INL_BF16))) return rc;
   DensePlan plan;
   int cus = 0;
-  if ((rc = dense_plan(*d, &plan, &cus))) return rc;
+  if ((rc = dense_plan(*d, true, &plan, &cus))) return rc;
   if ((rc = check_workspace("dense", ws, ws_bytes, plan.need(*d, true)))) return rc;
   Carve c(ws);
   char* dzb = acts ? c.take((size_t)d->m * d->n * 2) : nullptr;

@@ -32,11 +32,15 @@ struct FfnPlan {
   TilePlan h, y, dh, dwd, dx, dwgu;
   int cus = 0;
 };
-int ffn_plan(const inl_gated_ffn_desc& d, FfnPlan* p) {
+int ffn_plan(const inl_gated_ffn_desc& d, bool backward, FfnPlan* p) {
+  if (!backward && d.m <= FEW_DENSE_ROWS) return INL_OK;
   int rc = device_cus(&p->cus);
   if (rc) return rc;
-  p->h = tile_plan(d.m, d.inner, d.hidden, 0, true, MAX_SPLITS, p->cus);
-  p->y = tile_plan(d.m, d.hidden, d.inner, 0, false, MAX_SPLITS, p->cus);
+  if (!backward) {
+    p->h = tile_plan(d.m, d.inner, d.hidden, 0, true, MAX_SPLITS, p->cus);
+    p->y = tile_plan(d.m, d.hidden, d.inner, 0, false, MAX_SPLITS, p->cus);
+    return INL_OK;
+  }
   p->dh = tile_plan(d.m, d.inner, d.hidden, 1, false, MAX_SPLITS, p->cus);
   p->dwd = tile_plan(d.hidden, d.inner, d.m, 2, false, MAX_SPLITS, p->cus);
   p->dx = tile_plan(d.m, d.hidden, 2 * d.inner, 1, false, MAX_SPLITS, p->cus);
@@ -69,7 +73,7 @@ extern "C" int inl_gated_ffn_workspace_size(const inl_gated_ffn_desc* d, int32_t
   int rc = ffn_check(d);
   if (rc) return rc;
   FfnPlan plan;
-  if ((rc = ffn_plan(*d, &plan))) return rc;
+  if ((rc = ffn_plan(*d, backward != 0, &plan))) return rc;
   *bytes = ffn_need(*d, plan, backward != 0);
   return INL_OK;
 }
@@ -93,7 +97,7 @@ extern "C" int inl_gated_ffn_fwd(const inl_gated_ffn_desc* d, const void* x, con
   if (pre && (rc = check_rows("gated_ffn: pre", pre, 2 * d->inner, 2 * d->inner, INL_BF16))) return rc;
   if (h && (rc = check_rows("gated_ffn: h", h, d->inner, d->inner, INL_BF16))) return rc;
   FfnPlan plan;
-  if ((rc = ffn_plan(*d, &plan))) return rc;
+  if ((rc = ffn_plan(*d, false, &plan))) return rc;
   if ((rc = check_workspace("gated_ffn", ws, ws_bytes, ffn_need(*d, plan, false)))) return rc;
   Carve c(ws);
   char* hb = c.take(rows_bytes(*d, false));
@@ -159,7 +163,7 @@ extern "C" int inl_gated_ffn_bwd(const inl_gated_ffn_desc* d, const void* dy, co
   if (dw_gate_up && (rc = check_rows("gated_ffn: x", x, d->hidden, xs, INL_BF16))) return rc;
   if (dw_down && (rc = check_rows("gated_ffn: h", h, d->inner, d->inner, INL_BF16))) return rc;
   FfnPlan plan;
-  if ((rc = ffn_plan(*d, &plan))) return rc;
+  if ((rc = ffn_plan(*d, true, &plan))) return rc;
   if ((rc = check_workspace("gated_ffn", ws, ws_bytes, ffn_need(*d, plan, true)))) return rc;
   Carve c(ws);
   char* dgu = c.take(rows_bytes(*d, true));

@@ -9,11 +9,12 @@ captured into a graph.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 
-from . import (INL_BF16, INL_F32, InlError, NormRopeDesc, _check, _dtype_code, _lib, _sig, _stream_ptr, c_i32, c_i64,
-               c_void_p)
+import torch
+
+from . import INL_BF16, INL_F32, InlError, NormRopeDesc, _check, _dtype_code, _sig, c_i32, c_i64, c_void_p
 
 ACTS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu_tanh": 3, "gelu_erf": 4}
 ROPE_HALF, ROPE_AXIAL, ROPE_INTERLEAVED = 1, 2, 3
@@ -59,61 +60,85 @@ _rope_bwd = _sig("inl_norm_rope_qk_bwd", ctypes.c_int, ctypes.POINTER(NormRopeDe
                  *_ptrs(10), ctypes.c_size_t, c_void_p)
 
 
-def _on(t):
-    """The device of ``t`` as the current one: the library launches there."""
-    import torch
-    if not t.is_cuda:
-        raise InlError(-1, f"not a device tensor ({t.device})")
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+_BF16, _F32 = torch.bfloat16, torch.float32
+_B16, _ANY = (_BF16,), (_BF16, _F32)
+_CODE = {_BF16: INL_BF16, _F32: INL_F32}
 
 
-def _mat(name, t, shape, dtypes, like):
+def _at_home(call):
+    """Runs ``call`` with the device of its first tensor as the current one: the
+    library launches there, and workspaces and outputs belong there."""
+    @functools.wraps(call)
+    def wrapped(first, *args, **kwargs):
+        dev = first.get_device()
+        if dev < 0:
+            raise InlError(-1, f"not a device tensor ({first.device})")
+        if dev == torch._C._cuda_getDevice():
+            return call(dev, first, *args, **kwargs)
+        with torch.cuda.device(dev):
+            return call(dev, first, *args, **kwargs)
+    return wrapped
+
+
+def _mat(name, t, rows, cols, dtypes, dev):
     """``t`` as rows of a matrix for the library, which sees only a pointer: its
     shape, type and device, and contiguous rows. Returns the row stride."""
-    if tuple(t.shape) != tuple(shape):
-        raise InlError(-1, f"{name}: shape {tuple(t.shape)}, need {tuple(shape)}")
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != rows or shape[1] != cols:
+        raise InlError(-1, f"{name}: shape {tuple(shape)}, need {(rows, cols)}")
     if t.dtype not in dtypes:
         raise InlError(-1, f"{name}: dtype {t.dtype}, need {' or '.join(str(d) for d in dtypes)}")
-    if t.device != like.device:
-        raise InlError(-1, f"{name}: on {t.device}, x is on {like.device}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if t.get_device() != dev:
+        raise InlError(-1, f"{name}: on {t.device}, need cuda:{dev}")
+    stride = t.stride()
+    if stride[1] != 1 and cols > 1:
         raise InlError(-1, f"{name}: rows must be contiguous")
-    return t.stride(0) if t.dim() > 1 and t.shape[0] > 1 else t.shape[-1]
+    return stride[0] if rows > 1 else cols
 
 
-def _vec(name, t, n, dtype, like):
+def _packed(name, t, rows, cols, dev):
+    if _mat(name, t, rows, cols, _B16, dev) != cols:
+        raise InlError(-1, f"{name}: must be packed")
+
+
+def _vec(name, t, n, dtype, dev):
     if t is None:
         return None
-    if tuple(t.shape) != (n,) or t.dtype != dtype or t.device != like.device or (n > 1 and t.stride(0) != 1):
-        raise InlError(-1, f"{name}: need contiguous {dtype} [{n}] on {like.device}, got {t.dtype} {tuple(t.shape)} "
-                           f"on {t.device}")
+    if t.dtype != dtype or tuple(t.shape) != (n,) or t.get_device() != dev or (n > 1 and t.stride(0) != 1):
+        raise InlError(-1, f"{name}: need contiguous {dtype} [{n}] on cuda:{dev}, got {t.dtype} {tuple(t.shape)} on "
+                           f"{t.device}")
     return t.data_ptr()
 
 
-def _types():
-    import torch
-    return (torch.bfloat16,), (torch.bfloat16, torch.float32)
-
-
 def _act(act, gated=False):
-    if act not in ACTS or (gated and not ACTS[act]):
+    code = ACTS.get(act)
+    if code is None or (gated and not code):
         raise InlError(-1, f"unknown act {act!r}")
-    return ACTS[act]
+    return code
 
 
-def _workspace(size_fn, desc, like, *args):
-    import torch
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(op, dev, backward, *sizes):
+    """By the sizes alone (``dev``: the plan behind them counts compute units)."""
+    desc, size_fn, fields = {"dense": (DenseDesc, _dense_ws, ("m", "n", "k", "act")),
+                             "gated_ffn": (GatedFfnDesc, _ffn_ws, ("m", "hidden", "inner", "act")),
+                             "softmax_xent": (SoftmaxXentDesc, _xent_ws, ("m", "vocab", "hidden"))}[op]
     n = ctypes.c_size_t()
-    _check(size_fn(ctypes.byref(desc), *args, ctypes.byref(n)))
-    return torch.empty(n.value, dtype=torch.uint8, device=like.device) if n.value else None
+    _check(size_fn(desc(**dict(zip(fields, sizes))), backward, ctypes.byref(n)))
+    return n.value
+
+
+def _room(n, dev):
+    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+
+
+def _stream(stream, dev):
+    return torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
 
 
 def _done(stream, *tensors):
     """Tensors allocated here that work on another stream than the current one
     uses: the allocator must not hand their memory out before it is done."""
-    import torch
     if stream is None or stream == torch.cuda.current_stream():
         return
     for t in tensors:
@@ -129,34 +154,62 @@ def _ptr(t):
 # Linear layer
 # ---------------------------------------------------------------------------
 
+@_at_home
+def _dense(dev, x, w, bias, act, residual, pre, out, out_dtype, stream):
+    m, k = x.shape
+    n = w.shape[0]
+    code = _act(act)
+    xs, ws = _mat("x", x, m, k, _B16, dev), _mat("w", w, n, k, _B16, dev)
+    made = None
+    if out is None:
+        made = out = torch.empty((m, n), dtype=out_dtype or _BF16, device=dev)
+    ys = _mat("out", out, m, n, _ANY, dev)
+    rs = rd = ps = 0
+    if residual is not None:
+        rs, rd = _mat("residual", residual, m, n, _ANY, dev), _CODE[residual.dtype]
+    if pre is not None:
+        ps = _mat("pre", pre, m, n, _B16, dev)
+    bp = _vec("bias", bias, n, _F32, dev)
+    d = DenseDesc(m, n, k, xs, ws, ys, rs, ps, 0, 0, code, _CODE[out.dtype], rd, 0, 0)
+    size = _workspace_bytes("dense", dev, 0, m, n, k, code)
+    room = _room(size, dev)
+    _check(_dense_fwd(d, x.data_ptr(), w.data_ptr(), bp, _ptr(residual), out.data_ptr(), _ptr(pre), _ptr(room), size,
+                      _stream(stream, dev)))
+    _done(stream, room, made)
+    return out
+
+
 def dense(x, w, bias=None, *, act=None, residual=None, pre=None, out=None, out_dtype=None, stream=None):
     """``act(x @ w.T + bias) + residual`` (``inl_dense_fwd``): bf16 ``x [m, k]``
     and ``w [n, k]``, f32 ``bias [n]``, ``act`` one of None, "relu", "silu",
     "gelu_tanh", "gelu_erf", ``residual [m, n]`` bf16 or f32 (it may be
     ``out``). ``pre``: a bf16 ``[m, n]`` tensor that receives ``x @ w.T + bias`` for
     ``dense_bwd``. n and k are multiples of 8; rows may be strided."""
-    import torch
-    b16, any_ = _types()
+    return _dense(x, w, bias, act, residual, pre, out, out_dtype, stream)
+
+
+@_at_home
+def _dense_grads(dev, x, dy, w, act, pre, bias_grad, dx_grad, dw_grad, dx_dtype, dw_dtype, stream):
     m, k = x.shape
     n = w.shape[0]
-    with _on(x):
-        d = DenseDesc(m=m, n=n, k=k, act=_act(act))
-        d.x_stride, d.w_stride = _mat("x", x, (m, k), b16, x), _mat("w", w, (n, k), b16, x)
-        made = out is None
-        if made:
-            out = torch.empty((m, n), dtype=out_dtype or torch.bfloat16, device=x.device)
-        d.y_stride, d.out_dtype = _mat("out", out, (m, n), any_, x), _dtype_code(out.dtype)
-        if residual is not None:
-            d.residual_stride = _mat("residual", residual, (m, n), any_, x)
-            d.residual_dtype = _dtype_code(residual.dtype)
-        if pre is not None:
-            d.pre_stride = _mat("pre", pre, (m, n), b16, x)
-        ws = _workspace(_dense_ws, d, x, 0)
-        _check(_dense_fwd(ctypes.byref(d), x.data_ptr(), w.data_ptr(), _vec("bias", bias, n, torch.float32, x),
-                          _ptr(residual), out.data_ptr(), _ptr(pre), _ptr(ws), ws.numel() if ws is not None else 0,
-                          _stream_ptr(stream)))
-        _done(stream, ws, out if made else None)
-    return out
+    code = _act(act)
+    if not code:
+        pre = None
+    elif pre is None:
+        raise InlError(-1, "dense_bwd: an activation needs pre")
+    xs, ws, ys = _mat("x", x, m, k, _B16, dev), _mat("w", w, n, k, _B16, dev), _mat("dy", dy, m, n, _B16, dev)
+    ps = _mat("pre", pre, m, n, _B16, dev) if pre is not None else 0
+    dx = torch.empty((m, k), dtype=dx_dtype or _BF16, device=dev) if dx_grad else None
+    dw = torch.empty((n, k), dtype=dw_dtype or _BF16, device=dev) if dw_grad else None
+    db = torch.empty(n, dtype=_F32, device=dev) if bias_grad else None
+    d = DenseDesc(m, n, k, xs, ws, ys, 0, ps, 0, 0, code, 0, 0, _dtype_code(dx_dtype or _BF16),
+                  _dtype_code(dw_dtype or _BF16))
+    size = _workspace_bytes("dense", dev, 1, m, n, k, code)
+    room = _room(size, dev)
+    _check(_dense_bwd(d, dy.data_ptr(), x.data_ptr(), w.data_ptr(), _ptr(pre), _ptr(dx), _ptr(dw), _ptr(db),
+                      _ptr(room), size, _stream(stream, dev)))
+    _done(stream, room, dx, dw, db)
+    return dx, dw, db
 
 
 def dense_bwd(dy, x, w, *, act=None, pre=None, bias_grad=False, dx_grad=True, dw_grad=True, dx_dtype=None,
@@ -165,35 +218,38 @@ def dense_bwd(dy, x, w, *, act=None, pre=None, bias_grad=False, dx_grad=True, dw
     ``pre`` is what the forward stored (not needed without an activation). dx and dw are
     bf16 unless ``dx_dtype``/``dw_dtype`` say float32, dbias f32; what is not asked
     for is None. The residual's gradient is ``dy``."""
-    import torch
-    b16, _ = _types()
-    m, n = dy.shape
-    k = x.shape[1]
-    with _on(x):
-        d = DenseDesc(m=m, n=n, k=k, act=_act(act))
-        d.x_stride, d.w_stride = _mat("x", x, (m, k), b16, x), _mat("w", w, (n, k), b16, x)
-        d.y_stride = _mat("dy", dy, (m, n), b16, x)
-        if d.act:
-            if pre is None:
-                raise InlError(-1, "dense_bwd: an activation needs pre")
-            d.pre_stride = _mat("pre", pre, (m, n), b16, x)
-        else:
-            pre = None
-        dx = torch.empty((m, k), dtype=dx_dtype or torch.bfloat16, device=x.device) if dx_grad else None
-        dw = torch.empty((n, k), dtype=dw_dtype or torch.bfloat16, device=x.device) if dw_grad else None
-        db = torch.empty(n, dtype=torch.float32, device=x.device) if bias_grad else None
-        d.dx_dtype = _dtype_code(dx.dtype) if dx_grad else INL_BF16
-        d.dw_dtype = _dtype_code(dw.dtype) if dw_grad else INL_BF16
-        ws = _workspace(_dense_ws, d, x, 1)
-        _check(_dense_bwd(ctypes.byref(d), dy.data_ptr(), x.data_ptr(), w.data_ptr(), _ptr(pre), _ptr(dx), _ptr(dw),
-                          _ptr(db), _ptr(ws), ws.numel() if ws is not None else 0, _stream_ptr(stream)))
-        _done(stream, ws, dx, dw, db)
-    return dx, dw, db
+    return _dense_grads(x, dy, w, act, pre, bias_grad, dx_grad, dw_grad, dx_dtype, dw_dtype, stream)
 
 
 # ---------------------------------------------------------------------------
 # Gated feed-forward block
 # ---------------------------------------------------------------------------
+
+@_at_home
+def _ffn(dev, x, w_gate_up, w_down, act, residual, save, out, out_dtype, stream):
+    m, hidden = x.shape
+    inner = w_down.shape[1]
+    code = _act(act, True)
+    xs = _mat("x", x, m, hidden, _B16, dev)
+    _packed("w_gate_up", w_gate_up, 2 * inner, hidden, dev)
+    _packed("w_down", w_down, hidden, inner, dev)
+    made = None
+    if out is None:
+        made = out = torch.empty((m, hidden), dtype=out_dtype or _BF16, device=dev)
+    ys = _mat("out", out, m, hidden, _ANY, dev)
+    rs = rd = 0
+    if residual is not None:
+        rs, rd = _mat("residual", residual, m, hidden, _ANY, dev), _CODE[residual.dtype]
+    pre = torch.empty((m, 2 * inner), dtype=_BF16, device=dev) if save else None
+    h = torch.empty((m, inner), dtype=_BF16, device=dev) if save else None
+    d = GatedFfnDesc(m, hidden, inner, xs, ys, rs, 0, code, _CODE[out.dtype], rd, 0, 0)
+    size = _workspace_bytes("gated_ffn", dev, 0, m, hidden, inner, code)
+    room = _room(size, dev)
+    _check(_ffn_fwd(d, x.data_ptr(), w_gate_up.data_ptr(), w_down.data_ptr(), _ptr(residual), out.data_ptr(),
+                    _ptr(pre), _ptr(h), _ptr(room), size, _stream(stream, dev)))
+    _done(stream, room, pre, h, made)
+    return (out, pre, h) if save else out
+
 
 def gated_ffn(x, w_gate_up, w_down, *, act="silu", residual=None, save=False, out=None, out_dtype=None, stream=None):
     """``(act(x @ w_gate.T) * (x @ w_up.T)) @ w_down.T + residual``
@@ -202,35 +258,29 @@ def gated_ffn(x, w_gate_up, w_down, *, act="silu", residual=None, save=False, ou
     "silu", "gelu_tanh", "gelu_erf" or "relu". ``save=True`` returns ``(out, pre,
     h)`` with what ``gated_ffn_bwd`` reads: the gate and up products ``[m, 2
     inner]`` and ``h [m, inner]``, bf16."""
-    import torch
-    b16, any_ = _types()
+    return _ffn(x, w_gate_up, w_down, act, residual, save, out, out_dtype, stream)
+
+
+@_at_home
+def _ffn_grads(dev, x, dy, w_gate_up, w_down, pre, h, act, dx_grad, dw_grad, dx_dtype, dw_dtype, stream):
     m, hidden = x.shape
     inner = w_down.shape[1]
-    with _on(x):
-        d = GatedFfnDesc(m=m, hidden=hidden, inner=inner, act=_act(act, True))
-        d.x_stride = _mat("x", x, (m, hidden), b16, x)
-        _packed("w_gate_up", w_gate_up, (2 * inner, hidden), x)
-        _packed("w_down", w_down, (hidden, inner), x)
-        made = out is None
-        if made:
-            out = torch.empty((m, hidden), dtype=out_dtype or torch.bfloat16, device=x.device)
-        d.y_stride, d.out_dtype = _mat("out", out, (m, hidden), any_, x), _dtype_code(out.dtype)
-        if residual is not None:
-            d.residual_stride = _mat("residual", residual, (m, hidden), any_, x)
-            d.residual_dtype = _dtype_code(residual.dtype)
-        pre = torch.empty((m, 2 * inner), dtype=torch.bfloat16, device=x.device) if save else None
-        h = torch.empty((m, inner), dtype=torch.bfloat16, device=x.device) if save else None
-        ws = _workspace(_ffn_ws, d, x, 0)
-        _check(_ffn_fwd(ctypes.byref(d), x.data_ptr(), w_gate_up.data_ptr(), w_down.data_ptr(), _ptr(residual),
-                        out.data_ptr(), _ptr(pre), _ptr(h), _ptr(ws), ws.numel() if ws is not None else 0,
-                        _stream_ptr(stream)))
-        _done(stream, ws, pre, h, out if made else None)
-    return (out, pre, h) if save else out
-
-
-def _packed(name, t, shape, like):
-    if _mat(name, t, shape, _types()[0], like) != shape[1]:
-        raise InlError(-1, f"{name}: must be packed")
+    code = _act(act, True)
+    xs, ys = _mat("x", x, m, hidden, _B16, dev), _mat("dy", dy, m, hidden, _B16, dev)
+    for name, t, rows, cols in (("w_gate_up", w_gate_up, 2 * inner, hidden), ("w_down", w_down, hidden, inner),
+                                ("pre", pre, m, 2 * inner), ("h", h, m, inner)):
+        _packed(name, t, rows, cols, dev)
+    wd = dw_dtype or _BF16
+    dx = torch.empty((m, hidden), dtype=dx_dtype or _BF16, device=dev) if dx_grad else None
+    dgu = torch.empty((2 * inner, hidden), dtype=wd, device=dev) if dw_grad else None
+    ddown = torch.empty((hidden, inner), dtype=wd, device=dev) if dw_grad else None
+    d = GatedFfnDesc(m, hidden, inner, xs, ys, 0, 0, code, 0, 0, _dtype_code(dx_dtype or _BF16), _dtype_code(wd))
+    size = _workspace_bytes("gated_ffn", dev, 1, m, hidden, inner, code)
+    room = _room(size, dev)
+    _check(_ffn_bwd(d, dy.data_ptr(), x.data_ptr(), w_gate_up.data_ptr(), w_down.data_ptr(), pre.data_ptr(),
+                    h.data_ptr(), _ptr(dx), _ptr(dgu), _ptr(ddown), _ptr(room), size, _stream(stream, dev)))
+    _done(stream, room, dx, dgu, ddown)
+    return dx, dgu, ddown
 
 
 def gated_ffn_bwd(dy, x, w_gate_up, w_down, pre, h, *, act="silu", dx_grad=True, dw_grad=True, dx_dtype=None,
@@ -238,40 +288,35 @@ def gated_ffn_bwd(dy, x, w_gate_up, w_down, pre, h, *, act="silu", dx_grad=True,
     """``(dx, dw_gate_up, dw_down)`` of ``gated_ffn`` from bf16 ``dy [m, hidden]`` and
     the ``pre`` and ``h`` that the forward saved (``inl_gated_ffn_bwd``); bf16 unless
     ``dx_dtype``/``dw_dtype`` say float32."""
-    import torch
-    b16, _ = _types()
-    m, hidden = x.shape
-    inner = w_down.shape[1]
-    with _on(x):
-        d = GatedFfnDesc(m=m, hidden=hidden, inner=inner, act=_act(act, True))
-        d.x_stride, d.y_stride = _mat("x", x, (m, hidden), b16, x), _mat("dy", dy, (m, hidden), b16, x)
-        for name, t, shape in (("w_gate_up", w_gate_up, (2 * inner, hidden)), ("w_down", w_down, (hidden, inner)),
-                               ("pre", pre, (m, 2 * inner)), ("h", h, (m, inner))):
-            _packed(name, t, shape, x)
-        wd = dw_dtype or torch.bfloat16
-        dx = torch.empty((m, hidden), dtype=dx_dtype or torch.bfloat16, device=x.device) if dx_grad else None
-        dgu = torch.empty((2 * inner, hidden), dtype=wd, device=x.device) if dw_grad else None
-        ddown = torch.empty((hidden, inner), dtype=wd, device=x.device) if dw_grad else None
-        d.dx_dtype = _dtype_code(dx.dtype) if dx_grad else INL_BF16
-        d.dw_dtype = _dtype_code(wd)
-        ws = _workspace(_ffn_ws, d, x, 1)
-        _check(_ffn_bwd(ctypes.byref(d), dy.data_ptr(), x.data_ptr(), w_gate_up.data_ptr(), w_down.data_ptr(),
-                        pre.data_ptr(), h.data_ptr(), _ptr(dx), _ptr(dgu), _ptr(ddown), _ptr(ws),
-                        ws.numel() if ws is not None else 0, _stream_ptr(stream)))
-        _done(stream, ws, dx, dgu, ddown)
-    return dx, dgu, ddown
+    return _ffn_grads(x, dy, w_gate_up, w_down, pre, h, act, dx_grad, dw_grad, dx_dtype, dw_dtype, stream)
 
 
 # ---------------------------------------------------------------------------
 # Softmax cross entropy
 # ---------------------------------------------------------------------------
 
-def _xent_desc(x, w, scale, ignore_index):
-    b16, _ = _types()
+def _xent_desc(dev, x, w, scale, ignore_index, dx_dtype=None, dw_dtype=None):
     m, hidden = x.shape
-    d = SoftmaxXentDesc(m=m, vocab=w.shape[0], hidden=hidden, scale=float(scale), ignore_index=int(ignore_index))
-    d.x_stride, d.w_stride = _mat("x", x, (m, hidden), b16, x), _mat("w", w, (w.shape[0], hidden), b16, x)
-    return d
+    vocab = w.shape[0]
+    return SoftmaxXentDesc(m, vocab, hidden, _mat("x", x, m, hidden, _B16, dev), _mat("w", w, vocab, hidden, _B16, dev),
+                           0, 0, scale, ignore_index, _dtype_code(dx_dtype or _BF16), _dtype_code(dw_dtype or _BF16))
+
+
+def _xent_room(d, dev, backward):
+    size = _workspace_bytes("softmax_xent", dev, backward, d.m, d.vocab, d.hidden)
+    return _room(size, dev), size
+
+
+@_at_home
+def _xent(dev, x, w, targets, bias, scale, ignore_index, stream):
+    d = _xent_desc(dev, x, w, scale, ignore_index)
+    loss, lse = torch.empty((2, d.m), dtype=_F32, device=dev).unbind(0)
+    room, size = _xent_room(d, dev, 0)
+    _check(_xent_fwd(d, x.data_ptr(), w.data_ptr(), _vec("bias", bias, d.vocab, _F32, dev),
+                     _vec("targets", targets, d.m, torch.int32, dev), loss.data_ptr(), lse.data_ptr(), _ptr(room), size,
+                     _stream(stream, dev)))
+    _done(stream, room, loss, lse)
+    return loss, lse
 
 
 def softmax_xent(x, w, targets, *, bias=None, scale=1.0, ignore_index=-100, stream=None):
@@ -280,17 +325,23 @@ def softmax_xent(x, w, targets, *, bias=None, scale=1.0, ignore_index=-100, stre
     hidden]`` (a decoder, or the documents of a batch with ``scale`` = 1 /
     temperature), f32 ``bias [vocab]``, int32 ``targets [m]``. Rows whose target is
     ``ignore_index`` have loss 0; a target outside the vocabulary gives NaN."""
-    import torch
-    m = x.shape[0]
-    with _on(x):
-        d = _xent_desc(x, w, scale, ignore_index)
-        loss, lse = torch.empty((2, m), dtype=torch.float32, device=x.device).unbind(0)
-        ws = _workspace(_xent_ws, d, x, 0)
-        _check(_xent_fwd(ctypes.byref(d), x.data_ptr(), w.data_ptr(), _vec("bias", bias, d.vocab, torch.float32, x),
-                         _vec("targets", targets, m, torch.int32, x), loss.data_ptr(), lse.data_ptr(), _ptr(ws),
-                         ws.numel() if ws is not None else 0, _stream_ptr(stream)))
-        _done(stream, ws, loss, lse)
-    return loss, lse
+    return _xent(x, w, targets, bias, scale, ignore_index, stream)
+
+
+@_at_home
+def _xent_grads(dev, x, dloss, lse, w, targets, bias, scale, ignore_index, dx_grad, dw_grad, bias_grad, dx_dtype,
+                dw_dtype, stream):
+    d = _xent_desc(dev, x, w, scale, ignore_index, dx_dtype, dw_dtype)
+    dx = torch.empty(x.shape, dtype=dx_dtype or _BF16, device=dev) if dx_grad else None
+    dw = torch.empty(w.shape, dtype=dw_dtype or _BF16, device=dev) if dw_grad else None
+    db = torch.empty(d.vocab, dtype=_F32, device=dev) if bias_grad else None
+    room, size = _xent_room(d, dev, 1)
+    _check(_xent_bwd(d, _vec("dloss", dloss, d.m, _F32, dev), _vec("lse", lse, d.m, _F32, dev), x.data_ptr(),
+                     w.data_ptr(), _vec("bias", bias, d.vocab, _F32, dev),
+                     _vec("targets", targets, d.m, torch.int32, dev), _ptr(dx), _ptr(dw), _ptr(db), _ptr(room), size,
+                     _stream(stream, dev)))
+    _done(stream, room, dx, dw, db)
+    return dx, dw, db
 
 
 def softmax_xent_bwd(dloss, lse, x, w, targets, *, bias=None, scale=1.0, ignore_index=-100, dx_grad=True,
@@ -298,34 +349,67 @@ def softmax_xent_bwd(dloss, lse, x, w, targets, *, bias=None, scale=1.0, ignore_
     """``(dx, dw, dbias)`` of ``softmax_xent`` from f32 ``dloss [m]`` and the forward's
     ``lse`` (``inl_softmax_xent_bwd``); dx and dw bf16 unless ``dx_dtype``/``dw_dtype``
     say float32, dbias f32; what is not asked for is None."""
-    import torch
-    m, f32 = x.shape[0], torch.float32
-    with _on(x):
-        d = _xent_desc(x, w, scale, ignore_index)
-        dx = torch.empty(x.shape, dtype=dx_dtype or torch.bfloat16, device=x.device) if dx_grad else None
-        dw = torch.empty(w.shape, dtype=dw_dtype or torch.bfloat16, device=x.device) if dw_grad else None
-        db = torch.empty(d.vocab, dtype=f32, device=x.device) if bias_grad else None
-        d.dx_dtype = _dtype_code(dx.dtype) if dx_grad else INL_BF16
-        d.dw_dtype = _dtype_code(dw.dtype) if dw_grad else INL_BF16
-        ws = _workspace(_xent_ws, d, x, 1)
-        _check(_xent_bwd(ctypes.byref(d), _vec("dloss", dloss, m, f32, x), _vec("lse", lse, m, f32, x), x.data_ptr(),
-                         w.data_ptr(), _vec("bias", bias, d.vocab, f32, x), _vec("targets", targets, m, torch.int32, x),
-                         _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), ws.numel() if ws is not None else 0,
-                         _stream_ptr(stream)))
-        _done(stream, ws, dx, dw, db)
-    return dx, dw, db
+    return _xent_grads(x, dloss, lse, w, targets, bias, scale, ignore_index, dx_grad, dw_grad, bias_grad, dx_dtype,
+                       dw_dtype, stream)
 
 
 # ---------------------------------------------------------------------------
 # q/k prologue
 # ---------------------------------------------------------------------------
 
-def _heads(name, t, shape, like):
-    if tuple(t.shape) != tuple(shape) or t.device != like.device:
-        raise InlError(-1, f"{name}: shape {tuple(t.shape)} on {t.device}, need {tuple(shape)} on {like.device}")
-    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+def _heads(name, t, shape, dev):
+    if tuple(t.shape) != shape or t.get_device() != dev:
+        raise InlError(-1, f"{name}: shape {tuple(t.shape)} on {t.device}, need {shape} on cuda:{dev}")
+    stride = t.stride()
+    if stride[2] != 1 or (shape[1] > 1 and stride[1] != shape[2]):
         raise InlError(-1, f"{name}: heads must be contiguous inside a token row")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    return stride[0] if shape[0] > 1 else shape[1] * shape[2]
+
+
+@_at_home
+def _rope_grads(dev, x, dy, q_heads, rows, cos, sin, q_weight, k_weight, eps, norm, rotary_dim, sections, cos2, sin2,
+                round_tables, out, weight_grad, stream):
+    shape = tuple(x.shape)
+    if len(shape) != 3:
+        raise InlError(-1, f"x: shape {shape}, need [tokens, heads, head_dim]")
+    n, heads, hd = shape
+    d = NormRopeDesc()
+    d.n_tokens, d.heads, d.head_dim = shape
+    d.x_row_stride, d.y_row_stride = _heads("x", x, shape, dev), _heads("dy", dy, shape, dev)
+    d.dtype, d.out_dtype = _dtype_code(x.dtype), _dtype_code(dy.dtype)
+    d.norm, d.eps = int(bool(norm)), eps
+    d.rotary_dim = int((hd if cos is not None else 0) if rotary_dim is None else rotary_dim)
+    d.sections, d.round_tables = int(sections), int(bool(round_tables))
+    d.table_rows = int(cos.shape[0]) if cos is not None else 0
+    if d.rotary_dim:
+        tables = (("cos", cos), ("sin", sin))
+        if sections == ROPE_AXIAL:
+            tables += (("cos2", cos2), ("sin2", sin2))
+        width = hd // 4 if sections == ROPE_AXIAL else d.rotary_dim // 2
+        for name, t in tables:
+            if t is None or tuple(t.shape) != (d.table_rows, width) or t.dtype != _F32 or not t.is_contiguous() \
+                    or t.get_device() != dev:
+                raise InlError(-1, f"{name}: need contiguous f32 [{d.table_rows}, {width}] on cuda:{dev}")
+        _vec("rows", rows, n, torch.int32, dev)
+    made = None
+    if out is None:
+        made = out = torch.empty(shape, dtype=x.dtype, device=dev)
+    elif out.dtype != x.dtype:
+        raise InlError(-1, f"out: dtype {out.dtype}, need {x.dtype}")
+    ds = _heads("out", out, shape, dev)
+    grads = bool(norm and weight_grad)
+    dq = torch.empty(hd, dtype=_F32, device=dev) if grads else None
+    dk = torch.empty(hd, dtype=_F32, device=dev) if grads and q_heads < heads else None
+    size = ctypes.c_size_t()
+    if grads:
+        _check(_rope_bwd_ws(d, ctypes.byref(size)))
+    room = _room(size.value, dev)
+    _check(_rope_bwd(d, int(q_heads), dy.data_ptr(), x.data_ptr(), out.data_ptr(), ds,
+                     _vec("q_weight", q_weight, hd, x.dtype, dev), _vec("k_weight", k_weight, hd, x.dtype, dev),
+                     _ptr(rows), _ptr(cos), _ptr(sin), _ptr(cos2), _ptr(sin2), _ptr(dq), _ptr(dk), _ptr(room),
+                     size.value, _stream(stream, dev)))
+    _done(stream, room, dq, dk, made)
+    return out, dq, dk
 
 
 def norm_rope_qk_bwd(dy, x, q_heads, rows=None, cos=None, sin=None, *, q_weight=None, k_weight=None, eps=1e-6,
@@ -336,39 +420,5 @@ def norm_rope_qk_bwd(dy, x, q_heads, rows=None, cos=None, sin=None, *, q_weight=
     arguments as in the forward. dx has x's dtype (``out`` may be a slice of wider rows), the
     weight gradients are f32 ``[head_dim]`` and None without a norm, with
     ``weight_grad=False`` or, dk_weight, where all heads are q heads."""
-    import torch
-    n, heads, hd = x.shape
-    with _on(x):
-        d = NormRopeDesc()
-        d.n_tokens, d.heads, d.head_dim = n, heads, hd
-        d.x_row_stride, d.y_row_stride = _heads("x", x, (n, heads, hd), x), _heads("dy", dy, (n, heads, hd), x)
-        d.dtype, d.out_dtype = _dtype_code(x.dtype), _dtype_code(dy.dtype)
-        d.norm, d.eps = int(bool(norm)), float(eps)
-        d.rotary_dim = int((hd if cos is not None else 0) if rotary_dim is None else rotary_dim)
-        d.sections, d.round_tables = int(sections), int(bool(round_tables))
-        d.table_rows = int(cos.shape[0]) if cos is not None else 0
-        if d.rotary_dim:
-            width = hd // 4 if sections == ROPE_AXIAL else d.rotary_dim // 2
-            for name, t in (("cos", cos), ("sin", sin), ("cos2", cos2), ("sin2", sin2)):
-                if t is None and name in ("cos2", "sin2") and sections != ROPE_AXIAL:
-                    continue
-                if t is None or tuple(t.shape) != (d.table_rows, width) or t.dtype != torch.float32 \
-                        or not t.is_contiguous() or t.device != x.device:
-                    raise InlError(-1, f"{name}: need contiguous f32 [{d.table_rows}, {width}] on {x.device}")
-            _vec("rows", rows, n, torch.int32, x)
-        made = out is None
-        if made:
-            out = torch.empty((n, heads, hd), dtype=x.dtype, device=x.device)
-        elif out.dtype != x.dtype:
-            raise InlError(-1, f"out: dtype {out.dtype}, need {x.dtype}")
-        ds = _heads("out", out, (n, heads, hd), x)
-        grads = bool(norm and weight_grad)
-        dq = torch.empty(hd, dtype=torch.float32, device=x.device) if grads else None
-        dk = torch.empty(hd, dtype=torch.float32, device=x.device) if grads and q_heads < heads else None
-        ws = _workspace(_rope_bwd_ws, d, x) if grads else None
-        _check(_rope_bwd(ctypes.byref(d), int(q_heads), dy.data_ptr(), x.data_ptr(), out.data_ptr(), ds,
-                         _vec("q_weight", q_weight, hd, x.dtype, x), _vec("k_weight", k_weight, hd, x.dtype, x),
-                         _ptr(rows), _ptr(cos), _ptr(sin), _ptr(cos2), _ptr(sin2), _ptr(dq), _ptr(dk), _ptr(ws),
-                         ws.numel() if ws is not None else 0, _stream_ptr(stream)))
-        _done(stream, ws, dq, dk, out if made else None)
-    return out, dq, dk
+    return _rope_grads(x, dy, q_heads, rows, cos, sin, q_weight, k_weight, eps, norm, rotary_dim, sections, cos2, sin2,
+                       round_tables, out, weight_grad, stream)
