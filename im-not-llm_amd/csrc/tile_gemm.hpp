@@ -28,8 +28,9 @@
 //
 // Unit order: split-major, then groups of GROUP m-tiles, n outer and m inner
 // within a group, cut into 8 contiguous ranges, one per XCD (workgroup b runs
-// on XCD b % 8). The ~32 units an XCD runs at one time form a rectangle of 8 x
-// 4 tiles, 12 operand slices per stage instead of 33 for a row of tiles.
+// on XCD b % 8). The ~32 units an XCD runs at one time form a rectangle of 4 x
+// 8 tiles: 12 operand slices per stage instead of 33 for a row of tiles, and output
+// rows of 4 KiB at a time (8 x 4 tiles: the gate gradients of 16,384 x 4,096 took 8 % longer).
 #pragma once
 
 #include <algorithm>
@@ -87,7 +88,7 @@ constexpr int TG_KS = TG_BK / 32;   // MFMA k steps of it
 constexpr int TG_ROW = TG_BK * 2;
 constexpr int TG_STG = 4096;   // per-wave epilogue staging: 32 rows x 128 bytes
 constexpr int TG_XCDS = 8;
-constexpr int TG_GROUP = 8;
+constexpr int TG_GROUP = 4;
 
 template <int NWN_, int NWM_, int WNB_, int WMB_, int STAGES_, int WPC_>
 struct TileShape {
@@ -381,8 +382,7 @@ __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) voi
 
   // ---- epilogue: acc[a][b][e] is row (wm WMB + b) 16 + l16, w row (wn WNB + a) 16 + 4 quad + e ----
   // Staging of one wave: 32 rows (two x blocks) x 128 bytes, 16-byte chunk c of row r at
-  // r * 128 + ((c ^ ((r >> 1) & 7)) << 4); 64 bf16 columns, or 32 f32 ones where
-  // the value still meets memory (RES, EPI_DGATED) or is stored in f32.
+  // r * 128 + ((c ^ ((r >> 1) & 7)) << 4); 64 bf16 columns, or 32 f32 ones.
   const uint32_t stg = lds0 + C::RING + (uint32_t)wave * TG_STG;
   // (the lane anew for each tile: what an epilogue derives from it would otherwise
   // be kept in registers through the k loop)
@@ -413,8 +413,34 @@ __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) voi
       if (row < p.m && col < end && c * 8 < width) *reinterpret_cast<u32x4*>(dst + (row * stride + col) * 2) = v;
     }
   };
-  // The same from f32 staging, with what the value meets in memory
-  auto flush32 = [&](char* dst, int64_t row0, int col0, int width) __attribute__((always_inline)) {
+  // f32 rows (32 x 32): 128-byte row segments, plus a residual that was asked for
+  // before (res_load): a load behind the last block's stores would wait for them
+  struct Res {
+    f32x4 v[4];
+    f32x4 bias[2];   // of the block's columns (here and not with the tile's: registers)
+  };
+  auto res_load = [&](int64_t row0, int col0, int width, Res& q) __attribute__((always_inline)) {
+    const int c = (el & 7) * 4, col = col0 + c;
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      q.bias[a] = zero;
+      if (p.bias) q.bias[a] = *reinterpret_cast<const f32x4*>(p.bias + min(col0 + a * 16 + 4 * (el >> 4), p.n - 4));
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t row = row0 + (el >> 3) + 8 * j;
+      q.v[j] = zero;
+      if (row >= p.m || col >= p.n || c >= width) continue;
+      if (p.res_bf16) {
+        const bf16x4 o = *reinterpret_cast<const bf16x4*>(p.res + (row * p.rs + col) * 2);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q.v[j][e] = (float)o[e];
+      } else {
+        q.v[j] = *reinterpret_cast<const f32x4*>(p.res + (row * p.rs + col) * 4);
+      }
+    }
+  };
+  auto flush32 = [&](char* dst, int64_t row0, int col0, int width, const Res& q) __attribute__((always_inline)) {
     const int c = el & 7;
     const int col = col0 + c * 4;
 #pragma unroll
@@ -422,43 +448,79 @@ __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) voi
       const int r = (el >> 3) + 8 * j;
       f32x4 t = __builtin_bit_cast(f32x4, lds_load<u32x4>(stg_at(r, c)));
       const int64_t row = row0 + r;
-      if (row < p.m && col < p.n && c * 4 < width) {
-        if constexpr (EPI == EPI_DGATED) {
-          const char* g0 = p.pre + (row * p.ps + col) * 2;
-          const bf16x4 gv = *reinterpret_cast<const bf16x4*>(g0);
-          const bf16x4 uv = *reinterpret_cast<const bf16x4*>(g0 + (int64_t)p.n * 2);
-          bf16x4 dg, du;
+      if constexpr (RES) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const ActPair q = act_pair(p.act, (float)gv[e]);
-            dg[e] = (bf16)(t[e] * (float)uv[e] * q.slope);
-            du[e] = (bf16)(t[e] * q.value);
-          }
-          char* o = dst + (row * p.ys + col) * 2;
-          *reinterpret_cast<bf16x4*>(o) = dg;
-          *reinterpret_cast<bf16x4*>(o + (int64_t)p.n * 2) = du;
-        } else {
-          if constexpr (RES) {
-            if (p.res_bf16) {
-              const bf16x4 o = *reinterpret_cast<const bf16x4*>(p.res + (row * p.rs + col) * 2);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) t[e] += p.beta * (float)o[e];
-            } else {
-              const f32x4 o = *reinterpret_cast<const f32x4*>(p.res + (row * p.rs + col) * 4);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) t[e] += p.beta * o[e];
-            }
-          }
-          if constexpr (OUT16) {
-            bf16x4 o;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = (bf16)t[e];
-            *reinterpret_cast<bf16x4*>(dst + (row * p.ys + col) * 2) = o;
-          } else {
-            *reinterpret_cast<f32x4*>(dst + (row * p.ys + col) * 4) = t;
-          }
-        }
+        for (int e = 0; e < 4; ++e) t[e] += p.beta * q.v[j][e];
       }
+      if (row < p.m && col < p.n && c * 4 < width) *reinterpret_cast<f32x4*>(dst + (row * p.ys + col) * 4) = t;
+    }
+  };
+  // bf16 rows of values that meet others in memory first (MEET): 16 rows x 64 f32
+  // columns are staged, so that both are read and written in 128-byte row segments,
+  // 8 values per lane; chunk c of 16 of row r at r * 256 + ((c ^ r) << 4). The
+  // other values are asked for some blocks ahead (meet_load).
+  constexpr bool MEET = EPI == EPI_DGATED || (EPI == EPI_LINEAR && OUT16 && RES);
+  struct Met {
+    u32x4 v[2][2];
+  };
+  auto meet_row = [&](int64_t row0, int j) __attribute__((always_inline)) { return row0 + (el >> 3) + 8 * j; };
+  auto meet_load = [&](int64_t row0, int col0, int width, Met& q) __attribute__((always_inline)) {
+    const int c = (el & 7) * 8, col = col0 + c;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int64_t row = meet_row(row0, j);
+      if (row >= p.m || col >= p.n || c >= width) continue;
+      if constexpr (EPI == EPI_DGATED) {
+        const char* g0 = p.pre + (row * p.ps + col) * 2;
+        q.v[j][0] = *reinterpret_cast<const u32x4*>(g0);
+        q.v[j][1] = *reinterpret_cast<const u32x4*>(g0 + (int64_t)p.n * 2);
+      } else if (p.res_bf16) {
+        q.v[j][0] = *reinterpret_cast<const u32x4*>(p.res + (row * p.rs + col) * 2);
+      } else {
+        const char* r0 = p.res + (row * p.rs + col) * 4;
+        q.v[j][0] = *reinterpret_cast<const u32x4*>(r0);
+        q.v[j][1] = *reinterpret_cast<const u32x4*>(r0 + 16);
+      }
+    }
+  };
+  auto meet_at = [&](int r, int c) __attribute__((always_inline)) {
+    return stg + (uint32_t)r * 256 + (((uint32_t)c ^ (uint32_t)r) << 4);
+  };
+  auto meet_flush = [&](char* dst, int64_t row0, int col0, int width, const Met& q) __attribute__((always_inline)) {
+    const int c = (el & 7) * 8, col = col0 + c;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = (el >> 3) + 8 * j;
+      float t[8];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const f32x4 v = __builtin_bit_cast(f32x4, lds_load<u32x4>(meet_at(r, (el & 7) * 2 + i)));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[4 * i + e] = v[e];
+      }
+      const int64_t row = meet_row(row0, j);
+      if (row >= p.m || col >= p.n || c >= width) continue;
+      const bf16x8 a = __builtin_bit_cast(bf16x8, q.v[j][0]), b = __builtin_bit_cast(bf16x8, q.v[j][1]);
+      bf16x8 o;
+      char* at = dst + (row * p.ys + col) * 2;
+      if constexpr (EPI == EPI_DGATED) {
+        bf16x8 du;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const ActPair s = act_pair(p.act, (float)a[e]);
+          o[e] = (bf16)(t[e] * (float)b[e] * s.slope);
+          du[e] = (bf16)(t[e] * s.value);
+        }
+        *reinterpret_cast<bf16x8*>(at + (int64_t)p.n * 2) = du;
+      } else if (p.res_bf16) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = (bf16)(t[e] + p.beta * (float)a[e]);
+      } else {
+        const f32x4 lo = __builtin_bit_cast(f32x4, q.v[j][0]), hi = __builtin_bit_cast(f32x4, q.v[j][1]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = (bf16)(t[e] + p.beta * (e < 4 ? lo[e & 3] : hi[e & 3]));
+      }
+      *reinterpret_cast<bf16x8*>(at) = o;
     }
   };
   constexpr bool STG16 = EPI == EPI_GATED || EPI == EPI_DXENT || (EPI == EPI_LINEAR && OUT16 && !RES);
@@ -467,6 +529,83 @@ __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) voi
     el = (int)opaque((uint32_t)lane);
     const int ncol0 = q.nt * BNO;
     const int er = el & 15, ec = 4 * (el >> 4);   // this lane's row and first column of a block
+    // What the epilogue reads of vectors comes first: a load behind a store waits
+    // for the store (one counter, in order).
+    constexpr bool XENT = EPI == EPI_XENT || EPI == EPI_DXENT;
+    f32x4 bv[WNB];
+#pragma unroll
+    for (int a = 0; a < WNB; ++a) bv[a] = zero;
+    if constexpr ((EPI == EPI_LINEAR && !(RES && !OUT16)) || XENT) {
+      if (p.bias) {
+        const int c0 = ncol0 + wn * WNB * 16 + ec;
+        if (!XENT || ncol0 + BN <= p.n) {
+#pragma unroll
+          for (int a = 0; a < WNB; ++a) bv[a] = *reinterpret_cast<const f32x4*>(p.bias + min(c0 + a * 16, p.n - 4));
+        } else {   // any number of columns
+#pragma unroll
+          for (int a = 0; a < WNB; ++a)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bv[a][e] = p.bias[min(c0 + a * 16 + e, p.n - 1)];
+        }
+      }
+    }
+    int tcol[WMB];          // the target's column, if it is in [0, n)
+    float row_lse[WMB], row_dl[WMB];
+#pragma unroll
+    for (int b = 0; b < WMB; ++b) {
+      tcol[b] = -1;
+      row_lse[b] = row_dl[b] = 0.f;
+      if constexpr (XENT) {
+        const int64_t row = (int64_t)q.mt * BM + (wm * WMB + b) * 16 + er;
+        if (row < p.m) {
+          const int t = p.target[row];
+          if (t != p.ignore) tcol[b] = t - p.col0;
+          if constexpr (EPI == EPI_DXENT) {
+            row_lse[b] = p.lse[row];
+            if (t != p.ignore) row_dl[b] = p.dl[row];
+          }
+        }
+      }
+    }
+    Res res[2];   // (RES, f32 rows)
+    if constexpr (MEET) {
+      // 16 rows x 64 columns at a time, what they meet asked for DEPTH blocks ahead
+      constexpr int PER = WNB < 4 ? WNB : 4, WIDE = WNB / PER, STEPS = WMB * WIDE, DEPTH = STEPS < 4 ? STEPS : EPI == EPI_DGATED ? 4 : 2;
+      auto step_row = [&](int i) __attribute__((always_inline)) { return (int64_t)q.mt * BM + (wm * WMB + i / WIDE) * 16; };
+      auto step_col = [&](int i) __attribute__((always_inline)) { return ncol0 + (wn * WNB + i % WIDE * PER) * 16; };
+      Met met[DEPTH];
+#pragma unroll
+      for (int i = 0; i < DEPTH; ++i) meet_load(step_row(i), step_col(i), PER * 16, met[i]);
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const int b = i / WIDE, a0 = i % WIDE * PER;
+#pragma unroll
+        for (int a = 0; a < PER; ++a) {
+          f32x4 z = acc[a0 + a][b];
+          if constexpr (EPI == EPI_LINEAR) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[e] *= p.alpha;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[e] += bv[a0 + a][e];
+            if (p.pre) {   // straight from the accumulators, 8 bytes per lane
+              const int64_t row = step_row(i) + er;
+              const int col = step_col(i) + a * 16 + ec;
+              if (row < p.m && col < p.n) {
+                bf16x4 o;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = (bf16)z[e];
+                *reinterpret_cast<bf16x4*>(p.pre + (row * p.ps + col) * 2) = o;
+              }
+            }
+            z = act_apply4(p.act, z);
+          }
+          lds_store<u32x4>(meet_at(er, a * 4 + (el >> 4)), __builtin_bit_cast(u32x4, z));
+        }
+        meet_flush(p.y, step_row(i), step_col(i), PER * 16, met[i % DEPTH]);
+        if (i + DEPTH < STEPS) meet_load(step_row(i + DEPTH), step_col(i + DEPTH), PER * 16, met[i % DEPTH]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else
 #pragma unroll
     for (int b0 = 0; b0 < WMB; b0 += 2) {
       const int64_t row0 = (int64_t)q.mt * BM + (wm * WMB + b0) * 16;
@@ -497,37 +636,27 @@ __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) voi
       } else if constexpr (EPI == EPI_XENT || EPI == EPI_DXENT) {
         const int colb = ncol0 + wn * WNB * 16 + ec;   // this lane's first column
         const bool whole = ncol0 + BN <= p.n;
-        // Scores in place of the products, columns past n -inf. (One block of
-        // columns at a time: with all bias loads in flight at once the 256 x 256
-        // shape spills.)
-#pragma unroll
-        for (int a = 0; a < WNB; ++a) {
-          f32x4 bv = zero;
-          if (p.bias) {
-            if (whole) {
-              bv = *reinterpret_cast<const f32x4*>(p.bias + colb + a * 16);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) bv[e] = p.bias[min(colb + a * 16 + e, p.n - 1)];
-            }
-          }
-#pragma unroll
-          for (int b = b0; b < b0 + 2; ++b)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float s = __builtin_fmaf(p.alpha, acc[a][b][e], bv[e]);
-              if (!whole && colb + a * 16 + e >= p.n) s = -INFINITY;
-              acc[a][b][e] = s;
-            }
-          __builtin_amdgcn_sched_barrier(0);
-        }
+        constexpr float LOG2E = 1.44269504088896f;
         if constexpr (EPI == EPI_XENT) {
+          // scores in units of ln 2 in place of the products, columns past n -inf
+          const float alpha2 = p.alpha * LOG2E;
+#pragma unroll
+          for (int a = 0; a < WNB; ++a) {
+#pragma unroll
+            for (int b = b0; b < b0 + 2; ++b)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float s = __builtin_fmaf(alpha2, acc[a][b][e], bv[a][e] * LOG2E);
+                if (!whole && colb + a * 16 + e >= p.n) s = -INFINITY;
+                acc[a][b][e] = s;
+              }
+            __builtin_amdgcn_sched_barrier(0);
+          }
 #pragma unroll
           for (int b = b0; b < b0 + 2; ++b) {
             const int64_t row = row0 + (b - b0) * 16 + er;
             const bool in = row < p.m;
-            const int t = in ? p.target[row] : p.ignore;
-            const int tc = t == p.ignore ? -1 : t - p.col0;   // the target's column, if it is in [0, n)
+            const int tc = tcol[b];
             if (__any(tc >= colb - ec && tc < colb - ec + WNB * 16)) {
 #pragma unroll
               for (int a = 0; a < WNB; ++a)
@@ -547,43 +676,48 @@ __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) voi
 #pragma unroll
             for (int a = 0; a < WNB; ++a)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f((acc[a][b][e] - base) * 1.44269504088896f);
+              for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(acc[a][b][e] - base);
             sum += __shfl_xor(sum, 16, 64);
             sum += __shfl_xor(sum, 32, 64);
             if (in && el < 16) p.part[(int64_t)(q.nt * C::NWN + wn) * p.m + row] = make_float2(top, sum);
           }
         } else {
-          float lse[2], f[2];
-          int tc[2];
+          const float lse[2] = {row_lse[b0], row_lse[b0 + 1]}, f[2] = {row_dl[b0], row_dl[b0 + 1]};
+          const int tc[2] = {tcol[b0], tcol[b0 + 1]};
           bool live[2];   // (an ignored row is zeros whatever its scores are)
+          bool hit = false;
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
-            const int64_t row = row0 + b * 16 + er;
-            const bool in = row < p.m;
-            const int t = in ? p.target[row] : p.ignore;
-            tc[b] = t == p.ignore ? -1 : t - p.col0;
-            lse[b] = in ? p.lse[row] : 0.f;
-            f[b] = t != p.ignore ? p.dl[row] : 0.f;
+            hit |= tc[b] >= colb - ec && tc[b] < colb - ec + WNB * 16;
             live[b] = f[b] != 0.f || f[b] != f[b];
           }
+          // the common case has no target, end or dead row among the wave's columns
+          const bool plain = whole && !__any(hit) && __all(live[0] && live[1]);
           constexpr int PER = WNB < 4 ? WNB : 4;
 #pragma unroll
           for (int a0 = 0; a0 < WNB; a0 += PER) {
 #pragma unroll
-            for (int a = a0; a < a0 + PER; ++a)
+            for (int a = a0; a < a0 + PER; ++a) {
 #pragma unroll
               for (int b = 0; b < 2; ++b) {
                 f32x4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const int col = colb + a * 16 + e;
-                  float pr = __builtin_amdgcn_exp2f((acc[a][b0 + b][e] - lse[b]) * 1.44269504088896f);
-                  if (col == tc[b]) pr -= 1.f;
-                  v[e] = live[b] && (whole || col < p.n) ? pr * f[b] : 0.f;
+                for (int e = 0; e < 4; ++e)
+                  v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p.alpha, acc[a][b0 + b][e], bv[a][e] - lse[b]) * LOG2E);
+                if (!plain) {
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    const int col = colb + a * 16 + e;
+                    if (col == tc[b]) v[e] -= 1.f;
+                    if (!live[b] || col >= p.n) v[e] = 0.f;
+                  }
                 }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = live[b] ? v[e] * f[b] : 0.f;
                 put16(b * 16 + er, (a - a0) * 16 + ec, v);
                 __builtin_amdgcn_sched_barrier(0);
               }
+            }
             flush16(p.y, p.ys, row0, ncol0 + (wn * WNB + a0) * 16, PER * 16, p.n_store);
           }
         }
@@ -591,8 +725,13 @@ __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) voi
         constexpr int COLS = STG16 ? 64 : 32;
         constexpr int PER = COLS / 16 < WNB ? COLS / 16 : WNB;
         char* dst = EPI == EPI_PART ? p.y + (int64_t)q.s * p.m * p.n * 4 : p.y;
+        if constexpr (RES) {
+          if (b0 == 0) res_load(row0, ncol0 + wn * WNB * 16, PER * 16, res[0]);
+        }
 #pragma unroll
         for (int a0 = 0; a0 < WNB; a0 += PER) {
+          constexpr int NA = WNB / PER;
+          const int step = b0 / 2 * NA + a0 / PER;
           const int col0 = ncol0 + (wn * WNB + a0) * 16;
           f32x4 z[PER][2];
 #pragma unroll
@@ -603,16 +742,12 @@ __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) voi
               for (int e = 0; e < 4; ++e)
                 z[a][b][e] = EPI == EPI_LINEAR ? p.alpha * acc[a0 + a][b0 + b][e] : acc[a0 + a][b0 + b][e];
           if constexpr (EPI == EPI_LINEAR) {
-            if (p.bias) {
 #pragma unroll
-              for (int a = 0; a < PER; ++a) {
-                const f32x4 bv = *reinterpret_cast<const f32x4*>(p.bias + min(col0 + a * 16 + ec, p.n - 4));
+            for (int a = 0; a < PER; ++a)
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+              for (int b = 0; b < 2; ++b)
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) z[a][b][e] += bv[e];
-              }
-            }
+                for (int e = 0; e < 4; ++e) z[a][b][e] += RES ? res[step & 1].bias[a & 1][e] : bv[a0 + a][e];
             if (p.pre) {
 #pragma unroll
               for (int a = 0; a < PER; ++a)
@@ -634,8 +769,14 @@ __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) voi
               if constexpr (STG16) put16(b * 16 + er, a * 16 + ec, z[a][b]);
               else put32(b * 16 + er, a * 16 + ec, z[a][b]);
             }
+          if constexpr (RES) {   // the next block's, in front of this one's stores
+            __builtin_amdgcn_sched_barrier(0);
+            if (step + 1 < WMB / 2 * NA)
+              res_load(row0 + (a0 + PER == WNB ? 32 : 0), ncol0 + (wn * WNB + (a0 + PER) % WNB) * 16, PER * 16,
+                       res[(step + 1) & 1]);
+          }
           if constexpr (STG16) flush16(dst, p.ys, row0, col0, PER * 16, p.n);
-          else flush32(dst, row0, col0, PER * 16);
+          else flush32(dst, row0, col0, PER * 16, res[step & 1]);
           __builtin_amdgcn_sched_barrier(0);
         }
       }

@@ -36,36 +36,38 @@ int64_t stat_blocks(int shape, int64_t vocab) {
   return tiles * (tile_cols(shape) / stat_cols(shape));
 }
 
-// lse and loss from the blocks' statistics: 4 waves of a workgroup take every
-// 4th block for 64 rows, then meet in LDS.
-__global__ __launch_bounds__(256) void xent_join_kernel(const float2* part, int64_t blocks, int64_t m,
-                                                        const int32_t* target, const float* at, int32_t ignore,
-                                                        int64_t vocab, float* loss, float* lse) {
-  __shared__ float2 red[4][64];
+// lse and loss from the blocks' statistics (scores in units of ln 2): the 16 waves
+// of a workgroup take every 16th block for 64 rows, then meet in LDS.
+constexpr int JOIN_WAVES = 16;
+__global__ __launch_bounds__(JOIN_WAVES * 64) void xent_join_kernel(const float2* part, int64_t blocks, int64_t m,
+                                                                    const int32_t* target, const float* at,
+                                                                    int32_t ignore, int64_t vocab, float* loss,
+                                                                    float* lse) {
+  __shared__ float2 red[JOIN_WAVES][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = blockIdx.x * 64LL + lane;
   float top = -INFINITY, sum = 0.f;
   auto fold = [&](float2 q) {
     const float t = fmaxf(top, q.x);
     const float base = t == -INFINITY ? 0.f : t;
-    sum = sum * __builtin_amdgcn_exp2f((top - base) * 1.44269504088896f) +
-          q.y * __builtin_amdgcn_exp2f((q.x - base) * 1.44269504088896f);
+    sum = sum * __builtin_amdgcn_exp2f(top - base) + q.y * __builtin_amdgcn_exp2f(q.x - base);
     top = t;
   };
   if (row < m) {
 #pragma unroll 4
-    for (int64_t b = wave; b < blocks; b += 4) fold(part[b * m + row]);
+    for (int64_t b = wave; b < blocks; b += JOIN_WAVES) fold(part[b * m + row]);
   }
   red[wave][lane] = make_float2(top, sum);
   __syncthreads();
   if (wave || row >= m) return;
 #pragma unroll
-  for (int w = 1; w < 4; ++w) fold(red[w][lane]);
-  const float logs = logf(sum);
-  lse[row] = top + logs;
+  for (int w = 1; w < JOIN_WAVES; ++w) fold(red[w][lane]);
+  constexpr float LN2 = 0.693147180559945f;
+  const float logs = log2f(sum);
+  lse[row] = (top + logs) * LN2;
   const int32_t t = target[row];
   // (top - score) + log: a small loss beside large scores keeps its digits
-  loss[row] = t == ignore ? 0.f : (t < 0 || t >= vocab) ? __builtin_nanf("") : (top - at[row]) + logs;
+  loss[row] = t == ignore ? 0.f : (t < 0 || t >= vocab) ? __builtin_nanf("") : ((top - at[row]) + logs) * LN2;
 }
 
 // Rows whose target is neither ignored nor in [0, vocab): their gradient is NaN.
@@ -169,7 +171,7 @@ extern "C" int inl_softmax_xent_fwd(const inl_softmax_xent_desc* d, const void* 
   p.at = at;
   p.part = part;
   if ((rc = tile_nt_xent(p, plan.s, plan.cus, st))) return rc;
-  hipLaunchKernelGGL(xent_join_kernel, dim3((unsigned)((d->m + 63) / 64)), dim3(256), 0, st, part, blocks, d->m,
+  hipLaunchKernelGGL(xent_join_kernel, dim3((unsigned)((d->m + 63) / 64)), dim3(JOIN_WAVES * 64), 0, st, part, blocks, d->m,
                      targets, at, d->ignore_index, d->vocab, loss, lse);
   INL_HIP_TRY(hipGetLastError());
   return INL_OK;
