@@ -638,15 +638,16 @@ __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) voi
         const bool whole = ncol0 + BN <= p.n;
         constexpr float LOG2E = 1.44269504088896f;
         if constexpr (EPI == EPI_XENT) {
-          // scores in units of ln 2 in place of the products, columns past n -inf
-          const float alpha2 = p.alpha * LOG2E;
+          // Scores in place of the products, columns past n -inf. (Not in units of
+          // ln 2, which would save a product each: a bias of the lowest float would
+          // leave the range.)
 #pragma unroll
           for (int a = 0; a < WNB; ++a) {
 #pragma unroll
             for (int b = b0; b < b0 + 2; ++b)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                float s = __builtin_fmaf(alpha2, acc[a][b][e], bv[a][e] * LOG2E);
+                float s = __builtin_fmaf(p.alpha, acc[a][b][e], bv[a][e]);
                 if (!whole && colb + a * 16 + e >= p.n) s = -INFINITY;
                 acc[a][b][e] = s;
               }
@@ -676,7 +677,7 @@ __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) voi
 #pragma unroll
             for (int a = 0; a < WNB; ++a)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(acc[a][b][e] - base);
+              for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f((acc[a][b][e] - base) * LOG2E);
             sum += __shfl_xor(sum, 16, 64);
             sum += __shfl_xor(sum, 32, 64);
             if (in && el < 16) p.part[(int64_t)(q.nt * C::NWN + wn) * p.m + row] = make_float2(top, sum);

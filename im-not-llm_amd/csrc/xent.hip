@@ -36,21 +36,21 @@ int64_t stat_blocks(int shape, int64_t vocab) {
   return tiles * (tile_cols(shape) / stat_cols(shape));
 }
 
-// lse and loss from the blocks' statistics (scores in units of ln 2): the 16 waves
-// of a workgroup take every 16th block for 64 rows, then meet in LDS.
+// lse and loss from the blocks' statistics: the 16 waves of a workgroup take every 16th block for 64 rows, then meet in LDS.
 constexpr int JOIN_WAVES = 16;
 __global__ __launch_bounds__(JOIN_WAVES * 64) void xent_join_kernel(const float2* part, int64_t blocks, int64_t m,
                                                                     const int32_t* target, const float* at,
                                                                     int32_t ignore, int64_t vocab, float* loss,
                                                                     float* lse) {
   __shared__ float2 red[JOIN_WAVES][64];
+  constexpr float LOG2E = 1.44269504088896f;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = blockIdx.x * 64LL + lane;
   float top = -INFINITY, sum = 0.f;
   auto fold = [&](float2 q) {
     const float t = fmaxf(top, q.x);
     const float base = t == -INFINITY ? 0.f : t;
-    sum = sum * __builtin_amdgcn_exp2f(top - base) + q.y * __builtin_amdgcn_exp2f(q.x - base);
+    sum = sum * __builtin_amdgcn_exp2f((top - base) * LOG2E) + q.y * __builtin_amdgcn_exp2f((q.x - base) * LOG2E);
     top = t;
   };
   if (row < m) {
@@ -62,12 +62,11 @@ __global__ __launch_bounds__(JOIN_WAVES * 64) void xent_join_kernel(const float2
   if (wave || row >= m) return;
 #pragma unroll
   for (int w = 1; w < JOIN_WAVES; ++w) fold(red[w][lane]);
-  constexpr float LN2 = 0.693147180559945f;
-  const float logs = log2f(sum);
-  lse[row] = (top + logs) * LN2;
+  const float logs = logf(sum);
+  lse[row] = top + logs;
   const int32_t t = target[row];
   // (top - score) + log: a small loss beside large scores keeps its digits
-  loss[row] = t == ignore ? 0.f : (t < 0 || t >= vocab) ? __builtin_nanf("") : ((top - at[row]) + logs) * LN2;
+  loss[row] = t == ignore ? 0.f : (t < 0 || t >= vocab) ? __builtin_nanf("") : (top - at[row]) + logs;
 }
 
 // Rows whose target is neither ignored nor in [0, vocab): their gradient is NaN.

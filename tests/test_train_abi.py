@@ -1,0 +1,142 @@
+"""The C entries of include/inl_train.h refuse bad arguments on the host, before any
+GPU call: pointers here are made up and never read."""
+import ctypes
+
+import pytest
+
+P, ODD = 1 << 20, (1 << 20) + 8   # 16-byte aligned, and not
+
+
+@pytest.fixture(scope="module")
+def T():
+    from inl_hip import train
+    return train
+
+
+def _dense(T, **kw):
+    d = dict(m=4, n=16, k=40, out_dtype=1, residual_dtype=1, dx_dtype=1, dw_dtype=1)
+    d.update(kw)
+    return T.DenseDesc(**d)
+
+
+def _ffn(T, **kw):
+    d = dict(m=4, hidden=40, inner=16, act=2, out_dtype=1, residual_dtype=1, dx_dtype=1, dw_dtype=1)
+    d.update(kw)
+    return T.GatedFfnDesc(**d)
+
+
+def _xent(T, **kw):
+    d = dict(m=4, vocab=17, hidden=40, scale=1.0, ignore_index=-100, dx_dtype=1, dw_dtype=1)
+    d.update(kw)
+    return T.SoftmaxXentDesc(**d)
+
+
+@pytest.mark.parametrize("fields,code,word", [
+    (dict(m=-1), -1, "m must be"), (dict(n=0), -1, "n and k"), (dict(k=36), -2, "multiples of 8"),
+    (dict(n=12), -2, "multiples of 8"), (dict(n=1 << 22), -2, "at most"), (dict(m=1 << 31), -2, "below"),
+    (dict(act=5), -1, "unknown act"), (dict(act=-1), -1, "unknown act"), (dict(x_stride=32), -1, "x: the row stride"),
+    (dict(w_stride=44), -2, "w: the row stride"), (dict(y_stride=1 << 22), -2, "2^21"),
+    (dict(out_dtype=2), -1, "dtype"), (dict(residual_dtype=7), -1, "dtype"), (dict(pre_stride=8), -1, "pre")])
+def test_dense_refusals(fields, code, word, T):
+    import inl_hip
+    assert T._dense_fwd(_dense(T, **fields), P, P, P, P, P, P, None, 0, None) == code
+    assert word in inl_hip.last_error(), inl_hip.last_error()
+
+
+def test_dense_pointers(T):
+    import inl_hip
+    for i in range(6):
+        for bad in (ODD, None) if i not in (2, 3, 5) else (ODD,):
+            args = [P] * 6
+            args[i] = bad
+            assert T._dense_fwd(_dense(T), *args, None, 0, None) == -1
+    assert T._dense_fwd(None, P, P, P, P, P, P, None, 0, None) == -1
+    for i in (0, 1, 2, 3):   # dy, x, w, pre
+        args = [P] * 7
+        args[i] = None
+        assert T._dense_bwd(_dense(T, act=2), *args, None, 0, None) == -1
+    assert T._dense_bwd(_dense(T, dw_dtype=3), *[P] * 7, None, 0, None) == -1
+    assert T._dense_bwd(_dense(T, dx_stride=8), *[P] * 7, None, 0, None) == -1 and "dx" in inl_hip.last_error()
+    n = ctypes.c_size_t()
+    assert T._dense_ws(_dense(T, k=4), 0, ctypes.byref(n)) == -2
+    assert T._dense_ws(_dense(T), 0, None) == -1
+    # a few rows need none; nothing to do needs nothing
+    assert T._dense_ws(_dense(T), 0, ctypes.byref(n)) == 0 and n.value == 0
+    assert T._dense_fwd(_dense(T, m=0), None, None, None, None, None, None, None, 0, None) == 0
+
+
+@pytest.mark.parametrize("fields,code,word", [
+    (dict(m=-1), -1, "m must be"), (dict(hidden=36), -2, "multiples of 8"), (dict(inner=0), -1, "inner"),
+    (dict(act=0), -1, "act"), (dict(act=9), -1, "act"), (dict(inner=1 << 21), -2, "at most"),
+    (dict(x_stride=8), -1, "x: the row stride"), (dict(out_dtype=3), -1, "dtype")])
+def test_gated_ffn_refusals(fields, code, word, T):
+    import inl_hip
+    assert T._ffn_fwd(_ffn(T, **fields), P, P, P, P, P, P, P, None, 0, None) == code
+    assert word in inl_hip.last_error(), inl_hip.last_error()
+
+
+def test_gated_ffn_pointers(T):
+    import inl_hip
+    assert T._ffn_fwd(_ffn(T), P, P, P, None, P, P, None, None, 0, None) == -1 and "together" in inl_hip.last_error()
+    for i in (0, 1, 2, 4):
+        args = [P] * 7
+        args[i] = None
+        assert T._ffn_fwd(_ffn(T), *args, None, 0, None) == -1
+    for i in range(6):
+        args = [P] * 9
+        args[i] = ODD
+        assert T._ffn_bwd(_ffn(T), *args, None, 0, None) == -1
+    # the few-row forward keeps h in the workspace
+    assert T._ffn_fwd(_ffn(T), *[P] * 7, None, 0, None) == -1 and "workspace" in inl_hip.last_error()
+    assert T._ffn_fwd(_ffn(T), *[P] * 7, P, 8, None) == -1 and "need" in inl_hip.last_error()
+
+
+@pytest.mark.parametrize("fields,code,word", [
+    (dict(m=-1), -1, "m must be"), (dict(vocab=0), -1, "vocab"), (dict(hidden=36), -2, "multiple of 8"),
+    (dict(vocab=1 << 29), -2, "at most"), (dict(w_stride=8), -1, "w: the row stride")])
+def test_softmax_xent_refusals(fields, code, word, T):
+    import inl_hip
+    assert T._xent_fwd(_xent(T, **fields), *[P] * 6, None, 0, None) == code
+    assert word in inl_hip.last_error(), inl_hip.last_error()
+    assert T._xent_bwd(_xent(T, **fields), *[P] * 9, None, 0, None) == code
+
+
+def test_softmax_xent_pointers(T):
+    for i in (0, 1, 3, 4, 5):
+        args = [P] * 6
+        args[i] = None
+        assert T._xent_fwd(_xent(T), *args, None, 0, None) == -1
+    assert T._xent_fwd(_xent(T), P, P, ODD, P, P, P, None, 0, None) == -1
+    for i in (0, 1, 2, 3, 5):
+        args = [P] * 9
+        args[i] = None
+        assert T._xent_bwd(_xent(T), *args, None, 0, None) == -1
+    assert T._xent_bwd(_xent(T, dx_dtype=5), *[P] * 9, None, 0, None) == -1
+
+
+def test_norm_rope_bwd_refusals(T):
+    import inl_hip
+    def call(q=2, dq=P, dk=P, kw=P, dx_stride=0, x=P, dy=P, **kw_):
+        d = inl_hip.NormRopeDesc()
+        d.n_tokens, d.heads, d.head_dim, d.dtype, d.out_dtype, d.norm, d.eps = 4, 3, 64, 1, 1, 1, 1e-6
+        d.rotary_dim, d.sections, d.table_rows = 64, 1, 9
+        for k, v in kw_.items():
+            setattr(d, k, v)
+        return T._rope_bwd(d, q, dy, x, P, dx_stride, P, kw, P, P, P, None, None, dq, dk, None, 0, None)
+    assert call(head_dim=48) == -2 and call(rotary_dim=60, sections=3) == -2 and call(sections=4) == -1
+    assert call(q=0) == -1 and call(q=4) == -1 and call(q=3) == -1 and "k heads" in inl_hip.last_error()
+    assert call(norm=0) == -1 and "no norm" in inl_hip.last_error()
+    assert call(dx_stride=100) == -1 and call(x_row_stride=100) == -1 and call(x=ODD) == -1 and call(dy=None) == -1
+    assert call(sections=2, rotary_dim=64) == -1   # axial without its second tables
+    n = ctypes.c_size_t()
+    assert T._rope_bwd_ws(None, ctypes.byref(n)) == -1
+
+
+def test_adjacent_pairs_refusals():
+    import inl_hip
+    d = inl_hip.NormRopeDesc()
+    d.n_tokens, d.heads, d.head_dim, d.dtype, d.out_dtype = 4, 3, 64, 1, 1
+    d.sections, d.table_rows = 3, 9
+    for rd in (4, 12, 72):
+        d.rotary_dim = rd
+        assert inl_hip._norm_rope(d, P, P, None, P, P, P, None, None, None) == -2

@@ -622,3 +622,109 @@ def test_refusals(cuda, inl):
         with pytest.raises(inl.InlError):
             f()
             print("not refused:", i)
+
+
+def test_softmax_xent_lowest_float_everywhere(cuda, inl):
+    """A bias of the lowest float on every entry: all scores are that float, the
+    softmax is uniform. -inf on all but one: that one has all of it."""
+    import torch
+    m, vocab, hidden = 20, 333, 72
+    x, w, b, t = _xent_inputs(torch, cuda, m, vocab, hidden, 1.0, ignored=False)
+    low = torch.full_like(b, torch.finfo(torch.float32).min)
+    loss, lse = inl.softmax_xent(x, w, t, bias=low)
+    assert (lse == low[0]).all()
+    assert ((loss.double() - math.log(vocab)).abs() <= 2.0 ** -20).all()
+    one = torch.full_like(b, float("-inf"))
+    one[7] = 0
+    t.fill_(7)
+    loss, lse = inl.softmax_xent(x, w, t, bias=one)
+    s, tol = _scores(x, w, None, 1.0)
+    assert not loss.any() and ((lse.double() - s[:, 7]).abs() <= tol[:, 7]).all()
+    dx, dw, db = inl.softmax_xent_bwd(torch.ones(m, device=cuda), lse, x, w, t, bias=one, bias_grad=True)
+    # p of the one is 1 within the score's error, the others 0
+    e = m * (tol[:, 7].max().item() * 2 + 2.0 ** -20)
+    assert db.abs().max().item() <= e and dx.double().abs().max().item() <= e * w.double().abs().max().item() + 1e-30
+    assert not dw[:7].any() and not dw[8:].any()
+
+
+def test_dense_far_rows(cuda, inl):
+    """Rows that start past 2^32 bytes, of x, y, the stored pre and the gradients."""
+    import torch
+    rows, wide, k, n = 280_000, 8192, 72, 40
+    buf = torch.empty(rows, wide, dtype=torch.bfloat16, device=cuda)
+    x, y, pre, dy = buf[:, 1024:1024 + k], buf[:, 2048:2048 + n], buf[:, 4096:4096 + n], buf[:, 6000:6000 + n]
+    x.copy_(_rand(torch, cuda, (rows, k), 1))
+    dy.copy_(_rand(torch, cuda, (rows, n), 2, 0.1))
+    w = _rand(torch, cuda, (n, k), 3, k ** -0.5)
+    print("case=dense far rows", flush=True)
+    inl.dense(x, w, act="silu", pre=pre, out=y)
+    z, ref, tol = _dense_ref(x, w, None, "silu", None)
+    R.check(y, ref, tol + R.out_tol(ref, torch.bfloat16), "y")
+    R.check(pre, z, tol + R.out_tol(z, torch.bfloat16), "pre")
+    dx, dw, db = inl.dense_bwd(dy, x, w, act="silu", pre=pre, bias_grad=True)
+    dz = R.r16(dy.double() * R.act("silu", pre.double())[1])
+    ref = dz @ w.double()
+    R.check(dx, ref, R.out_tol(ref, torch.bfloat16) + R.sum_tol(n) * (dz.abs() @ w.double().abs()) + R.flips(dz, w.double()), "dx")
+    ref = dz.T.contiguous() @ x.double()
+    # some 280,000 x 2^-14 values near the middle of two bf16 numbers, of either sign
+    R.check(dw, ref, R.out_tol(ref, torch.bfloat16) + R.sum_tol(rows) * (dz.abs().T.contiguous() @ x.double().abs()) +
+            2 * R.flips(dz, x.double()), "dw")
+
+
+def test_first_call_in_a_capture(cuda, inl):
+    """A shape that was never called before, captured at once."""
+    import torch
+    x, w = _rand(torch, cuda, (777, 200), 1), _rand(torch, cuda, (456, 200), 2, 0.07)
+    dy = _rand(torch, cuda, (777, 456), 3, 0.1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = inl.dense(x, w)
+        grads = inl.dense_bwd(dy, x, w, bias_grad=True)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        want = (inl.dense(x, w), *inl.dense_bwd(dy, x, w, bias_grad=True))
+        assert all(torch.equal(a, b) for a, b in zip((y, *grads), want))
+
+
+def test_results_do_not_depend_on_the_workspace(cuda, inl):
+    """The C entries with a workspace of NaN and one of zeros, exactly as large as
+    asked for, with guards behind it that stay as they were."""
+    import ctypes
+
+    import torch
+    from inl_hip import train as T
+    m, hidden, inner, vocab = 300, 136, 200, 1001
+    x, dy = _rand(torch, cuda, (m, hidden), 1), _rand(torch, cuda, (m, hidden), 2, 0.1)
+    wgu, wd = _rand(torch, cuda, (2 * inner, hidden), 3, 0.08), _rand(torch, cuda, (hidden, inner), 4, 0.07)
+    wv = _rand(torch, cuda, (vocab, hidden), 5, 0.08)
+    t = torch.arange(m, device=cuda, dtype=torch.int32)
+    _, pre, h = inl.gated_ffn(x, wgu, wd, save=True)
+    _, lse = inl.softmax_xent(x, wv, t)
+    dl = torch.ones(m, device=cuda)
+    st = torch.cuda.current_stream().cuda_stream
+    p = lambda v: v.data_ptr()
+    got = []
+    for fill in (0, 255):
+        def room(size_fn, desc, backward):
+            n = ctypes.c_size_t()
+            assert size_fn(desc, backward, ctypes.byref(n)) == 0
+            buf = torch.full((n.value + 256,), fill, dtype=torch.uint8, device=cuda)
+            return buf, n.value
+        fd = T.GatedFfnDesc(m, hidden, inner, 0, 0, 0, 0, 2, 1, 0, 1, 1)
+        xd = T.SoftmaxXentDesc(m, vocab, hidden, 0, 0, 0, 0, 1.0, -100, 1, 1)
+        y, dx, dgu, dd = (torch.empty(s, dtype=torch.bfloat16, device=cuda)
+                          for s in ((m, hidden), (m, hidden), (2 * inner, hidden), (hidden, inner)))
+        loss, lse2 = torch.empty(m, device=cuda), torch.empty(m, device=cuda)
+        dxx, dwv, db = torch.empty_like(x), torch.empty_like(wv), torch.empty(vocab, device=cuda)
+        rooms = [room(T._ffn_ws, fd, 0), room(T._ffn_ws, fd, 1), room(T._xent_ws, xd, 0), room(T._xent_ws, xd, 1)]
+        (a, na), (b, nb), (c, nc), (d, nd) = rooms
+        assert T._ffn_fwd(fd, p(x), p(wgu), p(wd), None, p(y), None, None, p(a), na, st) == 0
+        assert T._ffn_bwd(fd, p(dy), p(x), p(wgu), p(wd), p(pre), p(h), p(dx), p(dgu), p(dd), p(b), nb, st) == 0
+        assert T._xent_fwd(xd, p(x), p(wv), None, p(t), p(loss), p(lse2), p(c), nc, st) == 0
+        assert T._xent_bwd(xd, p(dl), p(lse), p(x), p(wv), None, p(t), p(dxx), p(dwv), p(db), p(d), nd, st) == 0
+        torch.cuda.synchronize()
+        assert all((buf[n:] == fill).all() for buf, n in rooms)
+        got.append((y, dx, dgu, dd, loss, lse2, dxx, dwv, db))
+    assert all(torch.equal(u, v) for u, v in zip(*got))
