@@ -5,12 +5,15 @@
 //   dweight += dn * xhat
 //   dx   = (weight dn - xhat mean(weight dn xhat)) / rms(x)
 //
-// Bound by memory: x and dy read once, dx written once. The layout is the
-// forward's (norm_rope.hip): G = head_dim / 8 lanes own a token, 8 values of every
-// head each, so the two sums of a row are one cross-lane reduction each and a
-// rotation partner is a lane away. A lane keeps its 8 columns of dq_weight and
-// dk_weight in f32 registers over all tokens of its workgroup; the groups of a
-// workgroup meet in LDS, the workgroups in a second kernel, in a fixed order.
+// Bound by memory: x and dy read once, dx written once (125 us for 32,003 tokens of
+// 16 + 8 heads of 128 in bf16, 4.7 TB/s; a copy reaches 4.8; f32 5.2). The layout is
+// the forward's (norm_rope.hip): G = head_dim / 8 lanes own a unit of four heads (f32:
+// two) of a token, 8 values of every head each, so the two sums of a row are one
+// cross-lane reduction each and a rotation partner is a lane away. Units, not whole
+// tokens, so that a short batch fills the card too: 500 tokens took 28 us when a lane
+// group walked all the heads of its token, and take 11.6. A lane keeps its 8 columns of
+// dq_weight and dk_weight in f32 registers over all units of its workgroup; the groups
+// of a workgroup meet in LDS, the workgroups in a second kernel, in a fixed order.
 #include <type_traits>
 
 #include "norm_rope.hpp"
@@ -84,15 +87,34 @@ __global__ __launch_bounds__(256) void norm_rope_bwd_kernel(NormRopeBwdParams p)
   if (p.norm && p.qw) load8<TX>(p.qw + 8 * j * (int)sizeof(TX), wq);
   if (p.norm && p.kw) load8<TX>(p.kw + 8 * j * (int)sizeof(TX), wk);
 
-  const int64_t step = (int64_t)gridDim.x * GROUPS;
-  // every lane of a wave runs the same iterations (the reductions need all of them)
-  for (int64_t t0 = (int64_t)blockIdx.x * GROUPS; t0 < p.n_tokens; t0 += step) {
-    const int64_t tok = t0 + grp;
+  // units: HB heads of a token, a lane group each; every lane of a wave runs the
+  // same iterations (the reductions need all of them)
+  const int chunks = (p.heads + HB - 1) / HB;
+  const int64_t units = p.n_tokens * chunks, step = (int64_t)gridDim.x * GROUPS;
+  const int64_t step_tok = step / chunks;
+  const int step_chunk = (int)(step - step_tok * chunks);
+  int64_t u = (int64_t)blockIdx.x * GROUPS + grp, tok = u / chunks;
+  int chunk = (int)(u - tok * chunks);
+  for (int64_t u0 = u - grp; u0 < units; u0 += step) {
     const bool valid = tok < p.n_tokens;
     const int64_t tc = valid ? tok : 0;
+    const int h0 = chunk * HB;
+    tok += step_tok;
+    chunk += step_chunk;
+    if (chunk >= chunks) {
+      chunk -= chunks;
+      ++tok;
+    }
     const char* yt = p.dy + (tc * p.y_stride + 8 * j) * (int64_t)sizeof(TY);
     const char* xt = p.x + (tc * p.x_stride + 8 * j) * (int64_t)sizeof(TX);
     char* dt = p.dx + (tc * p.d_stride + 8 * j) * (int64_t)sizeof(TX);
+    Raw8 ry[HB], rx[HB];
+#pragma unroll
+    for (int i = 0; i < HB; ++i) {
+      const int64_t h = min(h0 + i, p.heads - 1) * (int64_t)p.head_dim;
+      load_raw<TY>(yt + h * (int64_t)sizeof(TY), ry[i]);
+      if (p.norm) load_raw<TX>(xt + h * (int64_t)sizeof(TX), rx[i]);
+    }
     float c[8], sn[8];
     bool bad = false;
     if (p.rotary_dim > 0) {
@@ -114,75 +136,66 @@ __global__ __launch_bounds__(256) void norm_rope_bwd_kernel(NormRopeBwdParams p)
 #pragma unroll
         for (int e = 0; e < 8; ++e) { c[e] = round_bf16(c[e]); sn[e] = round_bf16(sn[e]); }
     }
-    for (int h0 = 0; h0 < p.heads; h0 += HB) {
-      Raw8 ry[HB], rx[HB];
 #pragma unroll
-      for (int i = 0; i < HB; ++i) {
-        const int64_t h = min(h0 + i, p.heads - 1) * (int64_t)p.head_dim;
-        load_raw<TY>(yt + h * (int64_t)sizeof(TY), ry[i]);
-        if (p.norm) load_raw<TX>(xt + h * (int64_t)sizeof(TX), rx[i]);
+    for (int i = 0; i < HB; ++i) {
+      const bool live = valid && h0 + i < p.heads;
+      float d[8];
+      unpack8<TY>(ry[i], d);
+      if (mode == 1) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float a = d[e], b = d[e + 4];
+          d[e] = a * c[e] + b * sn[e];
+          d[e + 4] = b * c[e] - a * sn[e];
+        }
+      } else if (mode == 3) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float a = d[e], b = d[e + 1];
+          d[e] = a * c[e] + b * sn[e];
+          d[e + 1] = b * c[e] - a * sn[e];
+        }
       }
+      if (p.rotary_dim > 0 && !inner8 && !adjacent) {   // uniform
+        float pv[8];
+        if (xor_partner)
+          xor_lanes8(d, pv, half, lane);
+        else
 #pragma unroll
-      for (int i = 0; i < HB; ++i) {
-        const bool live = valid && h0 + i < p.heads;
-        float d[8];
-        unpack8<TY>(ry[i], d);
-        if (mode == 1) {
+          for (int e = 0; e < 8; ++e) pv[e] = __shfl(d[e], partner, 64);
+        if (mode == 2)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float a = d[e], b = d[e + 4];
-            d[e] = a * c[e] + b * sn[e];
-            d[e + 4] = b * c[e] - a * sn[e];
-          }
-        } else if (mode == 3) {
-#pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const float a = d[e], b = d[e + 1];
-            d[e] = a * c[e] + b * sn[e];
-            d[e + 1] = b * c[e] - a * sn[e];
-          }
-        }
-        if (p.rotary_dim > 0 && !inner8 && !adjacent) {   // uniform
-          float pv[8];
-          if (xor_partner)
-            xor_lanes8(d, pv, half, lane);
-          else
-#pragma unroll
-            for (int e = 0; e < 8; ++e) pv[e] = __shfl(d[e], partner, 64);
-          if (mode == 2)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) d[e] = first ? d[e] * c[e] + pv[e] * sn[e] : d[e] * c[e] - pv[e] * sn[e];
-        }
-        if (bad)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) d[e] = __builtin_nanf("");
-        if (p.norm) {
-          const bool is_q = h0 + i < p.q_heads;
-          float v[8];
-          unpack8<TX>(rx[i], v);
-          float ss = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
-          ss = group_sum<G>(ss);
-          const float inv = 1.0f / sqrtf(ss / (float)p.head_dim + p.eps);
-          float dot = 0.f, wd[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            v[e] *= inv;
-            const float dw = d[e] * v[e];
-            if (live) {
-              dq[e] += is_q ? dw : 0.f;
-              dk[e] += is_q ? 0.f : dw;
-            }
-            wd[e] = d[e] * (is_q ? wq[e] : wk[e]);
-            dot += wd[e] * v[e];
-          }
-          dot = group_sum<G>(dot) / (float)p.head_dim;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) d[e] = inv * (wd[e] - v[e] * dot);
-        }
-        if (live) store8<TX>(dt + (h0 + i) * (int64_t)p.head_dim * (int64_t)sizeof(TX), d);
+          for (int e = 0; e < 8; ++e) d[e] = first ? d[e] * c[e] + pv[e] * sn[e] : d[e] * c[e] - pv[e] * sn[e];
       }
+      if (bad)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] = __builtin_nanf("");
+      if (p.norm) {
+        const bool is_q = h0 + i < p.q_heads;
+        float v[8];
+        unpack8<TX>(rx[i], v);
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
+        ss = group_sum<G>(ss);
+        const float inv = 1.0f / sqrtf(ss / (float)p.head_dim + p.eps);
+        float dot = 0.f, wd[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[e] *= inv;
+          const float dw = d[e] * v[e];
+          if (live) {
+            dq[e] += is_q ? dw : 0.f;
+            dk[e] += is_q ? 0.f : dw;
+          }
+          wd[e] = d[e] * (is_q ? wq[e] : wk[e]);
+          dot += wd[e] * v[e];
+        }
+        dot = group_sum<G>(dot) / (float)p.head_dim;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] = inv * (wd[e] - v[e] * dot);
+      }
+      if (live) store8<TX>(dt + (h0 + i) * (int64_t)p.head_dim * (int64_t)sizeof(TX), d);
     }
   }
   if (!p.part) return;   // uniform
@@ -201,11 +214,12 @@ __global__ __launch_bounds__(256) void norm_rope_bwd_kernel(NormRopeBwdParams p)
   }
 }
 
-// Workgroups: two waves per SIMD on every CU keep the memory busy; more would
-// only add partial sums to join.
-int64_t bwd_groups(int64_t n_tokens, int head_dim, int cus) {
-  const int64_t per = 256 / (head_dim / 8);
-  return std::max<int64_t>(1, std::min<int64_t>((n_tokens + per - 1) / per, (int64_t)cus * 2));
+// Workgroups, at most four per CU: each adds a row of partial sums to join. Eight take
+// 29 us for 4,000 tokens where four take 24, and no less for 32,003. (A unit has two
+// heads or more.)
+int64_t bwd_groups(int64_t n_tokens, int heads, int head_dim, int cus) {
+  const int64_t per = 256 / (head_dim / 8), units = n_tokens * ((heads + 1) / 2);
+  return std::max<int64_t>(1, std::min<int64_t>((units + per - 1) / per, (int64_t)cus * 4));
 }
 
 }  // namespace
@@ -215,11 +229,11 @@ int64_t bwd_groups(int64_t n_tokens, int head_dim, int cus) {
 extern "C" int inl_norm_rope_bwd_workspace_size(const inl_norm_rope_desc* d, size_t* bytes) {
   using namespace inl;
   if (!d || !bytes) return fail(INL_E_INVALID, "norm_rope_bwd: desc or bytes is NULL");
-  if (d->n_tokens < 0 || d->head_dim < 8 || d->head_dim > 512)
-    return fail(INL_E_INVALID, "norm_rope_bwd: bad n_tokens/head_dim");
+  if (d->n_tokens < 0 || d->heads <= 0 || d->head_dim < 8 || d->head_dim > 512)
+    return fail(INL_E_INVALID, "norm_rope_bwd: bad n_tokens/heads/head_dim");
   int cus = 0, rc = device_cus(&cus);
   if (rc) return rc;
-  *bytes = d->norm ? (size_t)bwd_groups(d->n_tokens, d->head_dim, cus) * 2 * d->head_dim * 4 : 0;
+  *bytes = d->norm ? (size_t)bwd_groups(d->n_tokens, d->heads, d->head_dim, cus) * 2 * d->head_dim * 4 : 0;
   return INL_OK;
 }
 
@@ -251,7 +265,7 @@ extern "C" int inl_norm_rope_qk_bwd(const inl_norm_rope_desc* d, int32_t q_heads
     return fail(INL_E_INVALID, "norm_rope_bwd: dy, x, dx and the weights must be non-null and 16-byte aligned");
   int cus = 0;
   if ((rc = device_cus(&cus))) return rc;
-  const int64_t groups = bwd_groups(d->n_tokens, hd, cus);
+  const int64_t groups = bwd_groups(d->n_tokens, d->heads, hd, cus);
   const bool sums = dq_weight || dk_weight;
   if (sums && (rc = check_workspace("norm_rope_bwd", ws, ws_bytes, (size_t)groups * 2 * hd * 4))) return rc;
   NormRopeBwdParams p{};
