@@ -233,12 +233,13 @@ int act_bwd(int64_t m, int64_t n, const void* dy, int64_t dys, const void* pre, 
             float* colsum, float* part, hipStream_t stream) {
   ActBwdParams p{(const char*)dy, (const char*)pre, (char*)dz, part, m, dys, pres, (int32_t)n, act};
   const int64_t blocks = colsum_blocks(m);
+  if (colsum && blocks == 1) p.part = colsum;   // nothing to join
   const dim3 grid((unsigned)((n + CS_COLS - 1) / CS_COLS), (unsigned)blocks), block(256);
   if (pre && colsum) hipLaunchKernelGGL((act_bwd_kernel<true, true>), grid, block, 0, stream, p);
   else if (pre) hipLaunchKernelGGL((act_bwd_kernel<true, false>), grid, block, 0, stream, p);
   else hipLaunchKernelGGL((act_bwd_kernel<false, true>), grid, block, 0, stream, p);
   INL_HIP_TRY(hipGetLastError());
-  return colsum ? colsum_join(part, blocks, (int32_t)n, colsum, (int32_t)n, nullptr, stream) : INL_OK;
+  return colsum && blocks > 1 ? colsum_join(part, blocks, (int32_t)n, colsum, (int32_t)n, nullptr, stream) : INL_OK;
 }
 
 int fill_zero(void* p, int64_t rows, int64_t cols, int64_t stride, int32_t dtype, hipStream_t stream) {

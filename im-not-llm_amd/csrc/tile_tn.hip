@@ -148,7 +148,8 @@ TilePlan tile_plan(int64_t m, int64_t n, int64_t k, int by_cols, bool gated, int
     const Cost& c = costs[i];
     const int64_t bno = gated ? c.bn / 2 : c.bn;
     const int64_t tiles = ((m + c.bm - 1) / c.bm) * ((n + bno - 1) / bno);
-    for (int s = 1; s <= max_splits && s <= kst; ++s) {
+    // (past two units per CU a split only adds partials)
+    for (int s = 1; s <= max_splits && s <= kst && (s == 1 || tiles * (s - 1) < 2 * cus); ++s) {
       const int64_t kper = (kst + s - 1) / s;
       if ((kst + kper - 1) / kper != s) continue;   // a split would have no work
       const int64_t units = tiles * s;
