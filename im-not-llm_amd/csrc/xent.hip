@@ -81,9 +81,10 @@ __global__ __launch_bounds__(256) void xent_dloss_kernel(const float* dl, const 
 constexpr int MAX_SPLITS = 32;
 
 // Vocabulary entries per piece: g of a piece is some 128 MiB, so that dw and dx
-// read it from the 256 MB Infinity Cache, in whole 256-column tiles.
+// read it from the 256 MB Infinity Cache, in whole 256-column tiles; at most 2^21, the
+// longest row that the products' descriptors take.
 int64_t piece_cols(int64_t m, int64_t vocab) {
-  int64_t p = ((int64_t)1 << 26) / std::max<int64_t>(m, 1);
+  int64_t p = std::min<int64_t>(((int64_t)1 << 26) / std::max<int64_t>(m, 1), (int64_t)1 << 21);
   p = std::min(std::max<int64_t>(p, 4096), vocab);
   return (p + 255) / 256 * 256;
 }

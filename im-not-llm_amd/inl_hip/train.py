@@ -93,7 +93,18 @@ def _mat(name, t, rows, cols, dtypes, dev):
     stride = t.stride()
     if stride[1] != 1 and cols > 1:
         raise InlError(-1, f"{name}: rows must be contiguous")
-    return stride[0] if rows > 1 else cols
+    if rows <= 1:
+        return cols
+    if stride[0] < cols:   # expanded rows, too: the library reads a stride of 0 as packed
+        raise InlError(-1, f"{name}: rows overlap (strides {stride})")
+    return stride[0]
+
+
+def _matrix(name, t):
+    shape = t.shape
+    if len(shape) != 2:
+        raise InlError(-1, f"{name}: shape {tuple(shape)}, need two dimensions")
+    return shape
 
 
 def _packed(name, t, rows, cols, dev):
@@ -156,8 +167,8 @@ def _ptr(t):
 
 @_at_home
 def _dense(dev, x, w, bias, act, residual, pre, out, out_dtype, stream):
-    m, k = x.shape
-    n = w.shape[0]
+    m, k = _matrix("x", x)
+    n = _matrix("w", w)[0]
     code = _act(act)
     xs, ws = _mat("x", x, m, k, _B16, dev), _mat("w", w, n, k, _B16, dev)
     made = None
@@ -190,8 +201,8 @@ def dense(x, w, bias=None, *, act=None, residual=None, pre=None, out=None, out_d
 
 @_at_home
 def _dense_grads(dev, x, dy, w, act, pre, bias_grad, dx_grad, dw_grad, dx_dtype, dw_dtype, stream):
-    m, k = x.shape
-    n = w.shape[0]
+    m, k = _matrix("x", x)
+    n = _matrix("w", w)[0]
     code = _act(act)
     if not code:
         pre = None
@@ -227,8 +238,8 @@ def dense_bwd(dy, x, w, *, act=None, pre=None, bias_grad=False, dx_grad=True, dw
 
 @_at_home
 def _ffn(dev, x, w_gate_up, w_down, act, residual, save, out, out_dtype, stream):
-    m, hidden = x.shape
-    inner = w_down.shape[1]
+    m, hidden = _matrix("x", x)
+    inner = _matrix("w_down", w_down)[1]
     code = _act(act, True)
     xs = _mat("x", x, m, hidden, _B16, dev)
     _packed("w_gate_up", w_gate_up, 2 * inner, hidden, dev)
@@ -263,8 +274,8 @@ def gated_ffn(x, w_gate_up, w_down, *, act="silu", residual=None, save=False, ou
 
 @_at_home
 def _ffn_grads(dev, x, dy, w_gate_up, w_down, pre, h, act, dx_grad, dw_grad, dx_dtype, dw_dtype, stream):
-    m, hidden = x.shape
-    inner = w_down.shape[1]
+    m, hidden = _matrix("x", x)
+    inner = _matrix("w_down", w_down)[1]
     code = _act(act, True)
     xs, ys = _mat("x", x, m, hidden, _B16, dev), _mat("dy", dy, m, hidden, _B16, dev)
     for name, t, rows, cols in (("w_gate_up", w_gate_up, 2 * inner, hidden), ("w_down", w_down, hidden, inner),
@@ -296,8 +307,10 @@ def gated_ffn_bwd(dy, x, w_gate_up, w_down, pre, h, *, act="silu", dx_grad=True,
 # ---------------------------------------------------------------------------
 
 def _xent_desc(dev, x, w, scale, ignore_index, dx_dtype=None, dw_dtype=None):
-    m, hidden = x.shape
-    vocab = w.shape[0]
+    m, hidden = _matrix("x", x)
+    vocab = _matrix("w", w)[0]
+    if not -2 ** 31 <= ignore_index < 2 ** 31:
+        raise InlError(-1, f"ignore_index {ignore_index} is no int32")
     return SoftmaxXentDesc(m, vocab, hidden, _mat("x", x, m, hidden, _B16, dev), _mat("w", w, vocab, hidden, _B16, dev),
                            0, 0, scale, ignore_index, _dtype_code(dx_dtype or _BF16), _dtype_code(dw_dtype or _BF16))
 
@@ -363,7 +376,12 @@ def _heads(name, t, shape, dev):
     stride = t.stride()
     if stride[2] != 1 or (shape[1] > 1 and stride[1] != shape[2]):
         raise InlError(-1, f"{name}: heads must be contiguous inside a token row")
-    return stride[0] if shape[0] > 1 else shape[1] * shape[2]
+    row = shape[1] * shape[2]
+    if shape[0] <= 1:
+        return row
+    if stride[0] < row:
+        raise InlError(-1, f"{name}: token rows overlap (strides {stride})")
+    return stride[0]
 
 
 @_at_home

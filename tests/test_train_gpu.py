@@ -728,3 +728,35 @@ def test_results_do_not_depend_on_the_workspace(cuda, inl):
         assert all((buf[n:] == fill).all() for buf, n in rooms)
         got.append((y, dx, dgu, dd, loss, lse2, dxx, dwv, db))
     assert all(torch.equal(u, v) for u, v in zip(*got))
+
+
+def test_overlapping_rows_and_wrong_ranks_are_refused(cuda, inl):
+    """Expanded rows (the gradient of a sum) have a stride of 0, which the library
+    reads as packed rows: they are refused, as are vectors for matrices."""
+    import torch
+    dev = cuda
+    m, n, k = 24, 64, 32
+    x, w, dy = (_rand(torch, dev, s, 7 + i) for i, s in enumerate([(m, k), (n, k), (m, n)]))
+    wide = lambda cols: torch.ones((1, cols), dtype=torch.bfloat16, device=dev).expand(m, cols)
+    gu, down = _rand(torch, dev, (2 * n, k), 20), _rand(torch, dev, (k, n), 21)
+    targets = torch.zeros(m, dtype=torch.int32, device=dev)
+    ones = torch.ones(m, device=dev)
+    heads = _rand(torch, dev, (m, 3, 64), 22)
+    flat = torch.ones((1, 3, 64), dtype=torch.bfloat16, device=dev).expand(m, 3, 64)
+    slid = torch.zeros(m + k, dtype=torch.bfloat16, device=dev).as_strided((m, k), (1, 1))
+    for call in (lambda: inl.dense(wide(k), w), lambda: inl.dense(slid, w), lambda: inl.dense(x[0], w),
+                 lambda: inl.dense(x, w[0]), lambda: inl.dense(x, w, residual=wide(n)),
+                 lambda: inl.dense(x, w, out=wide(n)), lambda: inl.dense_bwd(wide(n), x, w),
+                 lambda: inl.dense_bwd(dy, x, w, act="silu", pre=wide(n)),
+                 lambda: inl.gated_ffn(wide(k), gu, down), lambda: inl.gated_ffn(x, gu, down[0]),
+                 lambda: inl.gated_ffn(x, gu, down, residual=wide(k)),
+                 lambda: inl.softmax_xent(wide(k), w, targets), lambda: inl.softmax_xent(x[0], w, targets),
+                 lambda: inl.softmax_xent(x, w, targets, ignore_index=2 ** 32),
+                 lambda: inl.softmax_xent_bwd(ones[:1].expand(m), ones, x, w, targets),
+                 lambda: inl.softmax_xent_bwd(ones, ones, x, wide(k), targets),
+                 lambda: inl.norm_rope_qk_bwd(flat, heads, 2), lambda: inl.norm_rope_qk_bwd(heads, flat, 2),
+                 lambda: inl.norm_rope_qk_bwd(heads, heads, 2, out=flat)):
+        with pytest.raises(inl.InlError):
+            call()
+    one = torch.ones((1, k), dtype=torch.bfloat16, device=dev).expand(1, k)   # one row has no stride
+    assert torch.equal(inl.dense(one, w), inl.dense(one.contiguous(), w))
