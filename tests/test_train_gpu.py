@@ -760,3 +760,10 @@ def test_overlapping_rows_and_wrong_ranks_are_refused(cuda, inl):
             call()
     one = torch.ones((1, k), dtype=torch.bfloat16, device=dev).expand(1, k)   # one row has no stride
     assert torch.equal(inl.dense(one, w), inl.dense(one.contiguous(), w))
+
+
+@pytest.mark.parametrize("m", [1, 2])
+def test_softmax_xent_very_wide(m, cuda, inl):
+    """More vocabulary than a piece may be wide with a few rows."""
+    test_softmax_xent(m, 2 ** 21 + 4099, 8, 1.0, True, cuda, inl)
+    test_softmax_xent_bwd(m, 2 ** 21 + 4099, 8, 1.0, True, cuda, inl)
