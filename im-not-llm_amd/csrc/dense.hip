@@ -13,14 +13,16 @@ namespace inl {
 
 namespace {
 
-// ---- a few rows: y[m, n], m <= 8 ----
+// ---- one to four rows ----
 //
 // Bound by the weights, read once: a wave takes one output column (or the gate
 // and up rows of one) and walks its row of w in contiguous KiB, 16 bytes per
 // lane, next to the same k of the M rows of x (from L1 after the first wave);
-// products by v_dot2_f32_bf16, f32 sums, one cross-lane sum at the end.
+// f32 products and sums, one cross-lane sum at the end. (The instruction that adds
+// two bf16 products rounds too coarsely.) One row through 1,024 x 1,024 takes 2.6 us,
+// through 50,000 x 768 13.5 us (5.7 TB/s). Its vector instructions grow with M.
 template <int M, int R, bool OUT16>
-__global__ __launch_bounds__(256) void few_dense_kernel(TileParams p) {
+__global__ __launch_bounds__(256) void row_dense_kernel(TileParams p) {
   const int lane = threadIdx.x & 63;
   const int c = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (c >= p.n) return;   // a whole wave
@@ -85,6 +87,119 @@ __global__ __launch_bounds__(256) void few_dense_kernel(TileParams p) {
   }
   if constexpr (OUT16) *reinterpret_cast<bf16*>(p.y + (row * p.ys + c) * 2) = (bf16)y;
   else *reinterpret_cast<float*>(p.y + (row * p.ys + c) * 4) = y;
+}
+
+// ---- up to 16 XB rows ----
+//
+// Bound by latency, and by what one CU can load: no LDS stage, no ring. A workgroup
+// takes 16 output columns (R = 2: their gate and up rows), its waves share k in units
+// of 64 (whole 128-byte lines of 16 rows of w). Operands go from memory to
+// v_mfma_f32_16x16x32_bf16 as they lie, U units asked for at a time (x from L2 after
+// the first workgroups); the waves' sums meet in LDS, in order. 8 rows through 1,024 x
+// 1,024 take 3.7 us, 16 take 4.0 (tiled product: 9.4).
+constexpr int FEW_WAVES = 4;   // (eight: 5.8 us instead of 4.0 for 16 rows, 1,024 x 1,024)
+
+template <int R, int XB, bool OUT16>
+__global__ __launch_bounds__(FEW_WAVES * 64) void few_dense_kernel(TileParams p) {
+  constexpr int U = XB == 1 ? 4 : 2;
+  __shared__ f32x4 red[FEW_WAVES][R * XB][64];
+  const int lane = threadIdx.x & 63, l16 = lane & 15, quad = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c0 = blockIdx.x * 16, m = (int)p.m;
+  const char* wr[R];
+  const char* xr[XB];
+#pragma unroll
+  for (int r = 0; r < R; ++r) wr[r] = p.w + (min(c0 + l16, p.n - 1) + (int64_t)r * p.n) * p.ws_b;
+#pragma unroll
+  for (int b = 0; b < XB; ++b) xr[b] = p.x + min(b * 16 + l16, m - 1) * p.xs_b;
+  f32x4 acc[R][XB] = {};
+  const u32x4 none = {};
+  for (int k0 = wave * 64; k0 < p.k; k0 += FEW_WAVES * 64 * U) {
+    u32x4 wv[U][2][R], xv[U][2][XB];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int k = k0 + i * FEW_WAVES * 64 + s * 32 + quad * 8;
+        const bool in = k < p.k;
+        const int64_t off = in ? (int64_t)k * 2 : 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) wv[i][s][r] = *reinterpret_cast<const u32x4*>(wr[r] + off);
+#pragma unroll
+        for (int b = 0; b < XB; ++b) xv[i][s][b] = *reinterpret_cast<const u32x4*>(xr[b] + off);
+      }
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const bool in = k0 + i * FEW_WAVES * 64 + s * 32 + quad * 8 < p.k;
+#pragma unroll
+        for (int r = 0; r < R; ++r) wv[i][s][r] = in ? wv[i][s][r] : none;
+#pragma unroll
+        for (int b = 0; b < XB; ++b) {
+          const u32x4 x = in ? xv[i][s][b] : none;
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            acc[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv[i][s][r]),
+                                                                __builtin_bit_cast(bf16x8, x), acc[r][b], 0, 0, 0);
+        }
+      }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int b = 0; b < XB; ++b) red[wave][r * XB + b][lane] = acc[r][b];
+  __syncthreads();
+  // element e: row b 16 + l16, column c0 + 4 quad + e; a wave per block of rows
+  if (wave >= XB) return;
+  const int row = wave * 16 + l16, c = c0 + 4 * quad;
+  if (row >= m || c >= p.n) return;
+  f32x4 v[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    v[r] = red[0][r * XB + wave][lane];
+#pragma unroll
+    for (int i = 1; i < FEW_WAVES; ++i) {
+      const f32x4 q = red[i][r * XB + wave][lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[r][e] += q[e];
+    }
+  }
+  auto put16 = [](char* at, const f32x4& z) {
+    bf16x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = (bf16)z[e];
+    *reinterpret_cast<bf16x4*>(at) = o;
+  };
+  f32x4 y = v[0];
+  if constexpr (R == 2) {
+    if (p.pre) {
+      put16(p.pre + (row * p.ps + c) * 2, v[0]);
+      put16(p.pre + (row * p.ps + p.n + c) * 2, v[1]);
+    }
+    y = act_apply4(p.act, y);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] *= v[1][e];
+  } else {
+    if (p.bias) {
+      const f32x4 b = *reinterpret_cast<const f32x4*>(p.bias + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] += b[e];
+    }
+    if (p.pre) put16(p.pre + (row * p.ps + c) * 2, y);
+    y = act_apply4(p.act, y);
+    if (p.res && p.res_bf16) {
+      const bf16x4 q = *reinterpret_cast<const bf16x4*>(p.res + (row * p.rs + c) * 2);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] += p.beta * (float)q[e];
+    } else if (p.res) {
+      const f32x4 q = *reinterpret_cast<const f32x4*>(p.res + (row * p.rs + c) * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] += p.beta * q[e];
+    }
+  }
+  if constexpr (OUT16) put16(p.y + (row * p.ys + c) * 2, y);
+  else *reinterpret_cast<f32x4*>(p.y + (row * p.ys + c) * 4) = y;
 }
 
 // ---- dz and column sums ----
@@ -176,16 +291,29 @@ __global__ __launch_bounds__(256) void fill_zero_kernel(char* p, int64_t rows, i
 
 template <int R, bool OUT16>
 int few_launch(const TileParams& p, hipStream_t stream) {
-  const dim3 grid((unsigned)((p.n + 3) / 4)), block(256);
-  if (p.m == 1) hipLaunchKernelGGL((few_dense_kernel<1, R, OUT16>), grid, block, 0, stream, p);
-  else if (p.m == 2) hipLaunchKernelGGL((few_dense_kernel<2, R, OUT16>), grid, block, 0, stream, p);
-  else if (p.m <= 4) hipLaunchKernelGGL((few_dense_kernel<4, R, OUT16>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((few_dense_kernel<8, R, OUT16>), grid, block, 0, stream, p);
+  const dim3 rows((unsigned)((p.n + 3) / 4)), blocks((unsigned)((p.n + 15) / 16)), t(256), tb(FEW_WAVES * 64);
+  if (p.m == 1) hipLaunchKernelGGL((row_dense_kernel<1, R, OUT16>), rows, t, 0, stream, p);
+  else if (p.m == 2) hipLaunchKernelGGL((row_dense_kernel<2, R, OUT16>), rows, t, 0, stream, p);
+  else if (p.m <= 4) hipLaunchKernelGGL((row_dense_kernel<4, R, OUT16>), rows, t, 0, stream, p);
+  else if (p.m <= 16) hipLaunchKernelGGL((few_dense_kernel<R, 1, OUT16>), blocks, tb, 0, stream, p);
+  else hipLaunchKernelGGL((few_dense_kernel<R, 2, OUT16>), blocks, tb, 0, stream, p);
   INL_HIP_TRY(hipGetLastError());
   return INL_OK;
 }
 
 }  // namespace
+
+// Measured, us, few rows against the tiled product, by (n, k): up to four rows
+// (1,024, 1,024) 3.1 / 9, (8,192, 2,048) 8.6 / 10, (16,384, 1,024) 9.1 / 8, (50,000, 768)
+// 21 / 16, two rows of the last 15 / 16. 16 rows (1,024, 1,024) 4.0 / 9.4, (4,096, 1,024)
+// 4.2 / 7.1, (1,024, 4,096) 9.3 / 10.0, (8,192, 2,048) 10.0 / 10.0, (50,000, 768) 25 / 16. 32
+// rows (1,024, 1,024) 5.0 / 7.7, (8,192, 1,024) 7.8 / 7.4, (1,024, 4,096) 12.7 / 10.6. (A
+// workgroup's time goes with k and its blocks of rows; 256 of them are 4,096 columns.)
+bool few_rows(int64_t m, int64_t n, int64_t k) {
+  if (m <= 2) return true;
+  if (m <= 4) return n * k <= ((int64_t)1 << 24);
+  return m <= 32 && (m + 15) / 16 * ((n + 4095) / 4096) * k <= 4096;
+}
 
 int few_dense(const TileParams& p, bool gated, bool out_bf16, hipStream_t stream) {
   if (gated) return few_launch<2, true>(p, stream);
@@ -276,7 +404,7 @@ constexpr int MAX_SPLITS = 32;
 struct DensePlan {
   TilePlan y, dx, dw;
   size_t need(const inl_dense_desc& d, bool backward) const {
-    if (!backward) return d.m <= FEW_DENSE_ROWS ? 0 : tile_part_bytes(y, d.m, d.n);
+    if (!backward) return few_rows(d.m, d.n, d.k) ? 0 : tile_part_bytes(y, d.m, d.n);
     Carve c(nullptr);
     if (d.act != INL_ACT_NONE) c.take((size_t)d.m * d.n * 2);
     c.take(colsum_bytes(d.m, d.n));
@@ -286,7 +414,7 @@ struct DensePlan {
 };
 
 int dense_plan(const inl_dense_desc& d, bool backward, DensePlan* p, int* cus) {
-  if (!backward && d.m <= FEW_DENSE_ROWS) return INL_OK;
+  if (!backward && few_rows(d.m, d.n, d.k)) return INL_OK;
   int rc = device_cus(cus);
   if (rc) return rc;
   if (!backward) {
@@ -350,7 +478,7 @@ extern "C" int inl_dense_fwd(const inl_dense_desc* d, const void* x, const void*
   p.ps = s.pre;
   p.act = d->act;
   const bool out16 = d->out_dtype == INL_BF16;
-  if (d->m <= FEW_DENSE_ROWS) return few_dense(p, false, out16, (hipStream_t)stream);
+  if (few_rows(d->m, d->n, d->k)) return few_dense(p, false, out16, (hipStream_t)stream);
   return tile_nt_linear(p, plan.y, out16, (float*)ws, cus, (hipStream_t)stream);
 }
 

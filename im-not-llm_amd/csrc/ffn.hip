@@ -29,16 +29,17 @@ int ffn_check(const inl_gated_ffn_desc* d) {
 constexpr int MAX_SPLITS = 32;
 
 struct FfnPlan {
-  TilePlan h, y, dh, dwd, dx, dwgu;
+  TilePlan h{}, y{}, dh, dwd, dx, dwgu;   // h and y without tiles: splits 0
   int cus = 0;
 };
 int ffn_plan(const inl_gated_ffn_desc& d, bool backward, FfnPlan* p) {
-  if (!backward && d.m <= FEW_DENSE_ROWS) return INL_OK;
+  const bool few_h = few_rows(d.m, d.inner, d.hidden), few_y = few_rows(d.m, d.hidden, d.inner);
+  if (!backward && few_h && few_y) return INL_OK;
   int rc = device_cus(&p->cus);
   if (rc) return rc;
   if (!backward) {
-    p->h = tile_plan(d.m, d.inner, d.hidden, 0, true, MAX_SPLITS, p->cus);
-    p->y = tile_plan(d.m, d.hidden, d.inner, 0, false, MAX_SPLITS, p->cus);
+    if (!few_h) p->h = tile_plan(d.m, d.inner, d.hidden, 0, true, MAX_SPLITS, p->cus);
+    if (!few_y) p->y = tile_plan(d.m, d.hidden, d.inner, 0, false, MAX_SPLITS, p->cus);
     return INL_OK;
   }
   p->dh = tile_plan(d.m, d.inner, d.hidden, 1, false, MAX_SPLITS, p->cus);
@@ -58,7 +59,7 @@ size_t ffn_need(const inl_gated_ffn_desc& d, const FfnPlan& p, bool backward) {
   if (backward)
     c.take(std::max(std::max(tile_part_bytes(p.dh, d.m, d.inner), tile_part_bytes(p.dwd, d.hidden, d.inner)),
                     std::max(tile_part_bytes(p.dx, d.m, d.hidden), tile_part_bytes(p.dwgu, 2 * d.inner, d.hidden))));
-  else if (d.m > FEW_DENSE_ROWS)
+  else
     c.take(std::max(tile_part_bytes(p.h, d.m, 2 * d.inner), tile_part_bytes(p.y, d.m, d.hidden)));
   return c.used;
 }
@@ -103,7 +104,6 @@ extern "C" int inl_gated_ffn_fwd(const inl_gated_ffn_desc* d, const void* x, con
   char* hb = c.take(rows_bytes(*d, false));
   float* part = (float*)c.take(0);
   if (h) hb = (char*)h;
-  const bool few = d->m <= FEW_DENSE_ROWS;
   TileParams p{};
   p.x = (const char*)x;
   p.xs_b = xs * 2;
@@ -118,7 +118,7 @@ extern "C" int inl_gated_ffn_fwd(const inl_gated_ffn_desc* d, const void* x, con
   p.pre = (char*)pre;
   p.ps = 2 * d->inner;
   p.act = d->act;
-  if ((rc = few ? few_dense(p, true, true, st) : tile_nt_gated(p, plan.h, part, plan.cus, st))) return rc;
+  if ((rc = !plan.h.splits ? few_dense(p, true, true, st) : tile_nt_gated(p, plan.h, part, plan.cus, st))) return rc;
   p.x = hb;
   p.xs_b = d->inner * 2;
   p.w = (const char*)w_down;
@@ -133,7 +133,7 @@ extern "C" int inl_gated_ffn_fwd(const inl_gated_ffn_desc* d, const void* x, con
   p.pre = nullptr;
   p.act = ACT_NONE;
   const bool out16 = d->out_dtype == INL_BF16;
-  return few ? few_dense(p, false, out16, st) : tile_nt_linear(p, plan.y, out16, part, plan.cus, st);
+  return !plan.y.splits ? few_dense(p, false, out16, st) : tile_nt_linear(p, plan.y, out16, part, plan.cus, st);
 }
 
 extern "C" int inl_gated_ffn_bwd(const inl_gated_ffn_desc* d, const void* dy, const void* x, const void* w_gate_up,

@@ -30,7 +30,7 @@ def _dense_ref(x, w, b, act, res):
     return z, y, tol
 
 
-# 1 to 8 rows take the few-row kernel; sizes off every tile and off 32; k of many stages
+# 1 to 4 and 5 to 32 rows have kernels of their own; sizes off every tile and off 32; k of many stages
 SIZES = [(1, 8, 8), (2, 264, 72), (3, 72, 1032), (4, 1024, 512), (8, 40, 2048), (9, 8, 8), (64, 64, 64), (65, 136, 40),
          (129, 520, 264), (257, 72, 4104), (1000, 264, 96), (2051, 1032, 520)]
 
@@ -767,3 +767,35 @@ def test_softmax_xent_very_wide(m, cuda, inl):
     """More vocabulary than a piece may be wide with a few rows."""
     test_softmax_xent(m, 2 ** 21 + 4099, 8, 1.0, True, cuda, inl)
     test_softmax_xent_bwd(m, 2 ** 21 + 4099, 8, 1.0, True, cuda, inl)
+
+
+# both sides of the rules that choose a kernel for a few rows
+FEW = [(5, 24, 40), (16, 1000, 1032), (16, 4096, 1024), (16, 4104, 2056), (17, 520, 264), (32, 4104, 72), (31, 264, 2040),
+       (32, 8, 2056), (33, 264, 264), (4, 8200, 2040), (3, 8208, 2056)]
+
+
+@pytest.mark.parametrize("act", [None, "gelu_erf"])
+@pytest.mark.parametrize("m,n,k", FEW)
+def test_dense_few_rows(m, n, k, act, cuda, inl):
+    """With a neighbour on every side that stays as it was."""
+    import torch
+    x, w = _rand(torch, cuda, (m, k + 8), 1)[:, :k], _rand(torch, cuda, (n, k + 16), 2, k ** -0.5)[:, :k]
+    b = _rand(torch, cuda, (n,), 3, 0.5, torch.float32)
+    res = _rand(torch, cuda, (m, n), 4, 1.0, torch.float32 if m % 2 else torch.bfloat16)
+    out = torch.full((m + 2, n + 16), 7.0, dtype=torch.bfloat16 if n % 16 else torch.float32, device=cuda)
+    pre = torch.full((m + 2, n + 8), 7.0, dtype=torch.bfloat16, device=cuda)
+    print(f"case=few {m} {n} {k} act={act}", flush=True)
+    y = inl.dense(x, w, b, act=act, residual=res, pre=pre[1:-1, :n], out=out[1:-1, 8:-8])
+    z, ref, tol = _dense_ref(x, w, b, act, res)
+    R.check(y, ref, tol + R.out_tol(ref, out.dtype), "y")
+    R.check(pre[1:-1, :n], z, tol + R.out_tol(z, torch.bfloat16), "pre")
+    for t, inside in ((out, (slice(1, -1), slice(8, -8))), (pre, (slice(1, -1), slice(0, n)))):
+        t[inside] = 7.0
+        assert (t == 7.0).all()
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("m,hidden,inner", [(5, 40, 24), (16, 1024, 2816), (32, 1024, 4096), (24, 4104, 264), (33, 72, 136)])
+def test_gated_ffn_few_rows(m, hidden, inner, act, cuda, inl):
+    """Either product by either kernel."""
+    test_gated_ffn(m, hidden, inner, act, cuda, inl)
