@@ -8,6 +8,11 @@
 //             dw_down = dy^T . h                       2
 //             dx = [d_gate d_up] . w_gate_up           4
 //             dw_gate_up = [d_gate d_up]^T . x         4
+//
+// 20,011 rows, 768 x 1,152, forward: 110 to 120 us by card (gate and up 73, down 42; 890 to 960
+// TFLOP/s). 16,384 rows, 1,024 x 4,096, backward: 764 to 771 us (1,070); the gate gradients' product
+// stands beside the bytes of its epilogue (98 us of products, 537 MB), the others
+// under the power limit. One row of 1,024 x 2,816: 6.3 us.
 #include "train_ops.hpp"
 
 namespace inl {

@@ -14,7 +14,8 @@ struct FinishParams {
   int64_t quads;   // groups of 4 output columns
 };
 
-// One thread: 4 output columns of one row, the partials added in split order.
+// One thread: 4 output columns of one row, the partials added in split order. Bound by
+// memory (splits 4-byte reads per output).
 template <int EPI, bool OUT16>
 __global__ __launch_bounds__(256) void tile_finish_kernel(FinishParams f) {
   const TileParams& p = f.t;
