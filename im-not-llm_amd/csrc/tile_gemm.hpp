@@ -81,7 +81,7 @@ struct TileParams {
   const float* dl;          // [m]
   float* at;                // [m] the target's score
   float2* part;             // [column block][m] (maximum, sum)
-  int32_t col0;             // vocabulary id of column 0
+  int32_t col0, vocab;      // vocabulary id of column 0, and their number
   int32_t ignore;
   int32_t n_store;          // columns of y, past n zeros (EPI_DXENT)
   // schedule
@@ -569,7 +569,8 @@ __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) voi
           if (t != p.ignore) tcol[b] = t - p.col0;
           if constexpr (EPI == EPI_DXENT) {
             row_lse[b] = p.lse[row];
-            if (t != p.ignore) row_dl[b] = p.dl[row];
+            // (another target outside the vocabulary: NaN in the whole row)
+            if (t != p.ignore) row_dl[b] = (uint32_t)t < (uint32_t)p.vocab ? p.dl[row] : __builtin_nanf("");
           }
         }
       }

@@ -75,15 +75,6 @@ __global__ __launch_bounds__(JOIN_WAVES * 64) void xent_join_kernel(const float2
   loss[row] = t == ignore ? 0.f : (t < 0 || t >= vocab) ? __builtin_nanf("") : (top - at[row]) + logs;
 }
 
-// Rows whose target is neither ignored nor in [0, vocab): their gradient is NaN.
-__global__ __launch_bounds__(256) void xent_dloss_kernel(const float* dl, const int32_t* target, int32_t ignore,
-                                                         int64_t vocab, int64_t m, float* out) {
-  const int64_t i = blockIdx.x * 256LL + threadIdx.x;
-  if (i >= m) return;
-  const int32_t t = target[i];
-  out[i] = t != ignore && (t < 0 || t >= vocab) ? __builtin_nanf("") : dl[i];
-}
-
 constexpr int MAX_SPLITS = 32;
 
 // Vocabulary entries per piece: g of a piece is some 128 MiB, so that dw and dx
@@ -120,7 +111,6 @@ size_t xent_need(const inl_softmax_xent_desc& d, const XentPlan& p, bool backwar
     return c.used;
   }
   c.take((size_t)d.m * (size_t)p.piece * 2);
-  c.take((size_t)d.m * 4);
   c.take((size_t)d.m * (size_t)d.hidden * 4);
   c.take(colsum_bytes(d.m, p.piece));
   c.take(std::max(tile_part_bytes(p.dw, std::min(p.piece, d.vocab), d.hidden), tile_part_bytes(p.dx, d.m, d.hidden)));
@@ -209,13 +199,9 @@ extern "C" int inl_softmax_xent_bwd(const inl_softmax_xent_desc* d, const float*
   if ((rc = check_workspace("softmax_xent", ws, ws_bytes, xent_need(*d, plan, true)))) return rc;
   Carve c(ws);
   char* g = c.take((size_t)d->m * (size_t)plan.piece * 2);
-  float* dl = (float*)c.take((size_t)d->m * 4);
   float* dxf = (float*)c.take((size_t)d->m * (size_t)d->hidden * 4);
   float* sums = (float*)c.take(colsum_bytes(d->m, plan.piece));
   float* part = (float*)c.take(0);
-  hipLaunchKernelGGL(xent_dloss_kernel, dim3((unsigned)((d->m + 255) / 256)), dim3(256), 0, st, dloss, targets,
-                     d->ignore_index, d->vocab, d->m, dl);
-  INL_HIP_TRY(hipGetLastError());
   for (int64_t v0 = 0; v0 < d->vocab; v0 += plan.piece) {
     const int64_t cols = std::min(plan.piece, d->vocab - v0), cols8 = (cols + 7) / 8 * 8;
     const bool last = v0 + cols == d->vocab;
@@ -234,7 +220,8 @@ extern "C" int inl_softmax_xent_bwd(const inl_softmax_xent_desc* d, const float*
     p.ignore = d->ignore_index;
     p.col0 = (int32_t)v0;
     p.lse = lse;
-    p.dl = dl;
+    p.dl = dloss;
+    p.vocab = (int32_t)d->vocab;
     p.y = g;
     p.ys = plan.piece;
     p.n_store = (int32_t)cols8;
