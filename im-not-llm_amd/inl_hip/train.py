@@ -83,21 +83,20 @@ def _at_home(call):
 def _mat(name, t, rows, cols, dtypes, dev):
     """``t`` as rows of a matrix for the library, which sees only a pointer: its
     shape, type and device, and contiguous rows. Returns the row stride."""
-    shape = t.shape
-    if len(shape) != 2 or shape[0] != rows or shape[1] != cols:
-        raise InlError(-1, f"{name}: shape {tuple(shape)}, need {(rows, cols)}")
+    if t.shape != (rows, cols):
+        raise InlError(-1, f"{name}: shape {tuple(t.shape)}, need {(rows, cols)}")
     if t.dtype not in dtypes:
         raise InlError(-1, f"{name}: dtype {t.dtype}, need {' or '.join(str(d) for d in dtypes)}")
     if t.get_device() != dev:
         raise InlError(-1, f"{name}: on {t.device}, need cuda:{dev}")
-    stride = t.stride()
-    if stride[1] != 1 and cols > 1:
+    row, col = t.stride()
+    if col != 1 and cols > 1:
         raise InlError(-1, f"{name}: rows must be contiguous")
     if rows <= 1:
         return cols
-    if stride[0] < cols:   # expanded rows, too: the library reads a stride of 0 as packed
-        raise InlError(-1, f"{name}: rows overlap (strides {stride})")
-    return stride[0]
+    if row < cols:   # expanded rows, too: the library reads a stride of 0 as packed
+        raise InlError(-1, f"{name}: rows overlap (strides {(row, col)})")
+    return row
 
 
 def _matrix(name, t):
@@ -115,7 +114,7 @@ def _packed(name, t, rows, cols, dev):
 def _vec(name, t, n, dtype, dev):
     if t is None:
         return None
-    if t.dtype != dtype or tuple(t.shape) != (n,) or t.get_device() != dev or (n > 1 and t.stride(0) != 1):
+    if t.dtype != dtype or t.shape != (n,) or t.get_device() != dev or (n > 1 and t.stride(0) != 1):
         raise InlError(-1, f"{name}: need contiguous {dtype} [{n}] on cuda:{dev}, got {t.dtype} {tuple(t.shape)} on "
                            f"{t.device}")
     return t.data_ptr()
@@ -173,7 +172,7 @@ def _dense(dev, x, w, bias, act, residual, pre, out, out_dtype, stream):
     xs, ws = _mat("x", x, m, k, _B16, dev), _mat("w", w, n, k, _B16, dev)
     made = None
     if out is None:
-        made = out = torch.empty((m, n), dtype=out_dtype or _BF16, device=dev)
+        made = out = x.new_empty((m, n), dtype=out_dtype)
     ys = _mat("out", out, m, n, _ANY, dev)
     rs = rd = ps = 0
     if residual is not None:
@@ -210,9 +209,9 @@ def _dense_grads(dev, x, dy, w, act, pre, bias_grad, dx_grad, dw_grad, dx_dtype,
         raise InlError(-1, "dense_bwd: an activation needs pre")
     xs, ws, ys = _mat("x", x, m, k, _B16, dev), _mat("w", w, n, k, _B16, dev), _mat("dy", dy, m, n, _B16, dev)
     ps = _mat("pre", pre, m, n, _B16, dev) if pre is not None else 0
-    dx = torch.empty((m, k), dtype=dx_dtype or _BF16, device=dev) if dx_grad else None
-    dw = torch.empty((n, k), dtype=dw_dtype or _BF16, device=dev) if dw_grad else None
-    db = torch.empty(n, dtype=_F32, device=dev) if bias_grad else None
+    dx = x.new_empty((m, k), dtype=dx_dtype) if dx_grad else None
+    dw = x.new_empty((n, k), dtype=dw_dtype) if dw_grad else None
+    db = x.new_empty(n, dtype=_F32) if bias_grad else None
     d = DenseDesc(m, n, k, xs, ws, ys, 0, ps, 0, 0, code, 0, 0, _dtype_code(dx_dtype or _BF16),
                   _dtype_code(dw_dtype or _BF16))
     size = _workspace_bytes("dense", dev, 1, m, n, k, code)
@@ -246,13 +245,13 @@ def _ffn(dev, x, w_gate_up, w_down, act, residual, save, out, out_dtype, stream)
     _packed("w_down", w_down, hidden, inner, dev)
     made = None
     if out is None:
-        made = out = torch.empty((m, hidden), dtype=out_dtype or _BF16, device=dev)
+        made = out = x.new_empty((m, hidden), dtype=out_dtype)
     ys = _mat("out", out, m, hidden, _ANY, dev)
     rs = rd = 0
     if residual is not None:
         rs, rd = _mat("residual", residual, m, hidden, _ANY, dev), _CODE[residual.dtype]
-    pre = torch.empty((m, 2 * inner), dtype=_BF16, device=dev) if save else None
-    h = torch.empty((m, inner), dtype=_BF16, device=dev) if save else None
+    pre = x.new_empty((m, 2 * inner)) if save else None
+    h = x.new_empty((m, inner)) if save else None
     d = GatedFfnDesc(m, hidden, inner, xs, ys, rs, 0, code, _CODE[out.dtype], rd, 0, 0)
     size = _workspace_bytes("gated_ffn", dev, 0, m, hidden, inner, code)
     room = _room(size, dev)
@@ -282,9 +281,9 @@ def _ffn_grads(dev, x, dy, w_gate_up, w_down, pre, h, act, dx_grad, dw_grad, dx_
                                 ("pre", pre, m, 2 * inner), ("h", h, m, inner)):
         _packed(name, t, rows, cols, dev)
     wd = dw_dtype or _BF16
-    dx = torch.empty((m, hidden), dtype=dx_dtype or _BF16, device=dev) if dx_grad else None
-    dgu = torch.empty((2 * inner, hidden), dtype=wd, device=dev) if dw_grad else None
-    ddown = torch.empty((hidden, inner), dtype=wd, device=dev) if dw_grad else None
+    dx = x.new_empty((m, hidden), dtype=dx_dtype) if dx_grad else None
+    dgu = x.new_empty((2 * inner, hidden), dtype=wd) if dw_grad else None
+    ddown = x.new_empty((hidden, inner), dtype=wd) if dw_grad else None
     d = GatedFfnDesc(m, hidden, inner, xs, ys, 0, 0, code, 0, 0, _dtype_code(dx_dtype or _BF16), _dtype_code(wd))
     size = _workspace_bytes("gated_ffn", dev, 1, m, hidden, inner, code)
     room = _room(size, dev)
@@ -323,7 +322,7 @@ def _xent_room(d, dev, backward):
 @_at_home
 def _xent(dev, x, w, targets, bias, scale, ignore_index, stream):
     d = _xent_desc(dev, x, w, scale, ignore_index)
-    loss, lse = torch.empty((2, d.m), dtype=_F32, device=dev).unbind(0)
+    loss, lse = x.new_empty(d.m, dtype=_F32), x.new_empty(d.m, dtype=_F32)
     room, size = _xent_room(d, dev, 0)
     _check(_xent_fwd(d, x.data_ptr(), w.data_ptr(), _vec("bias", bias, d.vocab, _F32, dev),
                      _vec("targets", targets, d.m, torch.int32, dev), loss.data_ptr(), lse.data_ptr(), _ptr(room), size,
@@ -345,9 +344,9 @@ def softmax_xent(x, w, targets, *, bias=None, scale=1.0, ignore_index=-100, stre
 def _xent_grads(dev, x, dloss, lse, w, targets, bias, scale, ignore_index, dx_grad, dw_grad, bias_grad, dx_dtype,
                 dw_dtype, stream):
     d = _xent_desc(dev, x, w, scale, ignore_index, dx_dtype, dw_dtype)
-    dx = torch.empty(x.shape, dtype=dx_dtype or _BF16, device=dev) if dx_grad else None
-    dw = torch.empty(w.shape, dtype=dw_dtype or _BF16, device=dev) if dw_grad else None
-    db = torch.empty(d.vocab, dtype=_F32, device=dev) if bias_grad else None
+    dx = x.new_empty(x.shape, dtype=dx_dtype) if dx_grad else None
+    dw = x.new_empty(w.shape, dtype=dw_dtype) if dw_grad else None
+    db = x.new_empty(d.vocab, dtype=_F32) if bias_grad else None
     room, size = _xent_room(d, dev, 1)
     _check(_xent_bwd(d, _vec("dloss", dloss, d.m, _F32, dev), _vec("lse", lse, d.m, _F32, dev), x.data_ptr(),
                      w.data_ptr(), _vec("bias", bias, d.vocab, _F32, dev),
