@@ -131,7 +131,9 @@ int tile_tn_linear(TileParams p, const TilePlan& plan, bool out_bf16, float* par
 //   (8,192, 1,024, 2,048): 45 / 35 / 58                    (12,000, 768, 768): 24 / 24 / 29
 //   (20,011, 768, 768): 27 / 30 / 46                       (16,384, 2,304, 768): 63 / 60 / 103
 //   (16,384, 4,096, 1,024): 114 / 137 / 226                (2,048, 4,096, 1,024): 29 / 21 / 34
-// Joining s splits: a launch, and the partials written and read.
+// Joining s splits: a launch, a little for each (206 x 184 outputs, k 1,392: 9.3 us with
+// 11, 8.0 with 6; 64 x 1,024, k 4,096: 11.7 with 16, 10.2 with 8), and the partials
+// written and read.
 // An operand by columns costs two reads per fragment, which the smaller shapes
 // feel: `cols` us a stage more for each.
 TilePlan tile_plan(int64_t m, int64_t n, int64_t k, int by_cols, bool gated, int max_splits, int cus) {
@@ -157,7 +159,7 @@ TilePlan tile_plan(int64_t m, int64_t n, int64_t k, int by_cols, bool gated, int
       const float fill = std::min(1.f, (float)units / (float)cus);
       const float stage = c.stage + fill * (c.full - c.stage) + (float)by_cols * c.cols;
       float t = c.start + (float)((units + cus - 1) / cus) * ((float)kper * stage + c.drain);
-      if (s > 1) t += 3.f + (float)m * (float)n * (gated ? 2.f : 1.f) * 8.f * (float)s / 7e6f;
+      if (s > 1) t += 3.f + 0.15f * (float)s + (float)m * (float)n * (gated ? 2.f : 1.f) * 8.f * (float)s / 7e6f;
       if (least < 0.f || t < least) {
         least = t;
         best = {i, s, (int32_t)kper};
