@@ -59,7 +59,8 @@ struct NormRopeParams {
 // are normalised only (a fused q/k/v row: q and k rotated, v not). Every
 // lane of a wave runs the head step the same number of times (the shuffles
 // need all of them).
-template <typename TI, typename TO, int G, int HB>
+// ADJ: adjacent pairs, a kernel of its own (as a branch it cost the others 1 to 4 %).
+template <typename TI, typename TO, int G, int HB, bool ADJ>
 __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeParams p) {
   // G = head_dim / 8 lanes per row (a power of two <= 64)
   const int lane = threadIdx.x & 63;
@@ -110,10 +111,10 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeParams p) {
   // so the exchange runs on DPP / permlane instead of an LDS shuffle.
   int half_lanes = 0;
   bool xor_partner = false;
-  if (p.rotary_dim == 8 && p.sections == 1) {
-    mode = j == 0 ? 1 : 0;
-  } else if (p.sections == INL_ROPE_INTERLEAVED) {
+  if constexpr (ADJ) {
     mode = 8 * j < p.rotary_dim ? 3 : 0;
+  } else if (p.rotary_dim == 8 && p.sections == 1) {
+    mode = j == 0 ? 1 : 0;
   } else if (p.rotary_dim > 0) {
     if (p.sections == 2) {
       sec_lanes = G >> 1;
@@ -136,17 +137,17 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeParams p) {
     bad_pos = mode != 0 && valid && (pos < 0 || pos >= p.table_rows);
     const int64_t posc = pos < 0 ? 0 : (pos >= p.table_rows ? p.table_rows - 1 : pos);
     float tc[8], ts[8];
-    if (p.rotary_dim == 8 && p.sections == 1) {
-      const f32x4 c4 = *reinterpret_cast<const f32x4*>(p.cos + posc * 4);
-      const f32x4 s4 = *reinterpret_cast<const f32x4*>(p.sin + posc * 4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) { tc[e] = c4[e]; ts[e] = s4[e]; tc[e + 4] = 1.f; ts[e + 4] = 0.f; }
-    } else if (p.sections == INL_ROPE_INTERLEAVED) {
+    if constexpr (ADJ) {
       const int64_t at = posc * (p.rotary_dim >> 1) + (mode ? 4 * j : 0);
       const f32x4 c4 = *reinterpret_cast<const f32x4*>(p.cos + at);
       const f32x4 s4 = *reinterpret_cast<const f32x4*>(p.sin + at);
 #pragma unroll
       for (int e = 0; e < 8; ++e) { tc[e] = c4[e >> 1]; ts[e] = s4[e >> 1]; }
+    } else if (p.rotary_dim == 8 && p.sections == 1) {
+      const f32x4 c4 = *reinterpret_cast<const f32x4*>(p.cos + posc * 4);
+      const f32x4 s4 = *reinterpret_cast<const f32x4*>(p.sin + posc * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { tc[e] = c4[e]; ts[e] = s4[e]; tc[e + 4] = 1.f; ts[e + 4] = 0.f; }
     } else {
       const int half_lanes = sec_lanes >> 1;
       const int width = half_lanes * 8;              // table columns
@@ -202,7 +203,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeParams p) {
           v[0][e + 4] = b * c[e] + a * sn[e];
         }
       }
-      if (mode == 3 && rot) {
+      if (ADJ && mode == 3 && rot) {
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
           const float a = v[0][e], b = v[0][e + 1];
@@ -210,7 +211,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeParams p) {
           v[0][e + 1] = b * c[e] + a * sn[e];
         }
       }
-      if (p.rotary_dim > 0 && p.sections != INL_ROPE_INTERLEAVED && !(p.rotary_dim == 8 && p.sections == 1)) {
+      if (!ADJ && p.rotary_dim > 0 && !(p.rotary_dim == 8 && p.sections == 1)) {
         float pv[8];
         if (xor_partner)
           xor_lanes8(v[0], pv, half_lanes, lane);
@@ -322,7 +323,8 @@ int norm_rope_launch_ex(const inl_norm_rope_desc* d, const void* x, void* y, con
   // token), else 4 (8 was slower on 8 and 16 heads of head_dim 128). The
   // fused row of EmbeddingGemma (3 q + 1 k + 1 v heads of 256) takes exactly
   // 5: no repeated loads of its last head, and 16 fewer registers.
-  const int HB = d->heads == 5 && G == 32 ? 5 : (d->heads > 4 && d->heads < 8 ? 8 : 4);
+  const bool adjacent = d->rotary_dim > 0 && d->sections == INL_ROPE_INTERLEAVED;   // (four heads always)
+  const int HB = adjacent ? 4 : d->heads == 5 && G == 32 ? 5 : (d->heads > 4 && d->heads < 8 ? 8 : 4);
   const int64_t groups_per_block = 256 / G;
   const int64_t groups = d->n_tokens * ((d->heads + HB - 1) / HB);   // (token, HB-head chunk)
   if (groups + groups_per_block >= ((int64_t)1 << 31))
@@ -333,21 +335,23 @@ int norm_rope_launch_ex(const inl_norm_rope_desc* d, const void* x, void* y, con
     using TI = decltype(ti);
     using TO = decltype(to);
     const dim3 grid((unsigned)blocks), block(256);
-    auto go = [&](auto hb) {
+    auto go = [&](auto hb, auto adj) {
       constexpr int H = decltype(hb)::value;
+      constexpr bool A = decltype(adj)::value;
       switch (G) {
-        case 1: hipLaunchKernelGGL((norm_rope_kernel<TI, TO, 1, H>), grid, block, 0, st, p); break;
-        case 2: hipLaunchKernelGGL((norm_rope_kernel<TI, TO, 2, H>), grid, block, 0, st, p); break;
-        case 4: hipLaunchKernelGGL((norm_rope_kernel<TI, TO, 4, H>), grid, block, 0, st, p); break;
-        case 8: hipLaunchKernelGGL((norm_rope_kernel<TI, TO, 8, H>), grid, block, 0, st, p); break;
-        case 16: hipLaunchKernelGGL((norm_rope_kernel<TI, TO, 16, H>), grid, block, 0, st, p); break;
-        case 32: hipLaunchKernelGGL((norm_rope_kernel<TI, TO, 32, H>), grid, block, 0, st, p); break;
-        default: hipLaunchKernelGGL((norm_rope_kernel<TI, TO, 64, H>), grid, block, 0, st, p);
+        case 1: hipLaunchKernelGGL((norm_rope_kernel<TI, TO, 1, H, A>), grid, block, 0, st, p); break;
+        case 2: hipLaunchKernelGGL((norm_rope_kernel<TI, TO, 2, H, A>), grid, block, 0, st, p); break;
+        case 4: hipLaunchKernelGGL((norm_rope_kernel<TI, TO, 4, H, A>), grid, block, 0, st, p); break;
+        case 8: hipLaunchKernelGGL((norm_rope_kernel<TI, TO, 8, H, A>), grid, block, 0, st, p); break;
+        case 16: hipLaunchKernelGGL((norm_rope_kernel<TI, TO, 16, H, A>), grid, block, 0, st, p); break;
+        case 32: hipLaunchKernelGGL((norm_rope_kernel<TI, TO, 32, H, A>), grid, block, 0, st, p); break;
+        default: hipLaunchKernelGGL((norm_rope_kernel<TI, TO, 64, H, A>), grid, block, 0, st, p);
       }
     };
-    if (HB == 5) hipLaunchKernelGGL((norm_rope_kernel<TI, TO, 32, 5>), grid, block, 0, st, p);
-    else if (HB == 8) go(std::integral_constant<int, 8>{});
-    else go(std::integral_constant<int, 4>{});
+    if (adjacent) go(std::integral_constant<int, 4>{}, std::true_type{});
+    else if (HB == 5) hipLaunchKernelGGL((norm_rope_kernel<TI, TO, 32, 5, false>), grid, block, 0, st, p);
+    else if (HB == 8) go(std::integral_constant<int, 8>{}, std::false_type{});
+    else go(std::integral_constant<int, 4>{}, std::false_type{});
   };
   if (d->dtype == INL_BF16 && d->out_dtype == INL_BF16) launch(bf16{}, bf16{});
   else if (d->dtype == INL_BF16) launch(bf16{}, float{});
