@@ -1105,5 +1105,6 @@ def unit_lower_inverse(a, *, stream=None):
 # Layer and head ops with their gradients (include/inl_train.h)
 # ---------------------------------------------------------------------------
 
-from .train import (ROPE_AXIAL, ROPE_HALF, ROPE_INTERLEAVED, dense, dense_bwd, gated_ffn,  # noqa: E402,F401
-                    gated_ffn_bwd, norm_rope_qk_bwd, softmax_xent, softmax_xent_bwd)
+if "torch" in globals():   # the rest of the package does without it
+    from .train import (ROPE_AXIAL, ROPE_HALF, ROPE_INTERLEAVED, dense, dense_bwd, gated_ffn,  # noqa: E402,F401
+                        gated_ffn_bwd, norm_rope_qk_bwd, softmax_xent, softmax_xent_bwd)

@@ -140,3 +140,14 @@ def test_adjacent_pairs_refusals():
     for rd in (4, 12, 72):
         d.rotary_dim = rd
         assert inl_hip._norm_rope(d, P, P, None, P, P, P, None, None, None) == -2
+
+
+def test_package_imports_without_torch():
+    """The layer ops need torch; the host-side entries of the package do not."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    pkg = Path(__file__).resolve().parents[1] / "im-not-llm_amd"
+    code = (f"import sys; sys.modules['torch'] = None; sys.path.insert(0, {str(pkg)!r}); import inl_hip; "
+            "assert inl_hip.library_path().exists() and not hasattr(inl_hip, 'dense')")
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=120)
