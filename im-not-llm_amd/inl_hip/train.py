@@ -5,7 +5,10 @@ cross entropy without its scores, and the gradients of the q/k prologue.
 Gradients are plain functions of what the forward left (no autograd graph is
 kept): a ``torch.autograd.Function`` or a training loop calls them in its own
 backward. Outputs and workspaces come from torch's allocator, so calls can be
-captured into a graph.
+captured into a graph. With ``stream=`` a call works there and takes its memory there;
+that its inputs are ready on that stream, and that their memory is not handed on
+before it is done (``record_stream``), is up to the caller, as it is that the current
+stream waits before it uses the outputs.
 """
 from __future__ import annotations
 
@@ -66,17 +69,31 @@ _CODE = {_BF16: INL_BF16, _F32: INL_F32}
 
 
 def _at_home(call):
-    """Runs ``call`` with the device of its first tensor as the current one: the
-    library launches there, and workspaces and outputs belong there."""
+    """Runs ``call(device, first, *args)`` with the device of its first tensor as the
+    current one and ``stream`` (the last argument; None: the current one) as the
+    current stream: the library launches there, and workspaces and outputs come from
+    that stream's memory. A block of another stream's could still be in use by work
+    queued there, which ``stream`` does not wait for."""
     @functools.wraps(call)
-    def wrapped(first, *args, **kwargs):
+    def wrapped(first, *args):
+        *args, stream = args
         dev = first.get_device()
         if dev < 0:
             raise InlError(-1, f"not a device tensor ({first.device})")
+        if stream is not None:
+            callers = torch.cuda.current_stream(dev)
+            if stream != callers:
+                with torch.cuda.stream(stream):
+                    made = call(dev, first, *args)
+                # the caller goes on with them on its own stream, once that has waited
+                for t in made if isinstance(made, tuple) else (made,):
+                    if t is not None:
+                        t.record_stream(callers)
+                return made
         if dev == torch._C._cuda_getDevice():
-            return call(dev, first, *args, **kwargs)
+            return call(dev, first, *args)
         with torch.cuda.device(dev):
-            return call(dev, first, *args, **kwargs)
+            return call(dev, first, *args)
     return wrapped
 
 
@@ -142,18 +159,8 @@ def _room(n, dev):
     return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
 
 
-def _stream(stream, dev):
-    return torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
-
-
-def _done(stream, *tensors):
-    """Tensors allocated here that work on another stream than the current one
-    uses: the allocator must not hand their memory out before it is done."""
-    if stream is None or stream == torch.cuda.current_stream():
-        return
-    for t in tensors:
-        if t is not None:
-            t.record_stream(stream)
+def _stream(dev):
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _ptr(t):
@@ -165,14 +172,13 @@ def _ptr(t):
 # ---------------------------------------------------------------------------
 
 @_at_home
-def _dense(dev, x, w, bias, act, residual, pre, out, out_dtype, stream):
+def _dense(dev, x, w, bias, act, residual, pre, out, out_dtype):
     m, k = _matrix("x", x)
     n = _matrix("w", w)[0]
     code = _act(act)
     xs, ws = _mat("x", x, m, k, _B16, dev), _mat("w", w, n, k, _B16, dev)
-    made = None
     if out is None:
-        made = out = x.new_empty((m, n), dtype=out_dtype)
+        out = x.new_empty((m, n), dtype=out_dtype)
     ys = _mat("out", out, m, n, _ANY, dev)
     rs = rd = ps = 0
     if residual is not None:
@@ -184,8 +190,7 @@ def _dense(dev, x, w, bias, act, residual, pre, out, out_dtype, stream):
     size = _workspace_bytes("dense", dev, 0, m, n, k, code)
     room = _room(size, dev)
     _check(_dense_fwd(d, x.data_ptr(), w.data_ptr(), bp, _ptr(residual), out.data_ptr(), _ptr(pre), _ptr(room), size,
-                      _stream(stream, dev)))
-    _done(stream, room, made)
+                      _stream(dev)))
     return out
 
 
@@ -199,7 +204,7 @@ def dense(x, w, bias=None, *, act=None, residual=None, pre=None, out=None, out_d
 
 
 @_at_home
-def _dense_grads(dev, x, dy, w, act, pre, bias_grad, dx_grad, dw_grad, dx_dtype, dw_dtype, stream):
+def _dense_grads(dev, x, dy, w, act, pre, bias_grad, dx_grad, dw_grad, dx_dtype, dw_dtype):
     m, k = _matrix("x", x)
     n = _matrix("w", w)[0]
     code = _act(act)
@@ -217,8 +222,7 @@ def _dense_grads(dev, x, dy, w, act, pre, bias_grad, dx_grad, dw_grad, dx_dtype,
     size = _workspace_bytes("dense", dev, 1, m, n, k, code)
     room = _room(size, dev)
     _check(_dense_bwd(d, dy.data_ptr(), x.data_ptr(), w.data_ptr(), _ptr(pre), _ptr(dx), _ptr(dw), _ptr(db),
-                      _ptr(room), size, _stream(stream, dev)))
-    _done(stream, room, dx, dw, db)
+                      _ptr(room), size, _stream(dev)))
     return dx, dw, db
 
 
@@ -236,16 +240,15 @@ def dense_bwd(dy, x, w, *, act=None, pre=None, bias_grad=False, dx_grad=True, dw
 # ---------------------------------------------------------------------------
 
 @_at_home
-def _ffn(dev, x, w_gate_up, w_down, act, residual, save, out, out_dtype, stream):
+def _ffn(dev, x, w_gate_up, w_down, act, residual, save, out, out_dtype):
     m, hidden = _matrix("x", x)
     inner = _matrix("w_down", w_down)[1]
     code = _act(act, True)
     xs = _mat("x", x, m, hidden, _B16, dev)
     _packed("w_gate_up", w_gate_up, 2 * inner, hidden, dev)
     _packed("w_down", w_down, hidden, inner, dev)
-    made = None
     if out is None:
-        made = out = x.new_empty((m, hidden), dtype=out_dtype)
+        out = x.new_empty((m, hidden), dtype=out_dtype)
     ys = _mat("out", out, m, hidden, _ANY, dev)
     rs = rd = 0
     if residual is not None:
@@ -256,8 +259,7 @@ def _ffn(dev, x, w_gate_up, w_down, act, residual, save, out, out_dtype, stream)
     size = _workspace_bytes("gated_ffn", dev, 0, m, hidden, inner, code)
     room = _room(size, dev)
     _check(_ffn_fwd(d, x.data_ptr(), w_gate_up.data_ptr(), w_down.data_ptr(), _ptr(residual), out.data_ptr(),
-                    _ptr(pre), _ptr(h), _ptr(room), size, _stream(stream, dev)))
-    _done(stream, room, pre, h, made)
+                    _ptr(pre), _ptr(h), _ptr(room), size, _stream(dev)))
     return (out, pre, h) if save else out
 
 
@@ -272,7 +274,7 @@ def gated_ffn(x, w_gate_up, w_down, *, act="silu", residual=None, save=False, ou
 
 
 @_at_home
-def _ffn_grads(dev, x, dy, w_gate_up, w_down, pre, h, act, dx_grad, dw_grad, dx_dtype, dw_dtype, stream):
+def _ffn_grads(dev, x, dy, w_gate_up, w_down, pre, h, act, dx_grad, dw_grad, dx_dtype, dw_dtype):
     m, hidden = _matrix("x", x)
     inner = _matrix("w_down", w_down)[1]
     code = _act(act, True)
@@ -288,8 +290,7 @@ def _ffn_grads(dev, x, dy, w_gate_up, w_down, pre, h, act, dx_grad, dw_grad, dx_
     size = _workspace_bytes("gated_ffn", dev, 1, m, hidden, inner, code)
     room = _room(size, dev)
     _check(_ffn_bwd(d, dy.data_ptr(), x.data_ptr(), w_gate_up.data_ptr(), w_down.data_ptr(), pre.data_ptr(),
-                    h.data_ptr(), _ptr(dx), _ptr(dgu), _ptr(ddown), _ptr(room), size, _stream(stream, dev)))
-    _done(stream, room, dx, dgu, ddown)
+                    h.data_ptr(), _ptr(dx), _ptr(dgu), _ptr(ddown), _ptr(room), size, _stream(dev)))
     return dx, dgu, ddown
 
 
@@ -320,14 +321,13 @@ def _xent_room(d, dev, backward):
 
 
 @_at_home
-def _xent(dev, x, w, targets, bias, scale, ignore_index, stream):
+def _xent(dev, x, w, targets, bias, scale, ignore_index):
     d = _xent_desc(dev, x, w, scale, ignore_index)
     loss, lse = x.new_empty(d.m, dtype=_F32), x.new_empty(d.m, dtype=_F32)
     room, size = _xent_room(d, dev, 0)
     _check(_xent_fwd(d, x.data_ptr(), w.data_ptr(), _vec("bias", bias, d.vocab, _F32, dev),
                      _vec("targets", targets, d.m, torch.int32, dev), loss.data_ptr(), lse.data_ptr(), _ptr(room), size,
-                     _stream(stream, dev)))
-    _done(stream, room, loss, lse)
+                     _stream(dev)))
     return loss, lse
 
 
@@ -342,7 +342,7 @@ def softmax_xent(x, w, targets, *, bias=None, scale=1.0, ignore_index=-100, stre
 
 @_at_home
 def _xent_grads(dev, x, dloss, lse, w, targets, bias, scale, ignore_index, dx_grad, dw_grad, bias_grad, dx_dtype,
-                dw_dtype, stream):
+                dw_dtype):
     d = _xent_desc(dev, x, w, scale, ignore_index, dx_dtype, dw_dtype)
     dx = x.new_empty(x.shape, dtype=dx_dtype) if dx_grad else None
     dw = x.new_empty(w.shape, dtype=dw_dtype) if dw_grad else None
@@ -351,8 +351,7 @@ def _xent_grads(dev, x, dloss, lse, w, targets, bias, scale, ignore_index, dx_gr
     _check(_xent_bwd(d, _vec("dloss", dloss, d.m, _F32, dev), _vec("lse", lse, d.m, _F32, dev), x.data_ptr(),
                      w.data_ptr(), _vec("bias", bias, d.vocab, _F32, dev),
                      _vec("targets", targets, d.m, torch.int32, dev), _ptr(dx), _ptr(dw), _ptr(db), _ptr(room), size,
-                     _stream(stream, dev)))
-    _done(stream, room, dx, dw, db)
+                     _stream(dev)))
     return dx, dw, db
 
 
@@ -385,7 +384,7 @@ def _heads(name, t, shape, dev):
 
 @_at_home
 def _rope_grads(dev, x, dy, q_heads, rows, cos, sin, q_weight, k_weight, eps, norm, rotary_dim, sections, cos2, sin2,
-                round_tables, out, weight_grad, stream):
+                round_tables, out, weight_grad):
     shape = tuple(x.shape)
     if len(shape) != 3:
         raise InlError(-1, f"x: shape {shape}, need [tokens, heads, head_dim]")
@@ -408,9 +407,8 @@ def _rope_grads(dev, x, dy, q_heads, rows, cos, sin, q_weight, k_weight, eps, no
                     or t.get_device() != dev:
                 raise InlError(-1, f"{name}: need contiguous f32 [{d.table_rows}, {width}] on cuda:{dev}")
         _vec("rows", rows, n, torch.int32, dev)
-    made = None
     if out is None:
-        made = out = torch.empty(shape, dtype=x.dtype, device=dev)
+        out = torch.empty(shape, dtype=x.dtype, device=dev)
     elif out.dtype != x.dtype:
         raise InlError(-1, f"out: dtype {out.dtype}, need {x.dtype}")
     ds = _heads("out", out, shape, dev)
@@ -424,8 +422,7 @@ def _rope_grads(dev, x, dy, q_heads, rows, cos, sin, q_weight, k_weight, eps, no
     _check(_rope_bwd(d, int(q_heads), dy.data_ptr(), x.data_ptr(), out.data_ptr(), ds,
                      _vec("q_weight", q_weight, hd, x.dtype, dev), _vec("k_weight", k_weight, hd, x.dtype, dev),
                      _ptr(rows), _ptr(cos), _ptr(sin), _ptr(cos2), _ptr(sin2), _ptr(dq), _ptr(dk), _ptr(room),
-                     size.value, _stream(stream, dev)))
-    _done(stream, room, dq, dk, made)
+                     size.value, _stream(dev)))
     return out, dq, dk
 
 
