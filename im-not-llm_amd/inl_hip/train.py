@@ -81,6 +81,8 @@ def _at_home(call):
         if dev < 0:
             raise InlError(-1, f"not a device tensor ({first.device})")
         if stream is not None:
+            if stream.device.index != dev:   # a launch there would use this device's addresses
+                raise InlError(-1, f"the stream is on {stream.device}, the tensors on cuda:{dev}")
             callers = torch.cuda.current_stream(dev)
             if stream != callers:
                 with torch.cuda.stream(stream):

@@ -151,3 +151,19 @@ def test_package_imports_without_torch():
     code = (f"import sys; sys.modules['torch'] = None; sys.path.insert(0, {str(pkg)!r}); import inl_hip; "
             "assert inl_hip.library_path().exists() and not hasattr(inl_hip, 'dense')")
     subprocess.run([sys.executable, "-c", code], check=True, timeout=120)
+
+
+def test_stream_of_another_device(T):
+    """Refused before anything is allocated or launched."""
+    import types
+
+    import inl_hip
+    import torch
+    x = types.SimpleNamespace(get_device=lambda: 0)
+    s = types.SimpleNamespace(device=torch.device("cuda", 1), cuda_stream=P)
+    for call in (lambda: T.dense(x, x, stream=s), lambda: T.dense_bwd(x, x, x, stream=s),
+                 lambda: T.gated_ffn(x, x, x, stream=s), lambda: T.gated_ffn_bwd(x, x, x, x, x, x, stream=s),
+                 lambda: T.softmax_xent(x, x, x, stream=s), lambda: T.softmax_xent_bwd(x, x, x, x, x, stream=s),
+                 lambda: T.norm_rope_qk_bwd(x, x, 1, stream=s)):
+        with pytest.raises(inl_hip.InlError, match="the stream is on cuda:1"):
+            call()
