@@ -605,7 +605,7 @@ __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) voi
                 *reinterpret_cast<bf16x4*>(p.pre + (row * p.ps + col) * 2) = o;
               }
             }
-            z = act_apply4(p.act, z);
+            if constexpr (LW == OP_ROWS) z = act_apply4(p.act, z);
           }
           lds_store<u32x4>(meet_at(er, a * 4 + (el >> 4)), __builtin_bit_cast(u32x4, z));
         }
@@ -764,7 +764,7 @@ __global__ __launch_bounds__(TileShapeOf<SH>::NW * 64, TileShapeOf<SH>::WPC) voi
                 for (int b = 0; b < 2; ++b) put16(b * 16 + er, a * 16 + ec, z[a][b]);
               flush16(p.pre, p.ps, row0, col0, PER * 16, p.n);
             }
-            if (p.act != ACT_NONE) {
+            if (LW == OP_ROWS && p.act != ACT_NONE) {   // (the gradients' products have none)
 #pragma unroll
               for (int a = 0; a < PER; ++a)
 #pragma unroll

@@ -57,3 +57,48 @@ def test_memory_of_a_call_on_another_stream(op, cuda, inl):
         assert not any(lo < t.data_ptr() + t.numel() * t.element_size() and t.data_ptr() < hi for lo, hi in spans)
     assert all((t == 7).all() for t in seen)
     assert all(torch.equal(u, v) for u, v in zip(got, want))
+
+
+# row kernels, one per block of 16 columns, tiles of the three shapes, a split sum
+@pytest.mark.parametrize("m,k", [(1, 8), (4, 40), (16, 72), (64, 72), (300, 2056), (5000, 72), (9000, 72)])
+def test_gelu_erf_keeps_its_tail(m, k, cuda, inl):
+    """v Phi(v) and its slope for v from -8 to 8 by their own size: the tail Phi(-|v|) is
+    within 3e-4 of itself and 4e-7 of 1, and nothing cancels where it stands alone.
+    An identity for weights makes v an input exactly."""
+    import torch
+    n = 1024 if m > 4000 else 264
+    v = torch.linspace(-8, 8, n * 4, device=cuda).to(torch.bfloat16)
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device=cuda)
+    x[:, 5] = 1
+    w = torch.zeros(4 * n, k, dtype=torch.bfloat16, device=cuda)
+    w[:, 5] = v
+    print(f"case=gelu tail {m} {k}", flush=True)
+    d = v.double()
+    tail = torch.special.erfc(d.abs() / 2 ** 0.5) / 2
+    ref = torch.where(d < 0, d * tail, d * (1 - tail))
+    # v Phi(v): the tail's error times v, two roundings
+    tol = torch.where(d < 0, 3e-4 * ref.abs(), d.abs() * torch.minimum(3e-4 * tail, torch.full_like(tail, 4e-7))) + 2.0 ** -22 * ref.abs()
+    for i in range(4):
+        y = inl.dense(x, w[i * n:(i + 1) * n], act="gelu_erf", out_dtype=torch.float32)
+        s = slice(i * n, (i + 1) * n)
+        R.check(y, ref[s].expand(m, n), tol[s].expand(m, n), "y")
+    # one row's bias gradient is its slope, Phi(v) + v phi(v)
+    dens = d * torch.exp(-d * d / 2) / (2 * torch.pi) ** 0.5
+    got = inl.dense_bwd(torch.ones(1, 4 * n, dtype=torch.bfloat16, device=cuda), x[:1], w, act="gelu_erf", pre=v[None, :],
+                        bias_grad=True, dx_grad=False, dw_grad=False)[2]
+    ref = torch.where(d < 0, tail, 1 - tail) + dens
+    # (the exponent of the density, up to 47 in base 2, is off by 3 f32 steps of itself)
+    R.check(got, ref, torch.minimum(3e-4 * tail, torch.full_like(tail, 4e-7)) + 2.0 ** -17 * dens.abs() + 2.0 ** -22 * ref.abs(), "slope")
+
+
+def test_gelu_erf_far_values(cuda, inl):
+    import torch
+    v = torch.tensor([1e4, 3e38, float("inf"), -20, -1e4, -3e38, float("nan"), 0], device=cuda).to(torch.bfloat16)
+    for m in (1, 16, 70):
+        x = torch.ones(m, 8, dtype=torch.bfloat16, device=cuda)
+        x[:, 1:] = 0
+        w = torch.zeros(8, 8, dtype=torch.bfloat16, device=cuda)
+        w[:, 0] = v
+        y = inl.dense(x, w, act="gelu_erf", out_dtype=torch.float32)
+        assert torch.equal(y[:, :3], v[:3].float().expand(m, 3)) and not y[:, 3:6].any() and not y[:, 7].any()
+        assert torch.isnan(y[:, 6]).all()
