@@ -89,9 +89,11 @@ __device__ __forceinline__ ActPair act_pair(int32_t act, float v) {
       return {v * s, s * __builtin_fmaf(v, 1.0f - s, 1.0f)};
     }
     case ACT_GELU_TANH: {
-      const float s = act_gelu_gate(v);
-      const float d = __builtin_fmaf(v * v, 0.214064449f, 1.59576912f);   // d(2u) / dv
-      return {v * s, s * __builtin_fmaf(v * (1.0f - s), d, 1.0f)};
+      // (past 16, where s is 0 or 1, the square would leave the range before v does; the
+      // median drops NaN, which s carries)
+      const float s = act_gelu_gate(v), w = __builtin_amdgcn_fmed3f(v, -16.0f, 16.0f);
+      const float d = __builtin_fmaf(w * w, 0.214064449f, 1.59576912f);   // d(2u) / dv
+      return {v * s, s * __builtin_fmaf(w * (1.0f - s), d, 1.0f)};
     }
     case ACT_GELU_ERF: {
       const float q = __builtin_amdgcn_exp2f(-0.721347520444482f * v * v);

@@ -102,3 +102,28 @@ def test_gelu_erf_far_values(cuda, inl):
         y = inl.dense(x, w, act="gelu_erf", out_dtype=torch.float32)
         assert torch.equal(y[:, :3], v[:3].float().expand(m, 3)) and not y[:, 3:6].any() and not y[:, 7].any()
         assert torch.isnan(y[:, 6]).all()
+
+
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu_tanh", "gelu_erf"])
+def test_slopes_of_far_values(act, cuda, inl):
+    """Slopes of activations far out are 0 and 1, also where v^2 or v^3 leaves the range of
+    f32, and NaN stays NaN; in the element-wise pass and in the products' epilogues."""
+    import torch
+    far = torch.tensor([20, 1e3, 1e12, 1e14, 1e18, 1e20, 1e30, 3e38], device=cuda)
+    pre = torch.cat([far, -far, torch.full_like(far, float("nan"))]).to(torch.bfloat16)[None, :]
+    ones = torch.ones(1, 24, dtype=torch.bfloat16, device=cuda)
+    x, w = torch.zeros(1, 8, dtype=torch.bfloat16, device=cuda), torch.zeros(24, 8, dtype=torch.bfloat16, device=cuda)
+    db = inl.dense_bwd(ones, x, w, act=act, pre=pre, bias_grad=True)[2]
+    assert (db[:8] == 1).all() and (db[8:16].abs() <= 1e-7).all() and torch.isnan(db[16:]).all()
+    # d_gate = dh up act'(gate) with dh = dy; dx of w_gate = identity is d_gate
+    for m in (1, 300):
+        gate = pre[:, :16].expand(m, 16)
+        gu = torch.cat([gate, torch.ones_like(gate)], 1).contiguous()
+        w_gu = torch.cat([torch.eye(16, device=cuda), torch.zeros(16, 16, device=cuda)]).to(torch.bfloat16)
+        down = torch.zeros(16, 16, dtype=torch.bfloat16, device=cuda)
+        down[0] = 1
+        dy = torch.zeros(m, 16, dtype=torch.bfloat16, device=cuda)
+        dy[:, 0] = 2.0 ** -20   # d_up = dh act(gate) stays in the range
+        h = torch.zeros(m, 16, dtype=torch.bfloat16, device=cuda)
+        dx, _, _ = inl.gated_ffn_bwd(dy, x.new_zeros(m, 16), w_gu, down, gu, h, act=act, dx_dtype=torch.float32)
+        assert (dx[:, :8] == 2.0 ** -20).all() and (dx[:, 8:].abs() <= 1e-7 * 2.0 ** -20).all(), m
