@@ -176,10 +176,9 @@ def _cu_array(cu_seqlens: Sequence[int]):
 
 
 def _dtype_code(t) -> int:
-    import torch
-    if t == torch.bfloat16:
+    if t is torch.bfloat16:   # (one object per type)
         return INL_BF16
-    if t == torch.float32:
+    if t is torch.float32:
         return INL_F32
     raise InlError(-1, f"unsupported dtype {t}")
 
@@ -432,31 +431,135 @@ def positions(cu_seqlens):
     return out
 
 
+def _head_rows(name, t, shape, dev):
+    """The stride between the token rows of ``t [tokens, heads, head_dim]``, whose
+    heads the kernels take as contiguous."""
+    if t.shape != shape or t.get_device() != dev:
+        raise InlError(-1, f"{name}: shape {tuple(t.shape)} on {t.device}, need {tuple(shape)} on cuda:{dev}")
+    return _token_stride(name, t.stride(), *shape)
+
+
+def _token_stride(name, stride, n, heads, hd):
+    row, head, one = stride
+    if one != 1 or (head != hd and heads > 1):
+        raise InlError(-1, f"{name}: heads must be contiguous inside a token row")
+    if n <= 1:
+        return heads * hd
+    if row < heads * hd:
+        raise InlError(-1, f"{name}: token rows overlap (strides {stride})")
+    return row
+
+
+def _rope_tables(n, rows, rotary_dim, head_dim, sections, cos, sin, cos2, sin2, dev):
+    """Checks ``rows`` and the tables of a rotation, of which the library gets
+    addresses only. Returns the number of table rows."""
+    f32, shape = torch.float32, None if cos is None else cos.shape
+    width = head_dim // 4 if sections == 2 else rotary_dim // 2
+    # (the usual forms first, in as few calls as will do; short batches wait for these)
+    if shape is None or len(shape) != 2 or shape[1] != width or cos.dtype is not f32 or not cos.is_contiguous() \
+            or cos.get_device() != dev:
+        _table("cos", cos, 0, width, dev)
+    if sin is None or sin.shape != shape or sin.dtype is not f32 or not sin.is_contiguous() or sin.get_device() != dev:
+        _table("sin", sin, shape[0], width, dev)
+    if sections == 2:
+        _table("cos2", cos2, shape[0], width, dev)
+        _table("sin2", sin2, shape[0], width, dev)
+    if rows is None or rows.dtype is not torch.int32 or rows.get_device() != dev or rows.numel() < n \
+            or not rows.is_contiguous():
+        raise InlError(-1, f"rows: need contiguous int32 [{n}] on cuda:{dev}"
+                           + ("" if rows is None else f", got {rows.dtype} {tuple(rows.shape)} on {rows.device}"))
+    return shape[0]
+
+
+def _table(name, t, table_rows, width, dev):
+    """Rows of ``width`` values behind one another, ``table_rows`` of them or more."""
+    if t is None or t.dtype != torch.float32 or t.get_device() != dev or t.dim() < 2 or t.shape[0] < table_rows \
+            or t.numel() != t.shape[0] * width or not t.is_contiguous():
+        raise InlError(-1, f"{name}: need contiguous f32 [{table_rows or 'T'}, {width}] on cuda:{dev}"
+                           + ("" if t is None else f", got {t.dtype} {tuple(t.shape)} on {t.device}"))
+
+
+def _bad_weight(name, t, like, hd, dev):
+    raise InlError(-1, f"{name}: need contiguous {like} [{hd}] on cuda:{dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _prologue(entry, x, q_heads, w, w2, rows, cos, sin, eps, norm, rotary_dim, sections, cos2, sin2, out, out_dtype,
+              round_tables, round_norm, stream):
+    """``entry(desc, x, out, weights ..)``, or with ``q_heads`` the q/k form's, once
+    everything that it will read and write is known to be there."""
+    shape, dtype, dev = x.shape, x.dtype, x.get_device()
+    if len(shape) != 3:
+        raise InlError(-1, f"x: shape {tuple(shape)}, need [tokens, heads, head_dim]")
+    if dev < 0:
+        raise InlError(-1, f"x: not a device tensor ({x.device})")
+    if stream is not None and stream.device.index != dev:   # a launch there would use this device's addresses
+        raise InlError(-1, f"the stream is on {stream.device}, the tensors on cuda:{dev}")
+    n, heads, hd = shape
+    code = out_code = _dtype_code(dtype)
+    x_row = _token_stride("x", x.stride(), n, heads, hd)
+    if out is None:
+        if out_dtype is None:
+            out_dtype = dtype
+        else:
+            out_code = _dtype_code(out_dtype)
+        out = torch.empty_like(x, dtype=out_dtype) if stream is None else _new_on(stream, x, out_dtype)
+        out_row = heads * hd
+    else:
+        out_row, out_code = _head_rows("out", out, shape, dev), _dtype_code(out.dtype)
+    if rotary_dim is None:
+        rotary_dim = 0 if cos is None else hd
+    table_rows = 0
+    wp = wp2 = rp = cp = sp = cp2 = sp2 = None   # (tables without a rotation are not looked at)
+    if rotary_dim > 0:
+        table_rows = _rope_tables(n, rows, rotary_dim, hd, sections, cos, sin, cos2, sin2, dev)
+        rp, cp, sp = rows.data_ptr(), cos.data_ptr(), sin.data_ptr()
+        if sections == 2:
+            cp2, sp2 = cos2.data_ptr(), sin2.data_ptr()
+    if norm:
+        if w is not None:
+            if w.dtype is not dtype or w.numel() != hd or w.get_device() != dev or not w.is_contiguous():
+                _bad_weight("weight" if q_heads is None else "q_weight", w, dtype, hd, dev)
+            wp = w.data_ptr()
+        if w2 is not None:
+            if w2.dtype is not dtype or w2.numel() != hd or w2.get_device() != dev or not w2.is_contiguous():
+                _bad_weight("k_weight", w2, dtype, hd, dev)
+            wp2 = w2.data_ptr()
+    d = NormRopeDesc(n, heads, hd, x_row, out_row, code, out_code, bool(norm), float(eps),
+                     int(rotary_dim), int(sections), table_rows, bool(round_tables), bool(round_norm))
+    at = torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
+    args = (d, x.data_ptr(), out.data_ptr(), wp) if q_heads is None else (d, q_heads, x.data_ptr(), out.data_ptr(), wp, wp2)
+    if dev == torch._C._cuda_getDevice():
+        rc = entry(*args, rp, cp, sp, cp2, sp2, at)
+    else:
+        with torch.cuda.device(dev):
+            rc = entry(*args, rp, cp, sp, cp2, sp2, at)
+    if rc:
+        _check(rc)
+    return out
+
+
+def _new_on(stream, like, dtype):
+    """A packed output like ``like`` of a call that works on ``stream``, from that
+    stream's memory: a block of another's could still be in use by work queued there."""
+    callers = torch.cuda.current_stream(like.device)
+    if stream == callers:
+        return torch.empty_like(like, dtype=dtype)
+    with torch.cuda.stream(stream):
+        out = torch.empty_like(like, dtype=dtype)
+    out.record_stream(callers)   # the caller goes on with it there, once it has waited
+    return out
+
+
 def norm_rope(x, rows=None, cos=None, sin=None, *, weight=None, eps=1e-6, norm=True,
               rotary_dim=None, sections=1, cos2=None, sin2=None, out=None, out_dtype=None,
               round_tables=False, round_norm=False, stream=None):
     """Fused per-head RMSNorm + RoPE over ``x [N, heads, head_dim]`` (torch
     device tensor; token rows may be strided). ``rows`` (int32 device [N]) is
-    the table row of each token; ``cos``/``sin`` are f32 device tables.
-    ``rotary_dim=0`` (or no tables) skips the rope."""
-    import torch
-    n, heads, hd = x.shape
-    od = out_dtype if out_dtype is not None else x.dtype
-    if out is None:
-        out = torch.empty((n, heads, hd), dtype=od, device=x.device)
-    rd = (hd if cos is not None else 0) if rotary_dim is None else rotary_dim
-    d = NormRopeDesc()
-    d.n_tokens, d.heads, d.head_dim = n, heads, hd
-    d.x_row_stride, d.y_row_stride = x.stride(0), out.stride(0)
-    d.dtype, d.out_dtype = _dtype_code(x.dtype), _dtype_code(out.dtype)
-    d.norm, d.eps = int(bool(norm)), float(eps)
-    d.rotary_dim, d.sections = int(rd), int(sections)
-    d.table_rows = int(cos.shape[0]) if cos is not None else 0
-    d.round_tables, d.round_norm = int(bool(round_tables)), int(bool(round_norm))
-    ptr = lambda t: t.data_ptr() if t is not None else None
-    _check(_norm_rope(ctypes.byref(d), x.data_ptr(), out.data_ptr(), ptr(weight), ptr(rows),
-                      ptr(cos), ptr(sin), ptr(cos2), ptr(sin2), _stream_ptr(stream)))
-    return out
+    the table row of each token; ``cos``/``sin`` are f32 device tables ``[T, rotary_dim / 2]``
+    (axial, ``sections=2``: all four ``[T, head_dim / 4]``), one column per pair also where pairs are
+    adjacent (``sections=3``). ``weight`` has x's dtype. ``rotary_dim=0`` (or no tables) skips the rope."""
+    return _prologue(_norm_rope, x, None, weight, None, rows, cos, sin, eps, norm, rotary_dim, sections, cos2, sin2, out,
+                     out_dtype, round_tables, round_norm, stream)
 
 
 def norm_rope_qk(x, q_heads, rows=None, cos=None, sin=None, *, q_weight=None, k_weight=None, eps=1e-6,
@@ -465,25 +568,8 @@ def norm_rope_qk(x, q_heads, rows=None, cos=None, sin=None, *, q_weight=None, k_
     """norm_rope over the q heads (``x[:, :q_heads]``, ``q_weight``) and k
     heads (``x[:, q_heads:]``, ``k_weight``) of ``x [N, heads, head_dim]`` in
     one launch (inl_norm_rope_qk_fwd)."""
-    import torch
-    n, heads, hd = x.shape
-    od = out_dtype if out_dtype is not None else x.dtype
-    if out is None:
-        out = torch.empty((n, heads, hd), dtype=od, device=x.device)
-    rd = (hd if cos is not None else 0) if rotary_dim is None else rotary_dim
-    d = NormRopeDesc()
-    d.n_tokens, d.heads, d.head_dim = n, heads, hd
-    d.x_row_stride, d.y_row_stride = x.stride(0), out.stride(0)
-    d.dtype, d.out_dtype = _dtype_code(x.dtype), _dtype_code(out.dtype)
-    d.norm, d.eps = int(bool(norm)), float(eps)
-    d.rotary_dim, d.sections = int(rd), int(sections)
-    d.table_rows = int(cos.shape[0]) if cos is not None else 0
-    d.round_tables, d.round_norm = int(bool(round_tables)), int(bool(round_norm))
-    ptr = lambda t: t.data_ptr() if t is not None else None
-    _check(_norm_rope_qk(ctypes.byref(d), int(q_heads), x.data_ptr(), out.data_ptr(), ptr(q_weight),
-                         ptr(k_weight), ptr(rows), ptr(cos), ptr(sin), ptr(cos2), ptr(sin2),
-                         _stream_ptr(stream)))
-    return out
+    return _prologue(_norm_rope_qk, x, int(q_heads), q_weight, k_weight, rows, cos, sin, eps, norm, rotary_dim, sections,
+                     cos2, sin2, out, out_dtype, round_tables, round_norm, stream)
 
 
 # ---------------------------------------------------------------------------

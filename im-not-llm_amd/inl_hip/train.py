@@ -17,7 +17,8 @@ import functools
 
 import torch
 
-from . import INL_BF16, INL_F32, InlError, NormRopeDesc, _check, _dtype_code, _sig, c_i32, c_i64, c_void_p
+from . import (INL_BF16, INL_F32, InlError, NormRopeDesc, _check, _dtype_code, _head_rows, _rope_tables, _sig, c_i32,
+               c_i64, c_void_p)
 
 ACTS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu_tanh": 3, "gelu_erf": 4}
 ROPE_HALF, ROPE_AXIAL, ROPE_INTERLEAVED = 1, 2, 3
@@ -370,50 +371,27 @@ def softmax_xent_bwd(dloss, lse, x, w, targets, *, bias=None, scale=1.0, ignore_
 # q/k prologue
 # ---------------------------------------------------------------------------
 
-def _heads(name, t, shape, dev):
-    if tuple(t.shape) != shape or t.get_device() != dev:
-        raise InlError(-1, f"{name}: shape {tuple(t.shape)} on {t.device}, need {shape} on cuda:{dev}")
-    stride = t.stride()
-    if stride[2] != 1 or (shape[1] > 1 and stride[1] != shape[2]):
-        raise InlError(-1, f"{name}: heads must be contiguous inside a token row")
-    row = shape[1] * shape[2]
-    if shape[0] <= 1:
-        return row
-    if stride[0] < row:
-        raise InlError(-1, f"{name}: token rows overlap (strides {stride})")
-    return stride[0]
-
-
 @_at_home
 def _rope_grads(dev, x, dy, q_heads, rows, cos, sin, q_weight, k_weight, eps, norm, rotary_dim, sections, cos2, sin2,
                 round_tables, out, weight_grad):
-    shape = tuple(x.shape)
+    shape = x.shape
     if len(shape) != 3:
-        raise InlError(-1, f"x: shape {shape}, need [tokens, heads, head_dim]")
+        raise InlError(-1, f"x: shape {tuple(shape)}, need [tokens, heads, head_dim]")
     n, heads, hd = shape
     d = NormRopeDesc()
     d.n_tokens, d.heads, d.head_dim = shape
-    d.x_row_stride, d.y_row_stride = _heads("x", x, shape, dev), _heads("dy", dy, shape, dev)
+    d.x_row_stride, d.y_row_stride = _head_rows("x", x, shape, dev), _head_rows("dy", dy, shape, dev)
     d.dtype, d.out_dtype = _dtype_code(x.dtype), _dtype_code(dy.dtype)
     d.norm, d.eps = int(bool(norm)), eps
     d.rotary_dim = int((hd if cos is not None else 0) if rotary_dim is None else rotary_dim)
     d.sections, d.round_tables = int(sections), int(bool(round_tables))
-    d.table_rows = int(cos.shape[0]) if cos is not None else 0
-    if d.rotary_dim:
-        tables = (("cos", cos), ("sin", sin))
-        if sections == ROPE_AXIAL:
-            tables += (("cos2", cos2), ("sin2", sin2))
-        width = hd // 4 if sections == ROPE_AXIAL else d.rotary_dim // 2
-        for name, t in tables:
-            if t is None or tuple(t.shape) != (d.table_rows, width) or t.dtype != _F32 or not t.is_contiguous() \
-                    or t.get_device() != dev:
-                raise InlError(-1, f"{name}: need contiguous f32 [{d.table_rows}, {width}] on cuda:{dev}")
-        _vec("rows", rows, n, torch.int32, dev)
+    if d.rotary_dim > 0:
+        d.table_rows = _rope_tables(n, rows, d.rotary_dim, hd, d.sections, cos, sin, cos2, sin2, dev)
     if out is None:
         out = torch.empty(shape, dtype=x.dtype, device=dev)
     elif out.dtype != x.dtype:
         raise InlError(-1, f"out: dtype {out.dtype}, need {x.dtype}")
-    ds = _heads("out", out, shape, dev)
+    ds = _head_rows("out", out, shape, dev)
     grads = bool(norm and weight_grad)
     dq = torch.empty(hd, dtype=_F32, device=dev) if grads else None
     dk = torch.empty(hd, dtype=_F32, device=dev) if grads and q_heads < heads else None

@@ -167,3 +167,47 @@ def test_stream_of_another_device(T):
                  lambda: T.norm_rope_qk_bwd(x, x, 1, stream=s)):
         with pytest.raises(inl_hip.InlError, match="the stream is on cuda:1"):
             call()
+
+
+def test_prologue_tables_and_rows():
+    """What the prologue's kernels read by address is checked by the binding, forward
+    and backward (host tensors here, whose device number is -1)."""
+    import inl_hip
+    import torch
+    f = lambda *s, dtype=torch.float32: torch.zeros(*s, dtype=dtype)
+    rows = f(5, dtype=torch.int32)
+    ok = lambda *a: inl_hip._rope_tables(*a, -1)
+    assert ok(5, rows, 64, 128, 3, f(9, 32), f(9, 32), None, None) == 9
+    assert ok(4, rows, 64, 128, 1, f(9, 1, 32), f(12, 32), None, None) == 9   # more than is read
+    assert ok(5, rows, 128, 128, 2, f(5, 32), f(5, 32), f(5, 32), f(5, 32)) == 5
+    for a in ((5, rows, 64, 128, 3, f(9, 64), f(9, 64), None, None),        # a column per feature
+              (5, rows, 64, 128, 3, f(9, 32), f(9, 64), None, None),
+              (5, rows, 64, 128, 1, f(9, 16), f(9, 16), None, None),
+              (5, rows, 64, 128, 1, f(9, 32), f(8, 32), None, None),        # sin of fewer positions
+              (5, rows, 64, 128, 1, f(9, 32), None, None, None),
+              (5, rows, 64, 128, 1, None, f(9, 32), None, None),
+              (5, rows, 64, 128, 1, f(288), f(288), None, None),
+              (5, rows, 64, 128, 1, f(9, 32, dtype=torch.bfloat16), f(9, 32), None, None),
+              (5, rows, 64, 128, 1, f(9, 64)[:, :32], f(9, 32), None, None),
+              (5, rows, 64, 128, 1, f(32, 9).T, f(9, 32), None, None),
+              (6, rows, 64, 128, 1, f(9, 32), f(9, 32), None, None),        # fewer rows than tokens
+              (5, rows.long(), 64, 128, 1, f(9, 32), f(9, 32), None, None),
+              (3, rows[::2], 64, 128, 1, f(9, 32), f(9, 32), None, None),
+              (5, None, 64, 128, 1, f(9, 32), f(9, 32), None, None),
+              (5, rows, 128, 128, 2, f(5, 32), f(5, 32), None, None),
+              (5, rows, 128, 128, 2, f(5, 32), f(5, 32), f(5, 32), f(4, 32)),
+              (5, rows, 128, 128, 2, f(5, 64), f(5, 64), f(5, 64), f(5, 64))):
+        with pytest.raises(inl_hip.InlError):
+            ok(*a)
+    with pytest.raises(inl_hip.InlError, match="cuda:0"):   # another device than the tokens'
+        inl_hip._rope_tables(5, rows, 64, 128, 1, f(9, 32), f(9, 32), None, None, 0)
+    x = f(7, 5, 16)
+    shape = x[:, :3].shape
+    assert inl_hip._head_rows("x", x[:, :3], shape, -1) == 80
+    assert inl_hip._head_rows("x", x[:1, :3].expand(1, 3, 16), (1, 3, 16), -1) == 48
+    for t in (x, x[:, ::2], x[:, :3].float().transpose(1, 2), x[:1, :3].expand(7, 3, 16), x[:6, :3], f(7, 3, 32)[..., ::2]):
+        with pytest.raises(inl_hip.InlError):
+            inl_hip._head_rows("x", t, shape, -1)
+    for call in (lambda: inl_hip.norm_rope(x), lambda: inl_hip.norm_rope_qk(x, 2)):
+        with pytest.raises(inl_hip.InlError, match="not a device tensor"):
+            call()

@@ -127,3 +127,54 @@ def test_slopes_of_far_values(act, cuda, inl):
         h = torch.zeros(m, 16, dtype=torch.bfloat16, device=cuda)
         dx, _, _ = inl.gated_ffn_bwd(dy, x.new_zeros(m, 16), w_gu, down, gu, h, act=act, dx_dtype=torch.float32)
         assert (dx[:, :8] == 2.0 ** -20).all() and (dx[:, 8:].abs() <= 1e-7 * 2.0 ** -20).all(), m
+
+
+def test_prologue_forward_refusals(cuda, inl):
+    """The forward refuses what its gradient refuses: nothing of it reaches a kernel."""
+    import torch
+    f = lambda *s, dtype=torch.float32: torch.ones(*s, dtype=dtype, device=cuda)
+    x, rows, c = f(5, 3, 64), f(5, dtype=torch.int32), f(9, 32)
+    for kw in (dict(rows=rows, cos=f(9, 64), sin=f(9, 64), rotary_dim=64, sections=3),
+               dict(rows=rows.long(), cos=c, sin=c), dict(rows=rows[:4], cos=c, sin=c), dict(cos=c, sin=c),
+               dict(rows=rows, cos=c), dict(rows=rows, cos=c.bfloat16(), sin=c.bfloat16()), dict(rows=rows.cpu(), cos=c, sin=c),
+               dict(rows=rows, cos=c.cpu(), sin=c.cpu()), dict(out=f(5, 3, 32)), dict(out=f(4, 3, 64)), dict(out=f(1, 3, 64).expand(5, 3, 64)),
+               dict(rotary_dim=8)):
+        for call in (lambda: inl.norm_rope(x, **kw), lambda: inl.norm_rope_qk(x, 2, **kw)):
+            with pytest.raises(inl.InlError):
+                call()
+    for w in (f(32), f(64, dtype=torch.bfloat16), f(64).cpu(), f(128)[::2]):
+        for call in (lambda: inl.norm_rope(x, weight=w), lambda: inl.norm_rope_qk(x, 2, q_weight=w),
+                     lambda: inl.norm_rope_qk(x, 2, k_weight=w)):
+            with pytest.raises(inl.InlError):
+                call()
+    for t in (x[0], x.transpose(1, 2), f(5, 6, 64)[:, ::2], f(1, 3, 64).expand(5, 3, 64)):
+        with pytest.raises(inl.InlError):
+            inl.norm_rope_qk(t, 2)
+
+
+@pytest.mark.parametrize("sections", [1, 3])
+def test_prologue_forward_forms(sections, cuda, inl):
+    """Longer rows and tables than are read, one token of any row stride, a weight that
+    no norm uses, another stream: all as the plain call."""
+    import torch
+    x = _rand(torch, cuda, (5, 4, 64), 1)
+    rows = torch.tensor([3, 0, 8, 1, 1, 7], dtype=torch.int32, device=cuda)
+    c, s = _rand(torch, cuda, (9, 32), 2, 1, torch.float32), _rand(torch, cuda, (9, 32), 3, 1, torch.float32)
+    w = _rand(torch, cuda, (64,), 4)
+    kw = dict(rotary_dim=64, sections=sections)
+    want = inl.norm_rope_qk(x, 3, rows[:5], c, s, q_weight=w, **kw)
+    t64 = [v.double()[rows[:5].long()] for v in (c, s)]
+    weights = torch.cat([w.double().expand(3, 64), torch.ones(1, 64, dtype=torch.float64, device=cuda)])
+    ref = R.norm_rope(x.double(), weights, 1e-6, 64, sections, t64)
+    R.check(want, ref, R.out_tol(ref, torch.bfloat16) + 2.0 ** -20 * ref.abs().amax(-1, keepdim=True), "y")
+    assert torch.equal(inl.norm_rope_qk(x, 3, rows, c.view(9, 1, 32), torch.cat([s, s]), q_weight=w[None], **kw), want)
+    one = torch.empty(1, 9, 64, dtype=torch.bfloat16, device=cuda).expand(1, 9, 64)[:, :4]
+    one.copy_(x[2:3])
+    assert torch.equal(inl.norm_rope_qk(one, 3, rows[2:], c, s, q_weight=w, **kw), want[2:3])
+    plain = inl.norm_rope(x, rows, c, s, norm=False, **kw)
+    assert torch.equal(inl.norm_rope(x, rows, c, s, norm=False, weight=w.float()[:1], **kw), plain)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = inl.norm_rope_qk(x, 3, rows, c, s, q_weight=w, stream=side, **kw)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
