@@ -276,7 +276,8 @@ int norm_rope_launch_ex(const inl_norm_rope_desc* d, const void* x, void* y, con
                         const void* weight2, int32_t w2_heads, int32_t w3_heads, int32_t rope_heads,
                         const int32_t* rows, const float* cos, const float* sin, const float* cos2,
                         const float* sin2, void* stream) {
-  int rc = norm_rope_check(d, rows, cos, sin, cos2, sin2);
+  const int32_t none = 0;   // no tokens, no rows
+  int rc = norm_rope_check(d, d && d->n_tokens == 0 ? &none : rows, cos, sin, cos2, sin2);
   if (rc) return rc;
   const int hd = d->head_dim;
   const int64_t xs = d->x_row_stride ? d->x_row_stride : (int64_t)d->heads * hd;

@@ -211,3 +211,17 @@ def test_prologue_tables_and_rows():
     for call in (lambda: inl_hip.norm_rope(x), lambda: inl_hip.norm_rope_qk(x, 2)):
         with pytest.raises(inl_hip.InlError, match="not a device tensor"):
             call()
+
+
+def test_prologue_of_no_tokens():
+    """An empty tensor of rows has no address: no tokens is no error, forward or backward."""
+    import inl_hip
+    d = inl_hip.NormRopeDesc()
+    d.n_tokens, d.heads, d.head_dim, d.dtype, d.out_dtype, d.norm, d.eps = 0, 3, 64, 1, 1, 1, 1e-6
+    d.rotary_dim, d.table_rows = 64, 9
+    for sections in (1, 3):
+        d.sections = sections
+        assert inl_hip._norm_rope(d, None, None, P, None, P, P, None, None, None) == 0, inl_hip.last_error()
+        assert inl_hip._norm_rope_qk(d, 2, None, None, P, P, None, P, P, None, None, None) == 0
+    d.n_tokens = 1
+    assert inl_hip._norm_rope(d, P, P, P, None, P, P, None, None, None) == -1 and "rows" in inl_hip.last_error()
