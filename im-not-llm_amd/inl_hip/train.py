@@ -407,12 +407,14 @@ def _rope_grads(dev, x, dy, q_heads, rows, cos, sin, q_weight, k_weight, eps, no
 
 
 def norm_rope_qk_bwd(dy, x, q_heads, rows=None, cos=None, sin=None, *, q_weight=None, k_weight=None, eps=1e-6,
-                     norm=True, rotary_dim=None, sections=1, cos2=None, sin2=None, round_tables=False, out=None,
-                     weight_grad=True, stream=None):
+                     norm=True, rotary_dim=None, sections=1, cos2=None, sin2=None, round_tables=False, round_norm=False,
+                     out=None, weight_grad=True, stream=None):
     """``(dx, dq_weight, dk_weight)`` of ``norm_rope_qk`` from ``dy [N, heads,
     head_dim]`` and the forward's ``x`` (``inl_norm_rope_qk_bwd``); the other
-    arguments as in the forward. dx has x's dtype (``out`` may be a slice of wider rows), the
+    arguments as in the forward (``round_norm`` changes nothing, gradients pass the
+    rounding unchanged; dy has the forward's output dtype). dx has x's dtype (``out`` may be a slice of wider rows), the
     weight gradients are f32 ``[head_dim]`` and None without a norm, with
     ``weight_grad=False`` or, dk_weight, where all heads are q heads."""
+    del round_norm
     return _rope_grads(x, dy, q_heads, rows, cos, sin, q_weight, k_weight, eps, norm, rotary_dim, sections, cos2, sin2,
                        round_tables, out, weight_grad, stream)

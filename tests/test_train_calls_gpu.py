@@ -178,3 +178,13 @@ def test_prologue_forward_forms(sections, cuda, inl):
     got = inl.norm_rope_qk(x, 3, rows, c, s, q_weight=w, stream=side, **kw)
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+def test_prologue_gradient_takes_the_forwards_arguments(cuda, inl):
+    import torch
+    x, dy = _rand(torch, cuda, (9, 3, 64), 1), _rand(torch, cuda, (9, 3, 64), 2)
+    rows, c = torch.arange(9, dtype=torch.int32, device=cuda), _rand(torch, cuda, (9, 32), 3, 1, torch.float32)
+    kw = dict(q_weight=x[0, 0], k_weight=x[1, 1], eps=1e-5, rotary_dim=64, sections=3, round_tables=True)
+    inl.norm_rope_qk(x, 2, rows, c, c, round_norm=True, **kw)
+    got = inl.norm_rope_qk_bwd(dy, x, 2, rows, c, c, round_norm=True, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(got, inl.norm_rope_qk_bwd(dy, x, 2, rows, c, c, **kw)))
