@@ -304,16 +304,27 @@ int few_launch(const TileParams& p, hipStream_t stream) {
 
 }  // namespace
 
-// Measured, us, few rows against the tiled product, by (n, k): up to four rows
-// (1,024, 1,024) 3.1 / 9, (8,192, 2,048) 8.6 / 10, (16,384, 1,024) 9.1 / 8, (50,000, 768)
-// 21 / 16, two rows of the last 15 / 16. 16 rows (1,024, 1,024) 4.0 / 9.4, (4,096, 1,024)
-// 4.2 / 7.1, (1,024, 4,096) 9.3 / 10.0, (8,192, 2,048) 10.0 / 10.0, (50,000, 768) 25 / 16. 32
-// rows (1,024, 1,024) 5.0 / 7.7, (8,192, 1,024) 7.8 / 7.4, (1,024, 4,096) 12.7 / 10.6. (A
-// workgroup's time goes with k and its blocks of rows; 256 of them are 4,096 columns.)
-bool few_rows(int64_t m, int64_t n, int64_t k) {
-  if (m <= 2) return true;
-  if (m <= 4) return n * k <= ((int64_t)1 << 24);
-  return m <= 32 && (m + 15) / 16 * ((n + 4095) / 4096) * k <= 4096;
+// Measured, us, few rows against the tiled product, by (n, k), six sets of weights in turn:
+//   2 rows   (8,192, 256) 3.5 / 4.2   (16,384, 512) 6.4 / 6.0    (16,384, 1,024) 7.8 / 8.3   (50,000, 768) 18.8 / 18.3
+//   4        (8,192, 512) 5.2 / 5.6   (8,192, 2,048) 9.0 / 10.1  (12,288, 1,024) 8.2 / 7.8   (4,096, 8,192) 21.6 / 20.6
+//   5        (1,024, 1,024) 3.6 / 7.1 (8,192, 512) 5.4 / 5.7     (8,192, 2,048) 9.5 / 10.1   (1,024, 4,096) 8.2 / 9.5
+//   16       (1,024, 1,024) 4.1 / 7.2 (8,192, 256) 5.9 / 4.3     (8,192, 1,024) 6.4 / 7.8    (16,384, 1,024) 9.8 / 8.3
+//            (4,096, 2,048) 7.0 / 8.9 (4,096, 4,096) 10.4 / 10.8 (2,048, 8,192) 16.9 / 12.1
+//   32       (4,096, 2,048) 8.6 / 9.6 (8,192, 512) 5.6 / 6.0     (8,192, 768) 8.5 / 6.9      (1,024, 4,096) 13.3 / 9.8
+// Gate and up rows (n of each), few less tiled:
+//   2 rows   (16,384, 512) -1.4       (8,192, 2,048) -4.2
+//   4        (4,096, 512) -1.2        (8,192, 512) +0.4          (8,192, 1,024) -1.3         (12,288, 1,024) -0.8
+//   16       (4,096, 1,024) -1.8      (4,096, 2,048) -1.3        (6,144, 1,024) +0.6         (8,192, 512) +2.2
+//   32       (4,096, 2,048) -0.5      (1,024, 4,096) +4.5        (8,192, 512) +0.7           (8,192, 1,024) +2.3
+// (One row through 50,000 x 768: 13.5 / 16. A workgroup's time goes with k and its blocks of
+// rows; 256 workgroups of the kernel from 5 rows on are 4,096 columns, a round.)
+bool few_rows(int64_t m, int64_t n, int64_t k, bool gated) {
+  if (m == 1) return true;
+  if (m == 2) return gated || n <= 8192 || n <= 16 * k;
+  if (m <= 4) return gated ? n <= 6144 || (k >= 1024 && n <= 12288) : n <= 8192 && n * k <= ((int64_t)1 << 24);
+  const int64_t rounds = (n + 4095) / 4096;
+  if (m <= 16) return rounds * k <= 4096 && (rounds == 1 || (rounds == 2 && k >= (gated ? 1024 : 768)));
+  return m <= 32 && ((rounds == 1 && k <= 2048) || (rounds == 2 && !gated && k <= 512));
 }
 
 int few_dense(const TileParams& p, bool gated, bool out_bf16, hipStream_t stream) {
@@ -405,7 +416,7 @@ constexpr int MAX_SPLITS = 32;
 struct DensePlan {
   TilePlan y, dx, dw;
   size_t need(const inl_dense_desc& d, bool backward) const {
-    if (!backward) return few_rows(d.m, d.n, d.k) ? 0 : tile_part_bytes(y, d.m, d.n);
+    if (!backward) return few_rows(d.m, d.n, d.k, false) ? 0 : tile_part_bytes(y, d.m, d.n);
     Carve c(nullptr);
     if (d.act != INL_ACT_NONE) c.take((size_t)d.m * d.n * 2);
     c.take(colsum_bytes(d.m, d.n));
@@ -415,7 +426,7 @@ struct DensePlan {
 };
 
 int dense_plan(const inl_dense_desc& d, bool backward, DensePlan* p, int* cus) {
-  if (!backward && few_rows(d.m, d.n, d.k)) return INL_OK;
+  if (!backward && few_rows(d.m, d.n, d.k, false)) return INL_OK;
   int rc = device_cus(cus);
   if (rc) return rc;
   if (!backward) {
@@ -479,7 +490,7 @@ extern "C" int inl_dense_fwd(const inl_dense_desc* d, const void* x, const void*
   p.ps = s.pre;
   p.act = d->act;
   const bool out16 = d->out_dtype == INL_BF16;
-  if (few_rows(d->m, d->n, d->k)) return few_dense(p, false, out16, (hipStream_t)stream);
+  if (few_rows(d->m, d->n, d->k, false)) return few_dense(p, false, out16, (hipStream_t)stream);
   return tile_nt_linear(p, plan.y, out16, (float*)ws, cus, (hipStream_t)stream);
 }
 

@@ -38,7 +38,7 @@ struct FfnPlan {
   int cus = 0;
 };
 int ffn_plan(const inl_gated_ffn_desc& d, bool backward, FfnPlan* p) {
-  const bool few_h = few_rows(d.m, d.inner, d.hidden), few_y = few_rows(d.m, d.hidden, d.inner);
+  const bool few_h = few_rows(d.m, d.inner, d.hidden, true), few_y = few_rows(d.m, d.hidden, d.inner, false);
   if (!backward && few_h && few_y) return INL_OK;
   int rc = device_cus(&p->cus);
   if (rc) return rc;

@@ -28,7 +28,7 @@ int check_workspace(const char* what, const void* ws, size_t have, size_t need);
 
 // y[m, n] = act(x . w^T + bias) + residual, and act(x . w_gate^T) * (x . w_up^T), for
 // few rows of x: where few_rows says that they beat the tiled product.
-bool few_rows(int64_t m, int64_t n, int64_t k);
+bool few_rows(int64_t m, int64_t n, int64_t k, bool gated);
 int few_dense(const TileParams& p, bool gated, bool out_bf16, hipStream_t stream);
 
 // dz = dy * act'(pre) (bf16, packed [m, n]; NULL = not stored) and the column sums of the

@@ -188,3 +188,19 @@ def test_prologue_gradient_takes_the_forwards_arguments(cuda, inl):
     inl.norm_rope_qk(x, 2, rows, c, c, round_norm=True, **kw)
     got = inl.norm_rope_qk_bwd(dy, x, 2, rows, c, c, round_norm=True, **kw)
     assert all(torch.equal(a, b) for a, b in zip(got, inl.norm_rope_qk_bwd(dy, x, 2, rows, c, c, **kw)))
+
+
+# both sides of each border of the rules that choose a kernel for a few rows
+@pytest.mark.parametrize("m,n,k", [(2, 16384, 1024), (2, 16392, 1016), (3, 8192, 2048), (4, 8200, 1016), (4, 4096, 4104),
+                                   (5, 8192, 768), (16, 8192, 760), (16, 8200, 768), (16, 4104, 2048), (9, 40, 4096), (9, 40, 4104),
+                                   (17, 4096, 2048), (32, 72, 2056), (32, 8192, 512), (32, 4104, 520)])
+def test_dense_at_the_borders_of_few_rows(m, n, k, cuda, inl):
+    from test_train_gpu import test_dense_few_rows
+    test_dense_few_rows(m, n, k, "silu", cuda, inl)
+
+
+@pytest.mark.parametrize("m,hidden,inner", [(4, 520, 6144), (3, 520, 6152), (4, 1024, 12288), (3, 1024, 12296), (16, 512, 4096),
+                                            (5, 512, 4104), (16, 1024, 4104), (16, 1016, 4104), (32, 2048, 4096), (17, 2056, 264), (2, 264, 16400)])
+def test_gated_ffn_at_the_borders_of_few_rows(m, hidden, inner, cuda, inl):
+    from test_train_gpu import test_gated_ffn
+    test_gated_ffn(m, hidden, inner, "gelu_erf", cuda, inl)
