@@ -319,7 +319,7 @@ int few_launch(const TileParams& p, hipStream_t stream) {
 // (One row through 50,000 x 768: 13.5 / 16. A workgroup's time goes with k and its blocks of
 // rows; 256 workgroups of the kernel from 5 rows on are 4,096 columns, a round.)
 bool few_rows(int64_t m, int64_t n, int64_t k, bool gated) {
-  if (m == 1) return true;
+  if (m <= 1) return true;
   if (m == 2) return gated || n <= 8192 || n <= 16 * k;
   if (m <= 4) return gated ? n <= 6144 || (k >= 1024 && n <= 12288) : n <= 8192 && n * k <= ((int64_t)1 << 24);
   const int64_t rounds = (n + 4095) / 4096;

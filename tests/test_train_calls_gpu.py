@@ -204,3 +204,155 @@ def test_dense_at_the_borders_of_few_rows(m, n, k, cuda, inl):
 def test_gated_ffn_at_the_borders_of_few_rows(m, hidden, inner, cuda, inl):
     from test_train_gpu import test_gated_ffn
     test_gated_ffn(m, hidden, inner, "gelu_erf", cuda, inl)
+
+
+# ---------------------------------------------------------------------------
+# Padded rows in and out, with guards
+# ---------------------------------------------------------------------------
+
+def _padded(torch, dev, rows, cols, dtype, extra=24):
+    """A [rows, cols] part of wider rows, a row behind them, everything 7."""
+    whole = torch.full((rows + 2, cols + extra), 7.0, dtype=dtype, device=dev)
+    return whole, whole[:rows, 8:8 + cols] if dtype == torch.bfloat16 else whole[:rows, 4:4 + cols]
+
+
+def _only_inside_changed(torch, whole, part):
+    part.fill_(7.0)
+    return bool((whole == 7.0).all())
+
+
+def _room(torch, dev, size_fn, desc):
+    import ctypes
+    n = ctypes.c_size_t()
+    assert size_fn(desc, 1, ctypes.byref(n)) == 0
+    return torch.empty(max(n.value, 16), dtype=torch.uint8, device=dev), n.value
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("m,n,k", [(3, 40, 24), (300, 136, 72), (2500, 264, 520)])
+def test_gradients_into_padded_rows(m, n, k, dt, cuda, inl):
+    """dx and dw of the linear layer, the block and cross entropy (several pieces of the
+    vocabulary with the largest m) with row strides of their own: the bits of packed
+    outputs, and nothing beside them is written. The binding packs its outputs, so
+    these are calls of the C entries."""
+    import torch
+    from inl_hip import train as T
+    dtype, code = (torch.bfloat16, 1) if dt == "bf16" else (torch.float32, 0)
+    p, st = (lambda t: t.data_ptr()), torch.cuda.current_stream().cuda_stream
+    x, dy, w = _rand(torch, cuda, (m, k), 1), _rand(torch, cuda, (m, n), 2, 0.1), _rand(torch, cuda, (n, k), 3, k ** -0.5)
+    pre = _rand(torch, cuda, (m, n), 4)
+    print(f"case=padded {m} {n} {k} {dt}", flush=True)
+    want = inl.dense_bwd(dy, x, w, act="silu", pre=pre, dx_dtype=dtype, dw_dtype=dtype)
+    (dxw, dx), (dww, dw) = _padded(torch, cuda, m, k, dtype), _padded(torch, cuda, n, k, dtype)
+    d = T.DenseDesc(m, n, k, 0, 0, 0, 0, 0, dx.stride(0), dw.stride(0), 2, 0, 0, code, code)
+    room, size = _room(torch, cuda, T._dense_ws, d)
+    assert T._dense_bwd(d, p(dy), p(x), p(w), p(pre), p(dx), p(dw), None, p(room), size, st) == 0, inl.last_error()
+    assert torch.equal(dx, want[0]) and torch.equal(dw, want[1])
+    assert _only_inside_changed(torch, dxw, dx) and _only_inside_changed(torch, dww, dw)
+
+    gu, down = _rand(torch, cuda, (2 * n, k), 5, k ** -0.5), _rand(torch, cuda, (k, n), 6, n ** -0.5)
+    _, pre2, h = inl.gated_ffn(x, gu, down, save=True)
+    want = inl.gated_ffn_bwd(x, x, gu, down, pre2, h, dx_dtype=dtype, dw_dtype=dtype)
+    d = T.GatedFfnDesc(m, k, n, 0, 0, 0, dx.stride(0), 2, 0, 0, code, code)
+    room, size = _room(torch, cuda, T._ffn_ws, d)
+    dgu, dd = (torch.empty_like(t) for t in want[1:])
+    assert T._ffn_bwd(d, p(x), p(x), p(gu), p(down), p(pre2), p(h), p(dx), p(dgu), p(dd), p(room), size, st) == 0
+    assert all(torch.equal(a, b) for a, b in zip((dx, dgu, dd), want)) and _only_inside_changed(torch, dxw, dx)
+
+    vocab = 2 ** 26 // m // 256 * 256 + 1031 if m > 2000 else n + 3
+    wv, t = _rand(torch, cuda, (vocab, k), 7, k ** -0.5), torch.arange(m, device=cuda, dtype=torch.int32) % vocab
+    _, lse = inl.softmax_xent(x, wv, t)
+    dl = torch.full((m,), 1 / m, device=cuda)
+    want = inl.softmax_xent_bwd(dl, lse, x, wv, t, dx_dtype=dtype, dw_dtype=dtype)
+    dvw, dv = _padded(torch, cuda, vocab, k, dtype)
+    d = T.SoftmaxXentDesc(m, vocab, k, 0, 0, dx.stride(0), dv.stride(0), 1.0, -100, code, code)
+    room, size = _room(torch, cuda, T._xent_ws, d)
+    assert T._xent_bwd(d, p(dl), p(lse), p(x), p(wv), None, p(t), p(dx), p(dv), None, p(room), size, st) == 0
+    assert torch.equal(dx, want[0]) and torch.equal(dv, want[1])
+    assert _only_inside_changed(torch, dxw, dx) and _only_inside_changed(torch, dvw, dv)
+
+
+@pytest.mark.parametrize("m", [2, 20, 700])
+def test_block_and_loss_on_strided_rows(m, cuda, inl):
+    """Slices of wider rows in and out give what packed rows give."""
+    import torch
+    hidden, inner, vocab = 136, 200, 1001
+    wide = lambda rows, cols, seed, std=1.0: _rand(torch, cuda, (rows, cols + 24), seed, std)[:, 8:8 + cols]
+    x, dy, res, wv = wide(m, hidden, 1), wide(m, hidden, 2, 0.1), wide(m, hidden, 3), wide(vocab, hidden, 4, 0.08)
+    gu, down = _rand(torch, cuda, (2 * inner, hidden), 5, 0.08), _rand(torch, cuda, (hidden, inner), 6, 0.07)
+    c = lambda t: t.contiguous()
+    print(f"case=strided {m}", flush=True)
+    want = inl.gated_ffn(c(x), gu, down, residual=c(res), save=True)
+    whole, out = _padded(torch, cuda, m, hidden, torch.bfloat16)
+    got = inl.gated_ffn(x, gu, down, residual=res, save=True, out=out)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and _only_inside_changed(torch, whole, out)
+    _, pre, h = want
+    assert all(torch.equal(a, b) for a, b in zip(inl.gated_ffn_bwd(dy, x, gu, down, pre, h),
+                                                 inl.gated_ffn_bwd(c(dy), c(x), gu, down, pre, h)))
+    t = torch.arange(m, device=cuda, dtype=torch.int32)
+    want = inl.softmax_xent(c(x), c(wv), t)
+    assert all(torch.equal(a, b) for a, b in zip(inl.softmax_xent(x, wv, t), want))
+    dl = torch.full((m,), 1 / m, device=cuda)
+    want = inl.softmax_xent_bwd(dl, want[1], c(x), c(wv), t, bias_grad=True)
+    assert all(torch.equal(a, b) for a, b in zip(inl.softmax_xent_bwd(dl, inl.softmax_xent(x, wv, t)[1], x, wv, t, bias_grad=True), want))
+
+
+@pytest.mark.parametrize("m,vocab", [(9000, 9001), (17000, 9001)])
+def test_softmax_xent_bwd_of_several_pieces(m, vocab, cuda, inl):
+    """Two and three pieces of the vocabulary (2^26 / m columns each, 4,096 at least), the
+    last one odd: dx adds up over them in f32."""
+    from test_train_gpu import test_softmax_xent_bwd
+    test_softmax_xent_bwd(m, vocab, 72, 1.0, True, cuda, inl)
+
+
+# ---------------------------------------------------------------------------
+# Forms of the prologue's gradient
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("types", [("bf16", "f32"), ("f32", "bf16"), ("bf16", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("weights,rounded", [(True, True), (False, False), (False, True)])
+@pytest.mark.parametrize("n,hq,hk,d,rotary,sections", [(5, 2, 1, 64, 64, 1), (333, 16, 8, 128, 64, 3), (40, 6, 6, 64, 64, 2),
+                                                       (2500, 8, 2, 32, 24, 3), (4000, 4, 4, 128, 128, 1)])
+def test_prologue_gradient_forms(n, hq, hk, d, rotary, sections, weights, rounded, types, cuda, inl):
+    """dy of the other type than x, norms without weights, tables rounded to bf16. The
+    weight gradients' bound is of the sizes that are summed: a token's heads that
+    went missing would show."""
+    import torch
+    from test_train_gpu import _tables
+    tx, ty = ({"bf16": torch.bfloat16, "f32": torch.float32}[t] for t in types)
+    heads = hq + hk
+    x, dy = _rand(torch, cuda, (n, heads, d), 1, 1.0, tx), _rand(torch, cuda, (n, heads, d), 2, 1.0, ty)
+    wq, wk = ((1 + _rand(torch, cuda, (d,), s, 0.2, torch.float32)).to(tx) for s in (3, 4))
+    rows, tabs = _tables(torch, cuda, n, d, rotary, sections)
+    kw = dict(q_weight=wq, k_weight=wk) if weights else {}
+    print(f"case=rope_bwd forms {n} {hq} {hk} {d} {rotary} {sections} {types}", flush=True)
+    dx, dq, dk = inl.norm_rope_qk_bwd(dy, x, hq, rows, tabs[0], tabs[1], rotary_dim=rotary, sections=sections, cos2=tabs[2],
+                                      sin2=tabs[3], round_tables=rounded, **kw)
+    t64 = [None if v is None else (R.r16(v) if rounded else v.double())[rows.long()] for v in tabs]
+    w = torch.cat([wq.double().expand(hq, d), wk.double().expand(hk, d)]) if weights else torch.ones(heads, d, device=cuda, dtype=torch.float64)
+    xd, dyd = x.double(), dy.double()
+    ref, dw = R.norm_rope_bwd(dyd, xd, w, 1e-6, rotary, sections, t64)
+    assert dx.dtype == tx
+    inv = 1 / torch.sqrt((xd * xd).mean(-1, keepdim=True) + 1e-6)
+    hat = xd * inv
+    # sizes of what a rotation adds: |dy| turned by |cos| and -|sin|, backwards
+    sizes = [None if v is None else v.abs() for v in t64]
+    for i in (1, 3):
+        sizes[i] = None if sizes[i] is None else -sizes[i]
+    turned = R.turn(dyd.abs(), rotary, sections, *sizes)
+    if rotary:   # (one of a pair takes the difference there: the sum bounds both)
+        flip = R.turn(dyd.abs(), rotary, sections, *sizes, back=True)
+        turned = torch.maximum(turned.abs(), flip.abs())
+    # some 16 f32 roundings of each value's terms, and of the row's sum of d of them
+    size = (w * turned).abs()
+    mean = (size * hat.abs()).mean(-1, keepdim=True)
+    R.check(dx, ref, R.out_tol(ref, tx) + (16 + d / 8) * 2.0 ** -24 * inv * (size + hat.abs() * mean), "dx")
+    for got, q in ((dq, slice(0, hq)), (dk, slice(hq, heads))):
+        part, each = dw[:, q], (turned * hat.abs())[:, q]
+        terms = part.shape[0] * part.shape[1]
+        # in order per lane, then over the lanes' groups and the workgroups: at most
+        # 80 + terms / 64 additions on a value's way; 16 roundings of each term
+        tol = (80 + terms / 64) * 2.0 ** -24 * part.abs().sum((0, 1)) + 16 * 2.0 ** -24 * each.sum((0, 1))
+        R.check(got, part.sum((0, 1)), tol, "dweight")
+        lost = part[n // 2].sum(0).abs()   # one token's heads
+        assert (lost > 2 * tol).any(), "the bound would not see a lost token"
