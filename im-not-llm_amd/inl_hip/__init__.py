@@ -479,8 +479,14 @@ def _table(name, t, table_rows, width, dev):
                            + ("" if t is None else f", got {t.dtype} {tuple(t.shape)} on {t.device}"))
 
 
-def _bad_weight(name, t, like, hd, dev):
-    raise InlError(-1, f"{name}: need contiguous {like} [{hd}] on cuda:{dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+def _head_weight(name, t, like, hd, dev):
+    """The address of a weight per feature, of the heads' dtype ``like``."""
+    if t is None:
+        return None
+    if t.dtype is not like or t.numel() != hd or t.get_device() != dev or not t.is_contiguous():
+        raise InlError(-1, f"{name}: need contiguous {like} [{hd}] on cuda:{dev}, got {t.dtype} {tuple(t.shape)} on "
+                           f"{t.device}")
+    return t.data_ptr()
 
 
 def _prologue(entry, x, q_heads, w, w2, rows, cos, sin, eps, norm, rotary_dim, sections, cos2, sin2, out, out_dtype,
@@ -516,14 +522,8 @@ def _prologue(entry, x, q_heads, w, w2, rows, cos, sin, eps, norm, rotary_dim, s
         if sections == 2:
             cp2, sp2 = cos2.data_ptr(), sin2.data_ptr()
     if norm:
-        if w is not None:
-            if w.dtype is not dtype or w.numel() != hd or w.get_device() != dev or not w.is_contiguous():
-                _bad_weight("weight" if q_heads is None else "q_weight", w, dtype, hd, dev)
-            wp = w.data_ptr()
-        if w2 is not None:
-            if w2.dtype is not dtype or w2.numel() != hd or w2.get_device() != dev or not w2.is_contiguous():
-                _bad_weight("k_weight", w2, dtype, hd, dev)
-            wp2 = w2.data_ptr()
+        wp = _head_weight("weight" if q_heads is None else "q_weight", w, dtype, hd, dev)
+        wp2 = _head_weight("k_weight", w2, dtype, hd, dev)
     d = NormRopeDesc(n, heads, hd, x_row, out_row, code, out_code, bool(norm), float(eps),
                      int(rotary_dim), int(sections), table_rows, bool(round_tables), bool(round_norm))
     at = torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream

@@ -17,8 +17,8 @@ import functools
 
 import torch
 
-from . import (INL_BF16, INL_F32, InlError, NormRopeDesc, _check, _dtype_code, _head_rows, _rope_tables, _sig, c_i32,
-               c_i64, c_void_p)
+from . import (INL_BF16, INL_F32, InlError, NormRopeDesc, _check, _dtype_code, _head_rows, _head_weight,
+               _rope_tables, _sig, c_i32, c_i64, c_void_p)
 
 ACTS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu_tanh": 3, "gelu_erf": 4}
 ROPE_HALF, ROPE_AXIAL, ROPE_INTERLEAVED = 1, 2, 3
@@ -399,10 +399,11 @@ def _rope_grads(dev, x, dy, q_heads, rows, cos, sin, q_weight, k_weight, eps, no
     if grads:
         _check(_rope_bwd_ws(d, ctypes.byref(size)))
     room = _room(size.value, dev)
-    _check(_rope_bwd(d, int(q_heads), dy.data_ptr(), x.data_ptr(), out.data_ptr(), ds,
-                     _vec("q_weight", q_weight, hd, x.dtype, dev), _vec("k_weight", k_weight, hd, x.dtype, dev),
-                     _ptr(rows), _ptr(cos), _ptr(sin), _ptr(cos2), _ptr(sin2), _ptr(dq), _ptr(dk), _ptr(room),
-                     size.value, _stream(dev)))
+    wp = wp2 = None   # (as in the forward: not looked at without a norm)
+    if norm:
+        wp, wp2 = _head_weight("q_weight", q_weight, x.dtype, hd, dev), _head_weight("k_weight", k_weight, x.dtype, hd, dev)
+    _check(_rope_bwd(d, int(q_heads), dy.data_ptr(), x.data_ptr(), out.data_ptr(), ds, wp, wp2, _ptr(rows), _ptr(cos),
+                     _ptr(sin), _ptr(cos2), _ptr(sin2), _ptr(dq), _ptr(dk), _ptr(room), size.value, _stream(dev)))
     return out, dq, dk
 
 

@@ -356,3 +356,20 @@ def test_prologue_gradient_forms(n, hq, hk, d, rotary, sections, weights, rounde
         R.check(got, part.sum((0, 1)), tol, "dweight")
         lost = part[n // 2].sum(0).abs()   # one token's heads
         assert (lost > 2 * tol).any(), "the bound would not see a lost token"
+
+
+def test_prologue_gradient_weights_as_in_the_forward(cuda, inl):
+    """The forms of a weight that the forward takes: any shape of head_dim values, and
+    whatever it is where there is no norm."""
+    import torch
+    x, dy = _rand(torch, cuda, (9, 3, 64), 1), _rand(torch, cuda, (9, 3, 64), 2)
+    w = _rand(torch, cuda, (64,), 3)
+    for f in (inl.norm_rope_qk, inl.norm_rope_qk_bwd):
+        a = (x,) if f is inl.norm_rope_qk else (dy, x)
+        flat = lambda out: [t for t in (out if isinstance(out, tuple) else (out,)) if t is not None]
+        for one, two in ((dict(q_weight=w[None], k_weight=w.view(8, 8)), dict(q_weight=w, k_weight=w)),
+                         (dict(norm=False, q_weight=w.float()), dict(norm=False))):
+            assert all(torch.equal(u, v) for u, v in zip(flat(f(*a, 2, **one)), flat(f(*a, 2, **two))))
+        for bad in (w.float(), w[:32], w.cpu()):
+            with pytest.raises(inl.InlError):
+                f(*a, 2, q_weight=bad)
