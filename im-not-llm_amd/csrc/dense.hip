@@ -96,7 +96,7 @@ __global__ __launch_bounds__(256) void row_dense_kernel(TileParams p) {
 // of 64 (whole 128-byte lines of 16 rows of w). Operands go from memory to
 // v_mfma_f32_16x16x32_bf16 as they lie, U units asked for at a time (x from L2 after
 // the first workgroups); the waves' sums meet in LDS, in order. 8 rows through 1,024 x
-// 1,024 take 3.7 us, 16 take 4.0 (tiled product: 9.4).
+// 1,024 take 3.8 us, 16 take 4.1 (tiled product: 7.2).
 constexpr int FEW_WAVES = 4;   // (eight: 5.8 us instead of 4.0 for 16 rows, 1,024 x 1,024)
 
 template <int R, int XB, bool OUT16>
@@ -204,10 +204,11 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void few_dense_kernel(TileParams p)
 
 // ---- dz and column sums ----
 //
-// Bound by memory: dy and pre read once, dz written once (20,011 x 768: 20 us, 4.6 TB/s).
-// A thread takes 8
-// columns of every 8th row of its block's CS_ROWS rows; the 8 row groups meet in LDS,
-// the blocks in a second kernel that adds their sums in order.
+// Bound by memory: dy and pre read once, dz written once (20,011 x 768: 19.4 us, 4.75 TB/s).
+// A thread takes 8 columns of every 8th row of its block's CS_ROWS rows; the 8 row groups
+// meet in LDS, the blocks in a second kernel that adds their sums in order. dz is rounded
+// to bf16, the type of the products' operands, which dx and dw feel as much as their own
+// rounding (2.4e-3 of their norm from 64 bits, 1.7e-3 without); the sums take it unrounded.
 constexpr int CS_ROWS = 64, CS_COLS = 256;
 int64_t colsum_blocks(int64_t m) { return std::min<int64_t>((m + CS_ROWS - 1) / CS_ROWS, 65535); }
 

@@ -9,10 +9,15 @@
 //             dx = [d_gate d_up] . w_gate_up           4
 //             dw_gate_up = [d_gate d_up]^T . x         4
 //
-// 20,011 rows, 768 x 1,152, forward: 110 to 120 us by card (gate and up 73, down 42; 890 to 960
-// TFLOP/s). 16,384 rows, 1,024 x 4,096, backward: 764 to 771 us (1,070); the gate gradients' product
-// stands beside the bytes of its epilogue (98 us of products, 537 MB), the others
-// under the power limit. One row of 1,024 x 2,816: 6.3 us.
+// 20,011 rows, 768 x 1,152, forward: 107 to 120 us by card (gate and up 71, down 43; 890 to 990
+// TFLOP/s), 7 more where pre and h are stored. 16,384 rows, 1,024 x 4,096, backward: 764 to 786 us
+// (1,050 to 1,080): the gate gradients' product stands beside the bytes of its epilogue (98 us of
+// products, 537 MB, matrix cores 26 % busy), the others run at 2.0 to 2.1 GHz of 2.4 (58 to 65 %
+// busy). One row of 1,024 x 2,816: 6.3 us.
+//
+// h, d_gate and d_up are rounded to bf16, the type of the products' operands. The outputs feel
+// it: y is 1.9e-3 of its norm from 64 bits (1.7e-3 with its own rounding alone), dx and
+// dw_gate_up 2.3e-3 (1.7e-3). gate, up, dh and the activation stay in f32 in between.
 #include "train_ops.hpp"
 
 namespace inl {

@@ -7,7 +7,7 @@
 // An operand is stored as rows of k (OP_ROWS: x [M, K], w [N, K], the forward
 // products) or as rows of m or n (OP_COLS: [K, M], [K, N]; dx = dz . W reads
 // W that way, dW = dz^T . x both). Nothing is transposed in memory: a stage of
-// an OP_COLS operand sits in LDS as it is stored (32 rows of k) and its MFMA
+// an OP_COLS operand sits in LDS as it is stored (64 rows of k) and its MFMA
 // operands are read with ds_read_b64_tr_b16, which hands lane j of 16 the four
 // k values of column j.
 //
@@ -19,10 +19,13 @@
 //
 // Rates on random values, 8,192^3, TFLOP/s: 1,472 with both operands as rows of k, 1,453
 // with W as rows of n, about 1,430 with both as rows of m and n (a large library
-// product reached 1,422 on the card): bound by power. Products of one to three rounds
-// of tiles are bound by their first loads and epilogues, which nothing hides
-// (20,011 x 768 x 768 takes 27 us for 17), those in 128 x 128 tiles by LDS (0.94 us per two
-// stages of a CU for 0.43 of products).
+// product reached 1,422 on the card): bound by power (matrix cores 72 to 74 % busy at
+// 1.5 to 1.6 GHz of 2.4). Products of one to three rounds of tiles are bound by their first
+// loads and epilogues, which nothing hides (20,011 x 768 x 768 takes 27 us for 17, matrix
+// cores 31 % busy). In 128 x 128 tiles two stages of a CU take 0.94 us for 0.43 of products
+// (8,192 x 1,024 x 2,048: matrix cores 35 % busy, LDS 20 %; of the waves' time 30 % goes to
+// barriers and loads, 33 % to waiting for an instruction slot, 6 % for LDS's): no unit is
+// full, the pieces of a stage stand in line.
 //
 // The 16 x 16 x 32 instruction and not 32 x 32 x 16: both run at the same rate, but a large
 // product is bound by the card's power, and on values that toggle (normal

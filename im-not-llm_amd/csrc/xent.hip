@@ -11,8 +11,10 @@
 //   backward  g = dloss (exp(s - lse) - onehot), in pieces of the vocabulary: the
 //     scores again (EPI_DXENT writes g in bf16), dw of the piece = scale g^T . x,
 //     dx += scale g . w. 6 m vocab hidden flops. 2,048 rows, 151,669 entries, hidden
-//     1,024: 1.72 to 1.80 ms (1,060 to 1,110 TFLOP/s); a piece's scores 147 us, dw 120, dx 114
-//     and 14 for the join of its k splits.
+//     1,024: 1.72 to 1.80 ms (1,060 to 1,110 TFLOP/s); a piece's scores 139 us, dw 107, dx 103
+//     and 14 for the join of its k splits. g is rounded to bf16, the type of the products'
+//     operands: here dx and dw move by 2e-4 of their norm for it, under the rounding of a
+//     bf16 output (1.7e-3). dbias sums those values, which the pieces read anyway, in f32.
 #include "train_ops.hpp"
 
 namespace inl {
@@ -41,8 +43,9 @@ int64_t stat_blocks(int shape, int64_t vocab) {
 }
 
 // lse and loss from the blocks' statistics: the 16 waves of a workgroup take every
-// 16th block for 64 rows, then meet in LDS. Bound by memory: 782 blocks of 4,099 rows
-// (26 MB) take 6.1 us.
+// 16th block for 64 rows, then meet in LDS. Bound by latency: 4,099 rows are 65
+// workgroups for 256 CUs, and a wave folds some 25 of the 392 blocks (50,002 entries) one
+// after another: 6.0 us for 12.9 MB, 2.1 TB/s. 1,024 rows x 128 blocks 3.9 us, mostly launch.
 constexpr int JOIN_WAVES = 16;
 __global__ __launch_bounds__(JOIN_WAVES * 64) void xent_join_kernel(const float2* part, int64_t blocks, int64_t m,
                                                                     const int32_t* target, const float* at,

@@ -2,8 +2,8 @@
 layer with bias, activation and residual, the gated feed-forward block, softmax
 cross entropy without its scores, and the gradients of the q/k prologue.
 
-Gradients are plain functions of what the forward left (no autograd graph is
-kept): a ``torch.autograd.Function`` or a training loop calls them in its own
+Gradients are plain functions of what the forward left (outputs carry no autograd
+graph, whatever ``requires_grad`` says of the inputs): a ``torch.autograd.Function`` or a training loop calls them in its own
 backward. Outputs and workspaces come from torch's allocator, so calls can be
 captured into a graph. With ``stream=`` a call works there and takes its memory there;
 that its inputs are ready on that stream, and that their memory is not handed on

@@ -129,7 +129,8 @@ int inl_gated_ffn_bwd(const inl_gated_ffn_desc* desc, const void* dy, const void
  * whose target is ignore_index has loss 0 and a gradient of 0 whatever its scores
  * are (its lse is given; dw still multiplies its x by 0); another target outside
  * [0, vocab) gives a NaN loss and, in the backward, NaN in its row of dx and in all
- * of dw. A bias of -inf takes an entry out. x: [m, hidden], w: [vocab, hidden]; any vocab >= 1.
+ * of dw. A bias of -inf takes an entry out (with all of them out lse is -inf, loss
+ * NaN). x: [m, hidden], w: [vocab, hidden]; any vocab >= 1.
  * --------------------------------------------------------------------- */
 typedef struct inl_softmax_xent_desc {
   int64_t m;

@@ -373,3 +373,15 @@ def test_prologue_gradient_weights_as_in_the_forward(cuda, inl):
         for bad in (w.float(), w[:32], w.cpu()):
             with pytest.raises(inl.InlError):
                 f(*a, 2, q_weight=bad)
+
+
+def test_softmax_xent_without_any_entry(cuda, inl):
+    """A bias of -inf on the whole vocabulary leaves nothing: lse -inf, loss NaN but for
+    ignored rows."""
+    import torch
+    for m, vocab in ((1, 3), (70, 1001), (300, 70)):
+        x, w = _rand(torch, cuda, (m, 72), 1), _rand(torch, cuda, (vocab, 72), 2)
+        t = torch.arange(m, device=cuda, dtype=torch.int32) % vocab
+        t[m // 2] = -100
+        loss, lse = inl.softmax_xent(x, w, t, bias=torch.full((vocab,), float("-inf"), device=cuda))
+        assert (lse == float("-inf")).all() and loss[m // 2] == 0 and torch.isnan(loss[t >= 0]).all()
