@@ -352,6 +352,25 @@ int check_rows(const char* what, const void* p, int64_t cols, int64_t stride, in
   return INL_OK;
 }
 
+bool rows_meet(const Rows& a, const Rows& b) {
+  if (!a.at || !b.at || a.rows <= 0 || b.rows <= 0) return false;
+  const int64_t d = (int64_t)((uintptr_t)b.at - (uintptr_t)a.at);   // b's start from a's
+  if (d >= (a.rows - 1) * a.step + a.len || -d >= (b.rows - 1) * b.step + b.len) return false;
+  auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
+  // rows j of b meet row i of a where i a.step - b.len < d + j b.step < i a.step + a.len
+  auto met = [&](int64_t at) {   // a row of a that starts `at` bytes after a's start
+    const int64_t lo = floor_div(at - b.len - d, b.step) + 1, hi = -floor_div(d - at - a.len, b.step) - 1;
+    return std::max<int64_t>(lo, 0) <= std::min(hi, b.rows - 1);
+  };
+  if (a.step == b.step) {   // columns of one buffer, say: only j - i counts
+    const int64_t lo = floor_div(-b.len - d, b.step) + 1, hi = -floor_div(d - a.len, b.step) - 1;
+    return std::max(lo, 1 - a.rows) <= std::min(hi, b.rows - 1);
+  }
+  for (int64_t i = 0; i < a.rows; ++i)
+    if (met(i * a.step)) return true;
+  return false;
+}
+
 int check_workspace(const char* what, const void* ws, size_t have, size_t need) {
   if (!need) return INL_OK;
   if (!ws || ((uintptr_t)ws & 15)) return fail(INL_E_INVALID, std::string(what) + ": the workspace must be 16-byte aligned");
@@ -468,6 +487,21 @@ extern "C" int inl_dense_fwd(const inl_dense_desc* d, const void* x, const void*
   if (residual && (rc = check_rows("dense: residual", residual, d->n, s.res, d->residual_dtype))) return rc;
   if (pre && (rc = check_rows("dense: pre", pre, d->n, s.pre, INL_BF16))) return rc;
   if ((uintptr_t)bias & 15) return fail(INL_E_INVALID, "dense: bias must be 16-byte aligned");
+  // tiles are written while others still read x and w
+  auto rows = [](const void* at, int64_t n, int64_t cols, int64_t stride, int32_t dtype) {
+    return Rows{at, n, cols * dtype_size(dtype), stride * dtype_size(dtype)};
+  };
+  const Rows rx = rows(x, d->m, d->k, s.x, INL_BF16), rw = rows(w, d->n, d->k, s.w, INL_BF16);
+  const Rows ry = rows(y, d->m, d->n, s.y, d->out_dtype), rp = rows(pre, d->m, d->n, s.pre, INL_BF16);
+  const Rows rr = rows(residual, d->m, d->n, s.res, residual ? d->residual_dtype : INL_BF16);
+  const bool in_place = residual == y && d->residual_dtype == d->out_dtype && (s.res == s.y || d->m == 1);
+  auto meet = [](const char* what, const Rows& a, const Rows& b) {
+    return rows_meet(a, b) ? fail(INL_E_INVALID, std::string("dense: overlap of ") + what) : INL_OK;
+  };
+  if ((rc = meet("y and x", ry, rx)) || (rc = meet("y and w", ry, rw)) || (rc = meet("pre and x", rp, rx)) ||
+      (rc = meet("pre and w", rp, rw)) || (rc = meet("pre and y", rp, ry)) || (rc = meet("pre and residual", rp, rr)))
+    return rc;
+  if (!in_place && (rc = meet("y and residual, which are not the same rows", ry, rr))) return rc;
   DensePlan plan;
   int cus = 0;
   if ((rc = dense_plan(*d, false, &plan, &cus))) return rc;

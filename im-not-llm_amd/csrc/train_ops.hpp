@@ -13,6 +13,13 @@ int device_cus(int* cus);
 // 16-byte aligned; `what` names it in the error.
 int check_rows(const char* what, const void* p, int64_t cols, int64_t stride, int32_t dtype);
 
+// Whether two matrices share a byte: rows of `len` bytes, `step` apart.
+struct Rows {
+  const void* at;
+  int64_t rows, len, step;
+};
+bool rows_meet(const Rows& a, const Rows& b);
+
 // Pieces of a workspace, each on a 256-byte boundary.
 struct Carve {
   char* base;

@@ -201,7 +201,7 @@ def dense(x, w, bias=None, *, act=None, residual=None, pre=None, out=None, out_d
     """``act(x @ w.T + bias) + residual`` (``inl_dense_fwd``): bf16 ``x [m, k]``
     and ``w [n, k]``, f32 ``bias [n]``, ``act`` one of None, "relu", "silu",
     "gelu_tanh", "gelu_erf", ``residual [m, n]`` bf16 or f32 (it may be
-    ``out``). ``pre``: a bf16 ``[m, n]`` tensor that receives ``x @ w.T + bias`` for
+    ``out``; ``x`` may not). ``pre``: a bf16 ``[m, n]`` tensor that receives ``x @ w.T + bias`` for
     ``dense_bwd``. n and k are multiples of 8; rows may be strided."""
     return _dense(x, w, bias, act, residual, pre, out, out_dtype, stream)
 

@@ -62,9 +62,11 @@ typedef struct inl_dense_desc {
 
 int inl_dense_workspace_size(const inl_dense_desc* desc, int32_t backward, size_t* bytes);
 
-/* bias: f32 [n] or NULL; residual: [m, n] or NULL (it may be y itself); pre:
- * bf16 [m, n] or NULL, receives x . w^T + bias for the backward. Everything up
- * to y (and pre) stays in f32: one rounding each. */
+/* bias: f32 [n] or NULL; residual: [m, n] or NULL (it may be y itself, of its type
+ * and stride); pre: bf16 [m, n] or NULL, receives x . w^T + bias for the backward.
+ * Everything up to y (and pre) stays in f32: one rounding each. y and pre otherwise
+ * share no byte with another argument: x itself is refused, as x is read until the
+ * last of y is written. */
 int inl_dense_fwd(const inl_dense_desc* desc, const void* x, const void* w, const float* bias, const void* residual,
                   void* y, void* pre, void* workspace, size_t workspace_bytes, void* stream);
 
@@ -103,7 +105,7 @@ typedef struct inl_gated_ffn_desc {
 
 int inl_gated_ffn_workspace_size(const inl_gated_ffn_desc* desc, int32_t backward, size_t* bytes);
 
-/* residual: [m, hidden] or NULL (it may be y itself). pre (bf16 [m, 2 inner]:
+/* residual: [m, hidden] or NULL (it may be y itself, and either may be x). pre (bf16 [m, 2 inner]:
  * gate, then up) and h (bf16 [m, inner]), packed, are stored for the backward,
  * both or neither (NULL). h is rounded to bf16 before the down projection. */
 int inl_gated_ffn_fwd(const inl_gated_ffn_desc* desc, const void* x, const void* w_gate_up, const void* w_down,

@@ -225,3 +225,48 @@ def test_prologue_of_no_tokens():
         assert inl_hip._norm_rope_qk(d, 2, None, None, P, P, None, P, P, None, None, None) == 0
     d.n_tokens = 1
     assert inl_hip._norm_rope(d, P, P, P, None, P, P, None, None, None) == -1 and "rows" in inl_hip.last_error()
+
+
+def test_dense_outputs_overlap_nothing(T):
+    """y over x (a residual stream updated in place) would be written while it is read."""
+    import inl_hip
+    X, W, R, Y, PRE = (P + (i << 24) for i in range(5))
+    kw = dict(m=300, n=40, k=40)
+
+    def refused(x=X, w=W, res=None, y=Y, pre=None, **f):
+        d = _dense(T, **{**kw, **f})
+        rc = T._dense_fwd(d, x, w, None, res, y, pre, None, 0, None)
+        return rc == -1 and "overlap" in inl_hip.last_error()
+    assert refused(y=X) and refused(y=W) and refused(pre=X) and refused(pre=Y) and refused(res=R, pre=R)
+    assert refused(res=X, y=X)                                  # residual in place, and x too
+    assert refused(y=X + 16) and refused(y=X - 16)              # a shifted one
+    assert refused(y=X + 300 * 80 - 16) and refused(y=X - 300 * 80 + 16)   # the ends
+    assert refused(y=Y, res=Y, residual_dtype=0)                # another type at the same place
+    assert refused(y=Y, res=Y, y_stride=48, residual_stride=56)
+    assert refused(y=Y, res=Y + 16)
+    assert refused(y=X + 80, x_stride=80, y_stride=88)          # strides that drift into each other
+
+
+def test_rows_meet(T):
+    """Against all pairs of rows, by way of the entry's refusal."""
+    import random
+
+    import inl_hip
+    rng = random.Random(1)
+    seen = set()
+    for _ in range(4000):
+        m, n, k = rng.choice([1, 2, 5]), 8 * rng.randint(1, 3), 8 * rng.randint(1, 3)
+        xs = k + 8 * rng.randint(0, 6)
+        ys = rng.choice([xs, n + 8 * rng.randint(0, 6)])
+        if ys < n:
+            continue
+        at = P + 16 * rng.randint(-20, 20)
+        want = any(P + 2 * i * xs < at + 2 * (j * ys + n) and at + 2 * j * ys < P + 2 * (i * xs + k)
+                   for i in range(m) for j in range(m))
+        # (a call that is not refused would go on to the card: where y misses x, w lies on y,
+        # which is looked at next)
+        d = _dense(T, m=m, n=n, k=k, x_stride=xs, y_stride=ys)
+        assert T._dense_fwd(d, P, P + (1 << 24) if want else at, None, None, at, None, None, 0, None) == -1
+        assert inl_hip.last_error().endswith("overlap of y and x" if want else "overlap of y and w")
+        seen.add(want)
+    assert seen == {True, False}

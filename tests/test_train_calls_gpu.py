@@ -385,3 +385,22 @@ def test_softmax_xent_without_any_entry(cuda, inl):
         t[m // 2] = -100
         loss, lse = inl.softmax_xent(x, w, t, bias=torch.full((vocab,), float("-inf"), device=cuda))
         assert (lse == float("-inf")).all() and loss[m // 2] == 0 and torch.isnan(loss[t >= 0]).all()
+
+
+def test_columns_of_one_buffer_and_in_place(cuda, inl):
+    """x, y, the residual and pre as columns of one buffer; the block in place on its
+    residual stream; the linear layer there is refused."""
+    import torch
+    for m in (1, 9, 300):
+        buf = _rand(torch, cuda, (m, 400), 1)
+        x, y, res, pre = buf[:, :72], buf[:, 72:144], buf[:, 144:216], buf[:, 216:288]
+        w = _rand(torch, cuda, (72, 72), 2, 0.1)
+        want = inl.dense(x.clone(), w, act="silu", residual=res.clone())
+        assert torch.equal(inl.dense(x, w, act="silu", residual=res, out=y, pre=pre), want)
+        for kw in (dict(out=x), dict(out=x, residual=x), dict(pre=x), dict(out=y, pre=y), dict(residual=res, pre=res),
+                   dict(out=buf[:, 64:136])):
+            with pytest.raises(inl.InlError, match="overlap"):
+                inl.dense(x, w, **kw)
+        gu, down = _rand(torch, cuda, (400, 72), 3, 0.1), _rand(torch, cuda, (72, 200), 4, 0.1)
+        want = inl.gated_ffn(x.clone(), gu, down, residual=x.clone())
+        assert torch.equal(inl.gated_ffn(x, gu, down, residual=x, out=x), want) and torch.equal(x, want)
