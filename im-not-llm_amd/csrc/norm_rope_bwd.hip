@@ -263,6 +263,14 @@ extern "C" int inl_norm_rope_qk_bwd(const inl_norm_rope_desc* d, int32_t q_heads
   if (!dy || !dx || (d->norm && !x) ||
       (((uintptr_t)dy | (uintptr_t)dx | (uintptr_t)x | (uintptr_t)q_weight | (uintptr_t)k_weight) & 15))
     return fail(INL_E_INVALID, "norm_rope_bwd: dy, x, dx and the weights must be non-null and 16-byte aligned");
+  // a unit of heads is read before it is written: at its own place, or nowhere near
+  auto apart = [&](const void* at, int64_t stride, int32_t dtype) {
+    if (at == dx && dtype == d->dtype && (stride == ds || d->n_tokens == 1)) return true;
+    const int64_t in = dtype_size(dtype), out = dtype_size(d->dtype);
+    return !rows_meet({at, d->n_tokens, row * in, stride * in}, {dx, d->n_tokens, row * out, ds * out});
+  };
+  if (!apart(dy, ys, d->out_dtype) || (d->norm && !apart(x, xs, d->dtype)))
+    return fail(INL_E_INVALID, "norm_rope_bwd: dx overlaps dy or x, of another type or stride");
   int cus = 0;
   if ((rc = device_cus(&cus))) return rc;
   const int64_t groups = bwd_groups(d->n_tokens, d->heads, hd, cus);

@@ -14,7 +14,8 @@
 //     1,024: 1.72 to 1.80 ms (1,060 to 1,110 TFLOP/s); a piece's scores 139 us, dw 107, dx 103
 //     and 14 for the join of its k splits. g is rounded to bf16, the type of the products'
 //     operands: here dx and dw move by 2e-4 of their norm for it, under the rounding of a
-//     bf16 output (1.7e-3). dbias sums those values, which the pieces read anyway, in f32.
+//     bf16 output (1.7e-3); a dloss that is the same for every row moves them by its own
+//     rounding, 3.9e-3 at most (1 / 255; 1 / 2,048 is exact). dbias sums those values, which the pieces read anyway, in f32.
 #include "train_ops.hpp"
 
 namespace inl {

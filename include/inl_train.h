@@ -157,7 +157,8 @@ int inl_softmax_xent_fwd(const inl_softmax_xent_desc* desc, const void* x, const
 /* With g[r, v] = dloss[r] (exp(s[r, v] - lse[r]) - [v == targets[r]]):
  *   dx = scale g . w,  dw = scale g^T . x,  dbias = sum over rows of g
  * lse: the forward's; dloss: f32 [m]. The vocabulary is taken in pieces: g of
- * one piece (bf16) is all of it that exists at a time; dx adds up in f32.
+ * one piece (bf16, dloss rounded with it) is all of it that exists at a time; dx
+ * adds up in f32.
  * dbias (f32 [vocab]) sums the bf16 values. dx, dw, dbias: NULL = not
  * computed. */
 int inl_softmax_xent_bwd(const inl_softmax_xent_desc* desc, const float* dloss, const float* lse, const void* x,
@@ -175,7 +176,8 @@ int inl_softmax_xent_bwd(const inl_softmax_xent_desc* desc, const float* dloss, 
  * [head_dim], NULL = not computed. The roundings that the desc's round_norm
  * and round_tables ask for pass gradients through unchanged (tables rounded as
  * in the forward). A token whose table row is out of range gets NaN in dx and
- * in dweight. dx may be dy itself where types and strides are equal.
+ * in dweight. dx may be dy or x itself where types and strides are equal; it
+ * overlaps them nowhere else.
  * --------------------------------------------------------------------- */
 int inl_norm_rope_bwd_workspace_size(const inl_norm_rope_desc* desc, size_t* bytes);
 int inl_norm_rope_qk_bwd(const inl_norm_rope_desc* desc, int32_t q_heads, const void* dy, const void* x, void* dx,

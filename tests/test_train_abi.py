@@ -270,3 +270,19 @@ def test_rows_meet(T):
         assert inl_hip.last_error().endswith("overlap of y and x" if want else "overlap of y and w")
         seen.add(want)
     assert seen == {True, False}
+
+
+def test_norm_rope_bwd_overlaps(T):
+    """dx over dy or x of another type or stride, or shifted. (A call that passes ends at
+    the device or the workspace, which are looked at next.)"""
+    import inl_hip
+
+    def message(dx, dx_stride=0, dtype=1, out_dtype=1, ys=0):
+        d = inl_hip.NormRopeDesc(5, 3, 64, 0, ys, dtype, out_dtype, 1, 1e-6, 0, 1, 0, 0, 0)
+        assert T._rope_bwd(d, 2, P, P + (1 << 24), dx, dx_stride, None, None, None, None, None, None, None, P, P, None, 0, None) != 0
+        return inl_hip.last_error()
+    for dx, kw in ((P + 16, {}), (P, dict(dx_stride=200)), (P, dict(out_dtype=0)), (P, dict(dtype=0)), (P - 16, {}),
+                   (P + (1 << 24), dict(dx_stride=256)), (P + (1 << 24) + 5 * 384 - 16, {}), (P + 128, dict(ys=384, dx_stride=384))):
+        assert "overlaps" in message(dx, **kw), (dx, kw)
+    for dx, kw in ((P, {}), (P + (1 << 24), {}), (P + 5 * 384, {}), (P + 384, dict(ys=384, dx_stride=384)), (1 << 24, {})):
+        assert "overlaps" not in message(dx, **kw), (dx, kw)
