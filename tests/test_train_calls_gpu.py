@@ -404,3 +404,27 @@ def test_columns_of_one_buffer_and_in_place(cuda, inl):
         gu, down = _rand(torch, cuda, (400, 72), 3, 0.1), _rand(torch, cuda, (72, 200), 4, 0.1)
         want = inl.gated_ffn(x.clone(), gu, down, residual=x.clone())
         assert torch.equal(inl.gated_ffn(x, gu, down, residual=x, out=x), want) and torch.equal(x, want)
+
+
+def test_captured_on_a_forked_stream(cuda, inl):
+    """Calls with stream= inside a capture, on a stream that joined it: their memory is
+    the graph's, and eager work between the replays leaves it alone."""
+    import torch
+    m, n, k = 500, 264, 136
+    x, w, dy = _rand(torch, cuda, (m, k), 1), _rand(torch, cuda, (n, k), 2, 0.1), _rand(torch, cuda, (m, n), 3, 0.1)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        y = inl.dense(x, w, act="silu", stream=side)
+        grads = inl.dense_bwd(dy, x, w, bias_grad=True, stream=side)
+        also = inl.dense(x, w)
+        here.wait_stream(side)
+    for i in range(3):
+        x.copy_(_rand(torch, cuda, (m, k), 10 + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = (inl.dense(x, w, act="silu"), *inl.dense_bwd(dy, x, w, bias_grad=True), inl.dense(x, w))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip((y, *grads, also), want)), i
