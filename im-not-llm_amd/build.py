@@ -43,6 +43,7 @@ LINK_FLAGS = [f"--offload-arch={ARCH}", "-shared", "-fPIC", "-L/opt/rocm/lib", "
 # every tile; the MFMA operands then take the AGPRs.
 EXTRA = {
     "attn_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "attn_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 # Sources whose kernels issue global loads from inline asm and wait for them

@@ -1,0 +1,610 @@
+// Gradients of packed varlen attention (inl_attn_varlen_bwd), bf16 on gfx950.
+//
+//   S = scale q k^T, P = softmax(S) over the visible keys, dP = dO v^T,
+//   delta = rowsum(dO o), dS = P (dP - delta);
+//   dq = scale dS k,  dk = scale dS^T q,  dv = P^T dO  (k, v: summed over their heads)
+//
+// Two kernels and no atomics, so equal calls give equal bits: one owns query rows and
+// streams keys (dq), the other owns keys and streams the queries of every head of the
+// group (dk, dv). S and dP are computed in both: 14 flops per (pair, feature) where
+// one pass with atomics would take 10 and as many f32 additions to memory as there are
+// (query, key block) pairs. The probabilities are recomputed: the dq kernel runs the
+// forward's online softmax (its sum of exponentials and running maximum are per query
+// row, so dq is scaled once at the end), and leaves log-sum-exp and delta, f32 per (head,
+// row), for the other.
+//
+// Both kernels are one: a wave owns 32 rows whose two operands (q and dO, or k and v)
+// stay in registers as B operands, and streams tiles of the other pair through LDS:
+// X (k, or q) and Y (v, or dO).
+//   T1[s][o] = X own0^T  (S^T or S),  T2[s][o] = Y own1^T  (dP^T or dP)
+//   acc[d][o] += X^T dS  (dq^T or dk^T),  and for keys accv[d][o] += Y^T P
+// An own row is a lane (lane & 31), stream rows are the accumulators' registers, so P
+// and dS leave the first products in the layout in which the second ones read them: the
+// k index of a product is summed over, and both operands take it in the same order. X
+// and Y are stored once, row-major, and read both ways (ds_read_b128 for the first
+// products, ds_read_b64_tr_b16 for the second); the swizzle serves both.
+
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "attn_bwd.hpp"
+#include "attn_stream.hpp"
+#include "train_ops.hpp"
+
+namespace inl {
+
+namespace {
+
+constexpr uint32_t BWD_NOWHERE = 0xffff0000u;   // beyond every text's range: reads 0, not written
+constexpr int BWD_BM = 128;                     // own rows of a workgroup: 4 waves of 32
+
+template <int D>
+struct BwdShape {
+  static constexpr int BN = D <= 128 ? 64 : 32;   // stream rows of a tile
+  static constexpr int ROW = D * 2;
+  static constexpr int TILE = BN * ROW;           // bytes of X, and of Y
+  static constexpr int STAT = 2 * BN * 4;         // log-sum-exp and delta of the stream rows
+  static constexpr int STAGE = 2 * TILE + STAT;
+  static constexpr int LDS = 2 * STAGE;
+};
+
+// 16-byte chunk c of row r lies at chunk c ^ bwd_swz(r) of that row. The 16 rows that a
+// row read touches at one logical chunk fall into 16 different 16-byte slots of 256, and so do
+// the 4 rows x 4 chunks of a transposed read.
+template <int D>
+__device__ __forceinline__ int bwd_swz(int r) {
+  return D == 64 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
+}
+
+__device__ __forceinline__ bf16x8 pack8(const float* x) {
+  u32x4 o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    o[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){x[2 * e], x[2 * e + 1]}, bf16x2));
+  return __builtin_bit_cast(bf16x8, o);
+}
+
+// Rows r0 .. r0 + 31 of an output from acc[d][row] (D / 32 blocks of 32 features): one
+// v_permlane32_swap per register pair puts 8 consecutive features of a row into a lane.
+template <int D, bool OUT16>
+__device__ __forceinline__ void bwd_store(const f32x16 (&acc)[D / 32], float by, __amdgpu_buffer_rsrc_t rs, uint32_t at,
+                                          int hf, int head_dim) {
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db) {
+    if constexpr (OUT16) {
+#pragma unroll
+      for (int gp = 0; gp < 2; ++gp) {
+        uint32_t w[4];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const f32x2 x = {acc[db][8 * gp + 2 * h] * by, acc[db][8 * gp + 2 * h + 1] * by};
+          w[h] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
+        }
+        swap_lanes_32(w[0], w[2]);
+        swap_lanes_32(w[1], w[3]);
+        const int col = db * 32 + 16 * gp + 8 * hf;
+        __builtin_amdgcn_raw_buffer_store_b128((u32x4){w[0], w[1], w[2], w[3]}, rs,
+                                               col < head_dim ? at + col * 2 : BWD_NOWHERE, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int col = db * 32 + 8 * g + 4 * hf;
+        u32x4 val;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) val[e] = __builtin_bit_cast(uint32_t, acc[db][4 * g + e] * by);
+        __builtin_amdgcn_raw_buffer_store_b128(val, rs, col < head_dim ? at + col * 4 : BWD_NOWHERE, 0, 0);
+      }
+    }
+  }
+}
+
+// The text of unit u: texts' first units ascend, so it is the last one whose is not above u.
+__device__ __forceinline__ BwdText bwd_text(const BwdText* texts, int n, int u, int lane) {
+  int at = 0;
+  for (int i = 0; i < n; i += 64) {
+    const int first = i + lane < n ? texts[i + lane].unit : 0x7fffffff;
+    const int below = __builtin_popcountll(__builtin_amdgcn_ballot_w64(first <= u));
+    at = i + below - 1;
+    if (below < 64) break;
+  }
+  // (texts[i].unit <= u for the first of a block that is not the first block, or `at` is the
+  // last text of the block before)
+  const BwdText t = texts[at];
+  return {__builtin_amdgcn_readfirstlane(t.start), __builtin_amdgcn_readfirstlane(t.len),
+          __builtin_amdgcn_readfirstlane(t.unit)};
+}
+
+// KV: own rows are keys (dk, dv); otherwise queries (dq, and the row statistics).
+template <int D, bool KV, bool OUT16>
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwdParams p) {
+  using S = BwdShape<D>;
+  constexpr int KST = D / 16;            // k-steps of the products over features
+  constexpr int NDB = D / 32;            // 32-feature blocks of an accumulator
+  constexpr int NKB = S::BN / 32;        // 32-row blocks of a tile
+  constexpr int CH = D / 8;              // 16-byte chunks per row
+  constexpr int RPB = 64 / CH;           // rows of a 1 KB block
+  constexpr int PARTS = S::TILE / 4096;  // 1 KB blocks of X (and of Y) per wave
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lq = lane & 31;
+  const int hf = lane >> 5;
+  const uint32_t lds0 = lds_addr(smem);
+  const int heads = KV ? p.h_kv : p.h_q;
+  const int u = blockIdx.x / heads;
+  const int head = blockIdx.x - u * heads;          // own head
+  const int kvh = KV ? head : head / p.group;
+  const BwdText txt = bwd_text(p.texts ? p.texts : p.own, p.n_texts, u, lane);
+  const int T = txt.len;
+  const int b0 = (u - txt.unit) * BWD_BM;           // first own row of the workgroup
+  const int r0 = b0 + wave * 32;                    // and of this wave
+  const bool active = r0 < T;
+  const int blast = min(b0 + BWD_BM - 1, T - 1), rlast = min(r0 + 31, T - 1);
+  const int own = r0 + lq;
+
+  const char* const base_q = p.q + txt.start * p.q_stride;
+  const char* const base_k = p.k + txt.start * p.k_stride + (int64_t)kvh * p.head_dim * 2;
+  const char* const base_v = p.v + txt.start * p.v_stride + (int64_t)kvh * p.head_dim * 2;
+  const char* const base_do = p.dout + txt.start * p.do_stride;
+
+  // ---- own operands: lane lq's row, chunks 2 i + hf ----
+  bf16x8 own0[KST], own1[KST];
+  float delta = 0.f;
+  {
+    const int64_t ho = (int64_t)head * p.head_dim * 2;
+    const uint32_t st0 = (uint32_t)(KV ? p.k_stride : p.q_stride), st1 = (uint32_t)(KV ? p.v_stride : p.do_stride);
+    const __amdgpu_buffer_rsrc_t rs0 = pp_rsrc(KV ? base_k : base_q + ho, (uint32_t)T * st0);
+    const __amdgpu_buffer_rsrc_t rs1 = pp_rsrc(KV ? base_v : base_do + ho, (uint32_t)T * st1);
+    const bool in = own < T;
+#pragma unroll
+    for (int i = 0; i < KST; ++i) {
+      const int c = 2 * i + hf;
+      const bool ok = in && c * 8 < p.head_dim;
+      own0[i] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs0, ok ? own * st0 + c * 16 : BWD_NOWHERE, 0, 0));
+      own1[i] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs1, ok ? own * st1 + c * 16 : BWD_NOWHERE, 0, 0));
+    }
+    if constexpr (!KV) {
+      const uint32_t st2 = (uint32_t)p.o_stride;
+      const __amdgpu_buffer_rsrc_t rs2 = pp_rsrc(p.o + txt.start * p.o_stride + ho, (uint32_t)T * st2);
+#pragma unroll
+      for (int i = 0; i < KST; ++i) {
+        const int c = 2 * i + hf;
+        const bool ok = in && c * 8 < p.head_dim;
+        const bf16x8 ov =
+            __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs2, ok ? own * st2 + c * 16 : BWD_NOWHERE, 0, 0));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) delta += (float)ov[e] * (float)own1[i][e];
+      }
+      delta = half_sum(delta);
+    }
+  }
+
+  // ---- the stream: tiles [t_lo, t_hi) of every head that the own rows meet ----
+  int s_lo = 0, s_hi = T;
+  if (p.window >= 0) {
+    s_lo = max(0, b0 - p.window);
+    s_hi = min(T, blast + p.window + 1);
+  }
+  if (p.causal) {
+    if (KV) s_lo = max(s_lo, b0);
+    else s_hi = min(s_hi, blast + 1);
+  }
+  const int t_lo = s_lo / S::BN, t_hi = (s_hi + S::BN - 1) / S::BN;
+  const int n_tiles = (t_hi - t_lo) * (KV ? p.group : 1);
+
+  uint32_t xg[PARTS], yg[PARTS];   // byte offset in a tile of what this lane loads
+  const uint32_t xst = (uint32_t)(KV ? p.q_stride : p.k_stride), yst = (uint32_t)(KV ? p.do_stride : p.v_stride);
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    const int row = (i * 4 + wave) * RPB + lane / CH;
+    const int c = (lane % CH) ^ bwd_swz<D>(row);
+    const bool ok = c * 8 < p.head_dim;
+    xg[i] = ok ? row * xst + c * 16 : BWD_NOWHERE;
+    yg[i] = ok ? row * yst + c * 16 : BWD_NOWHERE;
+  }
+  int dh = 0, dt = t_lo;   // load cursor: head of the group, tile
+  i32x4 xrs, yrs, lrs, ers;
+  auto load_head = [&]() __attribute__((always_inline)) {
+    if constexpr (KV) {
+      const int h = kvh * p.group + dh;
+      const int64_t ho = (int64_t)h * p.head_dim * 2;
+      xrs = pp_rsrc_words(base_q + ho, (uint32_t)T * xst);
+      yrs = pp_rsrc_words(base_do + ho, (uint32_t)T * yst);
+      lrs = pp_rsrc_words(p.stat + (int64_t)h * p.rows + txt.start, (uint32_t)T * 4);
+      ers = pp_rsrc_words(p.stat + (int64_t)(p.h_q + h) * p.rows + txt.start, (uint32_t)T * 4);
+    } else {
+      xrs = pp_rsrc_words(base_k, (uint32_t)T * xst);
+      yrs = pp_rsrc_words(base_v, (uint32_t)T * yst);
+    }
+  };
+  auto issue = [&](uint32_t stage) __attribute__((always_inline)) {
+    const uint32_t at = lds0 + stage + wave * 1024;
+    const uint32_t s0 = (uint32_t)(dt * S::BN);
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+      dma_b128(xrs, at + i * 4096, xg[i] == BWD_NOWHERE ? BWD_NOWHERE : s0 * xst + xg[i]);
+      dma_b128(yrs, at + S::TILE + i * 4096, yg[i] == BWD_NOWHERE ? BWD_NOWHERE : s0 * yst + yg[i]);
+    }
+    if constexpr (KV) {
+      // 4 bytes a lane; a tile of 32 rows fills half of its 64 (the rest is overwritten by nothing:
+      // lanes from BN on are off)
+      if (wave < 2 && lane < S::BN) {
+        const uint32_t dst = lds0 + stage + 2 * S::TILE + wave * S::BN * 4;
+        const i32x4 rs = wave == 0 ? lrs : ers;
+        asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds"
+                     :: "v"((s0 + lane) * 4), "s"(rs), "{m0}"(dst) : "memory");
+      }
+    }
+    if (++dt == t_hi && KV) {
+      dt = t_lo;
+      if (++dh < p.group) load_head();
+    }
+  };
+
+  // ---- per-lane LDS offsets ----
+  const uint32_t xa = lq * S::ROW + ((hf ^ bwd_swz<D>(lq)) << 4);   // row reads: ^ (st << 5)
+  const int g16 = lane >> 4, j16 = lane & 15;
+  const int trow = 4 * hf + (j16 >> 2);
+  const uint32_t ta = trow * S::ROW + (((2 * (g16 & 1) + ((j16 & 3) >> 1)) ^ bwd_swz<D>(trow)) << 4) + ((j16 & 1) << 3);
+  auto rows_frag = [&](uint32_t tile, int kb, int st) __attribute__((always_inline)) {
+    return __builtin_bit_cast(bf16x8, lds_load<u32x4>(lds0 + (xa ^ (st << 5)) + tile + kb * 32 * S::ROW));
+  };
+  // 16 stream rows (k-step ks) x 32 features (block db), transposed: the order of the rows is
+  // that of the accumulators' registers
+  auto cols_frag = [&](uint32_t tile, int ks, int db) __attribute__((always_inline)) {
+    s16x4 a[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      a[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)(size_t)(lds0 + tile + (ta ^ (db << 6) ^ (h << 5)) + (ks * 16 + 8 * h) * S::ROW));
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    return __builtin_bit_cast(bf16x8, (s16x8){a[0][0], a[0][1], a[0][2], a[0][3], a[1][0], a[1][1], a[1][2], a[1][3]});
+  };
+
+  f32x16 acc[NDB], accv[KV ? NDB : 1];
+#pragma unroll
+  for (int i = 0; i < NDB; ++i) {
+    acc[i] = (f32x16){};
+    if constexpr (KV) accv[i] = (f32x16){};
+  }
+  float m_i = -INFINITY, l_i = 0.f;
+
+  // One 32-row block of the stream against this wave's rows.
+  auto block = [&](uint32_t stage, int kb, int s0) __attribute__((always_inline)) {
+    const uint32_t X = stage, Y = stage + S::TILE;
+    f32x16 s = {}, dp = {};
+    if constexpr (KV) {
+      const uint32_t la = lds0 + stage + 2 * S::TILE + (kb * 32 + 4 * hf) * 4;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 a = lds_load<f32x4>(la + g * 32);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[4 * g + e] = a[e];
+      }
+    }
+#pragma unroll
+    for (int st = 0; st < KST; ++st)
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rows_frag(X, kb, st), own0[st], s, 0, 0, 0);
+    // masks: stream row s0 + c of register r, c = 8 (r / 4) + 4 hf + r % 4
+    const bool whole = (KV || s0 + 31 < T) && (!p.causal || (KV ? s0 >= rlast : s0 + 31 <= r0)) &&
+                       (p.window < 0 || (s0 + 31 - r0 <= p.window && rlast - s0 <= p.window));
+    if (!whole) {
+      const int sb = s0 + 4 * hf;
+      int hi = KV ? 0x3fffffff : T - 1, lo = 0;
+      if (p.causal) {
+        if (KV) lo = own;
+        else hi = min(hi, own);
+      }
+      if (p.window >= 0) {
+        lo = max(lo, own - p.window);
+        hi = min(hi, own + p.window);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int at = sb + 8 * (r >> 2) + (r & 3);
+        s[r] = at >= lo && at <= hi ? s[r] : -INFINITY;
+      }
+    }
+    float pr[16], ds[16];
+    auto second = [&]() __attribute__((always_inline)) {
+      if constexpr (KV) {
+        const uint32_t la = lds0 + stage + 2 * S::TILE + (S::BN + kb * 32 + 4 * hf) * 4;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 a = lds_load<f32x4>(la + g * 32);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dp[4 * g + e] = a[e];
+        }
+      }
+#pragma unroll
+      for (int st = 0; st < KST; ++st)
+        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rows_frag(Y, kb, st), own1[st], dp, 0, 0, 0);
+    };
+    if constexpr (KV) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) pr[r] = __builtin_amdgcn_exp2f(s[r] * p.c);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const bf16x8 pb = pack8(pr + 8 * ks);
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+          accv[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cols_frag(Y, kb * 2 + ks, db), pb, accv[db], 0, 0, 0);
+      }
+      second();
+#pragma unroll
+      for (int r = 0; r < 16; ++r) ds[r] = pr[r] * dp[r];
+    } else {
+      second();
+      auto mx2 = [](float a, float b) __attribute__((always_inline)) { return __builtin_elementwise_maximum(a, b); };
+      float mx = s[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) mx = mx2(mx, s[r]);
+      mx = half_max(mx) * p.c;
+      // the reference maximum moves only when a row's grows by more than 2^8
+      if (__builtin_amdgcn_ballot_w64(!(mx <= m_i + 8.0f)) != 0) {
+        const float m_new = mx2(m_i, mx);
+        const float alpha = m_i == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_i - m_new);
+        m_i = m_new;
+        l_i *= alpha;
+#pragma unroll
+        for (int i = 0; i < NDB; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][r] *= alpha;
+      }
+      const float base = m_i == -INFINITY ? 0.f : m_i;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        pr[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c, -base));
+        l_i += pr[r];
+        ds[r] = pr[r] * (dp[r] - delta);
+      }
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const bf16x8 db8 = pack8(ds + 8 * ks);
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+        acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cols_frag(X, kb * 2 + ks, db), db8, acc[db], 0, 0, 0);
+    }
+  };
+
+  // stream rows that some row of this wave sees
+  int w_lo = 0, w_hi = T;
+  if (p.window >= 0) {
+    w_lo = max(0, r0 - p.window);
+    w_hi = min(T, rlast + p.window + 1);
+  }
+  if (p.causal) {
+    if (KV) w_lo = max(w_lo, r0);
+    else w_hi = min(w_hi, rlast + 1);
+  }
+  if (!active) w_hi = 0;
+
+  load_head();
+  if (n_tiles > 0) issue(0);
+  int t = t_lo;
+  for (int i = 0; i < n_tiles; ++i) {
+    const uint32_t stage = (i & 1) * S::STAGE;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();
+    if (i + 1 < n_tiles) issue(((i + 1) & 1) * S::STAGE);
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb) {
+      const int s0 = t * S::BN + kb * 32;
+      if (s0 < w_hi && s0 + 32 > w_lo) block(stage, kb, s0);
+    }
+    if (++t == t_hi) t = t_lo;
+  }
+
+  // ---- results ----
+  const int osz = OUT16 ? 2 : 4;
+  const int64_t ho = (int64_t)head * p.head_dim * osz;
+  auto out = [&](char* at, int64_t stride, const f32x16 (&a)[NDB], float by) __attribute__((always_inline)) {
+    const __amdgpu_buffer_rsrc_t rs = pp_rsrc(at + txt.start * stride + ho, (uint32_t)T * (uint32_t)stride);
+    bwd_store<D, OUT16>(a, by, rs, own < T ? (uint32_t)own * (uint32_t)stride : BWD_NOWHERE, hf, p.head_dim);
+  };
+  if constexpr (KV) {
+    out(p.dk, p.dk_stride, acc, p.scale);
+    out(p.dv, p.dv_stride, accv, 1.f);
+  } else {
+    const float l = half_sum(l_i);
+    if (p.dq) out(p.dq, p.dq_stride, acc, p.scale / l);
+    if (hf == 0 && own < T) {
+      float* st = p.stat + (int64_t)head * p.rows + txt.start + own;
+      st[0] = -(m_i + log2f(l)) / p.c;
+      st[(int64_t)p.h_q * p.rows] = -delta;
+    }
+  }
+}
+
+struct BwdTable {
+  BwdText at[BWD_INLINE];
+};
+__global__ __launch_bounds__(BWD_INLINE) void bwd_table_kernel(BwdTable t, BwdText* out, int n) {
+  if ((int)threadIdx.x < n) out[threadIdx.x] = t.at[threadIdx.x];
+}
+
+}  // namespace
+
+}  // namespace inl
+
+namespace inl {
+
+namespace {
+
+typedef void (*AttnBwdFn)(AttnBwdParams);
+
+template <int D>
+AttnBwdFn bwd_fn(bool kv, bool out16) {
+  return kv ? (out16 ? attn_bwd_kernel<D, true, true> : attn_bwd_kernel<D, true, false>)
+            : (out16 ? attn_bwd_kernel<D, false, true> : attn_bwd_kernel<D, false, false>);
+}
+
+size_t bwd_stat_bytes(const inl_attn_desc& d, int64_t rows) { return ((size_t)2 * d.h_q * rows * 4 + 255) & ~(size_t)255; }
+
+// Checks what the forward's desc leaves open, and lists the texts that have tokens.
+int bwd_texts(const inl_attn_desc* d, int64_t* rows, std::vector<BwdText>* texts) {
+  int rc = attn_check(d, rows);
+  if (rc) return rc;
+  if (d->dtype != INL_BF16 || d->out_dtype != INL_BF16)
+    return fail(INL_E_UNSUPPORTED, "attention backward: q, k, v, out and dout must be bf16");
+  texts->reserve(d->n_texts);
+  for (int32_t b = 0; b < d->n_texts; ++b) {
+    const int32_t at = d->cu_seqlens_host[b], len = d->cu_seqlens_host[b + 1] - at;
+    if (len > 0) texts->push_back({d->seq_starts_host ? d->seq_starts_host[b] : at, len, 0});
+  }
+  if (d->seq_starts_host) {   // a row of two texts would get two gradients
+    std::vector<BwdText> by(*texts);
+    std::sort(by.begin(), by.end(), [](const BwdText& a, const BwdText& b) { return a.start < b.start; });
+    for (size_t i = 1; i < by.size(); ++i)
+      if (by[i].start < by[i - 1].start + by[i - 1].len)
+        return fail(INL_E_INVALID, "attention backward: texts overlap (seq_starts_host)");
+  }
+  return INL_OK;
+}
+
+size_t bwd_bytes(const inl_attn_desc& d, int64_t rows, size_t texts) {
+  return texts == 0 ? 0 : bwd_stat_bytes(d, rows) + (texts > (size_t)BWD_INLINE ? texts * sizeof(BwdText) : 0);
+}
+
+struct BwdTensor {
+  const char* what;
+  const void* at;
+  int64_t heads, stride;   // elements
+  int32_t dtype;
+};
+
+int bwd_run(const inl_attn_desc* d, const inl_attn_grads* g, const void* q, const void* k, const void* v, const void* o,
+            const void* dout, void* dq, void* dk, void* dv, void* ws, size_t ws_bytes, hipStream_t st) {
+  if (!g) return fail(INL_E_INVALID, "attention backward: grads is NULL");
+  int64_t rows = 0;
+  std::vector<BwdText> texts;
+  int rc = bwd_texts(d, &rows, &texts);
+  if (rc) return rc;
+  if (!dtype_ok(g->grad_dtype)) return fail(INL_E_INVALID, "attention backward: grad_dtype must be INL_F32 or INL_BF16");
+  if (!dk != !dv) return fail(INL_E_INVALID, "attention backward: dk and dv are computed together (or both NULL)");
+  const int64_t qr = (int64_t)d->h_q * d->head_dim, kr = (int64_t)d->h_kv * d->head_dim;
+  const BwdTensor t[8] = {{"q", q, d->h_q, d->q_row_stride ? d->q_row_stride : qr, INL_BF16},
+                          {"k", k, d->h_kv, d->k_row_stride ? d->k_row_stride : kr, INL_BF16},
+                          {"v", v, d->h_kv, d->v_row_stride ? d->v_row_stride : kr, INL_BF16},
+                          {"out", o, d->h_q, d->o_row_stride ? d->o_row_stride : qr, INL_BF16},
+                          {"dout", dout, d->h_q, g->do_row_stride ? g->do_row_stride : qr, INL_BF16},
+                          {"dq", dq, d->h_q, g->dq_row_stride ? g->dq_row_stride : qr, g->grad_dtype},
+                          {"dk", dk, d->h_kv, g->dk_row_stride ? g->dk_row_stride : kr, g->grad_dtype},
+                          {"dv", dv, d->h_kv, g->dv_row_stride ? g->dv_row_stride : kr, g->grad_dtype}};
+  int64_t longest = 0;
+  for (const BwdText& x : texts) longest = std::max<int64_t>(longest, x.len);
+  Rows r[8];
+  for (int i = 0; i < 8; ++i) {
+    const int64_t es = dtype_size(t[i].dtype), len = t[i].heads * d->head_dim;
+    if (t[i].stride < len || (t[i].stride * es) % 16)
+      return fail(INL_E_INVALID, std::string("attention backward: ") + t[i].what +
+                                     ": the row stride must cover all heads and be a multiple of 16 bytes");
+    if ((!t[i].at && i < 5 && rows) || ((uintptr_t)t[i].at & 15))
+      return fail(INL_E_INVALID, std::string("attention backward: ") + t[i].what + " must be non-null and 16-byte aligned");
+    // rows of a text are addressed with 32 bits
+    if (longest * t[i].stride * es >= (int64_t)BWD_NOWHERE)
+      return fail(INL_E_UNSUPPORTED, std::string("attention backward: a text's rows of ") + t[i].what + " span 4 GiB or more");
+    r[i] = {t[i].at, rows, len * es, t[i].stride * es};
+  }
+  for (int i = 5; i < 8; ++i)
+    for (int j = 0; j < i; ++j)
+      if (rows_meet(r[i], r[j]))
+        return fail(INL_E_INVALID, std::string("attention backward: ") + t[i].what + " overlaps " + t[j].what);
+  if (texts.empty() || (!dq && !dk)) return INL_OK;
+  if ((rc = check_workspace("attention backward", ws, ws_bytes, bwd_bytes(*d, rows, texts.size())))) return rc;
+
+  // Longest texts first, so that the last workgroups are short ones.
+  std::sort(texts.begin(), texts.end(), [](const BwdText& a, const BwdText& b) {
+    return a.len != b.len ? a.len > b.len : a.start < b.start;
+  });
+  int64_t units = 0;
+  for (BwdText& x : texts) {
+    x.unit = (int32_t)units;
+    units += (x.len + BWD_BM - 1) / BWD_BM;
+  }
+  if (units * d->h_q > INT32_MAX)
+    return fail(INL_E_UNSUPPORTED, "attention backward: more than 2^31 blocks of query rows and heads");
+  AttnBwdParams p{};
+  p.q = (const char*)q;
+  p.k = (const char*)k;
+  p.v = (const char*)v;
+  p.o = (const char*)o;
+  p.dout = (const char*)dout;
+  p.dq = (char*)dq;
+  p.dk = (char*)dk;
+  p.dv = (char*)dv;
+  int64_t* const strides[8] = {&p.q_stride, &p.k_stride, &p.v_stride, &p.o_stride,
+                               &p.do_stride, &p.dq_stride, &p.dk_stride, &p.dv_stride};
+  for (int i = 0; i < 8; ++i) *strides[i] = t[i].stride * dtype_size(t[i].dtype);
+  p.stat = (float*)ws;
+  p.rows = rows;
+  p.n_texts = (int32_t)texts.size();
+  p.n_units = (int32_t)units;
+  p.h_q = d->h_q;
+  p.h_kv = d->h_kv;
+  p.group = d->h_q / d->h_kv;
+  p.head_dim = d->head_dim;
+  p.causal = d->causal;
+  p.window = d->window;
+  // (the statistics are divided by c, and must stay finite; scores times less than this are 0)
+  p.c = std::max(d->scale * kLog2e, 1e-30f);
+  p.scale = d->scale;
+  if (texts.size() <= (size_t)BWD_INLINE) {
+    std::copy(texts.begin(), texts.end(), p.own);
+  } else {
+    // More texts go through the workspace, by launches that carry them as arguments: a copy from
+    // host memory could not be captured, nor its source freed.
+    BwdText* table = (BwdText*)((char*)ws + bwd_stat_bytes(*d, rows));
+    for (size_t i = 0; i < texts.size(); i += BWD_INLINE) {
+      BwdTable part{};
+      const int n = (int)std::min<size_t>(BWD_INLINE, texts.size() - i);
+      std::copy(texts.begin() + i, texts.begin() + i + n, part.at);
+      hipLaunchKernelGGL(bwd_table_kernel, dim3(1), dim3(BWD_INLINE), 0, st, part, table + i, n);
+    }
+    p.texts = table;
+  }
+  const bool out16 = g->grad_dtype == INL_BF16;
+  for (int kv = 0; kv < (dk ? 2 : 1); ++kv) {
+    AttnBwdFn fn = d->head_dim <= 64 ? bwd_fn<64>(kv, out16) : d->head_dim <= 128 ? bwd_fn<128>(kv, out16) : bwd_fn<256>(kv, out16);
+    const int lds = d->head_dim <= 64 ? BwdShape<64>::LDS : d->head_dim <= 128 ? BwdShape<128>::LDS : BwdShape<256>::LDS;
+    if ((rc = set_max_dynamic_lds((const void*)fn, lds))) return rc;
+    hipLaunchKernelGGL(fn, dim3((unsigned)(units * (kv ? d->h_kv : d->h_q))), dim3(256), lds, st, p);
+    INL_HIP_TRY(hipGetLastError());
+  }
+  return INL_OK;
+}
+
+}  // namespace
+
+}  // namespace inl
+
+extern "C" int inl_attn_bwd_workspace_size(const inl_attn_desc* d, size_t* bytes) {
+  using namespace inl;
+  if (!bytes) return fail(INL_E_INVALID, "attention backward: bytes is NULL");
+  try {
+    int64_t rows = 0;
+    std::vector<BwdText> texts;
+    int rc = bwd_texts(d, &rows, &texts);
+    if (rc) return rc;
+    *bytes = bwd_bytes(*d, rows, texts.size());
+    return INL_OK;
+  } catch (const std::bad_alloc&) {
+    return fail(INL_E_NOMEM, "attention backward: out of host memory");
+  }
+}
+
+extern "C" int inl_attn_varlen_bwd(const inl_attn_desc* d, const inl_attn_grads* g, const void* q, const void* k,
+                                   const void* v, const void* out, const void* dout, void* dq, void* dk, void* dv,
+                                   void* ws, size_t ws_bytes, void* stream) {
+  using namespace inl;
+  try {
+    return bwd_run(d, g, q, k, v, out, dout, dq, dk, dv, ws, ws_bytes, (hipStream_t)stream);
+  } catch (const std::bad_alloc&) {
+    return fail(INL_E_NOMEM, "attention backward: out of host memory");
+  }
+}

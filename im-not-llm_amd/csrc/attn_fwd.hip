@@ -1440,6 +1440,9 @@ int check_ptrs(const void* q, const void* k, const void* v, const void* out, int
 }  // namespace inl
 
 namespace inl {
+
+int attn_check(const inl_attn_desc* desc, int64_t* rows) { return validate_desc(desc, rows); }
+
 namespace {
 
 // Upload a schedule into device memory `buf` (a caller workspace or the

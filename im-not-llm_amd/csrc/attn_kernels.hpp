@@ -37,6 +37,9 @@ struct AttnParams {
   float2* part_ml;    // [slot][32 rows] {max (log2 domain, scaled), sum}
 };
 
+// The checks of a desc that every attention entry makes. Returns the rows that it covers.
+int attn_check(const inl_attn_desc* desc, int64_t* rows);
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Max / sum of x over lanes l and l ^ 32, without an LDS round trip:

@@ -1193,4 +1193,4 @@ def unit_lower_inverse(a, *, stream=None):
 
 if "torch" in globals():   # the rest of the package does without it
     from .train import (ROPE_AXIAL, ROPE_HALF, ROPE_INTERLEAVED, dense, dense_bwd, gated_ffn,  # noqa: E402,F401
-                        gated_ffn_bwd, norm_rope_qk_bwd, softmax_xent, softmax_xent_bwd)
+                        gated_ffn_bwd, norm_rope_qk_bwd, softmax_xent, softmax_xent_bwd, varlen_attention_bwd)

@@ -17,8 +17,8 @@ import functools
 
 import torch
 
-from . import (INL_BF16, INL_F32, InlError, NormRopeDesc, _check, _dtype_code, _head_rows, _head_weight,
-               _rope_tables, _sig, c_i32, c_i64, c_void_p)
+from . import (INL_BF16, INL_F32, AttnDesc, InlError, NormRopeDesc, _check, _dtype_code, _head_rows, _head_weight,
+               _rope_tables, _sig, c_i32, c_i64, c_void_p, desc_rows, make_attn_desc)
 
 ACTS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu_tanh": 3, "gelu_erf": 4}
 ROPE_HALF, ROPE_AXIAL, ROPE_INTERLEAVED = 1, 2, 3
@@ -43,6 +43,11 @@ class SoftmaxXentDesc(ctypes.Structure):
                [("scale", ctypes.c_float)] + [(n, c_i32) for n in ("ignore_index", "dx_dtype", "dw_dtype")]
 
 
+class AttnGrads(ctypes.Structure):
+    _fields_ = [(n, c_i64) for n in ("do_row_stride", "dq_row_stride", "dk_row_stride", "dv_row_stride")] + \
+               [("grad_dtype", c_i32)]
+
+
 def _ptrs(n):
     return [c_void_p] * n
 
@@ -63,6 +68,10 @@ _rope_bwd_ws = _sig("inl_norm_rope_bwd_workspace_size", ctypes.c_int, ctypes.POI
 _rope_bwd = _sig("inl_norm_rope_qk_bwd", ctypes.c_int, ctypes.POINTER(NormRopeDesc), c_i32, *_ptrs(3), c_i64,
                  *_ptrs(10), ctypes.c_size_t, c_void_p)
 
+
+_attn_bwd_ws = _sig("inl_attn_bwd_workspace_size", ctypes.c_int, ctypes.POINTER(AttnDesc), _size_p)
+_attn_bwd = _sig("inl_attn_varlen_bwd", ctypes.c_int, ctypes.POINTER(AttnDesc), ctypes.POINTER(AttnGrads), *_ptrs(9),
+                 ctypes.c_size_t, c_void_p)
 
 _BF16, _F32 = torch.bfloat16, torch.float32
 _B16, _ANY = (_BF16,), (_BF16, _F32)
@@ -419,3 +428,66 @@ def norm_rope_qk_bwd(dy, x, q_heads, rows=None, cos=None, sin=None, *, q_weight=
     del round_norm
     return _rope_grads(x, dy, q_heads, rows, cos, sin, q_weight, k_weight, eps, norm, rotary_dim, sections, cos2, sin2,
                        round_tables, out, weight_grad, stream)
+
+
+# ---------------------------------------------------------------------------
+# Attention
+# ---------------------------------------------------------------------------
+
+def _head_tensor(name, t, rows, heads, hd, dtype, dev):
+    """The stride between the token rows of ``t [rows or more, heads, hd]``."""
+    if len(t.shape) != 3 or t.shape[1:] != (heads, hd):
+        raise InlError(-1, f"{name}: shape {tuple(t.shape)}, need [rows, {heads}, {hd}]")
+    if t.dtype is not dtype:
+        raise InlError(-1, f"{name}: dtype {t.dtype}, need {dtype}")
+    if t.shape[0] < rows:
+        raise InlError(-1, f"{name}: {t.shape[0]} rows, the texts cover {rows}")
+    return _head_rows(name, t, t.shape, dev)
+
+
+@_at_home
+def _attn_grads(dev, q, dout, k, v, out, cu_seqlens, causal, window, scale, seq_starts, grad_dtype, grads, kv_grad):
+    if len(q.shape) != 3 or len(k.shape) != 3:
+        raise InlError(-1, f"q, k: shapes {tuple(q.shape)}, {tuple(k.shape)}, need [rows, heads, head_dim]")
+    n, hq, hd = q.shape
+    hkv = k.shape[1]
+    d = make_attn_desc(cu_seqlens, hq, hkv, hd, causal=causal, window=window, scale=scale, seq_starts=seq_starts)
+    rows = desc_rows(d)
+    d.q_row_stride = _head_tensor("q", q, rows, hq, hd, _BF16, dev)
+    d.k_row_stride = _head_tensor("k", k, rows, hkv, hd, _BF16, dev)
+    d.v_row_stride = _head_tensor("v", v, rows, hkv, hd, _BF16, dev)
+    d.o_row_stride = _head_tensor("out", out, rows, hq, hd, _BF16, dev)
+    dos = _head_tensor("dout", dout, rows, hq, hd, _BF16, dev)
+    if grads is None:
+        # rows of no text have no gradient: they are zero in tensors made here
+        made = torch.zeros if seq_starts is not None or n != rows or k.shape[0] != rows else torch.empty
+        dt = grad_dtype or _BF16
+        dq = made((n, hq, hd), dtype=dt, device=q.device)
+        dk, dv = (made((k.shape[0], hkv, hd), dtype=dt, device=q.device) for _ in range(2)) if kv_grad else (None, None)
+    else:
+        dq, dk, dv = grads
+        dt = next((t.dtype for t in grads if t is not None), _BF16)
+        if grad_dtype is not None and grad_dtype is not dt:
+            raise InlError(-1, f"grads: dtype {dt}, grad_dtype {grad_dtype}")
+    strides = [0 if t is None else _head_tensor(name, t, rows, heads, hd, dt, dev)
+               for name, t, heads in (("dq", dq, hq), ("dk", dk, hkv), ("dv", dv, hkv))]
+    g = AttnGrads(dos, *strides, _dtype_code(dt))
+    size = ctypes.c_size_t()
+    _check(_attn_bwd_ws(d, ctypes.byref(size)))
+    room = _room(size.value, dev)
+    _check(_attn_bwd(d, g, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), _ptr(dq),
+                     _ptr(dk), _ptr(dv), _ptr(room), size.value, _stream(dev)))
+    return dq, dk, dv
+
+
+def varlen_attention_bwd(dout, q, k, v, out, cu_seqlens, *, causal, window=-1, scale=None, seq_starts=None,
+                         grad_dtype=None, grads=None, kv_grad=True, stream=None):
+    """``(dq, dk, dv)`` of ``varlen_attention`` from bf16 ``dout [N, Hq, D]`` and the
+    forward's bf16 ``out`` (``inl_attn_varlen_bwd``); the other arguments as in the
+    forward. The probabilities are recomputed. dq, dk and dv are bf16 unless
+    ``grad_dtype`` says float32 (P and dS are rounded to bf16 in between all the same);
+    ``kv_grad=False`` leaves dk and dv out (None). ``grads=(dq, dk, dv)`` are tensors to
+    write, slices of one ``[N, Hq + 2 Hkv, D]`` row among them, None where not wanted; their
+    rows outside every text are left as they were, and zero in tensors made here."""
+    return _attn_grads(q, dout, k, v, out, cu_seqlens, causal, window, scale, seq_starts, grad_dtype, grads, kv_grad,
+                       stream)

@@ -185,6 +185,36 @@ int inl_norm_rope_qk_bwd(const inl_norm_rope_desc* desc, int32_t q_heads, const 
                          const float* sin, const float* cos2, const float* sin2, float* dq_weight, float* dk_weight,
                          void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Gradients of inl_attn_varlen_fwd (inl_hip.h), with its desc: per text and head
+ *   P = softmax of scale q k^T over the visible keys, dP = dout v^T,
+ *   dS = P (dP - rowsum(dout out));
+ *   dq = scale dS k,  dk = scale dS^T q,  dv = P^T dout
+ * dk and dv summed over the query heads of their key head. The probabilities are
+ * recomputed from q and k, so the forward keeps nothing but its output. bf16 only:
+ * q, k, v, `out` (what the forward wrote, desc->out_dtype INL_BF16) and dout; P and
+ * dS are rounded to bf16 before the products that read them, all sums are f32, and
+ * the gradients are rounded once to grad_dtype. desc->flags change nothing.
+ * dq, dk, dv: NULL = not computed (dk and dv together); they share no byte with
+ * another argument or one another, but may be slices of one row. Rows outside every
+ * text are not written; with seq_starts_host the texts may not overlap. Infinities and
+ * NaNs in a text reach any gradient of that text and of no other. A text's rows of each tensor
+ * span less than 4 GiB. The texts' table travels with the launches: a captured call replays with
+ * the lengths it was captured with.
+ * --------------------------------------------------------------------- */
+typedef struct inl_attn_grads {
+  int64_t do_row_stride;   /* elements; 0 = h_q * head_dim */
+  int64_t dq_row_stride;   /* 0 = h_q * head_dim */
+  int64_t dk_row_stride;   /* 0 = h_kv * head_dim */
+  int64_t dv_row_stride;   /* 0 = h_kv * head_dim */
+  int32_t grad_dtype;      /* of dq, dk and dv: INL_BF16 or INL_F32 */
+} inl_attn_grads;
+
+int inl_attn_bwd_workspace_size(const inl_attn_desc* desc, size_t* bytes);
+int inl_attn_varlen_bwd(const inl_attn_desc* desc, const inl_attn_grads* grads, const void* q, const void* k,
+                        const void* v, const void* out, const void* dout, void* dq, void* dk, void* dv,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
