@@ -48,6 +48,12 @@ class AttnGrads(ctypes.Structure):
                [("grad_dtype", c_i32)]
 
 
+class AddNormDesc(ctypes.Structure):
+    _fields_ = [(n, c_i64) for n in ("m", "n", "x_stride", "residual_stride", "h_stride", "y_stride", "dh_stride")] + \
+               [("eps", ctypes.c_float)] + \
+               [(n, c_i32) for n in ("drop", "tag", "x_dtype", "stream_dtype", "out_dtype", "weight_dtype")]
+
+
 def _ptrs(n):
     return [c_void_p] * n
 
@@ -72,6 +78,14 @@ _rope_bwd = _sig("inl_norm_rope_qk_bwd", ctypes.c_int, ctypes.POINTER(NormRopeDe
 _attn_bwd_ws = _sig("inl_attn_bwd_workspace_size", ctypes.c_int, ctypes.POINTER(AttnDesc), _size_p)
 _attn_bwd = _sig("inl_attn_varlen_bwd", ctypes.c_int, ctypes.POINTER(AttnDesc), ctypes.POINTER(AttnGrads), *_ptrs(9),
                  ctypes.c_size_t, c_void_p)
+_add_norm = _sig("inl_add_rms_norm_fwd", ctypes.c_int, ctypes.POINTER(AddNormDesc), *_ptrs(7))
+_add_norm_ws = _sig("inl_add_rms_norm_bwd_workspace_size", ctypes.c_int, ctypes.POINTER(AddNormDesc), _size_p)
+_add_norm_bwd = _sig("inl_add_rms_norm_bwd", ctypes.c_int, ctypes.POINTER(AddNormDesc), *_ptrs(9), ctypes.c_size_t,
+                     c_void_p)
+_pool_mean_bwd = _sig("inl_pool_mean_bwd", ctypes.c_int, c_i32, c_void_p, c_i32, c_i64, c_i64, c_i32, *_ptrs(4))
+_pool_last_ws = _sig("inl_pool_last_bwd_workspace_size", ctypes.c_int, c_i32, c_i32, _size_p)
+_pool_last_bwd = _sig("inl_pool_last_bwd", ctypes.c_int, c_i32, c_void_p, c_i32, c_i64, c_i64, c_i32, *_ptrs(3),
+                      ctypes.c_float, c_i64, c_i32, *_ptrs(3), ctypes.c_size_t, c_void_p)
 
 _BF16, _F32 = torch.bfloat16, torch.float32
 _B16, _ANY = (_BF16,), (_BF16, _F32)
@@ -491,3 +505,183 @@ def varlen_attention_bwd(dout, q, k, v, out, cu_seqlens, *, causal, window=-1, s
     rows outside every text are left as they were, and zero in tensors made here."""
     return _attn_grads(q, dout, k, v, out, cu_seqlens, causal, window, scale, seq_starts, grad_dtype, grads, kv_grad,
                        stream)
+
+
+# ---------------------------------------------------------------------------
+# The residual stream: addition, dropout, norm
+# ---------------------------------------------------------------------------
+
+def _drop(dropout, rng, dev, draws=True):
+    """The dropped share in 1 / 65536 and the address of the generator's state."""
+    if not 0.0 <= dropout < 1.0 or round(dropout * 65536) > 65535:
+        raise InlError(-1, f"dropout {dropout} must be in [0, 1)")
+    drop = round(dropout * 65536)
+    if not drop or not draws:
+        return drop, None
+    if rng is None or rng.dtype is not torch.int64 or rng.shape != (2,) or rng.get_device() != dev or rng.stride(0) != 1:
+        raise InlError(-1, f"rng: dropout needs contiguous torch.int64 [2] on cuda:{dev}"
+                           + ("" if rng is None else f", got {rng.dtype} {tuple(rng.shape)} on {rng.device}"))
+    return drop, rng.data_ptr()
+
+
+def _tag(tag):
+    if not -2 ** 31 <= tag < 2 ** 32:
+        raise InlError(-1, f"tag {tag} is no 32-bit number")
+    return tag - 2 ** 32 if tag >= 2 ** 31 else tag
+
+
+def _norm_weight(weight, n, dev):
+    if weight is None:
+        return INL_F32, None
+    if weight.dtype not in _ANY:
+        raise InlError(-1, f"weight: dtype {weight.dtype}, need torch.bfloat16 or torch.float32")
+    return _CODE[weight.dtype], _vec("weight", weight, n, weight.dtype, dev)
+
+
+@_at_home
+def _norm_fwd(dev, x, weight, residual, eps, dropout, rng, tag, out, sum_out, out_dtype, sum_dtype):
+    m, n = _matrix("x", x)
+    drop, rp = _drop(dropout, rng, dev)
+    xs = _mat("x", x, m, n, _ANY, dev)
+    rs = 0
+    if residual is not None:
+        rs = _mat("residual", residual, m, n, _ANY, dev)
+        sum_dtype = sum_dtype or residual.dtype
+        if sum_dtype is not residual.dtype:
+            raise InlError(-1, f"sum_dtype {sum_dtype}: the residual is {residual.dtype}")
+    wd, wp = _norm_weight(weight, n, dev)
+    if out is None:
+        out = x.new_empty((m, n), dtype=out_dtype)
+    ys = _mat("out", out, m, n, _ANY, dev)
+    h = sum_out
+    if h is None:
+        sd = sum_dtype or x.dtype
+        # the sum of nothing is x itself
+        h = x if residual is None and not drop and sd is x.dtype else x.new_empty((m, n), dtype=sd)
+    elif sum_dtype is not None and sum_dtype is not h.dtype:
+        raise InlError(-1, f"sum_out: dtype {h.dtype}, need {sum_dtype}")
+    hs = _mat("sum_out", h, m, n, _ANY, dev)
+    d = AddNormDesc(m, n, xs, rs, hs, ys, 0, eps, drop, _tag(tag), _CODE[x.dtype], _CODE[h.dtype], _CODE[out.dtype], wd)
+    _check(_add_norm(d, x.data_ptr(), _ptr(residual), wp, rp, None if h is x else h.data_ptr(), out.data_ptr(),
+                     _stream(dev)))
+    return out, h
+
+
+def add_rms_norm(x, weight=None, *, residual=None, eps=1e-6, dropout=0.0, rng=None, tag=0, out=None, sum_out=None,
+                 out_dtype=None, sum_dtype=None, stream=None):
+    """``(y, h)`` with ``h = residual + drop(x)`` and ``y = h / sqrt(mean(h^2) + eps) * weight``
+    (``inl_add_rms_norm_fwd``): bf16 or f32 ``x [m, n]`` and ``weight [n]``, ``residual [m, n]`` or None; n a multiple of 8,
+    at most 16384; rows may be strided. h has the residual's dtype (without one ``sum_dtype``, x's by
+    default) and may go into ``sum_out``, which may be the residual itself; y has x's dtype unless
+    ``out_dtype`` says otherwise. ``dropout``: the probability (in steps of 1 / 65536); its draws come from
+    ``rng``, int64 ``[2]`` on the device (seed, step), and ``tag``, a number of this place
+    in the model; no mask is kept."""
+    return _norm_fwd(x, weight, residual, eps, dropout, rng, tag, out, sum_out, out_dtype, sum_dtype, stream)
+
+
+@_at_home
+def _norm_grads(dev, h, dy, weight, dh, eps, dropout, rng, tag, x_grad, residual_grad, weight_grad, dx_dtype):
+    m, n = _matrix("h", h)
+    drop, rp = _drop(dropout, rng, dev, x_grad)
+    hs, ys = _mat("h", h, m, n, _ANY, dev), _mat("dy", dy, m, n, _ANY, dev)
+    ds = 0
+    if dh is not None:
+        ds = _mat("dh", dh, m, n, (h.dtype,), dev)
+    wd, wp = _norm_weight(weight, n, dev)
+    if dx_dtype is None:
+        dx_dtype = dy.dtype
+    # without dropout x's gradient is the residual's, in its own dtype
+    same = x_grad and not drop and dx_dtype is h.dtype
+    dres = h.new_empty((m, n)) if residual_grad or same else None
+    dx = h.new_empty((m, n), dtype=dx_dtype) if x_grad and not same else None
+    dw = h.new_empty(n, dtype=_F32) if weight_grad and weight is not None else None
+    d = AddNormDesc(m, n, 0, 0, hs, ys, ds, eps, drop, _tag(tag), _dtype_code(dx_dtype), _CODE[h.dtype],
+                    _CODE[dy.dtype], wd)
+    size = ctypes.c_size_t()
+    if dw is not None:
+        _check(_add_norm_ws(d, ctypes.byref(size)))
+    room = _room(size.value, dev)
+    _check(_add_norm_bwd(d, dy.data_ptr(), h.data_ptr(), _ptr(dh), wp, rp, _ptr(dx), _ptr(dres), _ptr(dw), _ptr(room),
+                         size.value, _stream(dev)))
+    return dres if same else dx, dres if residual_grad else None, dw
+
+
+def add_rms_norm_bwd(dy, h, weight=None, *, dh=None, eps=1e-6, dropout=0.0, rng=None, tag=0, x_grad=True,
+                     residual_grad=True, weight_grad=True, dx_dtype=None, stream=None):
+    """``(dx, dresidual, dweight)`` of ``add_rms_norm`` from ``dy [m, n]`` (y's dtype) and the ``h`` that it
+    returned (``inl_add_rms_norm_bwd``); ``dh`` (h's dtype) is the gradient that reaches h past the norm. ``dropout``, ``rng``
+    and ``tag`` as in the forward, with the step it had. dresidual has h's dtype, dx dy's unless ``dx_dtype`` says
+    otherwise (without dropout, and of one dtype, they are one tensor), dweight f32 ``[n]`` (None without a
+    weight); what is not asked for is None."""
+    return _norm_grads(h, dy, weight, dh, eps, dropout, rng, tag, x_grad, residual_grad, weight_grad, dx_dtype, stream)
+
+
+# ---------------------------------------------------------------------------
+# Pooled embedding
+# ---------------------------------------------------------------------------
+
+def _pooled(name, t, texts, dim, dev):
+    if t.shape != (texts, dim) or t.dtype is not _F32 or t.get_device() != dev or not t.is_contiguous():
+        raise InlError(-1, f"{name}: need contiguous torch.float32 {(texts, dim)} on cuda:{dev}, got {t.dtype} "
+                           f"{tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _offsets(cu, dev):
+    if len(cu.shape) != 1 or cu.shape[0] < 1 or cu.dtype is not torch.int32 or cu.get_device() != dev or not cu.is_contiguous():
+        raise InlError(-1, f"cu: need contiguous torch.int32 [texts + 1] on cuda:{dev}, got {cu.dtype} {tuple(cu.shape)} "
+                           f"on {cu.device}")
+    return cu.shape[0] - 1
+
+
+def _grad_rows(out, shape, dtype, like, dev):
+    if out is None:
+        out = like.new_empty(shape, dtype=dtype)
+    elif dtype is not None and out.dtype is not dtype:
+        raise InlError(-1, f"out: dtype {out.dtype}, need {dtype}")
+    return out, _mat("out", out, *shape, _ANY, dev)
+
+
+@_at_home
+def _mean_grads(dev, dpooled, cu, rows, mean, dtype, out):
+    texts, dim = _matrix("dpooled", dpooled)
+    if _offsets(cu, dev) != texts:
+        raise InlError(-1, f"cu: {cu.shape[0] - 1} texts, dpooled has {texts}")
+    dp, mp = _pooled("dpooled", dpooled, texts, dim, dev), None if mean is None else _pooled("mean", mean, texts, dim, dev)
+    out, stride = _grad_rows(out, (int(rows), dim), dtype if out is not None else dtype or _BF16, dpooled, dev)
+    _check(_pool_mean_bwd(texts, cu.data_ptr(), dim, int(rows), stride, _CODE[out.dtype], dp, mp, out.data_ptr(),
+                          _stream(dev)))
+    return out
+
+
+def pool_mean_bwd(dpooled, cu, rows, *, mean=None, dtype=None, out=None, stream=None):
+    """The gradient ``[rows, dim]`` of ``pool_mean``'s hidden rows from f32 ``dpooled [texts, dim]``
+    (``inl_pool_mean_bwd``): bf16 unless ``dtype`` says float32, 0 in rows of no text. ``mean``: with
+    ``normalize=True`` in the forward, what it gives with ``normalize=False``, f32 ``[texts, dim]``."""
+    return _mean_grads(dpooled, cu, rows, mean, dtype, out, stream)
+
+
+@_at_home
+def _last_grads(dev, dpooled, hidden, cu, weight, eps, dtype, out, weight_grad):
+    rows, dim = _matrix("hidden", hidden)
+    texts = _offsets(cu, dev)
+    dp = _pooled("dpooled", dpooled, texts, dim, dev)
+    hs = _mat("hidden", hidden, rows, dim, _ANY, dev)
+    wp = _vec("weight", weight, dim, hidden.dtype, dev)
+    out, stride = _grad_rows(out, (rows, dim), dtype if out is not None else dtype or hidden.dtype, hidden, dev)
+    dw = hidden.new_empty(dim, dtype=_F32) if weight_grad and weight is not None else None
+    size = 4 * texts * dim if dw is not None and texts > 1 else 0
+    room = _room(size, dev)
+    _check(_pool_last_bwd(texts, cu.data_ptr(), dim, rows, hs, _CODE[hidden.dtype], dp, hidden.data_ptr(), wp, eps, stride,
+                          _CODE[out.dtype], out.data_ptr(), _ptr(dw), _ptr(room), size, _stream(dev)))
+    return out, dw
+
+
+def pool_last_bwd(dpooled, hidden, cu, weight=None, *, eps=1e-6, round_norm=False, dtype=None, out=None,
+                  weight_grad=True, stream=None):
+    """``(dhidden, dweight)`` of ``pool_last`` from f32 ``dpooled [texts, dim]`` and the forward's
+    arguments (``inl_pool_last_bwd``; ``round_norm`` changes nothing, gradients pass the rounding
+    unchanged). dhidden has hidden's dtype unless ``dtype`` says otherwise and is 0 but in the
+    texts' last rows; dweight is f32 ``[dim]``, None without a weight."""
+    del round_norm
+    return _last_grads(dpooled, hidden, cu, weight, eps, dtype, out, weight_grad, stream)

@@ -215,6 +215,77 @@ int inl_attn_varlen_bwd(const inl_attn_desc* desc, const inl_attn_grads* grads, 
                         const void* v, const void* out, const void* dout, void* dq, void* dk, void* dv,
                         void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * The residual stream's addition and the norm behind it:
+ *   h = residual + drop(x);  y = h / sqrt(mean(h^2) + eps) * weight
+ * per row of n values (a multiple of 8, at most 16384); beside inl_rms_norm_rows_fwd
+ * (inl_encoder.h), which norms a stream that has been added up already. x, y in x_dtype and
+ * out_dtype; residual and h in stream_dtype; weight: weight_dtype [n] or NULL (ones). y is
+ * made from h before that is rounded to the stream's type.
+ *   drop: each value is 0 with probability drop / 65536 and multiplied by
+ * 65536 / (65536 - drop) otherwise. The draws come from a counter, so no mask is kept: value
+ * i of 8 of group (row n + column) / 8 takes 16 bits, the low half of a word first, of Philox
+ * 4x32-10 of (group, group >> 32, tag, rng[1]) under the key rng[0], all 32-bit words, low
+ * word first. rng: two int64 on the device (seed, step), read when the call runs, so a replayed
+ * graph draws anew where the program advances the step; `tag` tells apart the places of a
+ * model that draw in one step. The gradient's call with the same three draws the same mask.
+ * --------------------------------------------------------------------- */
+typedef struct inl_add_norm_desc {
+  int64_t m;               /* rows, >= 0 */
+  int64_t n;
+  int64_t x_stride;        /* of x and dx; elements, 0 = n, as all */
+  int64_t residual_stride; /* of residual and dresidual */
+  int64_t h_stride;
+  int64_t y_stride;        /* of y and dy */
+  int64_t dh_stride;
+  float eps;
+  int32_t drop;            /* 0 (none) .. 65535 */
+  int32_t tag;
+  int32_t x_dtype;
+  int32_t stream_dtype;    /* of residual, h, dh, dresidual */
+  int32_t out_dtype;       /* of y and dy */
+  int32_t weight_dtype;
+} inl_add_norm_desc;
+
+/* residual: NULL = 0; rng: may be NULL without dropout; h: NULL = not stored. h and y may each be x or residual itself
+ * (same address, type and stride) and otherwise share no byte with another argument. */
+int inl_add_rms_norm_fwd(const inl_add_norm_desc* desc, const void* x, const void* residual, const void* weight,
+                         const int64_t* rng, void* h, void* y, void* stream);
+
+/* With dn = dy weight and rms = sqrt(mean(h^2) + eps) of the h that the forward stored:
+ *   g = (dn - h / rms mean(dn h / rms)) / rms + dh
+ *   dresidual = g,  dx = drop(g),  dweight = sum over rows of dy h / rms (f32 [n])
+ * dh: what reaches h past the norm (NULL = 0). dx, dresidual, dweight: NULL = not computed. dx and
+ * dresidual may each be dy, h or dh itself (not the same one). m = 0 gives dweight = 0. */
+int inl_add_rms_norm_bwd_workspace_size(const inl_add_norm_desc* desc, size_t* bytes);
+int inl_add_rms_norm_bwd(const inl_add_norm_desc* desc, const void* dy, const void* h, const void* dh,
+                         const void* weight, const int64_t* rng, void* dx, void* dresidual, float* dweight,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Gradients of the pooled embedding (inl_pool_mean_fwd, inl_pool_last_fwd of inl_hip.h): every row
+ * of dhidden [rows, hidden_dim] is written, in `dtype`; rows of no text get 0. cu: DEVICE
+ * int32 [n_texts + 1], read on the device; whatever it holds, nothing outside the rows is
+ * written. dpooled: f32 [n_texts, hidden_dim], packed.
+ * --------------------------------------------------------------------- */
+
+/* dhidden[r] = d / len of r's text, d = dpooled, or with `mean` (f32 [n_texts, hidden_dim]: what the
+ * forward gives with normalize = 0) its gradient through y = mean / s, s = sqrt(|mean|^2 + 1e-12):
+ *   d = (dpooled - y (y . dpooled)) / s */
+int inl_pool_mean_bwd(int32_t n_texts, const int32_t* cu, int32_t hidden_dim, int64_t rows, int64_t row_stride,
+                      int32_t dtype, const float* dpooled, const float* mean, void* dhidden, void* stream);
+
+/* With x the last row of a text in `hidden`, z = x / rms(x) * weight and y = z / sqrt(|z|^2 + 1e-12):
+ * the gradient of y in that row of dhidden (0 elsewhere), dweight = sum over texts (f32 [hidden_dim],
+ * NULL = not computed). hidden and weight (or NULL) in `dtype`; dhidden in dx_dtype with
+ * dx_stride. round_norm passes gradients through unchanged. Empty texts add nothing. dhidden shares no byte with
+ * hidden. */
+int inl_pool_last_bwd_workspace_size(int32_t n_texts, int32_t hidden_dim, size_t* bytes);
+int inl_pool_last_bwd(int32_t n_texts, const int32_t* cu, int32_t hidden_dim, int64_t rows, int64_t row_stride,
+                      int32_t dtype, const float* dpooled, const void* hidden, const void* weight, float eps,
+                      int64_t dx_stride, int32_t dx_dtype, void* dhidden, float* dweight, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
