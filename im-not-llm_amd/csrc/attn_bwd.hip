@@ -44,18 +44,18 @@ struct BwdShape {
   static constexpr int BN = D <= 128 ? 64 : 32;   // stream rows of a tile
   static constexpr int ROW = D * 2;
   static constexpr int TILE = BN * ROW;           // bytes of X, and of Y
-  static constexpr int STAT = 2 * BN * 4;         // log-sum-exp and delta of the stream rows
-  static constexpr int STAGE = 2 * TILE + STAT;
-  static constexpr int LDS = 2 * STAGE;
+  static constexpr int STAGE = 2 * TILE;          // a power of two: the other stage is an XOR away
+  static constexpr int STATS = 2 * STAGE;         // log-sum-exp and delta of the stream rows, per stage
+  static constexpr int STAT = 2 * BN * 4;
+  static constexpr int LDS = STATS + 2 * STAT;
 };
 
-// 16-byte chunk c of row r lies at chunk c ^ bwd_swz(r) of that row. The 16 rows that a
-// row read touches at one logical chunk fall into 16 different 16-byte slots of 256, and so do
-// the 4 rows x 4 chunks of a transposed read.
-template <int D>
-__device__ __forceinline__ int bwd_swz(int r) {
-  return D == 64 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
-}
+// A tile of BN rows lies in groups of 64 features (a 128-byte line): 16-byte chunk c of row r at
+//   ((c / 8) BN + r) 128 + ((c % 8) ^ bwd_swz(r)) 16.
+// 16 rows at one chunk (a row read) fill 256 bytes, and so do 4 rows at 4 chunks (a transposed read): no
+// bank conflicts; and an address is one of four of a lane plus a constant, for every k-step and
+// every block of features.
+__device__ __forceinline__ int bwd_swz(int r) { return (((r >> 1) & 1) << 2) | ((r >> 2) & 3); }
 
 __device__ __forceinline__ bf16x8 pack8(const float* x) {
   u32x4 o;
@@ -116,6 +116,126 @@ __device__ __forceinline__ BwdText bwd_text(const BwdText* texts, int n, int u, 
           __builtin_amdgcn_readfirstlane(t.unit)};
 }
 
+// acc += rows . opnd over the features of 32 stream rows, at base[step % 4] (a lane's row and chunk) + off;
+// fragments are read RD - 1 products ahead, so that a product waits for its own read only. `first`: what
+// acc starts from.
+template <int D, int BN, int RD>
+__device__ __forceinline__ void rows_product(f32x16& acc, const f32x16& first, const uint32_t (&base)[4], uint32_t off,
+                                             const bf16x8 (&opnd)[D / 16]) {
+  constexpr int KST = D / 16;
+  u32x4 fr[RD];
+  auto read = [&](int st) __attribute__((always_inline)) {
+    fr[st % RD] = lds_load<u32x4>(base[st & 3] + off + (st >> 2) * BN * 128);
+  };
+#pragma unroll
+  for (int st = 0; st < RD - 1 && st < KST; ++st) read(st);
+#pragma unroll
+  for (int st = 0; st < KST; ++st) {
+    if (st + RD - 1 < KST) read(st + RD - 1);
+    __builtin_amdgcn_sched_barrier(0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, fr[st % RD]), opnd[st],
+                                                  st == 0 ? first : acc, 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// acc[d][own] += (32 stream rows, transposed) . x, likewise: base[2 (block of 32 features % 2) + (8 rows of 16)].
+template <int D, int BN, int RD>
+__device__ __forceinline__ void cols_product(f32x16 (&acc)[D / 32], const uint32_t (&base)[4], uint32_t off,
+                                             const bf16x8 (&x)[2]) {
+  constexpr int NDB = D / 32;
+  typedef short s16x8 __attribute__((ext_vector_type(8)));
+  s16x8 fr[RD];
+  auto read = [&](int i) __attribute__((always_inline)) {
+    const int ks = i / NDB, db = i % NDB;
+    s16x4 a[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      a[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(size_t)(
+          base[2 * (db & 1) + h] + off + (db >> 1) * BN * 128 + (ks * 16 + 8 * h) * 128));
+    fr[i % RD] = (s16x8){a[0][0], a[0][1], a[0][2], a[0][3], a[1][0], a[1][1], a[1][2], a[1][3]};
+  };
+#pragma unroll
+  for (int i = 0; i < RD - 1; ++i) read(i);
+#pragma unroll
+  for (int i = 0; i < 2 * NDB; ++i) {
+    if (i + RD - 1 < 2 * NDB) read(i + RD - 1);
+    __builtin_amdgcn_sched_barrier(0);
+    acc[i % NDB] =
+        __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, fr[i % RD]), x[i / NDB], acc[i % NDB], 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// 16 values, one per accumulator register, of 32 f32 values at `at` (+ 4 hf, a lane's)
+__device__ __forceinline__ f32x16 rows_stat(uint32_t at) {
+  f32x16 s;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const f32x4 a = lds_load<f32x4>(at + g * 32);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[4 * g + e] = a[e];
+  }
+  return s;
+}
+
+// 16 bytes a lane at rsrc + voff + off to LDS at lds + 16 lane. The instruction adds its offset to both
+// addresses; the s_nop is the wait between the write of M0 and the load.
+__device__ __forceinline__ void bwd_dma(i32x4 rsrc, uint32_t lds, uint32_t voff, int off) {
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen offset:%3 lds"
+               :: "v"(voff), "s"(rsrc), "{m0}"(lds - off), "n"(off) : "memory");
+}
+
+// A lane's LDS addresses in a tile at `tile`, from row `row0` on: row reads (k-steps of 16 features, modulo 4), and
+// transposed ones (blocks of 32 features modulo 2, rows 0-7 and 8-15 of 16): there 16 lanes read
+// 4 rows x 16 features, in the order of rows that the accumulators' registers have.
+__device__ __forceinline__ void bwd_row_reads(uint32_t (&at)[4], uint32_t tile, int row0, int lane) {
+  const int row = lane & 31, hf = lane >> 5;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) at[i] = tile + (row0 + row) * 128 + (((2 * i + hf) ^ bwd_swz(row)) << 4);
+}
+__device__ __forceinline__ void bwd_col_reads(uint32_t (&at)[4], uint32_t tile, int row0, int lane) {
+  const int g16 = lane >> 4, j16 = lane & 15, row = 4 * (lane >> 5) + (j16 >> 2);
+  const int c = 2 * (g16 & 1) + ((j16 & 3) >> 1);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    at[i] = tile + (row0 + row) * 128 + (((4 * (i >> 1) + c) ^ bwd_swz(row + 8 * (i & 1))) << 4) + ((j16 & 1) << 3);
+}
+
+// Tile loads by NW waves: 1 KB blocks of 8 rows x 128 bytes, the group's rows first; a wave's i-th
+// instruction loads block i NW + wave. Lanes whose chunk is behind the head load nothing, and find zeros there.
+template <int D, int BN, int NW>
+struct BwdLoad {
+  static constexpr int RBN = BN / 8;                              // blocks of a group
+  static constexpr int RP = RBN > NW ? RBN / NW : 1;              // a wave's blocks of one group
+  static constexpr int GP = D / 64 * RBN / NW / RP;               // groups that a wave takes part in
+  static constexpr int GSTEP = NW > RBN ? NW / RBN : 1;           // from one to the next
+  static_assert(RP * GP * NW == D / 64 * RBN && (NW * 8) % 16 == 0, "blocks of a tile");
+  uint32_t x, y;      // byte offset of this lane's chunk in X and Y, less the tile's first row
+  int chunk, g0;      // of the group; the wave's first group
+  __device__ __forceinline__ BwdLoad(int wave, int lane, uint32_t xst, uint32_t yst) {
+    const int row = 8 * (wave % RBN) + (lane >> 3);
+    g0 = wave / RBN;
+    chunk = (lane & 7) ^ bwd_swz(row);   // (the swizzle repeats every 16 rows)
+    x = row * xst + g0 * 128 + chunk * 16;
+    y = row * yst + g0 * 128 + chunk * 16;
+  }
+  __device__ __forceinline__ void issue(const i32x4& xrs, const i32x4& yrs, uint32_t at, uint32_t row, uint32_t xst,
+                                        uint32_t yst, int head_dim) const {
+#pragma unroll
+    for (int r = 0; r < RP; ++r) {
+      const uint32_t xa = x + (row + r * NW * 8) * xst, ya = y + (row + r * NW * 8) * yst;
+#pragma unroll
+      for (int g = 0; g < GP; ++g)
+        if (head_dim == D || (8 * (g0 + g * GSTEP) + chunk) * 8 < head_dim) {
+          const uint32_t lds = at + (g * GSTEP * RBN + r * NW) * 1024;
+          bwd_dma(xrs, lds, xa, g * GSTEP * 128);
+          bwd_dma(yrs, lds + D * 2 * BN, ya, g * GSTEP * 128);
+        }
+    }
+  }
+};
+
 // KV: own rows are keys (dk, dv); otherwise queries (dq, and the row statistics).
 template <int D, bool KV, bool OUT16>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwdParams p) {
@@ -123,10 +243,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwd
   constexpr int KST = D / 16;            // k-steps of the products over features
   constexpr int NDB = D / 32;            // 32-feature blocks of an accumulator
   constexpr int NKB = S::BN / 32;        // 32-row blocks of a tile
-  constexpr int CH = D / 8;              // 16-byte chunks per row
-  constexpr int RPB = 64 / CH;           // rows of a 1 KB block
-  constexpr int PARTS = S::TILE / 4096;  // 1 KB blocks of X (and of Y) per wave
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int RD = D == 128 && KV ? 3 : 4;   // fragments in flight
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -196,15 +314,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwd
   const int t_lo = s_lo / S::BN, t_hi = (s_hi + S::BN - 1) / S::BN;
   const int n_tiles = (t_hi - t_lo) * (KV ? p.group : 1);
 
-  uint32_t xg[PARTS], yg[PARTS];   // byte offset in a tile of what this lane loads
   const uint32_t xst = (uint32_t)(KV ? p.q_stride : p.k_stride), yst = (uint32_t)(KV ? p.do_stride : p.v_stride);
-#pragma unroll
-  for (int i = 0; i < PARTS; ++i) {
-    const int row = (i * 4 + wave) * RPB + lane / CH;
-    const int c = (lane % CH) ^ bwd_swz<D>(row);
-    const bool ok = c * 8 < p.head_dim;
-    xg[i] = ok ? row * xst + c * 16 : BWD_NOWHERE;
-    yg[i] = ok ? row * yst + c * 16 : BWD_NOWHERE;
+  const BwdLoad<D, S::BN, 4> load(wave, lane, xst, yst);
+  if (p.head_dim < D) {
+    for (int i = tid; i < S::LDS / 16; i += 256) lds_store<u32x4>(lds0 + i * 16, (u32x4){0u, 0u, 0u, 0u});
+    __syncthreads();
   }
   int dh = 0, dt = t_lo;   // load cursor: head of the group, tile
   i32x4 xrs, yrs, lrs, ers;
@@ -221,19 +335,15 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwd
       yrs = pp_rsrc_words(base_v, (uint32_t)T * yst);
     }
   };
-  auto issue = [&](uint32_t stage) __attribute__((always_inline)) {
-    const uint32_t at = lds0 + stage + wave * 1024;
+  auto issue = [&](int stage) __attribute__((always_inline)) {
+    const uint32_t at = lds0 + stage * S::STAGE + wave * 1024;
     const uint32_t s0 = (uint32_t)(dt * S::BN);
-#pragma unroll
-    for (int i = 0; i < PARTS; ++i) {
-      dma_b128(xrs, at + i * 4096, xg[i] == BWD_NOWHERE ? BWD_NOWHERE : s0 * xst + xg[i]);
-      dma_b128(yrs, at + S::TILE + i * 4096, yg[i] == BWD_NOWHERE ? BWD_NOWHERE : s0 * yst + yg[i]);
-    }
+    load.issue(xrs, yrs, at, s0, xst, yst, p.head_dim);
     if constexpr (KV) {
       // 4 bytes a lane; a tile of 32 rows fills half of its 64 (the rest is overwritten by nothing:
       // lanes from BN on are off)
       if (wave < 2 && lane < S::BN) {
-        const uint32_t dst = lds0 + stage + 2 * S::TILE + wave * S::BN * 4;
+        const uint32_t dst = lds0 + S::STATS + stage * S::STAT + wave * S::BN * 4;
         const i32x4 rs = wave == 0 ? lrs : ers;
         asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds"
                      :: "v"((s0 + lane) * 4), "s"(rs), "{m0}"(dst) : "memory");
@@ -245,25 +355,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwd
     }
   };
 
-  // ---- per-lane LDS offsets ----
-  const uint32_t xa = lq * S::ROW + ((hf ^ bwd_swz<D>(lq)) << 4);   // row reads: ^ (st << 5)
-  const int g16 = lane >> 4, j16 = lane & 15;
-  const int trow = 4 * hf + (j16 >> 2);
-  const uint32_t ta = trow * S::ROW + (((2 * (g16 & 1) + ((j16 & 3) >> 1)) ^ bwd_swz<D>(trow)) << 4) + ((j16 & 1) << 3);
-  auto rows_frag = [&](uint32_t tile, int kb, int st) __attribute__((always_inline)) {
-    return __builtin_bit_cast(bf16x8, lds_load<u32x4>(lds0 + (xa ^ (st << 5)) + tile + kb * 32 * S::ROW));
-  };
-  // 16 stream rows (k-step ks) x 32 features (block db), transposed: the order of the rows is
-  // that of the accumulators' registers
-  auto cols_frag = [&](uint32_t tile, int ks, int db) __attribute__((always_inline)) {
-    s16x4 a[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      a[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) s16x4*)(size_t)(lds0 + tile + (ta ^ (db << 6) ^ (h << 5)) + (ks * 16 + 8 * h) * S::ROW));
-    typedef short s16x8 __attribute__((ext_vector_type(8)));
-    return __builtin_bit_cast(bf16x8, (s16x8){a[0][0], a[0][1], a[0][2], a[0][3], a[1][0], a[1][1], a[1][2], a[1][3]});
-  };
+  // ---- per-lane LDS addresses in stage 0 ----
+  uint32_t xa[4], ta[4];
+  bwd_row_reads(xa, lds0, 0, lane);
+  bwd_col_reads(ta, lds0, 0, lane);
+  uint32_t la = lds0 + S::STATS + 16 * hf;
 
   f32x16 acc[NDB], accv[KV ? NDB : 1];
 #pragma unroll
@@ -272,23 +368,18 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwd
     if constexpr (KV) accv[i] = (f32x16){};
   }
   float m_i = -INFINITY, l_i = 0.f;
+  // dP^T - delta starts from -delta, where registers hold it 16 times
+  constexpr bool LESS = !KV && D <= 128;
+  f32x16 less = {};
+  if constexpr (LESS)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) less[r] = -delta;
 
   // One 32-row block of the stream against this wave's rows.
-  auto block = [&](uint32_t stage, int kb, int s0) __attribute__((always_inline)) {
-    const uint32_t X = stage, Y = stage + S::TILE;
-    f32x16 s = {}, dp = {};
-    if constexpr (KV) {
-      const uint32_t la = lds0 + stage + 2 * S::TILE + (kb * 32 + 4 * hf) * 4;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 a = lds_load<f32x4>(la + g * 32);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[4 * g + e] = a[e];
-      }
-    }
-#pragma unroll
-    for (int st = 0; st < KST; ++st)
-      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rows_frag(X, kb, st), own0[st], s, 0, 0, 0);
+  auto block = [&](int kb, int s0) __attribute__((always_inline)) {
+    const uint32_t X = kb * 32 * 128, Y = S::TILE + X;
+    f32x16 s, dp;
+    rows_product<D, S::BN, RD>(s, KV ? rows_stat(la + kb * 128) : (f32x16){}, xa, X, own0);
     // masks: stream row s0 + c of register r, c = 8 (r / 4) + 4 hf + r % 4
     const bool whole = (KV || s0 + 31 < T) && (!p.causal || (KV ? s0 >= rlast : s0 + 31 <= r0)) &&
                        (p.window < 0 || (s0 + 31 - r0 <= p.window && rlast - s0 <= p.window));
@@ -310,39 +401,21 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwd
       }
     }
     float pr[16], ds[16];
-    auto second = [&]() __attribute__((always_inline)) {
-      if constexpr (KV) {
-        const uint32_t la = lds0 + stage + 2 * S::TILE + (S::BN + kb * 32 + 4 * hf) * 4;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const f32x4 a = lds_load<f32x4>(la + g * 32);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) dp[4 * g + e] = a[e];
-        }
-      }
-#pragma unroll
-      for (int st = 0; st < KST; ++st)
-        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rows_frag(Y, kb, st), own1[st], dp, 0, 0, 0);
-    };
     if constexpr (KV) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) pr[r] = __builtin_amdgcn_exp2f(s[r] * p.c);
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        const bf16x8 pb = pack8(pr + 8 * ks);
-#pragma unroll
-        for (int db = 0; db < NDB; ++db)
-          accv[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cols_frag(Y, kb * 2 + ks, db), pb, accv[db], 0, 0, 0);
-      }
-      second();
+      const bf16x8 pb[2] = {pack8(pr), pack8(pr + 8)};
+      cols_product<D, S::BN, RD>(accv, ta, Y, pb);
+      rows_product<D, S::BN, RD>(dp, rows_stat(la + S::BN * 4 + kb * 128), xa, Y, own1);
 #pragma unroll
       for (int r = 0; r < 16; ++r) ds[r] = pr[r] * dp[r];
     } else {
-      second();
+      rows_product<D, S::BN, RD>(dp, less, xa, Y, own1);
       auto mx2 = [](float a, float b) __attribute__((always_inline)) { return __builtin_elementwise_maximum(a, b); };
-      float mx = s[0];
+      float m4[4];
 #pragma unroll
-      for (int r = 1; r < 16; ++r) mx = mx2(mx, s[r]);
+      for (int c = 0; c < 4; ++c) m4[c] = mx2(mx2(s[4 * c], s[4 * c + 1]), mx2(s[4 * c + 2], s[4 * c + 3]));
+      float mx = mx2(mx2(m4[0], m4[1]), mx2(m4[2], m4[3]));
       mx = half_max(mx) * p.c;
       // the reference maximum moves only when a row's grows by more than 2^8
       if (__builtin_amdgcn_ballot_w64(!(mx <= m_i + 8.0f)) != 0) {
@@ -360,16 +433,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwd
       for (int r = 0; r < 16; ++r) {
         pr[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c, -base));
         l_i += pr[r];
-        ds[r] = pr[r] * (dp[r] - delta);
+        ds[r] = pr[r] * (LESS ? dp[r] : dp[r] - delta);
       }
     }
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const bf16x8 db8 = pack8(ds + 8 * ks);
-#pragma unroll
-      for (int db = 0; db < NDB; ++db)
-        acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cols_frag(X, kb * 2 + ks, db), db8, acc[db], 0, 0, 0);
-    }
+    const bf16x8 db[2] = {pack8(ds), pack8(ds + 8)};
+    cols_product<D, S::BN, RD>(acc, ta, X, db);
   };
 
   // stream rows that some row of this wave sees
@@ -388,16 +456,21 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwd
   if (n_tiles > 0) issue(0);
   int t = t_lo;
   for (int i = 0; i < n_tiles; ++i) {
-    const uint32_t stage = (i & 1) * S::STAGE;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     lds_barrier();
-    if (i + 1 < n_tiles) issue(((i + 1) & 1) * S::STAGE);
+    if (i + 1 < n_tiles) issue((i + 1) & 1);
 #pragma unroll
     for (int kb = 0; kb < NKB; ++kb) {
       const int s0 = t * S::BN + kb * 32;
-      if (s0 < w_hi && s0 + 32 > w_lo) block(stage, kb, s0);
+      if (s0 < w_hi && s0 + 32 > w_lo) block(kb, s0);
     }
     if (++t == t_hi) t = t_lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      xa[e] ^= S::STAGE;
+      ta[e] ^= S::STAGE;
+    }
+    la = (i & 1) ? la - S::STAT : la + S::STAT;
   }
 
   // ---- results ----
@@ -421,6 +494,225 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwd
   }
 }
 
+// dk and dv of wide heads. One wave's registers do not hold the accumulators of both beside k
+// and v, so two waves share 32 keys, on one SIMD: the first makes P (from q and its k) and
+// accumulates dv, the second makes dP (from dO and its v), takes P from the first through LDS, and
+// accumulates dk. A stream tile is two phases with a barrier between: S and P beside dP, then dv
+// beside dS and dk; the first wave goes ahead of the second in the first phase (s_setprio), so
+// that its exponentials run under the other's products.
+// KG pairs of a workgroup's four own 32 keys each; where there are fewer, the others take
+// other rows of the stream for the same keys, and the sums meet in LDS at the end: half as
+// long a chain for a workgroup, for twice the tiles read.
+template <int D, int KG>
+struct PairShape {
+  static constexpr int QS = 4 / KG;               // parts of a stream tile
+  static constexpr int BN = 32 * QS;
+  static constexpr int ROW = D * 2;
+  static constexpr int TILE = BN * ROW;
+  static constexpr int STAGE = 2 * TILE;
+  static constexpr int SWAP = 2 * STAGE;          // P of every pair, f32
+  static constexpr int STATS = SWAP + 4 * 4096;
+  static constexpr int STAT = 2 * BN * 4;
+  static constexpr int LDS = STATS + 2 * STAT;
+};
+
+template <int D, int KG, bool OUT16>
+__global__ __launch_bounds__(512, 2) void attn_bwd_pair_kernel(AttnBwdParams p) {
+  using S = PairShape<D, KG>;
+  constexpr int KST = D / 16;
+  constexpr int NDB = D / 32;
+  constexpr int RD = 4;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int pair = wave & 3;
+  const bool second = wave >= 4;
+  const int kg = pair % KG, qg = pair / KG;
+  const int lq = lane & 31;
+  const int hf = lane >> 5;
+  const uint32_t lds0 = lds_addr(smem);
+  const int u = blockIdx.x / p.h_kv;
+  const int head = blockIdx.x - u * p.h_kv;
+  const BwdText txt = bwd_text(p.texts ? p.texts : p.own, p.n_texts, u, lane);
+  const int T = txt.len;
+  const int b0 = (u - txt.unit) * (32 * KG);
+  const int r0 = b0 + kg * 32;
+  const int blast = min(b0 + 32 * KG - 1, T - 1), rlast = min(r0 + 31, T - 1);
+  const int own = r0 + lq;
+
+  const char* const base_q = p.q + txt.start * p.q_stride;
+  const char* const base_do = p.dout + txt.start * p.do_stride;
+
+  // this wave's operand: k or v
+  bf16x8 opnd[KST];
+  {
+    const int64_t ho = (int64_t)head * p.head_dim * 2;
+    const uint32_t st = (uint32_t)(second ? p.v_stride : p.k_stride);
+    const __amdgpu_buffer_rsrc_t rs =
+        pp_rsrc((second ? p.v + txt.start * p.v_stride : p.k + txt.start * p.k_stride) + ho, (uint32_t)T * st);
+#pragma unroll
+    for (int i = 0; i < KST; ++i) {
+      const int c = 2 * i + hf;
+      const bool ok = own < T && c * 8 < p.head_dim;
+      opnd[i] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, ok ? own * st + c * 16 : BWD_NOWHERE, 0, 0));
+    }
+  }
+
+  int s_lo = 0, s_hi = T;
+  if (p.window >= 0) {
+    s_lo = max(0, b0 - p.window);
+    s_hi = min(T, blast + p.window + 1);
+  }
+  if (p.causal) s_lo = max(s_lo, b0);
+  const int t_lo = s_lo / S::BN, t_hi = (s_hi + S::BN - 1) / S::BN;
+  const int n_tiles = (t_hi - t_lo) * p.group;
+
+  const uint32_t xst = (uint32_t)p.q_stride, yst = (uint32_t)p.do_stride;
+  const BwdLoad<D, S::BN, 8> load(wave, lane, xst, yst);
+  if (p.head_dim < D) {
+    for (int i = tid; i < S::SWAP / 16; i += 512) lds_store<u32x4>(lds0 + i * 16, (u32x4){0u, 0u, 0u, 0u});
+    __syncthreads();
+  }
+  int dh = 0, dt = t_lo;
+  i32x4 xrs, yrs, lrs;
+  auto load_head = [&]() __attribute__((always_inline)) {
+    const int h = head * p.group + dh;
+    const int64_t ho = (int64_t)h * p.head_dim * 2;
+    xrs = pp_rsrc_words(base_q + ho, (uint32_t)T * xst);
+    yrs = pp_rsrc_words(base_do + ho, (uint32_t)T * yst);
+    lrs = pp_rsrc_words(p.stat + (int64_t)(second ? p.h_q + h : h) * p.rows + txt.start, (uint32_t)T * 4);
+  };
+  auto issue = [&](int stage) __attribute__((always_inline)) {
+    const uint32_t at = lds0 + stage * S::STAGE + wave * 1024;
+    const uint32_t s0 = (uint32_t)(dt * S::BN);
+    load.issue(xrs, yrs, at, s0, xst, yst, p.head_dim);
+    if (pair == 0 && lane < S::BN) {
+      const uint32_t dst = lds0 + S::STATS + stage * S::STAT + (second ? S::BN * 4 : 0);
+      asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds"
+                   :: "v"((s0 + lane) * 4), "s"(lrs), "{m0}"(dst) : "memory");
+    }
+    if (++dt == t_hi) {
+      dt = t_lo;
+      if (++dh < p.group) load_head();
+    }
+  };
+
+  // per-lane addresses in stage 0: row reads of q, or dO; transposed reads of dO, or q; statistics
+  uint32_t xa[4], ta[4];
+  bwd_row_reads(xa, lds0 + (second ? S::TILE : 0), qg * 32, lane);
+  bwd_col_reads(ta, lds0 + (second ? 0 : S::TILE), qg * 32, lane);
+  uint32_t la = lds0 + S::STATS + ((second ? S::BN : 0) + qg * 32 + 4 * hf) * 4;
+
+  f32x16 acc[NDB];
+#pragma unroll
+  for (int i = 0; i < NDB; ++i) acc[i] = (f32x16){};
+  const uint32_t swap = lds0 + S::SWAP + pair * 4096 + lane * 16;
+
+  // stream rows that some row of this wave sees
+  int w_lo = 0, w_hi = T;
+  if (p.window >= 0) {
+    w_lo = max(0, r0 - p.window);
+    w_hi = min(T, rlast + p.window + 1);
+  }
+  if (p.causal) w_lo = max(w_lo, r0);
+  if (r0 >= T) w_hi = 0;
+
+  load_head();
+  if (n_tiles > 0) issue(0);
+  int t = t_lo;
+  for (int i = 0; i < n_tiles; ++i) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();
+    if (i + 1 < n_tiles) issue((i + 1) & 1);
+    const int s0 = t * S::BN + qg * 32;
+    const bool seen = s0 < w_hi && s0 + 32 > w_lo;
+    bf16x8 x[2];
+    f32x16 s;
+    if (seen) {
+      if (!second) __builtin_amdgcn_s_setprio(1);
+      rows_product<D, S::BN, RD>(s, rows_stat(la), xa, 0, opnd);
+      if (!second) {
+        __builtin_amdgcn_s_setprio(0);
+        const bool whole = (!p.causal || s0 >= rlast) && (p.window < 0 || (s0 + 31 - r0 <= p.window && rlast - s0 <= p.window));
+        if (!whole) {
+          const int sb = s0 + 4 * hf;
+          int hi = 0x3fffffff, lo = 0;
+          if (p.causal) lo = own;
+          if (p.window >= 0) {
+            lo = max(lo, own - p.window);
+            hi = own + p.window;
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int at = sb + 8 * (r >> 2) + (r & 3);
+            s[r] = at >= lo && at <= hi ? s[r] : -INFINITY;
+          }
+        }
+        float pr[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) pr[r] = __builtin_amdgcn_exp2f(s[r] * p.c);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) lds_store<f32x4>(swap + g * 1024, (f32x4){pr[4 * g], pr[4 * g + 1], pr[4 * g + 2], pr[4 * g + 3]});
+        x[0] = pack8(pr);
+        x[1] = pack8(pr + 8);
+      }
+    }
+    lds_barrier();
+    if (seen) {
+      if (second) {
+        float ds[16];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 a = lds_load<f32x4>(swap + g * 1024);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ds[4 * g + e] = a[e] * s[4 * g + e];
+        }
+        x[0] = pack8(ds);
+        x[1] = pack8(ds + 8);
+      }
+      cols_product<D, S::BN, RD>(acc, ta, 0, x);
+    }
+    if (++t == t_hi) t = t_lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      xa[e] ^= S::STAGE;
+      ta[e] ^= S::STAGE;
+    }
+    la = (i & 1) ? la - S::STAT : la + S::STAT;
+  }
+
+  if constexpr (S::QS > 1) {
+    // the parts' sums: part 1 into the stages (16 KB per 64 features and pair), part 0 adds
+    static_assert(S::QS == 2 && 2 * KG * NDB * 4096 <= S::SWAP, "sums of the second half fit the stages");
+    const uint32_t at = lds0 + (kg * 2 + (second ? 1 : 0)) * NDB * 4096 + lane * 16;
+    lds_barrier();
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const uint32_t a = at + (db * 4 + g) * 1024;
+        if (qg == 1) lds_store<f32x4>(a, (f32x4){acc[db][4 * g], acc[db][4 * g + 1], acc[db][4 * g + 2], acc[db][4 * g + 3]});
+      }
+    lds_barrier();
+    if (qg == 1) return;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 v = lds_load<f32x4>(at + (db * 4 + g) * 1024);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[db][4 * g + e] += v[e];
+      }
+  }
+  char* const dst = second ? p.dk : p.dv;
+  const int64_t stride = second ? p.dk_stride : p.dv_stride;
+  const __amdgpu_buffer_rsrc_t rs =
+      pp_rsrc(dst + txt.start * stride + (int64_t)head * p.head_dim * (OUT16 ? 2 : 4), (uint32_t)T * (uint32_t)stride);
+  bwd_store<D, OUT16>(acc, second ? p.scale : 1.f, rs, own < T ? (uint32_t)own * (uint32_t)stride : BWD_NOWHERE, hf, p.head_dim);
+}
+
 struct BwdTable {
   BwdText at[BWD_INLINE];
 };
@@ -438,10 +730,30 @@ namespace {
 
 typedef void (*AttnBwdFn)(AttnBwdParams);
 
-template <int D>
-AttnBwdFn bwd_fn(bool kv, bool out16) {
-  return kv ? (out16 ? attn_bwd_kernel<D, true, true> : attn_bwd_kernel<D, true, false>)
-            : (out16 ? attn_bwd_kernel<D, false, true> : attn_bwd_kernel<D, false, false>);
+struct BwdLaunch {
+  AttnBwdFn fn;
+  int own;       // own rows of a workgroup
+  int threads, lds;
+};
+
+template <int D, bool KV>
+BwdLaunch bwd_plain(bool out16) {
+  return {out16 ? attn_bwd_kernel<D, KV, true> : attn_bwd_kernel<D, KV, false>, BWD_BM, 256, BwdShape<D>::LDS};
+}
+template <int D, int KG>
+BwdLaunch bwd_pair(bool out16) {
+  return {out16 ? attn_bwd_pair_kernel<D, KG, true> : attn_bwd_pair_kernel<D, KG, false>, 32 * KG, 512, PairShape<D, KG>::LDS};
+}
+
+BwdLaunch bwd_launch(const inl_attn_desc& d, const std::vector<BwdText>& texts, bool kv, bool out16) {
+  if (d.head_dim <= 64) return kv ? bwd_plain<64, true>(out16) : bwd_plain<64, false>(out16);
+  if (d.head_dim <= 128) return kv ? bwd_plain<128, true>(out16) : bwd_plain<128, false>(out16);
+  if (!kv) return bwd_plain<256, false>(out16);
+  int64_t blocks = 0;
+  for (const BwdText& x : texts) blocks += (x.len + 127) / 128;
+  static const char* f = getenv("KG");
+  if (f ? f[0] == '2' : blocks * d.h_kv < 1024) return bwd_pair<256, 2>(out16);
+  return bwd_pair<256, 4>(out16);
 }
 
 size_t bwd_stat_bytes(const inl_attn_desc& d, int64_t rows) { return ((size_t)2 * d.h_q * rows * 4 + 255) & ~(size_t)255; }
@@ -506,8 +818,8 @@ int bwd_run(const inl_attn_desc* d, const inl_attn_grads* g, const void* q, cons
                                      ": the row stride must cover all heads and be a multiple of 16 bytes");
     if ((!t[i].at && i < 5 && rows) || ((uintptr_t)t[i].at & 15))
       return fail(INL_E_INVALID, std::string("attention backward: ") + t[i].what + " must be non-null and 16-byte aligned");
-    // rows of a text are addressed with 32 bits
-    if (longest * t[i].stride * es >= (int64_t)BWD_NOWHERE)
+    // rows of a text, and those of its last tile behind it, are addressed with 32 bits
+    if ((longest + 128) * t[i].stride * es >= (int64_t)BWD_NOWHERE)
       return fail(INL_E_UNSUPPORTED, std::string("attention backward: a text's rows of ") + t[i].what + " span 4 GiB or more");
     r[i] = {t[i].at, rows, len * es, t[i].stride * es};
   }
@@ -522,13 +834,6 @@ int bwd_run(const inl_attn_desc* d, const inl_attn_grads* g, const void* q, cons
   std::sort(texts.begin(), texts.end(), [](const BwdText& a, const BwdText& b) {
     return a.len != b.len ? a.len > b.len : a.start < b.start;
   });
-  int64_t units = 0;
-  for (BwdText& x : texts) {
-    x.unit = (int32_t)units;
-    units += (x.len + BWD_BM - 1) / BWD_BM;
-  }
-  if (units * d->h_q > INT32_MAX)
-    return fail(INL_E_UNSUPPORTED, "attention backward: more than 2^31 blocks of query rows and heads");
   AttnBwdParams p{};
   p.q = (const char*)q;
   p.k = (const char*)k;
@@ -544,7 +849,6 @@ int bwd_run(const inl_attn_desc* d, const inl_attn_grads* g, const void* q, cons
   p.stat = (float*)ws;
   p.rows = rows;
   p.n_texts = (int32_t)texts.size();
-  p.n_units = (int32_t)units;
   p.h_q = d->h_q;
   p.h_kv = d->h_kv;
   p.group = d->h_q / d->h_kv;
@@ -554,26 +858,32 @@ int bwd_run(const inl_attn_desc* d, const inl_attn_grads* g, const void* q, cons
   // (the statistics are divided by c, and must stay finite; scores times less than this are 0)
   p.c = std::max(d->scale * kLog2e, 1e-30f);
   p.scale = d->scale;
-  if (texts.size() <= (size_t)BWD_INLINE) {
-    std::copy(texts.begin(), texts.end(), p.own);
-  } else {
-    // More texts go through the workspace, by launches that carry them as arguments: a copy from
-    // host memory could not be captured, nor its source freed.
-    BwdText* table = (BwdText*)((char*)ws + bwd_stat_bytes(*d, rows));
-    for (size_t i = 0; i < texts.size(); i += BWD_INLINE) {
-      BwdTable part{};
-      const int n = (int)std::min<size_t>(BWD_INLINE, texts.size() - i);
-      std::copy(texts.begin() + i, texts.begin() + i + n, part.at);
-      hipLaunchKernelGGL(bwd_table_kernel, dim3(1), dim3(BWD_INLINE), 0, st, part, table + i, n);
-    }
-    p.texts = table;
-  }
   const bool out16 = g->grad_dtype == INL_BF16;
   for (int kv = 0; kv < (dk ? 2 : 1); ++kv) {
-    AttnBwdFn fn = d->head_dim <= 64 ? bwd_fn<64>(kv, out16) : d->head_dim <= 128 ? bwd_fn<128>(kv, out16) : bwd_fn<256>(kv, out16);
-    const int lds = d->head_dim <= 64 ? BwdShape<64>::LDS : d->head_dim <= 128 ? BwdShape<128>::LDS : BwdShape<256>::LDS;
-    if ((rc = set_max_dynamic_lds((const void*)fn, lds))) return rc;
-    hipLaunchKernelGGL(fn, dim3((unsigned)(units * (kv ? d->h_kv : d->h_q))), dim3(256), lds, st, p);
+    const BwdLaunch l = bwd_launch(*d, texts, kv, out16);
+    int64_t units = 0;
+    for (BwdText& x : texts) {
+      x.unit = (int32_t)units;
+      units += (x.len + l.own - 1) / l.own;
+    }
+    const int64_t groups = units * (kv ? d->h_kv : d->h_q);
+    if (groups > INT32_MAX) return fail(INL_E_UNSUPPORTED, "attention backward: more than 2^31 blocks of rows and heads");
+    if (texts.size() <= (size_t)BWD_INLINE) {
+      std::copy(texts.begin(), texts.end(), p.own);
+    } else {
+      // More texts go through the workspace, by launches that carry them as arguments: a copy from
+      // host memory could not be captured, nor its source freed.
+      BwdText* table = (BwdText*)((char*)ws + bwd_stat_bytes(*d, rows));
+      for (size_t i = 0; i < texts.size(); i += BWD_INLINE) {
+        BwdTable part{};
+        const int n = (int)std::min<size_t>(BWD_INLINE, texts.size() - i);
+        std::copy(texts.begin() + i, texts.begin() + i + n, part.at);
+        hipLaunchKernelGGL(bwd_table_kernel, dim3(1), dim3(BWD_INLINE), 0, st, part, table + i, n);
+      }
+      p.texts = table;
+    }
+    if ((rc = set_max_dynamic_lds((const void*)l.fn, l.lds))) return rc;
+    hipLaunchKernelGGL(l.fn, dim3((unsigned)groups), dim3(l.threads), l.lds, st, p);
     INL_HIP_TRY(hipGetLastError());
   }
   return INL_OK;

@@ -27,7 +27,7 @@ struct AttnBwdParams {
   const BwdText* texts;    // null: in `own`
   int64_t q_stride, k_stride, v_stride, o_stride, do_stride, dq_stride, dk_stride, dv_stride;  // bytes
   int64_t rows;
-  int32_t n_texts, n_units, h_q, h_kv, group, head_dim, causal, window;
+  int32_t n_texts, h_q, h_kv, group, head_dim, causal, window;
   float c, scale;          // scale * log2(e) (the exponent's), scale
   BwdText own[BWD_INLINE];
 };
