@@ -243,3 +243,48 @@ if __name__ == "__main__":
         print(f"{path}: {count_asm_loads(txt)} register-writing asm loads, {len(v)} violations")
         for x in v[:20]:
             print("  ", x)
+
+
+# A vector instruction that wrote a scalar register (v_readfirstlane, v_readlane, a compare) needs five wait
+# states before a vector-memory instruction reads that register: with fewer the load takes the old value, and its
+# address from it. The compiler makes these waits for its own instructions and not for inline asm.
+_SGPR = re.compile(r"\bs\[(\d+):(\d+)\]|\bs(\d+)\b")
+_SGPR_STATES = 5
+
+
+def _sgprs(operands: str) -> set:
+    out = set()
+    for lo, hi, one in _SGPR.findall(operands):
+        out.update(range(int(lo), int(hi) + 1) if lo else (int(one),))
+    return out
+
+
+def check_sgpr_waits(listing: str) -> list[Violation]:
+    """Vector-memory instructions that read a scalar register fewer than five wait states after a vector
+    instruction wrote it, along the listing (a branch only adds states)."""
+    found, function, wrote, state = [], "", {}, 0
+    for number, raw in enumerate(listing.splitlines(), 1):
+        label = _LABEL.match(raw)
+        if label and not label.group(1).startswith("."):
+            function, wrote = label.group(1), {}
+            continue
+        text = raw.split(";")[0].strip()
+        if not text or text.startswith(".") or text.endswith(":"):
+            continue
+        mnemonic, _, operands = text.partition(" ")
+        if mnemonic == "s_nop":
+            state += int(operands.strip(), 0) + 1
+            continue
+        state += 1
+        first = operands.split(",")[0]
+        if _VMEM.match(mnemonic):
+            late = [r for r in _sgprs(operands) if r in wrote and state - wrote[r] - 1 < _SGPR_STATES]
+            if late:
+                found.append(Violation(function, number, text, [f"s{r} (too few waits)" for r in sorted(late)]))
+        elif mnemonic.startswith("v_"):
+            for r in _sgprs(first) if mnemonic.startswith(("v_readfirstlane", "v_readlane", "v_cmp")) else ():
+                wrote[r] = state
+        elif mnemonic.startswith("s_"):
+            for r in _sgprs(first):
+                wrote.pop(r, None)
+    return found

@@ -54,7 +54,7 @@ EXTRA = {
 # the compiler's resource-usage remarks and fails if any of them does.
 # gdn_chunk.hip and gemm_f32.hip load through builtins; they are held to the
 # same for speed, their loops filling the register file to a few registers.
-NO_SCRATCH = {"attn_pp.hip", "attn_pp64.hip", "attn_wide.hip", "gdn_chunk.hip", "gemm.hip", "gemm_f32.hip",
+NO_SCRATCH = {"attn_bwd.hip", "attn_pp.hip", "attn_pp64.hip", "attn_wide.hip", "gdn_chunk.hip", "gemm.hip", "gemm_f32.hip",
               "splade_decoder.hip", "tile_nt.hip", "tile_nn.hip", "tile_tn.hip"}
 RESOURCE_REMARKS = ["-Rpass-analysis=kernel-resource-usage", "-fno-caret-diagnostics"]
 # The same sources are also compiled to a device assembly listing, which
@@ -121,6 +121,11 @@ def check_inflight(src_name: str, listing: str) -> None:
         shown = "\n".join(str(v) for v in bad[:10])
         raise RuntimeError(f"{src_name}: {len(bad)} instructions name registers whose inline-asm loads are "
                            f"still in flight:\n{shown}")
+    bad = asmcheck.check_sgpr_waits(listing)
+    if bad:
+        shown = "\n".join(str(v) for v in bad[:10])
+        raise RuntimeError(f"{src_name}: {len(bad)} vector-memory instructions read scalar registers too soon after a "
+                           f"vector instruction wrote them:\n{shown}")
 
 
 def sources():

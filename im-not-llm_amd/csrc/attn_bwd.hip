@@ -37,17 +37,18 @@ namespace inl {
 namespace {
 
 constexpr uint32_t BWD_NOWHERE = 0xffff0000u;   // beyond every text's range: reads 0, not written
-constexpr int BWD_BM = 128;                     // own rows of a workgroup: 4 waves of 32
 
-template <int D>
+// QS parts of a workgroup's four waves take different rows of every stream tile for the same own rows.
+template <int D, bool KV, int QS>
 struct BwdShape {
-  static constexpr int BN = D <= 128 ? 64 : 32;   // stream rows of a tile
-  static constexpr int ROW = D * 2;
-  static constexpr int TILE = BN * ROW;           // bytes of X, and of Y
-  static constexpr int STAGE = 2 * TILE;          // a power of two: the other stage is an XOR away
-  static constexpr int STATS = 2 * STAGE;         // log-sum-exp and delta of the stream rows, per stage
-  static constexpr int STAT = 2 * BN * 4;
-  static constexpr int LDS = STATS + 2 * STAT;
+  static constexpr int KG = 4 / QS;               // waves with own rows of their own
+  static constexpr int OWN = 32 * KG;             // own rows of a workgroup
+  static constexpr int BN = D <= 64 || QS == 2 ? 64 : 32;    // stream rows of a tile
+  static constexpr int TILE = BN * D * 2;         // bytes of X, and of Y
+  static constexpr int STAT = KV ? 2 * BN * 4 : 0;   // log-sum-exp and delta of the stream rows
+  static constexpr int STAGE = 2 * TILE + STAT;
+  static constexpr int NS = D <= 64 ? 3 : BN == 32 ? 4 : 2;  // tiles in LDS: one in use, the others loading
+  static constexpr int LDS = NS * STAGE;
 };
 
 // A tile of BN rows lies in groups of 64 features (a 128-byte line): 16-byte chunk c of row r at
@@ -100,20 +101,34 @@ __device__ __forceinline__ void bwd_store(const f32x16 (&acc)[D / 32], float by,
   }
 }
 
-// The text of unit u: texts' first units ascend, so it is the last one whose is not above u.
-__device__ __forceinline__ BwdText bwd_text(const BwdText* texts, int n, int u, int lane) {
-  int at = 0;
-  for (int i = 0; i < n; i += 64) {
+// What a workgroup works on: a block of own rows of a text, for a key head and one of its query heads (of
+// `members`; all of them for members = 1).
+struct BwdUnit {
+  int start, len, block, kvh, member;
+};
+// False where there is nothing (classes have unequal numbers of units).
+__device__ __forceinline__ bool bwd_unit(const AttnBwdParams& p, int members, int lane, BwdUnit* out) {
+  const int width = p.h_kv * p.classes;
+  const int rest = blockIdx.x / width, x = blockIdx.x - rest * width;
+  const int cls = x / p.h_kv, u = rest / members;
+  out->kvh = x - cls * p.h_kv;
+  out->member = rest - u * members;
+  if (u >= p.units[cls]) return false;
+  // the class's first units ascend: the text is the last one whose is not above u
+  const BwdText* const texts = p.texts ? p.texts : p.own;
+  const int n = p.first[cls + 1];
+  int at = p.first[cls];
+  for (int i = at; i < n; i += 64) {
     const int first = i + lane < n ? texts[i + lane].unit : 0x7fffffff;
     const int below = __builtin_popcountll(__builtin_amdgcn_ballot_w64(first <= u));
-    at = i + below - 1;
+    at = below ? i + below - 1 : at;
     if (below < 64) break;
   }
-  // (texts[i].unit <= u for the first of a block that is not the first block, or `at` is the
-  // last text of the block before)
   const BwdText t = texts[at];
-  return {__builtin_amdgcn_readfirstlane(t.start), __builtin_amdgcn_readfirstlane(t.len),
-          __builtin_amdgcn_readfirstlane(t.unit)};
+  out->start = __builtin_amdgcn_readfirstlane(t.start);
+  out->len = __builtin_amdgcn_readfirstlane(t.len);
+  out->block = u - __builtin_amdgcn_readfirstlane(t.unit);
+  return true;
 }
 
 // acc += rows . opnd over the features of 32 stream rows, at base[step % 4] (a lane's row and chunk) + off;
@@ -180,9 +195,11 @@ __device__ __forceinline__ f32x16 rows_stat(uint32_t at) {
 }
 
 // 16 bytes a lane at rsrc + voff + off to LDS at lds + 16 lane. The instruction adds its offset to both
-// addresses; the s_nop is the wait between the write of M0 and the load.
+// addresses. The s_nop stands for two waits that the compiler does not see into asm to make: one state
+// from the write of M0, and five from a v_readfirstlane that wrote a word of the descriptor (with
+// fewer the load has taken the old word, and its address from it).
 __device__ __forceinline__ void bwd_dma(i32x4 rsrc, uint32_t lds, uint32_t voff, int off) {
-  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen offset:%3 lds"
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen offset:%3 lds"
                :: "v"(voff), "s"(rsrc), "{m0}"(lds - off), "n"(off) : "memory");
 }
 
@@ -221,10 +238,10 @@ struct BwdLoad {
     y = row * yst + g0 * 128 + chunk * 16;
   }
   __device__ __forceinline__ void issue(const i32x4& xrs, const i32x4& yrs, uint32_t at, uint32_t row, uint32_t xst,
-                                        uint32_t yst, int head_dim) const {
+                                        uint32_t yst, uint32_t off, int head_dim) const {
 #pragma unroll
     for (int r = 0; r < RP; ++r) {
-      const uint32_t xa = x + (row + r * NW * 8) * xst, ya = y + (row + r * NW * 8) * yst;
+      const uint32_t xa = x + ((row + r * NW * 8) * xst + off), ya = y + ((row + r * NW * 8) * yst + off);
 #pragma unroll
       for (int g = 0; g < GP; ++g)
         if (head_dim == D || (8 * (g0 + g * GSTEP) + chunk) * 8 < head_dim) {
@@ -236,14 +253,21 @@ struct BwdLoad {
   }
 };
 
+// The statistics of one head (log-sum-exp, or those of delta h_q behind) of a text's rows.
+__device__ __forceinline__ i32x4 bwd_stat_rsrc(const AttnBwdParams& p, int64_t h, const BwdUnit& txt) {
+  const uint64_t a = (uint64_t)(p.stat + h * p.rows + txt.start);
+  return (i32x4){(int)(uint32_t)a, (int)((uint32_t)(a >> 32) & 0xffffu), txt.len * 4, 0x00020000};
+}
+
 // KV: own rows are keys (dk, dv); otherwise queries (dq, and the row statistics).
-template <int D, bool KV, bool OUT16>
+template <int D, bool KV, int QS, bool OUT16>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwdParams p) {
-  using S = BwdShape<D>;
+  using S = BwdShape<D, KV, QS>;
   constexpr int KST = D / 16;            // k-steps of the products over features
   constexpr int NDB = D / 32;            // 32-feature blocks of an accumulator
-  constexpr int NKB = S::BN / 32;        // 32-row blocks of a tile
-  constexpr int RD = D == 128 && KV ? 3 : 4;   // fragments in flight
+  constexpr int NKB = S::BN / 32 / QS;   // 32-row blocks of a tile for a wave
+  static_assert(QS == 1 || NKB == 1, "parts of a tile");
+  constexpr int RR = D == 128 && KV ? 3 : 4, RC = 4;   // fragments in flight (eight are no faster)
   extern __shared__ __attribute__((aligned(1024))) char smem[];
 
   const int tid = threadIdx.x;
@@ -252,22 +276,71 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwd
   const int lq = lane & 31;
   const int hf = lane >> 5;
   const uint32_t lds0 = lds_addr(smem);
-  const int heads = KV ? p.h_kv : p.h_q;
-  const int u = blockIdx.x / heads;
-  const int head = blockIdx.x - u * heads;          // own head
-  const int kvh = KV ? head : head / p.group;
-  const BwdText txt = bwd_text(p.texts ? p.texts : p.own, p.n_texts, u, lane);
+  BwdUnit txt;
+  if (!bwd_unit(p, KV ? 1 : p.group, lane, &txt)) return;
+  const int kvh = txt.kvh, head = KV ? kvh : kvh * p.group + txt.member;   // own head
   const int T = txt.len;
-  const int b0 = (u - txt.unit) * BWD_BM;           // first own row of the workgroup
-  const int r0 = b0 + wave * 32;                    // and of this wave
+  const int kg = QS == 1 ? wave : wave % S::KG, qg = QS == 1 ? 0 : wave / S::KG;
+  const int b0 = txt.block * S::OWN;                // first own row of the workgroup
+  const int r0 = b0 + kg * 32;                      // and of this wave
   const bool active = r0 < T;
-  const int blast = min(b0 + BWD_BM - 1, T - 1), rlast = min(r0 + 31, T - 1);
+  const int blast = min(b0 + S::OWN - 1, T - 1), rlast = min(r0 + 31, T - 1);
   const int own = r0 + lq;
 
   const char* const base_q = p.q + txt.start * p.q_stride;
   const char* const base_k = p.k + txt.start * p.k_stride + (int64_t)kvh * p.head_dim * 2;
   const char* const base_v = p.v + txt.start * p.v_stride + (int64_t)kvh * p.head_dim * 2;
   const char* const base_do = p.dout + txt.start * p.do_stride;
+
+  // ---- the stream: tiles [t_lo, t_hi) of every head that the own rows meet ----
+  int s_lo = 0, s_hi = T;
+  if (p.window >= 0) {
+    s_lo = max(0, b0 - p.window);
+    s_hi = min(T, blast + p.window + 1);
+  }
+  if (p.causal) {
+    if (KV) s_lo = max(s_lo, b0);
+    else s_hi = min(s_hi, blast + 1);
+  }
+  const int t_lo = s_lo / S::BN, t_hi = (s_hi + S::BN - 1) / S::BN;
+  const int n_tiles = (t_hi - t_lo) * (KV ? p.group : 1);
+
+  const uint32_t xst = (uint32_t)(KV ? p.q_stride : p.k_stride), yst = (uint32_t)(KV ? p.do_stride : p.v_stride);
+  const BwdLoad<D, S::BN, 4> load(wave, lane, xst, yst);
+  if (p.head_dim < D) {
+    for (int i = tid; i < S::LDS / 16; i += 256) lds_store<u32x4>(lds0 + i * 16, (u32x4){0u, 0u, 0u, 0u});
+    __syncthreads();
+  }
+  int dh = 0, dt = t_lo;   // load cursor: head of the group (its heads take a tile after one another), tile
+  const int64_t h0 = (int64_t)kvh * p.group;
+  const i32x4 xrs = pp_rsrc_words(KV ? base_q + h0 * p.head_dim * 2 : base_k, (uint32_t)T * xst);
+  const i32x4 yrs = pp_rsrc_words(KV ? base_do + h0 * p.head_dim * 2 : base_v, (uint32_t)T * yst);
+  uint32_t put = lds0;     // the stage it goes to
+  auto issue = [&]() __attribute__((always_inline)) {
+    const uint32_t s0 = (uint32_t)(dt * S::BN);
+    load.issue(xrs, yrs, put + wave * 1024, s0, xst, yst, dh * p.head_dim * 2, p.head_dim);
+    if constexpr (KV) {
+      // BN / 2 statistics per wave, 4 bytes a lane
+      if (lane < S::BN / 2) {
+        const uint32_t dst = put + 2 * S::TILE + wave * (S::BN * 2);
+        const i32x4 rs = bwd_stat_rsrc(p, h0 + dh + (wave < 2 ? 0 : p.h_q), txt);
+        asm volatile("s_nop 4\n\tbuffer_load_dword %0, %1, 0 offen lds"
+                     :: "v"((s0 + (wave & 1) * (S::BN / 2) + lane) * 4), "s"(rs), "{m0}"(dst) : "memory");
+      }
+      if (++dh == p.group) {
+        dh = 0;
+        ++dt;
+      }
+    } else {
+      ++dt;
+    }
+    put = put == lds0 + (S::NS - 1) * S::STAGE ? lds0 : put + S::STAGE;
+  };
+
+  // The first tiles are under way while the own operands are loaded.
+#pragma unroll
+  for (int i = 0; i < S::NS - 1; ++i)
+    if (i < n_tiles) issue();
 
   // ---- own operands: lane lq's row, chunks 2 i + hf ----
   bf16x8 own0[KST], own1[KST];
@@ -301,65 +374,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwd
     }
   }
 
-  // ---- the stream: tiles [t_lo, t_hi) of every head that the own rows meet ----
-  int s_lo = 0, s_hi = T;
-  if (p.window >= 0) {
-    s_lo = max(0, b0 - p.window);
-    s_hi = min(T, blast + p.window + 1);
-  }
-  if (p.causal) {
-    if (KV) s_lo = max(s_lo, b0);
-    else s_hi = min(s_hi, blast + 1);
-  }
-  const int t_lo = s_lo / S::BN, t_hi = (s_hi + S::BN - 1) / S::BN;
-  const int n_tiles = (t_hi - t_lo) * (KV ? p.group : 1);
-
-  const uint32_t xst = (uint32_t)(KV ? p.q_stride : p.k_stride), yst = (uint32_t)(KV ? p.do_stride : p.v_stride);
-  const BwdLoad<D, S::BN, 4> load(wave, lane, xst, yst);
-  if (p.head_dim < D) {
-    for (int i = tid; i < S::LDS / 16; i += 256) lds_store<u32x4>(lds0 + i * 16, (u32x4){0u, 0u, 0u, 0u});
-    __syncthreads();
-  }
-  int dh = 0, dt = t_lo;   // load cursor: head of the group, tile
-  i32x4 xrs, yrs, lrs, ers;
-  auto load_head = [&]() __attribute__((always_inline)) {
-    if constexpr (KV) {
-      const int h = kvh * p.group + dh;
-      const int64_t ho = (int64_t)h * p.head_dim * 2;
-      xrs = pp_rsrc_words(base_q + ho, (uint32_t)T * xst);
-      yrs = pp_rsrc_words(base_do + ho, (uint32_t)T * yst);
-      lrs = pp_rsrc_words(p.stat + (int64_t)h * p.rows + txt.start, (uint32_t)T * 4);
-      ers = pp_rsrc_words(p.stat + (int64_t)(p.h_q + h) * p.rows + txt.start, (uint32_t)T * 4);
-    } else {
-      xrs = pp_rsrc_words(base_k, (uint32_t)T * xst);
-      yrs = pp_rsrc_words(base_v, (uint32_t)T * yst);
-    }
-  };
-  auto issue = [&](int stage) __attribute__((always_inline)) {
-    const uint32_t at = lds0 + stage * S::STAGE + wave * 1024;
-    const uint32_t s0 = (uint32_t)(dt * S::BN);
-    load.issue(xrs, yrs, at, s0, xst, yst, p.head_dim);
-    if constexpr (KV) {
-      // 4 bytes a lane; a tile of 32 rows fills half of its 64 (the rest is overwritten by nothing:
-      // lanes from BN on are off)
-      if (wave < 2 && lane < S::BN) {
-        const uint32_t dst = lds0 + S::STATS + stage * S::STAT + wave * S::BN * 4;
-        const i32x4 rs = wave == 0 ? lrs : ers;
-        asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds"
-                     :: "v"((s0 + lane) * 4), "s"(rs), "{m0}"(dst) : "memory");
-      }
-    }
-    if (++dt == t_hi && KV) {
-      dt = t_lo;
-      if (++dh < p.group) load_head();
-    }
-  };
-
   // ---- per-lane LDS addresses in stage 0 ----
   uint32_t xa[4], ta[4];
-  bwd_row_reads(xa, lds0, 0, lane);
-  bwd_col_reads(ta, lds0, 0, lane);
-  uint32_t la = lds0 + S::STATS + 16 * hf;
+  bwd_row_reads(xa, lds0, qg * 32, lane);
+  bwd_col_reads(ta, lds0, qg * 32, lane);
+  uint32_t la = lds0 + 2 * S::TILE + 16 * hf + qg * 128;
 
   f32x16 acc[NDB], accv[KV ? NDB : 1];
 #pragma unroll
@@ -379,7 +398,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwd
   auto block = [&](int kb, int s0) __attribute__((always_inline)) {
     const uint32_t X = kb * 32 * 128, Y = S::TILE + X;
     f32x16 s, dp;
-    rows_product<D, S::BN, RD>(s, KV ? rows_stat(la + kb * 128) : (f32x16){}, xa, X, own0);
+    rows_product<D, S::BN, RR>(s, KV ? rows_stat(la + kb * 128) : (f32x16){}, xa, X, own0);
     // masks: stream row s0 + c of register r, c = 8 (r / 4) + 4 hf + r % 4
     const bool whole = (KV || s0 + 31 < T) && (!p.causal || (KV ? s0 >= rlast : s0 + 31 <= r0)) &&
                        (p.window < 0 || (s0 + 31 - r0 <= p.window && rlast - s0 <= p.window));
@@ -405,12 +424,12 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwd
 #pragma unroll
       for (int r = 0; r < 16; ++r) pr[r] = __builtin_amdgcn_exp2f(s[r] * p.c);
       const bf16x8 pb[2] = {pack8(pr), pack8(pr + 8)};
-      cols_product<D, S::BN, RD>(accv, ta, Y, pb);
-      rows_product<D, S::BN, RD>(dp, rows_stat(la + S::BN * 4 + kb * 128), xa, Y, own1);
+      cols_product<D, S::BN, RC>(accv, ta, Y, pb);
+      rows_product<D, S::BN, RR>(dp, rows_stat(la + S::BN * 4 + kb * 128), xa, Y, own1);
 #pragma unroll
       for (int r = 0; r < 16; ++r) ds[r] = pr[r] * dp[r];
     } else {
-      rows_product<D, S::BN, RD>(dp, less, xa, Y, own1);
+      rows_product<D, S::BN, RR>(dp, less, xa, Y, own1);
       auto mx2 = [](float a, float b) __attribute__((always_inline)) { return __builtin_elementwise_maximum(a, b); };
       float m4[4];
 #pragma unroll
@@ -437,7 +456,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwd
       }
     }
     const bf16x8 db[2] = {pack8(ds), pack8(ds + 8)};
-    cols_product<D, S::BN, RD>(acc, ta, X, db);
+    cols_product<D, S::BN, RC>(acc, ta, X, db);
   };
 
   // stream rows that some row of this wave sees
@@ -452,25 +471,77 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwd
   }
   if (!active) w_hi = 0;
 
-  load_head();
-  if (n_tiles > 0) issue(0);
-  int t = t_lo;
+  using Load = BwdLoad<D, S::BN, 4>;
+  constexpr int LOADS = 2 * Load::RP * Load::GP + (KV ? 1 : 0);
+  int t = t_lo, th = 0, at = 0;
   for (int i = 0; i < n_tiles; ++i) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // this wave's loads of tile i are done once no more than those of the tiles behind it are in
+    // flight (a wave that loads no feature of a narrow head has fewer)
+    if (i + S::NS - 2 < n_tiles && p.head_dim == D)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S::NS - 2) * LOADS) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     lds_barrier();
-    if (i + 1 < n_tiles) issue((i + 1) & 1);
+    if (i + S::NS - 1 < n_tiles) issue();
 #pragma unroll
     for (int kb = 0; kb < NKB; ++kb) {
-      const int s0 = t * S::BN + kb * 32;
+      const int s0 = t * S::BN + (kb + qg) * 32;
       if (s0 < w_hi && s0 + 32 > w_lo) block(kb, s0);
     }
-    if (++t == t_hi) t = t_lo;
+    if (!KV || ++th == p.group) {
+      th = 0;
+      ++t;
+    }
+    const uint32_t step = at == S::NS - 1 ? (uint32_t)(-(S::NS - 1) * S::STAGE) : S::STAGE;
+    at = at == S::NS - 1 ? 0 : at + 1;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      xa[e] ^= S::STAGE;
-      ta[e] ^= S::STAGE;
+      xa[e] += step;
+      ta[e] += step;
     }
-    la = (i & 1) ? la - S::STAT : la + S::STAT;
+    la += step;
+  }
+
+  if constexpr (QS > 1) {
+    // The parts' sums meet in LDS, where the stages were. Queries' are brought to one maximum first: a part
+    // that saw no key of a row has none (-inf) and counts 0.
+    constexpr int PART = (KV ? 8 : 4) * NDB * 1024;   // a wave's
+    static_assert(QS == 2 && S::KG * (PART + 512) <= S::LDS, "sums of the second part fit");
+    const uint32_t to = lds0 + kg * PART + lane * 16, stat = lds0 + S::KG * PART + kg * 512 + lane * 4;
+    auto each = [&](auto&& f) __attribute__((always_inline)) {
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          f(acc[db], g, to + (db * 4 + g) * 1024);
+          if constexpr (KV) f(accv[db], g, to + ((NDB + db) * 4 + g) * 1024);
+        }
+    };
+    lds_barrier();
+    if (qg == 1) {
+      each([&](f32x16& a, int g, uint32_t at) __attribute__((always_inline)) {
+        lds_store<f32x4>(at, (f32x4){a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]});
+      });
+      if constexpr (!KV) {
+        lds_store<float>(stat, m_i);
+        lds_store<float>(stat + 256, l_i);
+      }
+    }
+    lds_barrier();
+    if (qg == 1) return;
+    float by0 = 1.f, by1 = 1.f;
+    if constexpr (!KV) {
+      const float m1 = lds_load<float>(stat), m = __builtin_elementwise_maximum(m_i, m1);
+      by0 = m_i == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_i - m);
+      by1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - m);
+      l_i = l_i * by0 + lds_load<float>(stat + 256) * by1;
+      m_i = m;
+    }
+    each([&](f32x16& a, int g, uint32_t at) __attribute__((always_inline)) {
+      const f32x4 v = lds_load<f32x4>(at);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a[4 * g + e] = KV ? a[4 * g + e] + v[e] : a[4 * g + e] * by0 + v[e] * by1;
+    });
   }
 
   // ---- results ----
@@ -500,12 +571,13 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwd
 // accumulates dk. A stream tile is two phases with a barrier between: S and P beside dP, then dv
 // beside dS and dk; the first wave goes ahead of the second in the first phase (s_setprio), so
 // that its exponentials run under the other's products.
-// KG pairs of a workgroup's four own 32 keys each; where there are fewer, the others take
-// other rows of the stream for the same keys, and the sums meet in LDS at the end: half as
-// long a chain for a workgroup, for twice the tiles read.
-template <int D, int KG>
+// Two of a workgroup's four pairs own 32 keys each, the others take other rows of the stream for
+// the same keys, and the sums meet in LDS at the end. Four pairs with keys of their own read half the tiles, but
+// make half as many workgroups of twice the length: 24 texts of 1,024 tokens with one key head take 176
+// us instead of 170, 4 x 4,096 of two 2.00 ms instead of 1.31, and 64 texts of 1,024 the same.
+template <int D>
 struct PairShape {
-  static constexpr int QS = 4 / KG;               // parts of a stream tile
+  static constexpr int QS = 2, KG = 2;            // parts of a stream tile, blocks of own keys
   static constexpr int BN = 32 * QS;
   static constexpr int ROW = D * 2;
   static constexpr int TILE = BN * ROW;
@@ -516,12 +588,13 @@ struct PairShape {
   static constexpr int LDS = STATS + 2 * STAT;
 };
 
-template <int D, int KG, bool OUT16>
+template <int D, bool OUT16>
 __global__ __launch_bounds__(512, 2) void attn_bwd_pair_kernel(AttnBwdParams p) {
-  using S = PairShape<D, KG>;
+  using S = PairShape<D>;
+  constexpr int KG = S::KG;
   constexpr int KST = D / 16;
   constexpr int NDB = D / 32;
-  constexpr int RD = 4;
+  constexpr int RR = 4, RC = 4;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
 
   const int tid = threadIdx.x;
@@ -533,32 +606,17 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_pair_kernel(AttnBwdParams p) 
   const int lq = lane & 31;
   const int hf = lane >> 5;
   const uint32_t lds0 = lds_addr(smem);
-  const int u = blockIdx.x / p.h_kv;
-  const int head = blockIdx.x - u * p.h_kv;
-  const BwdText txt = bwd_text(p.texts ? p.texts : p.own, p.n_texts, u, lane);
+  BwdUnit txt;
+  if (!bwd_unit(p, 1, lane, &txt)) return;
+  const int head = txt.kvh;
   const int T = txt.len;
-  const int b0 = (u - txt.unit) * (32 * KG);
+  const int b0 = txt.block * (32 * KG);
   const int r0 = b0 + kg * 32;
   const int blast = min(b0 + 32 * KG - 1, T - 1), rlast = min(r0 + 31, T - 1);
   const int own = r0 + lq;
 
   const char* const base_q = p.q + txt.start * p.q_stride;
   const char* const base_do = p.dout + txt.start * p.do_stride;
-
-  // this wave's operand: k or v
-  bf16x8 opnd[KST];
-  {
-    const int64_t ho = (int64_t)head * p.head_dim * 2;
-    const uint32_t st = (uint32_t)(second ? p.v_stride : p.k_stride);
-    const __amdgpu_buffer_rsrc_t rs =
-        pp_rsrc((second ? p.v + txt.start * p.v_stride : p.k + txt.start * p.k_stride) + ho, (uint32_t)T * st);
-#pragma unroll
-    for (int i = 0; i < KST; ++i) {
-      const int c = 2 * i + hf;
-      const bool ok = own < T && c * 8 < p.head_dim;
-      opnd[i] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, ok ? own * st + c * 16 : BWD_NOWHERE, 0, 0));
-    }
-  }
 
   int s_lo = 0, s_hi = T;
   if (p.window >= 0) {
@@ -575,29 +633,46 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_pair_kernel(AttnBwdParams p) 
     for (int i = tid; i < S::SWAP / 16; i += 512) lds_store<u32x4>(lds0 + i * 16, (u32x4){0u, 0u, 0u, 0u});
     __syncthreads();
   }
-  int dh = 0, dt = t_lo;
-  i32x4 xrs, yrs, lrs;
-  auto load_head = [&]() __attribute__((always_inline)) {
-    const int h = head * p.group + dh;
-    const int64_t ho = (int64_t)h * p.head_dim * 2;
-    xrs = pp_rsrc_words(base_q + ho, (uint32_t)T * xst);
-    yrs = pp_rsrc_words(base_do + ho, (uint32_t)T * yst);
-    lrs = pp_rsrc_words(p.stat + (int64_t)(second ? p.h_q + h : h) * p.rows + txt.start, (uint32_t)T * 4);
-  };
+  // From the last rows on, the heads of a tile after one another: so the blocks of a text, in their causal
+  // triangle too, stream the same rows at about the same time, and find them in L2 (4 x 4,096 tokens
+  // of 16/2 heads, whose q and dO are 32 MB a key head: 1.30 ms, and 1.83 head by head from the diagonal on).
+  int dh = 0, dt = t_hi - 1;
+  const int64_t h0 = (int64_t)head * p.group;
+  const i32x4 xrs = pp_rsrc_words(base_q + h0 * p.head_dim * 2, (uint32_t)T * xst);
+  const i32x4 yrs = pp_rsrc_words(base_do + h0 * p.head_dim * 2, (uint32_t)T * yst);
   auto issue = [&](int stage) __attribute__((always_inline)) {
     const uint32_t at = lds0 + stage * S::STAGE + wave * 1024;
     const uint32_t s0 = (uint32_t)(dt * S::BN);
-    load.issue(xrs, yrs, at, s0, xst, yst, p.head_dim);
+    load.issue(xrs, yrs, at, s0, xst, yst, dh * p.head_dim * 2, p.head_dim);
     if (pair == 0 && lane < S::BN) {
       const uint32_t dst = lds0 + S::STATS + stage * S::STAT + (second ? S::BN * 4 : 0);
-      asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds"
-                   :: "v"((s0 + lane) * 4), "s"(lrs), "{m0}"(dst) : "memory");
+      const i32x4 rs = bwd_stat_rsrc(p, h0 + dh + (second ? p.h_q : 0), txt);
+      asm volatile("s_nop 4\n\tbuffer_load_dword %0, %1, 0 offen lds"
+                   :: "v"((s0 + lane) * 4), "s"(rs), "{m0}"(dst) : "memory");
     }
-    if (++dt == t_hi) {
-      dt = t_lo;
-      if (++dh < p.group) load_head();
+    if (++dh == p.group) {
+      dh = 0;
+      --dt;
     }
   };
+
+  // (the first tile is under way while the operand is loaded)
+  if (n_tiles > 0) issue(0);
+
+  // this wave's operand: k or v
+  bf16x8 opnd[KST];
+  {
+    const int64_t ho = (int64_t)head * p.head_dim * 2;
+    const uint32_t st = (uint32_t)(second ? p.v_stride : p.k_stride);
+    const __amdgpu_buffer_rsrc_t rs =
+        pp_rsrc((second ? p.v + txt.start * p.v_stride : p.k + txt.start * p.k_stride) + ho, (uint32_t)T * st);
+#pragma unroll
+    for (int i = 0; i < KST; ++i) {
+      const int c = 2 * i + hf;
+      const bool ok = own < T && c * 8 < p.head_dim;
+      opnd[i] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, ok ? own * st + c * 16 : BWD_NOWHERE, 0, 0));
+    }
+  }
 
   // per-lane addresses in stage 0: row reads of q, or dO; transposed reads of dO, or q; statistics
   uint32_t xa[4], ta[4];
@@ -619,9 +694,7 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_pair_kernel(AttnBwdParams p) 
   if (p.causal) w_lo = max(w_lo, r0);
   if (r0 >= T) w_hi = 0;
 
-  load_head();
-  if (n_tiles > 0) issue(0);
-  int t = t_lo;
+  int t = t_hi - 1, th = 0;
   for (int i = 0; i < n_tiles; ++i) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     lds_barrier();
@@ -632,7 +705,7 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_pair_kernel(AttnBwdParams p) 
     f32x16 s;
     if (seen) {
       if (!second) __builtin_amdgcn_s_setprio(1);
-      rows_product<D, S::BN, RD>(s, rows_stat(la), xa, 0, opnd);
+      rows_product<D, S::BN, RR>(s, rows_stat(la), xa, 0, opnd);
       if (!second) {
         __builtin_amdgcn_s_setprio(0);
         const bool whole = (!p.causal || s0 >= rlast) && (p.window < 0 || (s0 + 31 - r0 <= p.window && rlast - s0 <= p.window));
@@ -672,9 +745,12 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_pair_kernel(AttnBwdParams p) 
         x[0] = pack8(ds);
         x[1] = pack8(ds + 8);
       }
-      cols_product<D, S::BN, RD>(acc, ta, 0, x);
+      cols_product<D, S::BN, RC>(acc, ta, 0, x);
     }
-    if (++t == t_hi) t = t_lo;
+    if (++th == p.group) {
+      th = 0;
+      --t;
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       xa[e] ^= S::STAGE;
@@ -736,24 +812,81 @@ struct BwdLaunch {
   int threads, lds;
 };
 
-template <int D, bool KV>
+template <int D, bool KV, int QS>
 BwdLaunch bwd_plain(bool out16) {
-  return {out16 ? attn_bwd_kernel<D, KV, true> : attn_bwd_kernel<D, KV, false>, BWD_BM, 256, BwdShape<D>::LDS};
+  using S = BwdShape<D, KV, QS>;
+  return {out16 ? attn_bwd_kernel<D, KV, QS, true> : attn_bwd_kernel<D, KV, QS, false>, S::OWN, 256, S::LDS};
 }
-template <int D, int KG>
+template <int D>
 BwdLaunch bwd_pair(bool out16) {
-  return {out16 ? attn_bwd_pair_kernel<D, KG, true> : attn_bwd_pair_kernel<D, KG, false>, 32 * KG, 512, PairShape<D, KG>::LDS};
+  using S = PairShape<D>;
+  return {out16 ? attn_bwd_pair_kernel<D, true> : attn_bwd_pair_kernel<D, false>, 32 * S::KG, 512, S::LDS};
 }
 
-BwdLaunch bwd_launch(const inl_attn_desc& d, const std::vector<BwdText>& texts, bool kv, bool out16) {
-  if (d.head_dim <= 64) return kv ? bwd_plain<64, true>(out16) : bwd_plain<64, false>(out16);
-  if (d.head_dim <= 128) return kv ? bwd_plain<128, true>(out16) : bwd_plain<128, false>(out16);
-  if (!kv) return bwd_plain<256, false>(out16);
-  int64_t blocks = 0;
-  for (const BwdText& x : texts) blocks += (x.len + 127) / 128;
-  static const char* f = getenv("KG");
-  if (f ? f[0] == '2' : blocks * d.h_kv < 1024) return bwd_pair<256, 2>(out16);
-  return bwd_pair<256, 4>(out16);
+// How many times the average load of a place for a workgroup (`places` per CU) the longest workgroup's stream
+// is, with blocks of 128 own rows: above 1 it is what the kernel takes.
+double bwd_longest(const inl_attn_desc& d, const std::vector<BwdText>& texts, bool kv, int cus, int places) {
+  double longest = 0, all = 0;
+  for (const BwdText& x : texts) {
+    const double rows = d.window >= 0 ? std::min<double>(x.len, 2.0 * d.window + 128) : x.len;
+    longest = std::max(longest, rows);
+    all += rows * ((x.len + 127) / 128) * (d.causal && d.window < 0 ? 0.5 : 1.0);
+  }
+  // (a key block streams its group of heads, a query block is one of as many)
+  return longest * cus * places / (all * (kv ? d.h_kv : d.h_q));
+}
+
+// Two parts of the waves (QS = 2) halve the longest workgroup's stream and make twice the
+// workgroups, for twice the tiles read. us with one part / two (texts x tokens, query / key heads x features):
+//   dq:     1 x 1,024 causal 16/8 x 128 (7.1 average loads) 36 / 24, 1 x 2,048 12/12 x 64 (4) 47 / 40,
+//           8 x 512 causal 16/8 x 128 (1.8) 34 / 41, 8 x 1,024 3/1 x 256 (1.5) 66 / 66, 16 x 256 16/16 x 64 (1.5) 18 / 20
+//   dk, dv: x 64: 1 x 2,048 12/12 (4) 58 / 49, 2 x 2,048 16/16 (1.5) 82 / 93;
+//           x 128: 64 ragged causal passages 16/8 (2.8) 182 / 134, 8 x 512 16/8 (2) 54 / 45, 4 x 2,048 (1) 276 / 293,
+//           causal, whose blocks are of unequal length: 8 x 2,048 (0.94) 370 / 313, 64 x 180 (0.7) 64 / 56
+BwdLaunch bwd_launch(const inl_attn_desc& d, const std::vector<BwdText>& texts, bool kv, int cus, bool out16) {
+  const int dim = d.head_dim <= 64 ? 64 : d.head_dim <= 128 ? 128 : 256;
+  if (kv && dim == 256) return bwd_pair<256>(out16);
+  const double over = bwd_longest(d, texts, kv, cus, dim == 64 ? 3 : dim == 128 ? 2 : 1);
+  const bool two = !kv ? over > 2.5 : dim == 64 ? over > 2 : d.causal || over > 1.2;
+  if (dim == 64) return kv ? (two ? bwd_plain<64, true, 2>(out16) : bwd_plain<64, true, 1>(out16))
+                           : (two ? bwd_plain<64, false, 2>(out16) : bwd_plain<64, false, 1>(out16));
+  if (dim == 128) return kv ? (two ? bwd_plain<128, true, 2>(out16) : bwd_plain<128, true, 1>(out16))
+                            : (two ? bwd_plain<128, false, 2>(out16) : bwd_plain<128, false, 1>(out16));
+  return two ? bwd_plain<256, false, 2>(out16) : bwd_plain<256, false, 1>(out16);
+}
+
+// Which texts a workgroup finds its unit among, longest first within a class, so that the last workgroups
+// are short ones. Workgroup i runs on XCD i mod 8, each with an L2 of its own: with the texts dealt to as many
+// classes as make key heads x classes a multiple of 8, all blocks of a (text, key head), which
+// stream the same rows, share one. Texts that do not fill the classes evenly, to 1.15 of the mean, run in
+// one class: an XCD without work costs more than L2 misses.
+void bwd_classes(const inl_attn_desc& d, std::vector<BwdText>* texts, AttnBwdParams* p) {
+  std::sort(texts->begin(), texts->end(), [](const BwdText& a, const BwdText& b) {
+    return a.len != b.len ? a.len > b.len : a.start < b.start;
+  });
+  const int h = d.h_kv;
+  p->classes = h % 8 == 0 ? 1 : h % 4 == 0 ? 2 : h % 2 == 0 ? 4 : 8;
+  p->first[1] = (int32_t)texts->size();
+  if (p->classes == 1) return;
+  std::vector<BwdText> in[BWD_CLASSES];
+  double load[BWD_CLASSES] = {}, all = 0;
+  for (const BwdText& x : *texts) {   // the next longest to the least loaded
+    const int c = (int)(std::min_element(load, load + p->classes) - load);
+    const double cost = (double)x.len * (d.window >= 0 ? std::min<double>(x.len, 2.0 * d.window + 128) : x.len);
+    in[c].push_back(x);
+    load[c] += cost;
+    all += cost;
+  }
+  if (*std::max_element(load, load + p->classes) * p->classes > 1.15 * all) {
+    p->classes = 1;
+    return;
+  }
+  int32_t at = 0;
+  for (int c = 0; c < p->classes; ++c) {
+    p->first[c] = at;
+    for (const BwdText& x : in[c]) (*texts)[at++] = x;
+    p->first[c + 1] = at;
+  }
 }
 
 size_t bwd_stat_bytes(const inl_attn_desc& d, int64_t rows) { return ((size_t)2 * d.h_q * rows * 4 + 255) & ~(size_t)255; }
@@ -830,10 +963,6 @@ int bwd_run(const inl_attn_desc* d, const inl_attn_grads* g, const void* q, cons
   if (texts.empty() || (!dq && !dk)) return INL_OK;
   if ((rc = check_workspace("attention backward", ws, ws_bytes, bwd_bytes(*d, rows, texts.size())))) return rc;
 
-  // Longest texts first, so that the last workgroups are short ones.
-  std::sort(texts.begin(), texts.end(), [](const BwdText& a, const BwdText& b) {
-    return a.len != b.len ? a.len > b.len : a.start < b.start;
-  });
   AttnBwdParams p{};
   p.q = (const char*)q;
   p.k = (const char*)k;
@@ -848,7 +977,6 @@ int bwd_run(const inl_attn_desc* d, const inl_attn_grads* g, const void* q, cons
   for (int i = 0; i < 8; ++i) *strides[i] = t[i].stride * dtype_size(t[i].dtype);
   p.stat = (float*)ws;
   p.rows = rows;
-  p.n_texts = (int32_t)texts.size();
   p.h_q = d->h_q;
   p.h_kv = d->h_kv;
   p.group = d->h_q / d->h_kv;
@@ -859,14 +987,22 @@ int bwd_run(const inl_attn_desc* d, const inl_attn_grads* g, const void* q, cons
   p.c = std::max(d->scale * kLog2e, 1e-30f);
   p.scale = d->scale;
   const bool out16 = g->grad_dtype == INL_BF16;
+  int cus = 0;
+  if ((rc = device_cus(&cus))) return rc;
+  bwd_classes(*d, &texts, &p);
   for (int kv = 0; kv < (dk ? 2 : 1); ++kv) {
-    const BwdLaunch l = bwd_launch(*d, texts, kv, out16);
-    int64_t units = 0;
-    for (BwdText& x : texts) {
-      x.unit = (int32_t)units;
-      units += (x.len + l.own - 1) / l.own;
+    const BwdLaunch l = bwd_launch(*d, texts, kv, cus, out16);
+    int64_t most = 0;
+    for (int c = 0; c < p.classes; ++c) {
+      int64_t units = 0;
+      for (int i = p.first[c]; i < p.first[c + 1]; ++i) {
+        texts[i].unit = (int32_t)units;
+        units += (texts[i].len + l.own - 1) / l.own;
+      }
+      p.units[c] = (int32_t)units;
+      most = std::max(most, units);
     }
-    const int64_t groups = units * (kv ? d->h_kv : d->h_q);
+    const int64_t groups = most * p.h_kv * p.classes * (kv ? 1 : p.group);
     if (groups > INT32_MAX) return fail(INL_E_UNSUPPORTED, "attention backward: more than 2^31 blocks of rows and heads");
     if (texts.size() <= (size_t)BWD_INLINE) {
       std::copy(texts.begin(), texts.end(), p.own);

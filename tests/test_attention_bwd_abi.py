@@ -104,3 +104,23 @@ def test_binding_checks_tensors():
     x = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
     with pytest.raises(inl_hip.InlError, match="not a device tensor"):
         inl_hip.varlen_attention_bwd(x, x, x, x, x, [0, 4], causal=True)
+
+
+def test_listing_check_finds_missing_waits():
+    """A descriptor word that v_readfirstlane wrote is read five wait states later at the earliest."""
+    import importlib.util
+    from pathlib import Path
+    path = Path(__file__).resolve().parent.parent / "im-not-llm_amd" / "asmcheck.py"
+    spec = importlib.util.spec_from_file_location("asmcheck_waits", path)
+    check = importlib.util.module_from_spec(spec)
+    import sys
+    sys.modules[spec.name] = check
+    spec.loader.exec_module(check)
+    head = "_kernel:\n\tv_readfirstlane_b32 s61, v3\n\ts_mov_b32 m0, s4\n"
+    load = "\tbuffer_load_dwordx4 v3, s[60:63], 0 offen lds\n"
+    assert len(check.check_sgpr_waits(head + "\ts_nop 0\n" + load)) == 1
+    assert len(check.check_sgpr_waits(head + "\ts_nop 2\n" + load)) == 1
+    assert not check.check_sgpr_waits(head + "\ts_nop 3\n" + load)
+    assert not check.check_sgpr_waits(head + "\ts_mov_b32 s61, s7\n" + load)
+    assert not check.check_sgpr_waits("_kernel:\n\tv_readfirstlane_b32 s40, v3\n" + load)
+    assert not check.check_sgpr_waits(head + "_other:\n" + load)
