@@ -824,7 +824,7 @@ BwdLaunch bwd_pair(bool out16) {
 }
 
 // How many times the average load of a place for a workgroup (`places` per CU) the longest workgroup's stream
-// is, with blocks of 128 own rows: above 1 it is what the kernel takes.
+// is, with blocks of 128 own rows: above 1 it is what the kernel takes. 0: nothing to share between parts.
 double bwd_longest(const inl_attn_desc& d, const std::vector<BwdText>& texts, bool kv, int cus, int places) {
   double longest = 0, all = 0;
   for (const BwdText& x : texts) {
@@ -832,6 +832,7 @@ double bwd_longest(const inl_attn_desc& d, const std::vector<BwdText>& texts, bo
     longest = std::max(longest, rows);
     all += rows * ((x.len + 127) / 128) * (d.causal && d.window < 0 ? 0.5 : 1.0);
   }
+  if (longest <= 64) return 0;
   // (a key block streams its group of heads, a query block is one of as many)
   return longest * cus * places / (all * (kv ? d.h_kv : d.h_q));
 }
@@ -847,7 +848,7 @@ BwdLaunch bwd_launch(const inl_attn_desc& d, const std::vector<BwdText>& texts, 
   const int dim = d.head_dim <= 64 ? 64 : d.head_dim <= 128 ? 128 : 256;
   if (kv && dim == 256) return bwd_pair<256>(out16);
   const double over = bwd_longest(d, texts, kv, cus, dim == 64 ? 3 : dim == 128 ? 2 : 1);
-  const bool two = !kv ? over > 2.5 : dim == 64 ? over > 2 : d.causal || over > 1.2;
+  const bool two = !kv ? over > 2.5 : dim == 64 ? over > 2 : (d.causal && over > 0) || over > 1.2;
   if (dim == 64) return kv ? (two ? bwd_plain<64, true, 2>(out16) : bwd_plain<64, true, 1>(out16))
                            : (two ? bwd_plain<64, false, 2>(out16) : bwd_plain<64, false, 1>(out16));
   if (dim == 128) return kv ? (two ? bwd_plain<128, true, 2>(out16) : bwd_plain<128, true, 1>(out16))

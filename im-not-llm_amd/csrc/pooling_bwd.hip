@@ -25,9 +25,19 @@ constexpr int PB_ROWS = 32;
 constexpr float PB_UNIT_EPS = 1e-12f;
 
 // Number of entries of cu[0 .. n] that are <= r: one more than the text of row r (if any). The
-// whole wave takes part.
+// whole wave takes part: up to 255 texts in one round of loads, more in a search of 64 ways.
 __device__ __forceinline__ int cu_upto(const int32_t* cu, int n, int64_t r) {
   const int lane = threadIdx.x & 63;
+  if (n < 256) {
+    int count = 0;
+    int32_t e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = cu[min(lane + 64 * i, n)];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane + 64 * i <= n && (int64_t)e[i] <= r));
+    return count;
+  }
   int lo = 0, hi = n + 1;   // the answer is in [lo, hi]
   while (hi > lo) {
     const int step = (hi - lo + 63) / 64;
@@ -40,12 +50,18 @@ __device__ __forceinline__ int cu_upto(const int32_t* cu, int n, int64_t r) {
   return lo;
 }
 
-__device__ float wg_sum(float v, float* red) {
-  v = wave_sum(v);
+// Sums of N values over the workgroup, in all lanes.
+template <int N>
+__device__ __forceinline__ void wg_sums(float (&v)[N], float (*red)[4]) {
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = wave_sum(v[i]);
+    if ((threadIdx.x & 63) == 0) red[i][threadIdx.x >> 6] = v[i];
+  }
   __syncthreads();
-  return (red[0] + red[1]) + (red[2] + red[3]);
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = (red[i][0] + red[i][1]) + (red[i][2] + red[i][3]);
 }
 
 template <typename T>
@@ -59,11 +75,17 @@ __device__ __forceinline__ void st1(char* p, int64_t i, float v) {
   else reinterpret_cast<float*>(p)[i] = v;
 }
 
+template <int V>
+__device__ __forceinline__ void load_cols(const float* p, float (&v)[V]) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) v[e] = p[e];
+}
+
 // V columns per lane: 8 (16-byte aligned rows of multiples of 8 columns) or 1.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void pool_mean_bwd_kernel(const int32_t* cu, int n_texts, int dim, int64_t rows,
                                                             const float* dp, const float* mean, char* out, int64_t stride) {
-  __shared__ float red[4];
+  __shared__ float red[2][4];
   const int64_t first = (int64_t)blockIdx.x * PB_ROWS, last = min(first + PB_ROWS, rows);
   const int lanes = dim / V;                         // lanes of a row
   const int pass = max(1, 256 / lanes);              // rows written side by side
@@ -75,30 +97,49 @@ __global__ __launch_bounds__(256) void pool_mean_bwd_kernel(const int32_t* cu, i
     const int64_t end = b < n_texts ? min(last, max(r, (int64_t)cu[b + 1])) : last;
     if (end == r) continue;                          // (b only grows, to n_texts at most)
     float by_d = 0.f, by_m = 0.f;                    // the gradient is by_d d - by_m mean
+    const int64_t row = some ? (int64_t)b * dim : 0;
+    // a lane's columns of the first round stay in registers from the sums to the gradient
+    float d0[V] = {}, m0[V] = {};
+    if (some && l0 < lanes) {
+      load_cols<V>(dp + row + (int64_t)l0 * V, d0);
+      if (mean) load_cols<V>(mean + row + (int64_t)l0 * V, m0);
+    }
     if (some) {
-      const int64_t at = (int64_t)b * dim;
       by_d = 1.f / (float)((int64_t)cu[b + 1] - cu[b]);
       if (mean) {
-        float mm = 0.f, md = 0.f;
-        for (int c = threadIdx.x; c < dim; c += 256) {
-          const float x = mean[at + c];
-          mm += x * x;
-          md += x * dp[at + c];
-        }
-        mm = wg_sum(mm, red);
-        md = wg_sum(md, red);
-        const float s2 = mm + PB_UNIT_EPS;
+        float s[2] = {0.f, 0.f};                     // |mean|^2, mean . d
+        if (sub == 0)
+          for (int l = l0; l < lanes; l += 256) {
+            float d[V], m[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              d[e] = d0[e];
+              m[e] = m0[e];
+            }
+            if (l != l0) {
+              load_cols<V>(dp + row + (int64_t)l * V, d);
+              load_cols<V>(mean + row + (int64_t)l * V, m);
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              s[0] += m[e] * m[e];
+              s[1] += m[e] * d[e];
+            }
+          }
+        wg_sums<2>(s, red);
+        const float s2 = s[0] + PB_UNIT_EPS;
         by_d /= sqrtf(s2);
-        by_m = by_d * md / s2;
+        by_m = by_d * s[1] / s2;
       }
     }
     for (int l = l0; l < lanes && sub < pass; l += 256) {
       float g[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const int64_t at = (int64_t)b * dim + (int64_t)l * V + e;
-        g[e] = some ? by_d * dp[at] - (mean ? by_m * mean[at] : 0.f) : 0.f;
+      if (l != l0 && some) {
+        load_cols<V>(dp + row + (int64_t)l * V, d0);
+        if (mean) load_cols<V>(mean + row + (int64_t)l * V, m0);
       }
+#pragma unroll
+      for (int e = 0; e < V; ++e) g[e] = some ? by_d * d0[e] - (mean ? by_m * m0[e] : 0.f) : 0.f;
       for (int64_t i = r + sub; i < end; i += pass) {
         if constexpr (V == 8) store8<T>(out + (i * stride + (int64_t)l * 8) * (int64_t)sizeof(T), g);
         else st1<T>(out, i * stride + l, g[0]);
@@ -115,7 +156,7 @@ __global__ __launch_bounds__(256) void pool_last_bwd_kernel(const int32_t* cu, i
                                                             float eps, const float* dp, char* out, int64_t os,
                                                             float* part) {
   if ((int)blockIdx.x < n_texts) {
-    __shared__ float red[4];
+    __shared__ float red[3][4];
     const int b = blockIdx.x;
     const int64_t row = (int64_t)cu[b + 1] - 1;
     const float* d = dp + (int64_t)b * dim;
@@ -126,16 +167,15 @@ __global__ __launch_bounds__(256) void pool_last_bwd_kernel(const int32_t* cu, i
       return;
     }
     const char* x = hidden + row * stride * (int64_t)sizeof(T);
-    float xx = 0.f, zz = 0.f, zd = 0.f;
+    float s[3] = {0.f, 0.f, 0.f};
     for (int c = threadIdx.x; c < dim; c += 256) {
       const float v = ld1<T>(x, c), z = weight ? v * ld1<T>(weight, c) : v;
-      xx += v * v;
-      zz += z * z;
-      zd += z * d[c];
+      s[0] += v * v;
+      s[1] += z * z;
+      s[2] += z * d[c];
     }
-    xx = wg_sum(xx, red);
-    zz = wg_sum(zz, red);
-    zd = wg_sum(zd, red);
+    wg_sums<3>(s, red);
+    const float xx = s[0], zz = s[1], zd = s[2];
     const float inv = 1.0f / sqrtf(xx / (float)dim + eps);
     const float s2 = inv * inv * zz + PB_UNIT_EPS, is = 1.0f / sqrtf(s2);
     const float along = inv * zd / s2;                                              // y . d / size

@@ -17,7 +17,7 @@ import functools
 
 import torch
 
-from . import (INL_BF16, INL_F32, AttnDesc, InlError, NormRopeDesc, _check, _dtype_code, _head_rows, _head_weight,
+from . import (INL_BF16, INL_F32, AttnDesc, InlError, NormRopeDesc, _check, _cu_array, _dtype_code, _head_rows, _head_weight,
                _rope_tables, _sig, c_i32, c_i64, c_void_p, desc_rows, make_attn_desc)
 
 ACTS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu_tanh": 3, "gelu_erf": 4}
@@ -450,13 +450,20 @@ def norm_rope_qk_bwd(dy, x, q_heads, rows=None, cos=None, sin=None, *, q_weight=
 
 def _head_tensor(name, t, rows, heads, hd, dtype, dev):
     """The stride between the token rows of ``t [rows or more, heads, hd]``."""
-    if len(t.shape) != 3 or t.shape[1:] != (heads, hd):
-        raise InlError(-1, f"{name}: shape {tuple(t.shape)}, need [rows, {heads}, {hd}]")
+    shape = t.shape
+    if len(shape) == 3:   # (the usual form first: a short batch waits for these checks)
+        row, head, one = t.stride()
+        n, h, d = shape
+        if n >= rows and n > 1 and h == heads and d == hd and t.dtype is dtype and one == 1 \
+                and (head == hd or heads == 1) and row >= heads * hd and t.get_device() == dev:
+            return row
+    if len(shape) != 3 or shape[1:] != (heads, hd):
+        raise InlError(-1, f"{name}: shape {tuple(shape)}, need [rows, {heads}, {hd}]")
     if t.dtype is not dtype:
         raise InlError(-1, f"{name}: dtype {t.dtype}, need {dtype}")
-    if t.shape[0] < rows:
-        raise InlError(-1, f"{name}: {t.shape[0]} rows, the texts cover {rows}")
-    return _head_rows(name, t, t.shape, dev)
+    if shape[0] < rows:
+        raise InlError(-1, f"{name}: {shape[0]} rows, the texts cover {rows}")
+    return _head_rows(name, t, shape, dev)
 
 
 @_at_home
@@ -464,33 +471,42 @@ def _attn_grads(dev, q, dout, k, v, out, cu_seqlens, causal, window, scale, seq_
     if len(q.shape) != 3 or len(k.shape) != 3:
         raise InlError(-1, f"q, k: shapes {tuple(q.shape)}, {tuple(k.shape)}, need [rows, heads, head_dim]")
     n, hq, hd = q.shape
-    hkv = k.shape[1]
-    d = make_attn_desc(cu_seqlens, hq, hkv, hd, causal=causal, window=window, scale=scale, seq_starts=seq_starts)
-    rows = desc_rows(d)
-    d.q_row_stride = _head_tensor("q", q, rows, hq, hd, _BF16, dev)
-    d.k_row_stride = _head_tensor("k", k, rows, hkv, hd, _BF16, dev)
-    d.v_row_stride = _head_tensor("v", v, rows, hkv, hd, _BF16, dev)
-    d.o_row_stride = _head_tensor("out", out, rows, hq, hd, _BF16, dev)
+    nk, hkv, _ = k.shape
+    texts = len(cu_seqlens) - 1
+    if seq_starts is None:
+        cu, starts = _cu_array(cu_seqlens), None
+        rows = cu[texts] if texts > 0 else 0
+    else:
+        d = make_attn_desc(cu_seqlens, hq, hkv, hd, causal=causal, seq_starts=seq_starts)   # checks the lengths
+        cu, starts, rows = d._cu_keepalive, d._starts_keepalive, desc_rows(d)
+    d = AttnDesc(texts, cu, hq, hkv, hd, bool(causal), -1 if window is None else int(window),
+                 hd ** -0.5 if scale is None else scale, INL_BF16, INL_BF16,
+                 _head_tensor("q", q, rows, hq, hd, _BF16, dev), _head_tensor("k", k, rows, hkv, hd, _BF16, dev),
+                 _head_tensor("v", v, rows, hkv, hd, _BF16, dev), _head_tensor("out", out, rows, hq, hd, _BF16, dev), 0,
+                 starts)
     dos = _head_tensor("dout", dout, rows, hq, hd, _BF16, dev)
     if grads is None:
         # rows of no text have no gradient: they are zero in tensors made here
-        made = torch.zeros if seq_starts is not None or n != rows or k.shape[0] != rows else torch.empty
+        made = torch.zeros if starts is not None or n != rows or nk != rows else torch.empty
         dt = grad_dtype or _BF16
         dq = made((n, hq, hd), dtype=dt, device=q.device)
-        dk, dv = (made((k.shape[0], hkv, hd), dtype=dt, device=q.device) for _ in range(2)) if kv_grad else (None, None)
+        dk = dv = None
+        if kv_grad:
+            dk, dv = made((nk, hkv, hd), dtype=dt, device=q.device), made((nk, hkv, hd), dtype=dt, device=q.device)
+        g = AttnGrads(dos, 0, 0, 0, _dtype_code(dt))
     else:
         dq, dk, dv = grads
         dt = next((t.dtype for t in grads if t is not None), _BF16)
         if grad_dtype is not None and grad_dtype is not dt:
             raise InlError(-1, f"grads: dtype {dt}, grad_dtype {grad_dtype}")
-    strides = [0 if t is None else _head_tensor(name, t, rows, heads, hd, dt, dev)
-               for name, t, heads in (("dq", dq, hq), ("dk", dk, hkv), ("dv", dv, hkv))]
-    g = AttnGrads(dos, *strides, _dtype_code(dt))
-    size = ctypes.c_size_t()
-    _check(_attn_bwd_ws(d, ctypes.byref(size)))
-    room = _room(size.value, dev)
+        strides = [0 if t is None else _head_tensor(name, t, rows, heads, hd, dt, dev)
+                   for name, t, heads in (("dq", dq, hq), ("dk", dk, hkv), ("dv", dv, hkv))]
+        g = AttnGrads(dos, *strides, _dtype_code(dt))
+    # inl_attn_bwd_workspace_size, or as much as a table of all the texts more
+    size = (8 * hq * max(rows, 0) + 255 & ~255) + (12 * texts if texts > 256 else 0)
+    room = _room(size, dev)
     _check(_attn_bwd(d, g, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), _ptr(dq),
-                     _ptr(dk), _ptr(dv), _ptr(room), size.value, _stream(dev)))
+                     _ptr(dk), _ptr(dv), _ptr(room), size, _stream(dev)))
     return dq, dk, dv
 
 
