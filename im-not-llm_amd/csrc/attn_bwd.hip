@@ -109,7 +109,8 @@ struct BwdUnit {
 // False where there is nothing (classes have unequal numbers of units).
 __device__ __forceinline__ bool bwd_unit(const AttnBwdParams& p, int members, int lane, BwdUnit* out) {
   const int width = p.h_kv * p.classes;
-  const int rest = blockIdx.x / width, x = blockIdx.x - rest * width;
+  const uint32_t wg = blockIdx.y * gridDim.x + blockIdx.x;
+  const int rest = wg / width, x = wg - rest * width;
   const int cls = x / p.h_kv, u = rest / members;
   out->kvh = x - cls * p.h_kv;
   out->member = rest - u * members;
@@ -943,7 +944,14 @@ int bwd_run(const inl_attn_desc* d, const inl_attn_grads* g, const void* q, cons
                           {"dk", dk, d->h_kv, g->dk_row_stride ? g->dk_row_stride : kr, g->grad_dtype},
                           {"dv", dv, d->h_kv, g->dv_row_stride ? g->dv_row_stride : kr, g->grad_dtype}};
   int64_t longest = 0;
-  for (const BwdText& x : texts) longest = std::max<int64_t>(longest, x.len);
+  int64_t blocks = 0;
+  for (const BwdText& x : texts) {
+    longest = std::max<int64_t>(longest, x.len);
+    blocks += (x.len + 63) / 64;
+  }
+  // (all classes are numbered like the one with the most blocks)
+  if (blocks * d->h_q * BWD_CLASSES > INT32_MAX)
+    return fail(INL_E_UNSUPPORTED, "attention backward: more than 2^28 blocks of 64 rows and a head");
   Rows r[8];
   for (int i = 0; i < 8; ++i) {
     const int64_t es = dtype_size(t[i].dtype), len = t[i].heads * d->head_dim;
@@ -983,7 +991,7 @@ int bwd_run(const inl_attn_desc* d, const inl_attn_grads* g, const void* q, cons
   p.group = d->h_q / d->h_kv;
   p.head_dim = d->head_dim;
   p.causal = d->causal;
-  p.window = d->window;
+  p.window = (int32_t)std::min<int64_t>(d->window, longest);   // (own + window stays in 32 bits)
   // (the statistics are divided by c, and must stay finite; scores times less than this are 0)
   p.c = std::max(d->scale * kLog2e, 1e-30f);
   p.scale = d->scale;
@@ -1004,7 +1012,8 @@ int bwd_run(const inl_attn_desc* d, const inl_attn_grads* g, const void* q, cons
       most = std::max(most, units);
     }
     const int64_t groups = most * p.h_kv * p.classes * (kv ? 1 : p.group);
-    if (groups > INT32_MAX) return fail(INL_E_UNSUPPORTED, "attention backward: more than 2^31 blocks of rows and heads");
+    // (a dimension of a grid has fewer than 2^32 threads; a multiple of 8 keeps workgroups on their XCDs)
+    const int64_t across = std::min<int64_t>(groups, 1 << 22);
     if (texts.size() <= (size_t)BWD_INLINE) {
       std::copy(texts.begin(), texts.end(), p.own);
     } else {
@@ -1020,7 +1029,7 @@ int bwd_run(const inl_attn_desc* d, const inl_attn_grads* g, const void* q, cons
       p.texts = table;
     }
     if ((rc = set_max_dynamic_lds((const void*)l.fn, l.lds))) return rc;
-    hipLaunchKernelGGL(l.fn, dim3((unsigned)groups), dim3(l.threads), l.lds, st, p);
+    hipLaunchKernelGGL(l.fn, dim3((unsigned)across, (unsigned)((groups + across - 1) / across)), dim3(l.threads), l.lds, st, p);
     INL_HIP_TRY(hipGetLastError());
   }
   return INL_OK;

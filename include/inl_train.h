@@ -6,10 +6,10 @@
  * buffer. Nothing is allocated and nothing synchronised, so every call can be
  * captured into a graph.
  *
- * Matrices are rows of bf16 (strides in elements between rows, 0 = packed),
- * 16-byte aligned, row lengths and strides multiples of 8 elements; products
- * accumulate in f32 on the matrix cores. Other shapes are refused
- * (INL_E_UNSUPPORTED).
+ * Matrices are rows of bf16, or of the dtypes that a section names (strides in
+ * elements between rows, 0 = packed), 16-byte aligned, row lengths and strides
+ * multiples of 8 elements where a section says nothing else; products accumulate
+ * in f32 on the matrix cores. Other shapes are refused (INL_E_UNSUPPORTED).
  *
  * Workspaces: device memory of at least the size the *_workspace_size call
  * gives for the same desc, 16-byte aligned, untouched until the call has
@@ -199,8 +199,8 @@ int inl_norm_rope_qk_bwd(const inl_norm_rope_desc* desc, int32_t q_heads, const 
  * another argument or one another, but may be slices of one row. Rows outside every
  * text are not written; with seq_starts_host the texts may not overlap. Infinities and
  * NaNs in a text reach any gradient of that text and of no other. A text's rows of each tensor
- * span less than 4 GiB. The texts' table travels with the launches: a captured call replays with
- * the lengths it was captured with.
+ * span less than 4 GiB; blocks of 64 rows times h_q stay below 2^28. The texts' table travels with
+ * the launches: a captured call replays with the lengths it was captured with.
  * --------------------------------------------------------------------- */
 typedef struct inl_attn_grads {
   int64_t do_row_stride;   /* elements; 0 = h_q * head_dim */
@@ -266,7 +266,7 @@ int inl_add_rms_norm_bwd(const inl_add_norm_desc* desc, const void* dy, const vo
  * Gradients of the pooled embedding (inl_pool_mean_fwd, inl_pool_last_fwd of inl_hip.h): every row
  * of dhidden [rows, hidden_dim] is written, in `dtype`; rows of no text get 0. cu: DEVICE
  * int32 [n_texts + 1], read on the device; whatever it holds, nothing outside the rows is
- * written. dpooled: f32 [n_texts, hidden_dim], packed.
+ * written. dpooled: f32 [n_texts, hidden_dim], packed. n_texts + rows / 32 stays below 2^24.
  * --------------------------------------------------------------------- */
 
 /* dhidden[r] = d / len of r's text, d = dpooled, or with `mean` (f32 [n_texts, hidden_dim]: what the

@@ -124,3 +124,9 @@ def test_listing_check_finds_missing_waits():
     assert not check.check_sgpr_waits(head + "\ts_mov_b32 s61, s7\n" + load)
     assert not check.check_sgpr_waits("_kernel:\n\tv_readfirstlane_b32 s40, v3\n" + load)
     assert not check.check_sgpr_waits(head + "_other:\n" + load)
+
+
+def test_too_many_blocks(T):
+    """The span of a text allows it, the number of blocks does not."""
+    far = {i: (i + 1) << 44 for i in range(8)}
+    assert _call(T, lengths=[1] * 300, hq=1 << 20, hkv=1, hd=8, ptrs=far) == -2 and _said("blocks")

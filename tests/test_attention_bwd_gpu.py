@@ -246,3 +246,31 @@ def test_nothing_to_do(cuda, inl):
     assert all(x.shape == (0, 2, 64) for x in inl.varlen_attention_bwd(e, e, e, e, e, [0, 0, 0], causal=True))
     z = torch.randn(4, 2, 64, device=cuda).to(torch.bfloat16)
     assert not any(x.any() for x in inl.varlen_attention_bwd(z, z, z, z, z, [0, 0], causal=False))
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_widest_window(causal, cuda, inl):
+    """A window of any size up to 2^31 - 1 that covers the texts is no window."""
+    import torch
+    for hd in (64, 128, 256):
+        lengths = [70, 1, 300]
+        q, k, v, dout, starts, cu = _inputs(torch, cuda, lengths, 2, 1, hd, 13)
+        out = A.forward(q, k, v, starts, lengths, causal, -1, hd ** -0.5).to(torch.bfloat16)
+        A.check(inl.varlen_attention_bwd(dout, q, k, v, out, cu, causal=causal, window=2 ** 31 - 1),
+                A.backward(dout, q, k, v, out, starts, lengths, causal, -1, hd ** -0.5), lengths)
+
+
+def test_more_blocks_than_one_grid_has_threads_for(cuda, inl):
+    """2^18 + 3 texts of one token and 64 heads: a key is all that its query sees, so dv is dout, and
+    dq and dk are 0."""
+    import torch
+    n, h, hd = 2 ** 18 + 3, 64, 8
+    g = torch.Generator(device=cuda).manual_seed(1)
+    q, k, v, dout = (torch.randn(n, h, hd, generator=g, device=cuda).to(torch.bfloat16) for _ in range(4))
+    dq, dk, dv = inl.varlen_attention_bwd(dout, q, k, v, v, list(range(n + 1)), causal=False)
+    assert torch.equal(dv, dout)
+    # dP - delta: delta has 8 roundings of 2^-24 at most of s = sum |dout v|; dP is added up from -delta on, 8
+    # steps of 2^-23 (matrix instructions need not round to nearest) of 2 s
+    few = (40 * 2.0 ** -24 * (dout.abs().float() * v.abs().float()).sum(-1, keepdim=True))
+    assert (dq.float().abs() <= few * hd ** -0.5 * k.abs().float() * (1 + 2.0 ** -6)).all()
+    assert (dk.float().abs() <= few * hd ** -0.5 * q.abs().float() * (1 + 2.0 ** -6)).all()
