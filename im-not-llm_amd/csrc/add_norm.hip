@@ -101,7 +101,7 @@ template <typename TX, typename TR, typename TY, int W, int K>
 __global__ __launch_bounds__(256) void add_norm_kernel(AddNormParams p) {
   constexpr int ROWS = 4 / W;
   __shared__ float red[4];
-  const int64_t r = (int64_t)blockIdx.x * ROWS + (W == 1 ? threadIdx.x >> 6 : 0);
+  const int64_t r = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * ROWS + (W == 1 ? threadIdx.x >> 6 : 0);
   if (r >= p.m) return;   // uniform over the waves of a row
   const int j = W == 1 ? threadIdx.x & 63 : threadIdx.x;
   const char* xr = p.x + r * p.xs * (int64_t)sizeof(TX);
@@ -308,7 +308,12 @@ int norm_weight(const inl_add_norm_desc* d, const void* weight, const void* rng,
 
 template <typename TX, typename TR, typename TY, bool BWD>
 void add_norm_launch(const AddNormParams& p, unsigned groups, hipStream_t st) {
-  const dim3 block(256), rows(BWD ? groups : (unsigned)((p.m + 3) / 4)), wide(BWD ? groups : (unsigned)p.m);
+  // (a dimension of a grid has fewer than 2^32 threads)
+  auto grid = [&](int64_t n) {
+    const int64_t x = std::min<int64_t>(n, 1 << 22);
+    return BWD ? dim3(groups) : dim3((unsigned)x, (unsigned)((n + x - 1) / x));
+  };
+  const dim3 block(256), rows = grid((p.m + 3) / 4), wide = grid(p.m);
 #define INL_NORM(W, K)                                                                                        \
   do {                                                                                                        \
     if constexpr (BWD) hipLaunchKernelGGL((add_norm_bwd_kernel<TX, TR, TY, W, K>), W == 1 ? rows : wide, block, 0, st, p); \

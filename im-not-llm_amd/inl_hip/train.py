@@ -569,16 +569,19 @@ def _norm_fwd(dev, x, weight, residual, eps, dropout, rng, tag, out, sum_out, ou
     if out is None:
         out = x.new_empty((m, n), dtype=out_dtype)
     ys = _mat("out", out, m, n, _ANY, dev)
-    h = sum_out
+    h, plain = sum_out, residual is None and not drop   # the sum of nothing is x itself
     if h is None:
         sd = sum_dtype or x.dtype
-        # the sum of nothing is x itself
-        h = x if residual is None and not drop and sd is x.dtype else x.new_empty((m, n), dtype=sd)
-    elif sum_dtype is not None and sum_dtype is not h.dtype:
-        raise InlError(-1, f"sum_out: dtype {h.dtype}, need {sum_dtype}")
+        # (and y may not take its place)
+        kept = plain and sd is x.dtype and out.untyped_storage().data_ptr() != x.untyped_storage().data_ptr()
+        h = x if kept else x.new_empty((m, n), dtype=sd)
+    else:
+        kept = False
+        if sum_dtype is not None and sum_dtype is not h.dtype:
+            raise InlError(-1, f"sum_out: dtype {h.dtype}, need {sum_dtype}")
     hs = _mat("sum_out", h, m, n, _ANY, dev)
     d = AddNormDesc(m, n, xs, rs, hs, ys, 0, eps, drop, _tag(tag), _CODE[x.dtype], _CODE[h.dtype], _CODE[out.dtype], wd)
-    _check(_add_norm(d, x.data_ptr(), _ptr(residual), wp, rp, None if h is x else h.data_ptr(), out.data_ptr(),
+    _check(_add_norm(d, x.data_ptr(), _ptr(residual), wp, rp, None if kept else h.data_ptr(), out.data_ptr(),
                      _stream(dev)))
     return out, h
 
@@ -588,8 +591,8 @@ def add_rms_norm(x, weight=None, *, residual=None, eps=1e-6, dropout=0.0, rng=No
     """``(y, h)`` with ``h = residual + drop(x)`` and ``y = h / sqrt(mean(h^2) + eps) * weight``
     (``inl_add_rms_norm_fwd``): bf16 or f32 ``x [m, n]`` and ``weight [n]``, ``residual [m, n]`` or None; n a multiple of 8,
     at most 16384; rows may be strided. h has the residual's dtype (without one ``sum_dtype``, x's by
-    default) and may go into ``sum_out``, which may be the residual itself; y has x's dtype unless
-    ``out_dtype`` says otherwise. ``dropout``: the probability (in steps of 1 / 65536); its draws come from
+    default; without dropout too it is x itself, where ``out`` is not) and may go into
+    ``sum_out``, which may be x or the residual itself; y has x's dtype unless ``out_dtype`` says otherwise. ``dropout``: the probability (in steps of 1 / 65536); its draws come from
     ``rng``, int64 ``[2]`` on the device (seed, step), and ``tag``, a number of this place
     in the model; no mask is kept."""
     return _norm_fwd(x, weight, residual, eps, dropout, rng, tag, out, sum_out, out_dtype, sum_dtype, stream)

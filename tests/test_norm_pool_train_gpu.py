@@ -301,3 +301,37 @@ def test_nothing_to_do(cuda, inl):
     assert not dx.any() and not dw.any()
     dx, dw = inl.pool_last_bwd(dp, none, cu, w)
     assert dx.shape == (0, 64) and not dw.any()
+
+
+def test_sum_in_x(cuda, inl):
+    """The sum in x's place, with and without something to add; y in x's place where the sum is x."""
+    import torch
+    m, n = 21, 264
+    r = _randn(torch, cuda, (m, n), 1, 1.0, torch.bfloat16)
+    rng = torch.tensor([5, 6], device=cuda)
+    for residual, dropout in ((r, 0.0), (None, 0.3), (r, 0.3), (None, 0.0)):
+        x = _randn(torch, cuda, (m, n), 2, 1.0, torch.bfloat16)
+        want = inl.add_rms_norm(x.clone(), residual=residual, dropout=dropout, rng=rng)
+        y, h = inl.add_rms_norm(x, residual=residual, dropout=dropout, rng=rng, sum_out=x)
+        assert h is x and torch.equal(y, want[0]) and torch.equal(x, want[1])
+    x = _randn(torch, cuda, (m, n), 2, 1.0, torch.bfloat16)
+    want = inl.add_rms_norm(x.clone())
+    with pytest.raises(inl.InlError, match="overlaps"):
+        inl.add_rms_norm(x, out=x, sum_out=x)
+    y, h = inl.add_rms_norm(x, out=x)
+    assert y is x and torch.equal(y, want[0]) and torch.equal(h, want[1])
+
+
+def test_more_rows_than_one_grid_has_threads_for(cuda, inl):
+    import torch
+    m, n = 2 ** 26 + 5, 8
+    x = torch.empty(m, n, dtype=torch.bfloat16, device=cuda)
+    x[:] = _randn(torch, cuda, (1, n), 1, 1.0, torch.bfloat16)
+    x[-3:] *= 2
+    r = torch.zeros_like(x)
+    y, h = inl.add_rms_norm(x, residual=r, eps=0.0)
+    assert torch.equal(h, x)
+    one = torch.ones((), dtype=torch.float64, device=cuda)
+    for rows in (slice(0, 9), slice(2 ** 24 - 4, 2 ** 24 + 4), slice(m - 9, m)):
+        S.check_add_norm(y[rows], h[rows], x[rows], None, None, one, 0.0, f"rows {rows}")
+    assert torch.equal(y[1:-3], y[:1].expand(m - 4, n))
