@@ -215,7 +215,9 @@ int pool_bwd_check(const char* what, int32_t n_texts, const int32_t* cu, int32_t
                    int32_t dtype, const float* dp, const void* out) {
   const std::string w(what);
   if (n_texts < 0 || dim <= 0 || rows < 0 || !dtype_ok(dtype)) return fail(INL_E_INVALID, w + ": bad n_texts, hidden_dim, rows or dtype");
-  if (rows > INT32_MAX) return fail(INL_E_UNSUPPORTED, w + ": more than 2^31 - 1 rows");
+  // (a grid has fewer than 2^32 threads: 256 for a text, and for PB_ROWS rows)
+  if (n_texts + (rows + PB_ROWS - 1) / PB_ROWS >= (int64_t)1 << 24)
+    return fail(INL_E_UNSUPPORTED, w + ": n_texts + rows / 32 must stay below 2^24");
   if (stride < dim) return fail(INL_E_INVALID, w + ": the row stride must cover hidden_dim");
   if (rows && (!out || (n_texts && (!cu || !dp)))) return fail(INL_E_INVALID, w + ": NULL pointer");
   if ((((uintptr_t)cu | (uintptr_t)dp) & 3) || ((uintptr_t)out % dtype_size(dtype)))
@@ -294,7 +296,6 @@ extern "C" int inl_pool_last_bwd(int32_t n_texts, const int32_t* cu, int32_t dim
   if (join && (rc = check_workspace("pool_last_bwd", ws, ws_bytes, (size_t)n_texts * (size_t)dim * 4))) return rc;
   float* part = join ? (float*)ws : dweight;
   const int64_t fills = (rows + PB_ROWS - 1) / PB_ROWS;
-  if (n_texts + fills > INT32_MAX) return fail(INL_E_UNSUPPORTED, "pool_last_bwd: too many texts and rows");
   const dim3 grid((unsigned)(n_texts + fills)), block(256);
 #define INL_POOL(T, TO, V)                                                                                            \
   hipLaunchKernelGGL((pool_last_bwd_kernel<T, TO, V>), grid, block, 0, st, cu, n_texts, dim, rows, (const char*)hidden, \

@@ -111,6 +111,14 @@ def test_pool_refusals(T):
     assert last(rows=0, out=None, cu=None, dp=None, h=None, dw=None) == 0
 
 
+def test_pool_grids(T):
+    far = [(i + 1) << 44 for i in range(6)]
+    for n, rows in ((3, 2 ** 29), (2 ** 24, 9), (2 ** 23, 2 ** 28), (2 ** 31 - 1, 9)):
+        assert T._pool_mean_bwd(n, far[0], 8, rows, 0, 1, far[1], far[2], far[3], None) == -2 and all(_said("2^24"))
+        assert T._pool_last_bwd(n, far[0], 8, rows, 0, 1, far[1], far[2], None, 1e-6, 0, 1, far[3], None, None, 0,
+                                None) == -2 and all(_said("2^24"))
+
+
 def test_bindings_check_tensors():
     import torch
 
