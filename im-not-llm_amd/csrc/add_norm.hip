@@ -15,6 +15,9 @@
 // Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011), one draw of 128
 // bits for 8 elements, 16 bits each: with 32 bits an element the generator's multiplications
 // would take longer than the memory does.
+//
+// 20,011 x 768, f32 stream, dropout 0.1: forward 36.5 us a call (5.0 TB/s), backward 51 and 5 for
+// the join of dweight (4.8 TB/s without it); 65,536 x 1,024 in bf16, backward 106 us in all (5.0 TB/s). One row: 2.5.
 #include <algorithm>
 
 #include "norm_rope.hpp"

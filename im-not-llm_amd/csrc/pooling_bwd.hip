@@ -10,6 +10,9 @@
 // epsilons: with size^2 = |z|^2 + e, e = 1e-12, the mean that the norm's gradient subtracts is
 // mean(dn x / rms) = (x w . d) e / (rms size^3 n), no difference of near values. So one pass of
 // three sums (x^2, (x w)^2, x w . d) gives the gradient.
+//
+// Mean of 26,923 x 768 rows in bf16: 10.8 us (3.9 TB/s; 17.1 with a search for the text in rounds of
+// dependent loads). Last token of 14,716 x 1,024: 9.8 (3.1 TB/s) and 3.9 for the join of dweight.
 #include <algorithm>
 
 #include "norm_rope.hpp"

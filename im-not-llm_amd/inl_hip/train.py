@@ -1,6 +1,7 @@
 """Layer and head ops with their gradients (``include/inl_train.h``): a linear
 layer with bias, activation and residual, the gated feed-forward block, softmax
-cross entropy without its scores, and the gradients of the q/k prologue.
+cross entropy without its scores, the residual stream's addition with dropout and
+norm, and the gradients of the q/k prologue, of attention and of the pooled embedding.
 
 Gradients are plain functions of what the forward left (outputs carry no autograd
 graph, whatever ``requires_grad`` says of the inputs): a ``torch.autograd.Function`` or a training loop calls them in its own

@@ -1,6 +1,6 @@
 /*
- * inl_train.h - C ABI of the layer and head ops with their gradients, on one
- * MI355X (gfx950): what fine-tuning the encoders of inl_encoder.h needs beside
+ * inl_train.h - C ABI of the layer and head ops with their gradients, and of the
+ * gradients of attention and pooling, on one MI355X (gfx950): what fine-tuning the encoders of inl_encoder.h needs beside
  * its forward. Conventions are those of inl_hip.h: device pointers, int status
  * + inl_last_error(), work on the caller's stream, the caller owns every
  * buffer. Nothing is allocated and nothing synchronised, so every call can be
