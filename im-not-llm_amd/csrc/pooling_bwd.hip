@@ -25,6 +25,7 @@ namespace inl {
 namespace {
 
 constexpr int PB_ROWS = 32;
+constexpr int PB_KEPT = 4;
 constexpr float PB_UNIT_EPS = 1e-12f;
 
 // Number of entries of cu[0 .. n] that are <= r: one more than the text of row r (if any). The
@@ -170,25 +171,44 @@ __global__ __launch_bounds__(256) void pool_last_bwd_kernel(const int32_t* cu, i
       return;
     }
     const char* x = hidden + row * stride * (int64_t)sizeof(T);
+    // the first PB_KEPT columns of a lane stay in registers: their loads are under way together
+    float kx[PB_KEPT], kw[PB_KEPT], kd[PB_KEPT];
     float s[3] = {0.f, 0.f, 0.f};
-    for (int c = threadIdx.x; c < dim; c += 256) {
-      const float v = ld1<T>(x, c), z = weight ? v * ld1<T>(weight, c) : v;
+#pragma unroll
+    for (int k = 0; k < PB_KEPT; ++k) {
+      const int c = min((int)threadIdx.x + 256 * k, dim - 1);
+      kx[k] = ld1<T>(x, c);
+      kw[k] = weight ? ld1<T>(weight, c) : 1.f;
+      kd[k] = d[c];
+    }
+    auto sums = [&](float v, float w, float g) {
+      const float z = v * w;
       s[0] += v * v;
       s[1] += z * z;
-      s[2] += z * d[c];
-    }
+      s[2] += z * g;
+    };
+#pragma unroll
+    for (int k = 0; k < PB_KEPT; ++k)
+      if ((int)threadIdx.x + 256 * k < dim) sums(kx[k], kw[k], kd[k]);
+    for (int c = threadIdx.x + 256 * PB_KEPT; c < dim; c += 256) sums(ld1<T>(x, c), weight ? ld1<T>(weight, c) : 1.f, d[c]);
     wg_sums<3>(s, red);
     const float xx = s[0], zz = s[1], zd = s[2];
     const float inv = 1.0f / sqrtf(xx / (float)dim + eps);
     const float s2 = inv * inv * zz + PB_UNIT_EPS, is = 1.0f / sqrtf(s2);
     const float along = inv * zd / s2;                                              // y . d / size
     const float mean = inv * zd * is * (PB_UNIT_EPS / s2) / (float)dim;             // of dn x / rms
-    for (int c = threadIdx.x; c < dim; c += 256) {
-      const float hat = ld1<T>(x, c) * inv, w = weight ? ld1<T>(weight, c) : 1.f;
-      const float dz = is * (d[c] - hat * w * along);
+    auto put = [&](int c, float v, float w, float g) {
+      const float hat = v * inv;
+      const float dz = is * (g - hat * w * along);
       st1<TO>(out, row * os + c, inv * (dz * w - hat * mean));
       if (dw) dw[c] = dz * hat;
+    };
+#pragma unroll
+    for (int k = 0; k < PB_KEPT; ++k) {
+      const int c = threadIdx.x + 256 * k;
+      if (c < dim) put(c, kx[k], kw[k], kd[k]);
     }
+    for (int c = threadIdx.x + 256 * PB_KEPT; c < dim; c += 256) put(c, ld1<T>(x, c), weight ? ld1<T>(weight, c) : 1.f, d[c]);
     return;
   }
   __shared__ int taken[PB_ROWS];
@@ -203,11 +223,14 @@ __global__ __launch_bounds__(256) void pool_last_bwd_kernel(const int32_t* cu, i
     if (end > cu[b] && end > first) taken[end - 1 - first] = 1;
   }
   __syncthreads();
-  const int lanes = dim / V;
+  const int lanes = dim / V;                         // lanes of a row; short rows are written side by side
+  const int pass = max(1, 256 / lanes), sub = lanes <= 256 ? threadIdx.x / lanes : 0;
+  const int l0 = lanes <= 256 ? threadIdx.x - sub * lanes : threadIdx.x;
   const float zero[8] = {};
-  for (int64_t i = first; i < last; ++i) {
+  if (sub >= pass) return;
+  for (int64_t i = first + sub; i < last; i += pass) {
     if (taken[i - first]) continue;
-    for (int l = threadIdx.x; l < lanes; l += 256) {
+    for (int l = l0; l < lanes; l += 256) {
       if constexpr (V == 8) store8<TO>(out + (i * os + (int64_t)l * 8) * (int64_t)sizeof(TO), zero);
       else st1<TO>(out, i * os + l, 0.f);
     }
