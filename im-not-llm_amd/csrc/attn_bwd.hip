@@ -25,7 +25,7 @@
 // products, ds_read_b64_tr_b16 for the second); the swizzle serves both.
 //
 // Bound by its products where texts are long: 8 x 2,048 tokens, 16/8 heads of 128, full: dq 990, dk and dv 1,040
-// TFLOP/s of those that they do; 4 x 4,096 causal, 16/2 heads of 256: 1.03 and 1.26 ms, matrix cores 36 and
+// TFLOP/s of those that they do; 4 x 4,096 causal, 16/2 heads of 256: 0.99 and 1.26 ms, matrix cores 38 and
 // 39 % busy, as one wave or a pair has a SIMD to itself and its exponentials stand between its products. By
 // bytes and the start of workgroups where they are short: 64 x 256 tokens of 16 heads of 64 take 50 and 54 us, for
 // 39 us of bytes each at 4.84 TB/s; 48 texts to 1,021 with a window of 64 and 12 heads 72 and 65 for 53.
@@ -160,6 +160,30 @@ __device__ __forceinline__ void rows_product(f32x16& acc, const f32x16& first, c
   }
 }
 
+// Two such products beside one another, of rows at base + off and base + off2: neither waits for its own
+// last step, which counts where a wave has its SIMD to itself (dq of 4 x 4,096 tokens, 16/2 heads of 256: 1.03 ms one
+// after the other, 0.99 so; the narrow heads' as long).
+template <int D, int BN, int RD>
+__device__ __forceinline__ void rows_products(f32x16& a, f32x16& b, const f32x16& first, const uint32_t (&base)[4], uint32_t off,
+                                              uint32_t off2, const bf16x8 (&opnd)[D / 16], const bf16x8 (&opnd2)[D / 16]) {
+  constexpr int KST = D / 16;
+  u32x4 fr[RD], fr2[RD];
+  auto read = [&](int st) __attribute__((always_inline)) {
+    fr[st % RD] = lds_load<u32x4>(base[st & 3] + off + (st >> 2) * BN * 128);
+    fr2[st % RD] = lds_load<u32x4>(base[st & 3] + off2 + (st >> 2) * BN * 128);
+  };
+#pragma unroll
+  for (int st = 0; st < RD - 1 && st < KST; ++st) read(st);
+#pragma unroll
+  for (int st = 0; st < KST; ++st) {
+    if (st + RD - 1 < KST) read(st + RD - 1);
+    __builtin_amdgcn_sched_barrier(0);
+    a = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, fr[st % RD]), opnd[st], st == 0 ? (f32x16){} : a, 0, 0, 0);
+    b = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, fr2[st % RD]), opnd2[st], st == 0 ? first : b, 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 // acc[d][own] += (32 stream rows, transposed) . x, likewise: base[2 (block of 32 features % 2) + (8 rows of 16)].
 template <int D, int BN, int RD>
 __device__ __forceinline__ void cols_product(f32x16 (&acc)[D / 32], const uint32_t (&base)[4], uint32_t off,
@@ -274,6 +298,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwd
   constexpr int NKB = S::BN / 32 / QS;   // 32-row blocks of a tile for a wave
   static_assert(QS == 1 || NKB == 1, "parts of a tile");
   constexpr int RR = D == 128 && KV ? 3 : 4, RC = 4;   // fragments in flight (eight are no faster)
+  constexpr int RB = 2;                                // of each of two products (three are no faster)
   extern __shared__ __attribute__((aligned(1024))) char smem[];
 
   const int tid = threadIdx.x;
@@ -404,7 +429,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwd
   auto block = [&](int kb, int s0) __attribute__((always_inline)) {
     const uint32_t X = kb * 32 * 128, Y = S::TILE + X;
     f32x16 s, dp;
-    rows_product<D, S::BN, RR>(s, KV ? rows_stat(la + kb * 128) : (f32x16){}, xa, X, own0);
+    if constexpr (KV) rows_product<D, S::BN, RR>(s, rows_stat(la + kb * 128), xa, X, own0);
+    else rows_products<D, S::BN, RB>(s, dp, less, xa, X, Y, own0, own1);
     // masks: stream row s0 + c of register r, c = 8 (r / 4) + 4 hf + r % 4
     const bool whole = (KV || s0 + 31 < T) && (!p.causal || (KV ? s0 >= rlast : s0 + 31 <= r0)) &&
                        (p.window < 0 || (s0 + 31 - r0 <= p.window && rlast - s0 <= p.window));
@@ -435,7 +461,6 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwd
 #pragma unroll
       for (int r = 0; r < 16; ++r) ds[r] = pr[r] * dp[r];
     } else {
-      rows_product<D, S::BN, RR>(dp, less, xa, Y, own1);
       auto mx2 = [](float a, float b) __attribute__((always_inline)) { return __builtin_elementwise_maximum(a, b); };
       float m4[4];
 #pragma unroll

@@ -12,7 +12,8 @@
 // three sums (x^2, (x w)^2, x w . d) gives the gradient.
 //
 // Mean of 26,923 x 768 rows in bf16: 10.8 us (3.9 TB/s; 17.1 with a search for the text in rounds of
-// dependent loads). Last token of 14,716 x 1,024: 9.8 (3.1 TB/s) and 3.9 for the join of dweight.
+// dependent loads). Last token of 14,716 x 1,024: 8.2 (3.7 TB/s; 9.1 with a text's columns loaded in turn) and
+// 3.6 for the join of dweight. 16 rows per workgroup instead of 32: the same; 64: 9.3.
 #include <algorithm>
 
 #include "norm_rope.hpp"
