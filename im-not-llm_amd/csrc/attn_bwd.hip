@@ -28,7 +28,7 @@
 // TFLOP/s of those that they do; 4 x 4,096 causal, 16/2 heads of 256: 0.99 and 1.26 ms, matrix cores 38 and
 // 39 % busy, as one wave or a pair has a SIMD to itself and its exponentials stand between its products. By
 // bytes and the start of workgroups where they are short: 64 x 256 tokens of 16 heads of 64 take 50 and 54 us, for
-// 39 us of bytes each at 4.84 TB/s; 48 texts to 1,021 with a window of 64 and 12 heads 72 and 65 for 53.
+// 42 us of bytes each at 4.84 TB/s; 48 texts to 1,021 with a window of 64 and 12 heads 72 and 65 for 53.
 #include <algorithm>
 #include <new>
 #include <vector>
