@@ -18,6 +18,9 @@ an in-flight register is reported, except as the destination of another
 load: loads write their registers in issue order, so the younger load's
 value is the one that stays (its address operands are still checked).
 Direct-to-LDS loads (``... lds``) write no register and are only counted.
+
+``check_sgpr_waits`` follows the same graph for scalar registers that vector
+instructions write.
 """
 from __future__ import annotations
 
@@ -39,10 +42,11 @@ class Violation:
     line: int          # 1-based line in the listing
     text: str
     registers: list
+    what: str = "names in-flight"
 
     def __str__(self) -> str:
         regs = ", ".join(self.registers)
-        return f"{self.function}: line {self.line}: `{self.text}` names in-flight {regs}"
+        return f"{self.function}: line {self.line}: `{self.text}` {self.what} {regs}"
 
 
 def _regs(operands: str) -> set:
@@ -78,19 +82,21 @@ class _Inst:
 
 
 def _functions(text: str):
-    """{name: [label or _Inst, ...]} for every function body in the listing."""
+    """{name: [label or _Inst, ...]} for every function body in the listing: from a global label to the
+    function's end or the next global label."""
     funcs, cur, name, in_asm = {}, None, None, False
     for no, raw in enumerate(text.splitlines(), 1):
         line = raw.rstrip()
         s = line.strip()
+        m = _LABEL.match(line)
+        if m and not m.group(1).startswith("."):
+            name, cur, in_asm = m.group(1), [], False
+            funcs[name] = cur
+            continue
         if cur is None:
-            m = _LABEL.match(line)
-            if m and not line.startswith((" ", "\t")) and not m.group(1).startswith(".L"):
-                name, cur = m.group(1), []
             continue
         if s.startswith(".Lfunc_end"):
-            funcs[name] = cur
-            cur, name, in_asm = None, None, False
+            cur = None
             continue
         if s.startswith(";;#ASMSTART"):
             in_asm = True
@@ -193,14 +199,16 @@ def _merge(a, b):
     return out
 
 
-def check_function(name, items):
+def check_function(name, items, transfer=_transfer):
+    """What `transfer` reports of the function's blocks, each from the least states that reach it along any
+    path, branches taken and not, loops included."""
     blocks, index = _blocks(items)
     entry = [None] * len(blocks)
     entry[0] = {}
     work = [0]
     while work:
         i = work.pop()
-        out = _transfer(blocks[i][1], entry[i], name, None)
+        out = transfer(blocks[i][1], entry[i], name, None)
         for s in blocks[i][2]:
             j = index[s]
             new = out if entry[j] is None else _merge(entry[j], out)
@@ -210,7 +218,7 @@ def check_function(name, items):
     report = []
     for i, b in enumerate(blocks):
         if entry[i] is not None:
-            _transfer(b[1], entry[i], name, report)
+            transfer(b[1], entry[i], name, report)
     return report
 
 
@@ -235,56 +243,63 @@ def count_asm_loads(text: str) -> int:
     return n
 
 
-if __name__ == "__main__":
-    import sys
-    for path in sys.argv[1:]:
-        txt = open(path).read()
-        v = check_listing(txt)
-        print(f"{path}: {count_asm_loads(txt)} register-writing asm loads, {len(v)} violations")
-        for x in v[:20]:
-            print("  ", x)
-
-
-# A vector instruction that wrote a scalar register (v_readfirstlane, v_readlane, a compare) needs five wait
-# states before a vector-memory instruction reads that register: with fewer the load takes the old value, and its
-# address from it. The compiler makes these waits for its own instructions and not for inline asm.
-_SGPR = re.compile(r"\bs\[(\d+):(\d+)\]|\bs(\d+)\b")
+# A vector instruction that wrote a scalar register (v_readfirstlane, v_readlane, a compare, a carry) needs
+# five wait states before a vector-memory instruction reads that register: with fewer the load takes the old
+# value, and its address from it. The compiler makes these waits for its own instructions and not for inline
+# asm. A state is an instruction of the path that ran, or one of the s_nop's: a taken branch skips those
+# between, and a loop's last instructions stand right before its first, so the states are carried along the
+# control flow like the loads in flight.
+_SGPR = re.compile(r"\bs\[(\d+):(\d+)\]|\bs(\d+)\b|\b(vcc|m0)\b")
 _SGPR_STATES = 5
+_SGPR_SECOND = re.compile(r"^v_(add|addc|sub|subb|subrev|subbrev)_co_|^v_div_scale_|^v_mad_[ui]64_[ui]32")
+# scalar instructions whose first operand is read, or is no register
+_SALU_READS = re.compile(r"^s_(cmp|cmpk|bitcmp|cbranch|branch|waitcnt|nop|barrier|set|sleep|sendmsg|endpgm)")
 
 
 def _sgprs(operands: str) -> set:
     out = set()
-    for lo, hi, one in _SGPR.findall(operands):
-        out.update(range(int(lo), int(hi) + 1) if lo else (int(one),))
+    for lo, hi, one, name in _SGPR.findall(operands):
+        out.update(f"s{i}" for i in (range(int(lo), int(hi) + 1) if lo else (one,) if one else ()))
+        if name:
+            out.add(name)
     return out
+
+
+def _transfer_sgpr(insts, state, function, report):
+    """Like _transfer, over {scalar register: wait states since a vector instruction wrote it}."""
+    st = dict(state)
+    for inst in insts:
+        ops = [o.strip() for o in inst.operands.split(",")]
+        if _VMEM.match(inst.mnemonic):
+            read = _sgprs(inst.operands)
+            if re.search(r"\blds\b", inst.operands):
+                read.add("m0")   # the LDS address
+            late = sorted(read & st.keys())
+            if late and report is not None:
+                report.append(Violation(function, inst.line, inst.text, late,
+                                        "has too few wait states behind the write of"))
+        states = int(ops[0], 0) + 1 if inst.mnemonic == "s_nop" else 1
+        st = {r: c + states for r, c in st.items() if c + states < _SGPR_STATES}
+        if inst.mnemonic.startswith("v_"):
+            written = _sgprs(ops[0]) | (_sgprs(ops[1]) if _SGPR_SECOND.match(inst.mnemonic) else set())
+            st.update(dict.fromkeys(written, 0))
+        elif inst.mnemonic.startswith("s_") and not _SALU_READS.match(inst.mnemonic):
+            for r in _sgprs(ops[0]):
+                st.pop(r, None)
+    return st
 
 
 def check_sgpr_waits(listing: str) -> list[Violation]:
     """Vector-memory instructions that read a scalar register fewer than five wait states after a vector
-    instruction wrote it, along the listing (a branch only adds states)."""
-    found, function, wrote, state = [], "", {}, 0
-    for number, raw in enumerate(listing.splitlines(), 1):
-        label = _LABEL.match(raw)
-        if label and not label.group(1).startswith("."):
-            function, wrote = label.group(1), {}
-            continue
-        text = raw.split(";")[0].strip()
-        if not text or text.startswith(".") or text.endswith(":"):
-            continue
-        mnemonic, _, operands = text.partition(" ")
-        if mnemonic == "s_nop":
-            state += int(operands.strip(), 0) + 1
-            continue
-        state += 1
-        first = operands.split(",")[0]
-        if _VMEM.match(mnemonic):
-            late = [r for r in _sgprs(operands) if r in wrote and state - wrote[r] - 1 < _SGPR_STATES]
-            if late:
-                found.append(Violation(function, number, text, [f"s{r} (too few waits)" for r in sorted(late)]))
-        elif mnemonic.startswith("v_"):
-            for r in _sgprs(first) if mnemonic.startswith(("v_readfirstlane", "v_readlane", "v_cmp")) else ():
-                wrote[r] = state
-        elif mnemonic.startswith("s_"):
-            for r in _sgprs(first):
-                wrote.pop(r, None)
-    return found
+    instruction wrote it, on any path of their function."""
+    return [v for name, items in _functions(listing).items() for v in check_function(name, items, _transfer_sgpr)]
+
+
+if __name__ == "__main__":
+    import sys
+    for path in sys.argv[1:]:
+        txt = open(path).read()
+        v = check_listing(txt) + check_sgpr_waits(txt)
+        print(f"{path}: {count_asm_loads(txt)} register-writing asm loads, {len(v)} violations")
+        for x in v[:20]:
+            print("  ", x)
