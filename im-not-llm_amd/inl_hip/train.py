@@ -496,8 +496,8 @@ def _attn_grads(dev, q, dout, k, v, out, cu_seqlens, causal, window, scale, seq_
             dk, dv = made((nk, hkv, hd), dtype=dt, device=q.device), made((nk, hkv, hd), dtype=dt, device=q.device)
         g = AttnGrads(dos, 0, 0, 0, _dtype_code(dt))
     else:
-        dq, dk, dv = grads
-        dt = next((t.dtype for t in grads if t is not None), _BF16)
+        dq, dk, dv = grads if kv_grad else (grads[0], None, None)
+        dt = next((t.dtype for t in (dq, dk, dv) if t is not None), _BF16)
         if grad_dtype is not None and grad_dtype is not dt:
             raise InlError(-1, f"grads: dtype {dt}, grad_dtype {grad_dtype}")
         strides = [0 if t is None else _head_tensor(name, t, rows, heads, hd, dt, dev)
@@ -517,9 +517,10 @@ def varlen_attention_bwd(dout, q, k, v, out, cu_seqlens, *, causal, window=-1, s
     forward's bf16 ``out`` (``inl_attn_varlen_bwd``); the other arguments as in the
     forward. The probabilities are recomputed. dq, dk and dv are bf16 unless
     ``grad_dtype`` says float32 (P and dS are rounded to bf16 in between all the same);
-    ``kv_grad=False`` leaves dk and dv out (None). ``grads=(dq, dk, dv)`` are tensors to
-    write, slices of one ``[N, Hq + 2 Hkv, D]`` row among them, None where not wanted; their
-    rows outside every text are left as they were, and zero in tensors made here."""
+    ``kv_grad=False`` leaves dk and dv out (None), those of ``grads`` as they were.
+    ``grads=(dq, dk, dv)`` are tensors to write, slices of one ``[N, Hq + 2 Hkv, D]`` row
+    among them, None where not wanted; their rows outside every text are left as they
+    were, and zero in tensors made here."""
     return _attn_grads(q, dout, k, v, out, cu_seqlens, causal, window, scale, seq_starts, grad_dtype, grads, kv_grad,
                        stream)
 

@@ -1,0 +1,41 @@
+"""What varlen_attention_bwd hands to the library, and what it refuses itself: its checks run here on tensors of the
+host, with the library's call recorded instead of made."""
+import pytest
+import torch
+
+
+@pytest.fixture
+def call(monkeypatch):
+    from inl_hip import train
+    made = []
+    monkeypatch.setattr(train, "_attn_bwd", lambda *a: made.append(a) or 0)
+    monkeypatch.setattr(train, "_stream", lambda dev: None)
+    monkeypatch.setattr(train, "_room", lambda n, dev: None)
+
+    def run(grads=None, kv_grad=True, window=-1, grad_dtype=None):
+        x = [torch.zeros(9, h, 64, dtype=torch.bfloat16) for h in (4, 2, 2, 4, 4)]
+        q, k, v, out, dout = x
+        del made[:]
+        got = train._attn_grads.__wrapped__(-1, q, dout, k, v, out, [0, 4, 9], False, window, None, None, grad_dtype, grads,
+                                            kv_grad)
+        return got, made[0]
+    return run
+
+
+def _grads(dtype=torch.bfloat16):
+    return tuple(torch.zeros(9, h, 64, dtype=dtype) for h in (4, 2, 2))
+
+
+def test_kv_grad_leaves_given_tensors_alone(call):
+    """Without kv_grad the dk and dv of `grads` are neither written nor returned."""
+    g = _grads()
+    got, args = call(grads=g, kv_grad=False)
+    assert got[0] is g[0] and got[1] is None and got[2] is None
+    assert args[7:10] == (g[0].data_ptr(), None, None)
+    got, args = call(grads=g)
+    assert all(a is b for a, b in zip(got, g)) and args[7:10] == tuple(t.data_ptr() for t in g)
+    # nor does their type count
+    got, args = call(grads=(g[0],) + _grads(torch.float32)[1:], kv_grad=False, grad_dtype=torch.bfloat16)
+    assert got[1] is None and args[1].grad_dtype == 1
+    got, args = call(kv_grad=False)
+    assert got[0].shape == (9, 4, 64) and got[1] is None and args[8:10] == (None, None)
