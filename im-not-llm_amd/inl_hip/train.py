@@ -474,13 +474,16 @@ def _attn_grads(dev, q, dout, k, v, out, cu_seqlens, causal, window, scale, seq_
     n, hq, hd = q.shape
     nk, hkv, _ = k.shape
     texts = len(cu_seqlens) - 1
+    window = -1 if window is None else int(window)
+    if not -1 <= window < 2 ** 31:   # (its low 32 bits would be another window)
+        raise InlError(-1, f"window {window} must be -1 or in [0, 2^31)")
     if seq_starts is None:
         cu, starts = _cu_array(cu_seqlens), None
         rows = cu[texts] if texts > 0 else 0
     else:
         d = make_attn_desc(cu_seqlens, hq, hkv, hd, causal=causal, seq_starts=seq_starts)   # checks the lengths
         cu, starts, rows = d._cu_keepalive, d._starts_keepalive, desc_rows(d)
-    d = AttnDesc(texts, cu, hq, hkv, hd, bool(causal), -1 if window is None else int(window),
+    d = AttnDesc(texts, cu, hq, hkv, hd, bool(causal), window,
                  hd ** -0.5 if scale is None else scale, INL_BF16, INL_BF16,
                  _head_tensor("q", q, rows, hq, hd, _BF16, dev), _head_tensor("k", k, rows, hkv, hd, _BF16, dev),
                  _head_tensor("v", v, rows, hkv, hd, _BF16, dev), _head_tensor("out", out, rows, hq, hd, _BF16, dev), 0,

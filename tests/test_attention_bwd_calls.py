@@ -39,3 +39,16 @@ def test_kv_grad_leaves_given_tensors_alone(call):
     assert got[1] is None and args[1].grad_dtype == 1
     got, args = call(kv_grad=False)
     assert got[0].shape == (9, 4, 64) and got[1] is None and args[8:10] == (None, None)
+
+
+@pytest.mark.parametrize("window", [2 ** 31, 2 ** 32, 2 ** 32 + 3, -2, -2 ** 32 - 1])
+def test_windows_beyond_32_bits_are_refused(window, call):
+    """They would reach the library as their low 32 bits: 2^32 as a window of 0."""
+    import inl_hip
+    with pytest.raises(inl_hip.InlError, match="window"):
+        call(window=window)
+
+
+def test_windows(call):
+    for window, want in ((None, -1), (-1, -1), (0, 0), (2 ** 31 - 1, 2 ** 31 - 1)):
+        assert call(window=window)[1][0].window == want
