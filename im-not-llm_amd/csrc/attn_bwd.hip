@@ -838,20 +838,21 @@ namespace {
 typedef void (*AttnBwdFn)(AttnBwdParams);
 
 struct BwdLaunch {
+  const char* name;
   AttnBwdFn fn;
   int own;       // own rows of a workgroup
   int threads, lds;
 };
 
 template <int D, bool KV, int QS>
-BwdLaunch bwd_plain(bool out16) {
+BwdLaunch bwd_plain(const char* name, bool out16) {
   using S = BwdShape<D, KV, QS>;
-  return {out16 ? attn_bwd_kernel<D, KV, QS, true> : attn_bwd_kernel<D, KV, QS, false>, S::OWN, 256, S::LDS};
+  return {name, out16 ? attn_bwd_kernel<D, KV, QS, true> : attn_bwd_kernel<D, KV, QS, false>, S::OWN, 256, S::LDS};
 }
 template <int D>
-BwdLaunch bwd_pair(bool out16) {
+BwdLaunch bwd_pair(const char* name, bool out16) {
   using S = PairShape<D>;
-  return {out16 ? attn_bwd_pair_kernel<D, true> : attn_bwd_pair_kernel<D, false>, 32 * S::KG, 512, S::LDS};
+  return {name, out16 ? attn_bwd_pair_kernel<D, true> : attn_bwd_pair_kernel<D, false>, 32 * S::KG, 512, S::LDS};
 }
 
 // How many times the average load of a place for a workgroup (`places` per CU) the longest workgroup's stream
@@ -877,14 +878,16 @@ double bwd_longest(const inl_attn_desc& d, const std::vector<BwdText>& texts, bo
 //           causal, whose blocks are of unequal length: 8 x 2,048 (0.94) 370 / 313, 64 x 180 (0.7) 64 / 56
 BwdLaunch bwd_launch(const inl_attn_desc& d, const std::vector<BwdText>& texts, bool kv, int cus, bool out16) {
   const int dim = d.head_dim <= 64 ? 64 : d.head_dim <= 128 ? 128 : 256;
-  if (kv && dim == 256) return bwd_pair<256>(out16);
+#define INL_BWD(D, KV, QS) bwd_plain<D, KV, QS>("attn_bwd_kernel<" #D ", " #KV ", " #QS ">", out16)
+  if (kv && dim == 256) return bwd_pair<256>("attn_bwd_pair_kernel<256>", out16);
   const double over = bwd_longest(d, texts, kv, cus, dim == 64 ? 3 : dim == 128 ? 2 : 1);
   const bool two = !kv ? over > 2.5 : dim == 64 ? over > 2 : (d.causal && over > 0) || over > 1.2;
-  if (dim == 64) return kv ? (two ? bwd_plain<64, true, 2>(out16) : bwd_plain<64, true, 1>(out16))
-                           : (two ? bwd_plain<64, false, 2>(out16) : bwd_plain<64, false, 1>(out16));
-  if (dim == 128) return kv ? (two ? bwd_plain<128, true, 2>(out16) : bwd_plain<128, true, 1>(out16))
-                            : (two ? bwd_plain<128, false, 2>(out16) : bwd_plain<128, false, 1>(out16));
-  return two ? bwd_plain<256, false, 2>(out16) : bwd_plain<256, false, 1>(out16);
+  if (dim == 64) return kv ? (two ? INL_BWD(64, true, 2) : INL_BWD(64, true, 1))
+                           : (two ? INL_BWD(64, false, 2) : INL_BWD(64, false, 1));
+  if (dim == 128) return kv ? (two ? INL_BWD(128, true, 2) : INL_BWD(128, true, 1))
+                            : (two ? INL_BWD(128, false, 2) : INL_BWD(128, false, 1));
+  return two ? INL_BWD(256, false, 2) : INL_BWD(256, false, 1);
+#undef INL_BWD
 }
 
 // Which texts a workgroup finds its unit among, longest first within a class, so that the last workgroups
@@ -1078,6 +1081,28 @@ extern "C" int inl_attn_bwd_workspace_size(const inl_attn_desc* d, size_t* bytes
     int rc = bwd_texts(d, &rows, &texts);
     if (rc) return rc;
     *bytes = bwd_bytes(*d, rows, texts.size());
+    return INL_OK;
+  } catch (const std::bad_alloc&) {
+    return fail(INL_E_NOMEM, "attention backward: out of host memory");
+  }
+}
+
+extern "C" int inl_attn_bwd_kernel_name(const inl_attn_desc* d, int32_t kv, const char** name) {
+  using namespace inl;
+  if (!name) return fail(INL_E_INVALID, "attention backward: name out-pointer is NULL");
+  *name = nullptr;
+  if (kv != 0 && kv != 1) return fail(INL_E_INVALID, "attention backward: kv must be 0 (dq) or 1 (dk, dv)");
+  try {
+    int64_t rows = 0;
+    std::vector<BwdText> texts;
+    int rc = bwd_texts(d, &rows, &texts);
+    if (rc) return rc;
+    int cus = 0;
+    if (device_cus(&cus)) {   // (no device: as an MI355X has them)
+      (void)hipGetLastError();
+      cus = 256;
+    }
+    *name = texts.empty() ? "none" : bwd_launch(*d, texts, kv != 0, cus, true).name;
     return INL_OK;
   } catch (const std::bad_alloc&) {
     return fail(INL_E_NOMEM, "attention backward: out of host memory");

@@ -1192,6 +1192,6 @@ def unit_lower_inverse(a, *, stream=None):
 # ---------------------------------------------------------------------------
 
 if "torch" in globals():   # the rest of the package does without it
-    from .train import (ROPE_AXIAL, ROPE_HALF, ROPE_INTERLEAVED, add_rms_norm, add_rms_norm_bwd, dense,  # noqa: E402,F401
-                        dense_bwd, gated_ffn, gated_ffn_bwd, norm_rope_qk_bwd, pool_last_bwd, pool_mean_bwd,
-                        softmax_xent, softmax_xent_bwd, varlen_attention_bwd)
+    from .train import (ROPE_AXIAL, ROPE_HALF, ROPE_INTERLEAVED, add_rms_norm, add_rms_norm_bwd,  # noqa: E402,F401
+                        attention_bwd_kernel_names, dense, dense_bwd, gated_ffn, gated_ffn_bwd, norm_rope_qk_bwd,
+                        pool_last_bwd, pool_mean_bwd, softmax_xent, softmax_xent_bwd, varlen_attention_bwd)

@@ -77,6 +77,8 @@ _rope_bwd = _sig("inl_norm_rope_qk_bwd", ctypes.c_int, ctypes.POINTER(NormRopeDe
 
 
 _attn_bwd_ws = _sig("inl_attn_bwd_workspace_size", ctypes.c_int, ctypes.POINTER(AttnDesc), _size_p)
+_attn_bwd_name = _sig("inl_attn_bwd_kernel_name", ctypes.c_int, ctypes.POINTER(AttnDesc), c_i32,
+                      ctypes.POINTER(ctypes.c_char_p))
 _attn_bwd = _sig("inl_attn_varlen_bwd", ctypes.c_int, ctypes.POINTER(AttnDesc), ctypes.POINTER(AttnGrads), *_ptrs(9),
                  ctypes.c_size_t, c_void_p)
 _add_norm = _sig("inl_add_rms_norm_fwd", ctypes.c_int, ctypes.POINTER(AddNormDesc), *_ptrs(7))
@@ -526,6 +528,17 @@ def varlen_attention_bwd(dout, q, k, v, out, cu_seqlens, *, causal, window=-1, s
     were, and zero in tensors made here."""
     return _attn_grads(q, dout, k, v, out, cu_seqlens, causal, window, scale, seq_starts, grad_dtype, grads, kv_grad,
                        stream)
+
+
+def attention_bwd_kernel_names(desc):
+    """The kernels that ``varlen_attention_bwd`` launches for ``desc`` (``make_attn_desc``): the one that
+    makes dq, and the one that makes dk and dv (``inl_attn_bwd_kernel_name``)."""
+    names = []
+    for kv in (0, 1):
+        name = ctypes.c_char_p()
+        _check(_attn_bwd_name(desc, kv, ctypes.byref(name)))
+        names.append(name.value.decode())
+    return tuple(names)
 
 
 # ---------------------------------------------------------------------------

@@ -211,6 +211,10 @@ typedef struct inl_attn_grads {
 } inl_attn_grads;
 
 int inl_attn_bwd_workspace_size(const inl_attn_desc* desc, size_t* bytes);
+/* Host only: the name of the kernel that makes dq (kv 0) or dk and dv (kv 1) of `desc` (a static string, e.g.
+ * "attn_bwd_kernel<128, false, 1>": feature width, keys, parts that its waves are divided into; "none" where no
+ * text has a token), for reporting and tests. */
+int inl_attn_bwd_kernel_name(const inl_attn_desc* desc, int32_t kv, const char** name);
 int inl_attn_varlen_bwd(const inl_attn_desc* desc, const inl_attn_grads* grads, const void* q, const void* k,
                         const void* v, const void* out, const void* dout, void* dq, void* dk, void* dv,
                         void* workspace, size_t workspace_bytes, void* stream);

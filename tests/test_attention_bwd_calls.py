@@ -52,3 +52,27 @@ def test_windows_beyond_32_bits_are_refused(window, call):
 def test_windows(call):
     for window, want in ((None, -1), (-1, -1), (0, 0), (2 ** 31 - 1, 2 ** 31 - 1)):
         assert call(window=window)[1][0].window == want
+
+
+def test_kernel_names():
+    """By the batch's fill of a GPU of 256 compute units, each by the widest of its features."""
+    import ctypes
+
+    import inl_hip
+    from inl_hip import train
+
+    def names(lengths, hq, hkv, hd, causal=False, window=-1):
+        cu = [sum(lengths[:i]) for i in range(len(lengths) + 1)]
+        return inl_hip.attention_bwd_kernel_names(inl_hip.make_attn_desc(cu, hq, hkv, hd, causal=causal, window=window))
+    assert names([257] * 64, 16, 16, 40) == ("attn_bwd_kernel<64, false, 1>", "attn_bwd_kernel<64, true, 1>")
+    assert names([900], 16, 16, 64) == ("attn_bwd_kernel<64, false, 2>", "attn_bwd_kernel<64, true, 2>")
+    assert names([257] * 64, 16, 8, 72, True) == ("attn_bwd_kernel<128, false, 1>", "attn_bwd_kernel<128, true, 2>")
+    assert names([300] * 32, 3, 1, 256, True) == ("attn_bwd_kernel<256, false, 1>", "attn_bwd_pair_kernel<256>")
+    assert names([23], 16, 8, 128, True) == ("attn_bwd_kernel<128, false, 1>", "attn_bwd_kernel<128, true, 1>")
+    assert names([0, 0], 2, 2, 64) == ("none", "none")
+    d = inl_hip.make_attn_desc([0, 5], 2, 2, 64, causal=False)
+    name = ctypes.c_char_p()
+    assert train._attn_bwd_name(d, 2, ctypes.byref(name)) == -1 and train._attn_bwd_name(d, 0, None) == -1
+    assert train._attn_bwd_name(None, 0, ctypes.byref(name)) == -1 and name.value is None
+    with pytest.raises(inl_hip.InlError, match="bf16"):
+        inl_hip.attention_bwd_kernel_names(inl_hip.make_attn_desc([0, 5], 2, 2, 64, causal=False, dtype="f32"))
