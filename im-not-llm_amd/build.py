@@ -7,6 +7,7 @@ the source tree; it is listed in .gitignore.
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -65,6 +66,9 @@ RESOURCE_REMARKS = ["-Rpass-analysis=kernel-resource-usage", "-fno-caret-diagnos
 # have register-writing asm loads; the check must find some there, so that a
 # listing format the parser no longer reads cannot pass silently.
 ASM_REGISTER_LOADS = {"attn_pp.hip", "attn_pp64.hip", "attn_wide.hip"}
+
+# Kernels that count on their dynamic LDS beginning at address 0, which static LDS would go before.
+NO_STATIC_LDS = {"attn_bwd.hip": "attn_bwd_pair_kernel"}
 
 
 def scratch_users(remarks: str) -> list[str]:
@@ -130,6 +134,20 @@ def check_inflight(src_name: str, listing: str) -> None:
                            f"vector instruction wrote them:\n{shown}")
 
 
+def check_no_static_lds(src_name: str, listing: str) -> None:
+    """Raise unless the listing of a source in NO_STATIC_LDS has its kernels, none of them with static LDS."""
+    kernel = NO_STATIC_LDS.get(src_name)
+    if kernel is None:
+        return
+    sizes = [(name, int(size)) for name, size in
+             re.findall(r"\.amdhsa_kernel (\S+)\n\s*\.amdhsa_group_segment_fixed_size (\d+)", listing) if kernel in name]
+    if not sizes:
+        raise RuntimeError(f"{src_name}: no static LDS size of {kernel} found in its listing")
+    users = [f"{name} ({size} bytes)" for name, size in sizes if size]
+    if users:
+        raise RuntimeError(f"{src_name}: kernels whose LDS addresses begin at 0 have static LDS: " + ", ".join(users))
+
+
 def sources():
     return sorted(CSRC.glob("*.hip"))
 
@@ -171,6 +189,7 @@ def build(verbose: bool = False) -> Path:
             if rc != 0:
                 raise RuntimeError(f"hipcc -S failed on {src.name} ({rc}):\n{err}")
             check_inflight(src.name, lst.read_text())
+            check_no_static_lds(src.name, lst.read_text())
         rc, err = _run([HIPCC, *LINK_FLAGS, *(str(o) for _, o, _ in jobs), "-o", str(tmp)])
         if rc != 0:
             raise RuntimeError(f"hipcc link failed ({rc}):\n{err}")

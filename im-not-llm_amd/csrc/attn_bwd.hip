@@ -617,6 +617,7 @@ struct PairShape {
   static constexpr int STATS = SWAP + 4 * 4096;
   static constexpr int STAT = 2 * BN * 4;
   static constexpr int LDS = STATS + 2 * STAT;
+  static_assert((STAGE & (STAGE - 1)) == 0, "stages differ in one bit of an address");
 };
 
 template <int D, bool OUT16>
@@ -782,6 +783,8 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_pair_kernel(AttnBwdParams p) 
       th = 0;
       --t;
     }
+    // to the other stage: a stage is a power of two and the first one begins at LDS address 0 (the build refuses
+    // static LDS in this kernel, which would go before it)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       xa[e] ^= S::STAGE;

@@ -79,3 +79,17 @@ def test_sources_with_asm_loads_are_checked():
     found = {s.name for s in (PKG / "csrc").glob("*.hip")
              if issues.search(s.read_text()) or any(re.search(rf"\b{c}\(", s.read_text()) for c in calls)}
     assert "attn_bwd.hip" in found and found <= held, found - held
+
+
+def test_static_lds_is_found():
+    """The kernel of wide heads' dk and dv tells its two stages apart by one bit of an LDS address."""
+    build = _module("build")
+    text = lambda size, name="attn_bwd_pair_kernel": (f"\t.amdhsa_kernel _Z20{name}ILi256ELb1EEvv\n"
+                                                      f"\t\t.amdhsa_group_segment_fixed_size {size}\n")
+    build.check_no_static_lds("attn_bwd.hip", text(0) + text(16, "another_kernel"))
+    with pytest.raises(RuntimeError, match="static LDS: .*pair_kernel.* .16 bytes"):
+        build.check_no_static_lds("attn_bwd.hip", text(0) + text(16))
+    with pytest.raises(RuntimeError, match="no static LDS size"):
+        build.check_no_static_lds("attn_bwd.hip", text(0, "another_kernel"))
+    build.check_no_static_lds("attn_pp.hip", "")
+    assert set(build.NO_STATIC_LDS) <= build.NO_SCRATCH
