@@ -353,7 +353,7 @@ int check_rows(const char* what, const void* p, int64_t cols, int64_t stride, in
 }
 
 bool rows_meet(const Rows& a, const Rows& b) {
-  if (!a.at || !b.at || a.rows <= 0 || b.rows <= 0) return false;
+  if (!a.at || !b.at || a.rows <= 0 || b.rows <= 0 || a.len <= 0 || b.len <= 0) return false;   // no byte
   const int64_t d = (int64_t)((uintptr_t)b.at - (uintptr_t)a.at);   // b's start from a's
   if (d >= (a.rows - 1) * a.step + a.len || -d >= (b.rows - 1) * b.step + b.len) return false;
   auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };

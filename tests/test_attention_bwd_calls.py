@@ -76,3 +76,26 @@ def test_kernel_names():
     assert train._attn_bwd_name(None, 0, ctypes.byref(name)) == -1 and name.value is None
     with pytest.raises(inl_hip.InlError, match="bf16"):
         inl_hip.attention_bwd_kernel_names(inl_hip.make_attn_desc([0, 5], 2, 2, 64, causal=False, dtype="f32"))
+
+
+_EMPTY = """
+import sys
+sys.path[:0] = {path!r}
+import inl_hip
+from inl_hip import train as T
+MB = 1 << 20
+# no texts: dpooled and mean are empty, wherever they point; cu lies in dhidden and is what is refused
+a = T._pool_mean_bwd(0, MB + 64, 8, 100, 8, 1, MB + 32, MB + 48, MB, None)
+assert a == -1 and "overlaps" in inl_hip.last_error(), (a, inl_hip.last_error())
+b = T._pool_last_bwd(0, MB + 64, 8, 100, 8, 1, MB + 32, 2 * MB, None, 1e-6, 8, 1, MB, None, None, 0, None)
+assert b == -1 and "overlaps" in inl_hip.last_error(), (b, inl_hip.last_error())
+"""
+
+
+def test_empty_tensors_inside_an_output():
+    """An empty dpooled whose address lies in dhidden shares no byte with it (in a process of its own: the check of the
+    overlap divided by its length)."""
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-c", _EMPTY.format(path=sys.path)], capture_output=True, text=True)
+    assert r.returncode == 0, (r.returncode, r.stderr[-800:])
