@@ -997,7 +997,7 @@ int bwd_run(const inl_attn_desc* d, const inl_attn_grads* g, const void* q, cons
     if ((!t[i].at && i < 5 && rows) || ((uintptr_t)t[i].at & 15))
       return fail(INL_E_INVALID, std::string("attention backward: ") + t[i].what + " must be non-null and 16-byte aligned");
     // rows of a text, and those of its last tile behind it, are addressed with 32 bits
-    if ((longest + 128) * t[i].stride * es >= (int64_t)BWD_NOWHERE)
+    if (t[i].stride >= (int64_t)BWD_NOWHERE || (longest + 128) * t[i].stride * es >= (int64_t)BWD_NOWHERE)
       return fail(INL_E_UNSUPPORTED, std::string("attention backward: a text's rows of ") + t[i].what + " span 4 GiB or more");
     r[i] = {t[i].at, rows, len * es, t[i].stride * es};
   }

@@ -99,3 +99,19 @@ def test_empty_tensors_inside_an_output():
     import sys
     r = subprocess.run([sys.executable, "-c", _EMPTY.format(path=sys.path)], capture_output=True, text=True)
     assert r.returncode == 0, (r.returncode, r.stderr[-800:])
+
+
+@pytest.mark.parametrize("stride", [1 << 24, 1 << 31, 1 << 40, 1 << 60, 1 << 61, 1 << 62])
+def test_rows_that_lie_far_apart_are_refused(stride):
+    """A text's rows are addressed with 32 bits: no stride passes as its low bits."""
+    import inl_hip
+    from inl_hip import train as T
+    far = [(i + 1) << 44 for i in range(8)]
+    for name in ("q", "k", "v", "o"):
+        d = inl_hip.make_attn_desc([0, 1], 2, 2, 64, causal=True, **{f"{name}_row_stride": stride})
+        assert T._attn_bwd(d, T.AttnGrads(grad_dtype=1), *far, None, 0, None) == -2, name
+        assert "4 GiB" in inl_hip.last_error()
+    d = inl_hip.make_attn_desc([0, 1], 2, 2, 64, causal=True)
+    for name in ("do", "dq", "dk", "dv"):
+        g = T.AttnGrads(**{f"{name}_row_stride": stride, "grad_dtype": 0})
+        assert T._attn_bwd(d, g, *far, None, 0, None) == -2 and "4 GiB" in inl_hip.last_error(), name
