@@ -4,8 +4,8 @@ cross entropy without its scores, the residual stream's addition with dropout an
 norm, and the gradients of the q/k prologue, of attention and of the pooled embedding.
 
 Gradients are plain functions of what the forward left (outputs carry no autograd
-graph, whatever ``requires_grad`` says of the inputs): a ``torch.autograd.Function`` or a training loop calls them in its own
-backward. Outputs and workspaces come from torch's allocator, so calls can be
+graph, whatever ``requires_grad`` says of the inputs): a ``torch.autograd.Function`` or
+a training loop calls them in its own backward. Outputs and workspaces come from torch's allocator, so calls can be
 captured into a graph. With ``stream=`` a call works there and takes its memory there;
 that its inputs are ready on that stream, and that their memory is not handed on
 before it is done (``record_stream``), is up to the caller, as it is that the current
@@ -18,8 +18,8 @@ import functools
 
 import torch
 
-from . import (INL_BF16, INL_F32, AttnDesc, InlError, NormRopeDesc, _check, _cu_array, _dtype_code, _head_rows, _head_weight,
-               _rope_tables, _sig, c_i32, c_i64, c_void_p, desc_rows, make_attn_desc)
+from . import (INL_BF16, INL_F32, AttnDesc, InlError, NormRopeDesc, _check, _cu_array, _dtype_code, _head_rows,
+               _head_weight, _rope_tables, _sig, c_i32, c_i64, c_void_p, desc_rows, make_attn_desc)
 
 ACTS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu_tanh": 3, "gelu_erf": 4}
 ROPE_HALF, ROPE_AXIAL, ROPE_INTERLEAVED = 1, 2, 3
@@ -552,7 +552,8 @@ def _drop(dropout, rng, dev, draws=True):
     drop = round(dropout * 65536)
     if not drop or not draws:
         return drop, None
-    if rng is None or rng.dtype is not torch.int64 or rng.shape != (2,) or rng.get_device() != dev or rng.stride(0) != 1:
+    if rng is None or rng.dtype is not torch.int64 or rng.shape != (2,) or rng.get_device() != dev \
+            or rng.stride(0) != 1:
         raise InlError(-1, f"rng: dropout needs contiguous torch.int64 [2] on cuda:{dev}"
                            + ("" if rng is None else f", got {rng.dtype} {tuple(rng.shape)} on {rng.device}"))
     return drop, rng.data_ptr()
@@ -607,12 +608,13 @@ def _norm_fwd(dev, x, weight, residual, eps, dropout, rng, tag, out, sum_out, ou
 def add_rms_norm(x, weight=None, *, residual=None, eps=1e-6, dropout=0.0, rng=None, tag=0, out=None, sum_out=None,
                  out_dtype=None, sum_dtype=None, stream=None):
     """``(y, h)`` with ``h = residual + drop(x)`` and ``y = h / sqrt(mean(h^2) + eps) * weight``
-    (``inl_add_rms_norm_fwd``): bf16 or f32 ``x [m, n]`` and ``weight [n]``, ``residual [m, n]`` or None; n a multiple of 8,
-    at most 16384; rows may be strided. h has the residual's dtype (without one ``sum_dtype``, x's by
-    default; without dropout too it is x itself, where ``out`` is not) and may go into
-    ``sum_out``, which may be x or the residual itself; y has x's dtype unless ``out_dtype`` says otherwise. ``dropout``: the probability (in steps of 1 / 65536); its draws come from
-    ``rng``, int64 ``[2]`` on the device (seed, step), and ``tag``, a number of this place
-    in the model; no mask is kept."""
+    (``inl_add_rms_norm_fwd``): bf16 or f32 ``x [m, n]`` and ``weight [n]``, ``residual [m, n]`` or
+    None; n a multiple of 8, at most 16384; rows may be strided. h has the residual's dtype (without
+    one ``sum_dtype``, x's by default; without dropout too it is x itself, where ``out`` is not) and may
+    go into ``sum_out``, which may be x or the residual itself; y has x's dtype unless ``out_dtype`` says
+    otherwise. ``dropout``: the probability (in steps of 1 / 65536); its draws come from ``rng``, int64
+    ``[2]`` on the device (seed, step), and ``tag``, a number of this place in the model; no mask is
+    kept."""
     return _norm_fwd(x, weight, residual, eps, dropout, rng, tag, out, sum_out, out_dtype, sum_dtype, stream)
 
 
@@ -645,11 +647,11 @@ def _norm_grads(dev, h, dy, weight, dh, eps, dropout, rng, tag, x_grad, residual
 
 def add_rms_norm_bwd(dy, h, weight=None, *, dh=None, eps=1e-6, dropout=0.0, rng=None, tag=0, x_grad=True,
                      residual_grad=True, weight_grad=True, dx_dtype=None, stream=None):
-    """``(dx, dresidual, dweight)`` of ``add_rms_norm`` from ``dy [m, n]`` (y's dtype) and the ``h`` that it
-    returned (``inl_add_rms_norm_bwd``); ``dh`` (h's dtype) is the gradient that reaches h past the norm. ``dropout``, ``rng``
-    and ``tag`` as in the forward, with the step it had. dresidual has h's dtype, dx dy's unless ``dx_dtype`` says
-    otherwise (without dropout, and of one dtype, they are one tensor), dweight f32 ``[n]`` (None without a
-    weight); what is not asked for is None."""
+    """``(dx, dresidual, dweight)`` of ``add_rms_norm`` from ``dy [m, n]`` (y's dtype) and the ``h`` that
+    it returned (``inl_add_rms_norm_bwd``); ``dh`` (h's dtype) is the gradient that reaches h past the
+    norm. ``dropout``, ``rng`` and ``tag`` as in the forward, with the step it had. dresidual has h's
+    dtype, dx dy's unless ``dx_dtype`` says otherwise (without dropout, and of one dtype, they are one
+    tensor), dweight f32 ``[n]`` (None without a weight); what is not asked for is None."""
     return _norm_grads(h, dy, weight, dh, eps, dropout, rng, tag, x_grad, residual_grad, weight_grad, dx_dtype, stream)
 
 
@@ -665,9 +667,10 @@ def _pooled(name, t, texts, dim, dev):
 
 
 def _offsets(cu, dev):
-    if len(cu.shape) != 1 or cu.shape[0] < 1 or cu.dtype is not torch.int32 or cu.get_device() != dev or not cu.is_contiguous():
-        raise InlError(-1, f"cu: need contiguous torch.int32 [texts + 1] on cuda:{dev}, got {cu.dtype} {tuple(cu.shape)} "
-                           f"on {cu.device}")
+    if len(cu.shape) != 1 or cu.shape[0] < 1 or cu.dtype is not torch.int32 or cu.get_device() != dev \
+            or not cu.is_contiguous():
+        raise InlError(-1, f"cu: need contiguous torch.int32 [texts + 1] on cuda:{dev}, got {cu.dtype} "
+                           f"{tuple(cu.shape)} on {cu.device}")
     return cu.shape[0] - 1
 
 
@@ -684,7 +687,8 @@ def _mean_grads(dev, dpooled, cu, rows, mean, dtype, out):
     texts, dim = _matrix("dpooled", dpooled)
     if _offsets(cu, dev) != texts:
         raise InlError(-1, f"cu: {cu.shape[0] - 1} texts, dpooled has {texts}")
-    dp, mp = _pooled("dpooled", dpooled, texts, dim, dev), None if mean is None else _pooled("mean", mean, texts, dim, dev)
+    dp = _pooled("dpooled", dpooled, texts, dim, dev)
+    mp = None if mean is None else _pooled("mean", mean, texts, dim, dev)
     out, stride = _grad_rows(out, (int(rows), dim), dtype if out is not None else dtype or _BF16, dpooled, dev)
     _check(_pool_mean_bwd(texts, cu.data_ptr(), dim, int(rows), stride, _CODE[out.dtype], dp, mp, out.data_ptr(),
                           _stream(dev)))
@@ -709,8 +713,8 @@ def _last_grads(dev, dpooled, hidden, cu, weight, eps, dtype, out, weight_grad):
     dw = hidden.new_empty(dim, dtype=_F32) if weight_grad and weight is not None else None
     size = 4 * texts * dim if dw is not None and texts > 1 else 0
     room = _room(size, dev)
-    _check(_pool_last_bwd(texts, cu.data_ptr(), dim, rows, hs, _CODE[hidden.dtype], dp, hidden.data_ptr(), wp, eps, stride,
-                          _CODE[out.dtype], out.data_ptr(), _ptr(dw), _ptr(room), size, _stream(dev)))
+    _check(_pool_last_bwd(texts, cu.data_ptr(), dim, rows, hs, _CODE[hidden.dtype], dp, hidden.data_ptr(), wp, eps,
+                          stride, _CODE[out.dtype], out.data_ptr(), _ptr(dw), _ptr(room), size, _stream(dev)))
     return out, dw
 
 

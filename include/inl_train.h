@@ -1,10 +1,10 @@
 /*
  * inl_train.h - C ABI of the layer and head ops with their gradients, and of the
- * gradients of attention and pooling, on one MI355X (gfx950): what fine-tuning the encoders of inl_encoder.h needs beside
- * its forward. Conventions are those of inl_hip.h: device pointers, int status
- * + inl_last_error(), work on the caller's stream, the caller owns every
- * buffer. Nothing is allocated and nothing synchronised, so every call can be
- * captured into a graph.
+ * gradients of attention and pooling, on one MI355X (gfx950): what fine-tuning
+ * the encoders of inl_encoder.h needs beside its forward. Conventions are those
+ * of inl_hip.h: device pointers, int status + inl_last_error(), work on the
+ * caller's stream, the caller owns every buffer. Nothing is allocated and nothing
+ * synchronised, so every call can be captured into a graph.
  *
  * Matrices are rows of bf16, or of the dtypes that a section names (strides in
  * elements between rows, 0 = packed), 16-byte aligned, row lengths and strides
