@@ -43,7 +43,7 @@ LINK_FLAGS = [f"--offload-arch={ARCH}", "-shared", "-fPIC", "-L/opt/rocm/lib", "
 # rescales with VALU instructions, is not copied between AGPRs and VGPRs on
 # every tile; the MFMA operands then take the AGPRs. attn_bwd.hip likewise: its S
 # and dP go from the MFMA to the VALU and back (dq of 256 features, 4 x 4,096 tokens:
-# 1.04 ms, 1.17 without).
+# 0.92 ms, 1.05 without; narrower heads take as long either way).
 EXTRA = {
     "attn_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "attn_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],

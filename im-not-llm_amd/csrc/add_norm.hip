@@ -17,7 +17,12 @@
 // would take longer than the memory does.
 //
 // 20,011 x 768, f32 stream, dropout 0.1: forward 36.5 us a call (5.0 TB/s), backward 51 and 5 for
-// the join of dweight (4.8 TB/s without it); 65,536 x 1,024 in bf16, backward 106 us in all (5.0 TB/s). One row: 2.5.
+// the join of dweight (4.8 TB/s without it); 65,536 x 1,024 in bf16, backward 107 us in all (5.0 TB/s). One row: 2.5.
+// Wide rows, 2^26 values, bf16 x and y, dropout, kernel alone, TB/s of forward and backward in a bf16 / f32
+// stream: 2,048 columns 5.6 and 4.4 / 5.5 and 5.1, 4,096 5.8 and 5.0 / 5.7 and 5.4, 8,192 5.5 and 4.6 / 5.5 and 5.1,
+// 16,384 5.1 and 4.2 / 5.2 and 4.0: a row of more than 8,192 fills up to 336 registers of a lane in the backward, so
+// one wave is on a SIMD in an f32 stream, and two in a bf16 one. The join of dweight takes 5 us to 4,096 columns, 7
+// to 9 at 8,192, 14 to 15 at 16,384.
 #include <algorithm>
 
 #include "norm_rope.hpp"

@@ -24,11 +24,17 @@
 // and Y are stored once, row-major, and read both ways (ds_read_b128 for the first
 // products, ds_read_b64_tr_b16 for the second); the swizzle serves both.
 //
-// Bound by its products where texts are long: 8 x 2,048 tokens, 16/8 heads of 128, full: dq 990, dk and dv 1,040
-// TFLOP/s of those that they do; 4 x 4,096 causal, 16/2 heads of 256: 0.99 and 1.26 ms, matrix cores 38 and
-// 39 % busy, as one wave or a pair has a SIMD to itself and its exponentials stand between its products. By
-// bytes and the start of workgroups where they are short: 64 x 256 tokens of 16 heads of 64 take 50 and 54 us, for
-// 42 us of bytes each at 4.84 TB/s; 48 texts to 1,021 with a window of 64 and 12 heads 72 and 65 for 53.
+// P and dS are rounded to bf16 before the second products. A matrix instruction takes one type for both operands,
+// and the others are the caller's bf16 q, k and dO: fp16, in which the forward keeps its P, would lose bits of
+// gradients below 6e-5 and all of those below 6e-8, and a mean over a large batch makes them that small; two bf16 terms
+// would double the second products (20 flops for 14). The two roundings put 0.0016 to 0.0017 of the gradients' norm
+// on them (what grad_dtype f32 is off by); with bf16 outputs, whose rounding alone is 0.0017, it is 0.0023 to 0.0024.
+//
+// Bound by its products where texts are long: 8 x 2,048 tokens, 16/8 heads of 128, full: dq 1,050, dk and dv
+// 1,120 TFLOP/s of those that they do; 4 x 4,096 causal, 16/2 heads of 256: 0.90 and 1.20 ms, matrix cores 38 % busy
+// in both, as one wave or a pair has a SIMD to itself and its exponentials stand between its products. By
+// bytes and the start of workgroups where they are short: 64 x 256 tokens of 16 heads of 64 take 50 to 57 and 55 to
+// 62 us, for 42 us of bytes each at 4.84 TB/s; 48 texts to 1,021 with a window of 64 and 12 heads 74 and 68 for 53.
 #include <algorithm>
 #include <new>
 #include <vector>
@@ -161,8 +167,8 @@ __device__ __forceinline__ void rows_product(f32x16& acc, const f32x16& first, c
 }
 
 // Two such products beside one another, of rows at base + off and base + off2: neither waits for its own
-// last step, which counts where a wave has its SIMD to itself (dq of 4 x 4,096 tokens, 16/2 heads of 256: 1.03 ms one
-// after the other, 0.99 so; the narrow heads' as long).
+// last step. dq, one after the other / so: 4 x 4,096 tokens of 16/2 heads of 256 0.92 / 0.92 ms, 8 x 2,048 of 16/8 x
+// 128 387 / 392 us, 64 x 256 of 16 heads of 64 53 / 51.5, 8 x 2,048 of them 226 / 225.
 template <int D, int BN, int RD>
 __device__ __forceinline__ void rows_products(f32x16& a, f32x16& b, const f32x16& first, const uint32_t (&base)[4], uint32_t off,
                                               uint32_t off2, const bf16x8 (&opnd)[D / 16], const bf16x8 (&opnd2)[D / 16]) {
@@ -604,8 +610,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_bwd_kernel(AttnBwd
 // that its exponentials run under the other's products.
 // Two of a workgroup's four pairs own 32 keys each, the others take other rows of the stream for
 // the same keys, and the sums meet in LDS at the end. Four pairs with keys of their own read half the tiles, but
-// make half as many workgroups of twice the length: 24 texts of 1,024 tokens with one key head take 176
-// us instead of 170, 4 x 4,096 of two 2.00 ms instead of 1.31, and 64 texts of 1,024 the same.
+// make half as many workgroups of twice the length. As here / so: 4 x 4,096 tokens, causal, of 16/2 heads 1.21 / 1.91
+// ms, 24 x 1,024 of 3/1 heads with a window of 512 155 / 162 us; but full, whose blocks are of equal length, 24 x
+// 1,024 199 / 172 and 64 x 1,024 501 / 403.
 template <int D>
 struct PairShape {
   static constexpr int QS = 2, KG = 2;            // parts of a stream tile, blocks of own keys
@@ -666,8 +673,9 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_pair_kernel(AttnBwdParams p) 
     __syncthreads();
   }
   // From the last rows on, the heads of a tile after one another: so the blocks of a text, in their causal
-  // triangle too, stream the same rows at about the same time, and find them in L2 (4 x 4,096 tokens
-  // of 16/2 heads, whose q and dO are 32 MB a key head: 1.30 ms, and 1.83 head by head from the diagonal on).
+  // triangle too, stream the same rows at about the same time, and find them in L2. That counts where they do not share
+  // one already (bwd_classes): 4 x 4,096 tokens of 16/2 heads, whose q and dO are 32 MB a key head, take 1.91 ms in
+  // one class, 1.21 in four; and there 1.12 head by head from the diagonal on. One key head: both the same.
   int dh = 0, dt = t_hi - 1;
   const int64_t h0 = (int64_t)head * p.group;
   const i32x4 xrs = pp_rsrc_words(base_q + h0 * p.head_dim * 2, (uint32_t)T * xst);
@@ -873,12 +881,17 @@ double bwd_longest(const inl_attn_desc& d, const std::vector<BwdText>& texts, bo
 }
 
 // Two parts of the waves (QS = 2) halve the longest workgroup's stream and make twice the
-// workgroups, for twice the tiles read. us with one part / two (texts x tokens, query / key heads x features):
-//   dq:     1 x 1,024 causal 16/8 x 128 (7.1 average loads) 36 / 24, 1 x 2,048 12/12 x 64 (4) 47 / 40,
-//           8 x 512 causal 16/8 x 128 (1.8) 34 / 41, 8 x 1,024 3/1 x 256 (1.5) 66 / 66, 16 x 256 16/16 x 64 (1.5) 18 / 20
-//   dk, dv: x 64: 1 x 2,048 12/12 (4) 58 / 49, 2 x 2,048 16/16 (1.5) 82 / 93;
-//           x 128: 64 ragged causal passages 16/8 (2.8) 182 / 134, 8 x 512 16/8 (2) 54 / 45, 4 x 2,048 (1) 276 / 293,
-//           causal, whose blocks are of unequal length: 8 x 2,048 (0.94) 370 / 313, 64 x 180 (0.7) 64 / 56
+// workgroups, for twice the tiles read. us with one part / two (texts x tokens, query / key heads x features;
+// average loads of the longest):
+//   dq:     two above 2.5: 1 x 1,024 causal 16/8 x 128 (8) 36 / 23, 1 x 2,048 12/12 x 64 (4) 47 / 39,
+//           8 x 512 causal 16/8 x 128 (2) 34 / 40, 64 ragged causal passages 16/8 x 128 (1.6) 109 / 131,
+//           8 x 1,024 3/1 x 256 (1.3) 63 / 78, 16 x 256 16/16 x 64 (1.5) 17 / 20
+//   dk, dv: x 64, two above 2: 1 x 2,048 12/12 (4) 57 / 47, 2 x 2,048 16/16 (1.5) 81 / 93;
+//           x 128, two above 1.2: 8 x 512 16/8 (2) 54 / 45, 4 x 2,048 (1) 256 / 275;
+//           x 128, causal, whose blocks are of unequal length, two: the passages (3.3) 179 / 123, 8 x 2,048 (1)
+//           374 / 323, 64 x 180 (1) 64 / 56; with a window, which makes long texts' equal: 64 x 180, 32 and 128:
+//           56 / 53 and 64 / 57; 32 x 512, 64 and 256: 75 / 77 and 113 / 110; 8 x 2,048, 64 and 512: 74 / 77 and
+//           176 / 172; 16 x 1,024, 16: 68 / 77; 4 x 4,096, 128: 90 / 92
 BwdLaunch bwd_launch(const inl_attn_desc& d, const std::vector<BwdText>& texts, bool kv, int cus, bool out16) {
   const int dim = d.head_dim <= 64 ? 64 : d.head_dim <= 128 ? 128 : 256;
 #define INL_BWD(D, KV, QS) bwd_plain<D, KV, QS>("attn_bwd_kernel<" #D ", " #KV ", " #QS ">", out16)
@@ -897,7 +910,12 @@ BwdLaunch bwd_launch(const inl_attn_desc& d, const std::vector<BwdText>& texts, 
 // are short ones. Workgroup i runs on XCD i mod 8, each with an L2 of its own: with the texts dealt to as many
 // classes as make key heads x classes a multiple of 8, all blocks of a (text, key head), which
 // stream the same rows, share one. Texts that do not fill the classes evenly, to 1.15 of the mean, run in
-// one class: an XCD without work costs more than L2 misses.
+// one class: an XCD without work costs more than L2 misses. us (dq, and dk and dv) in one class / several:
+//   4 x 4,096 causal 16/2 x 256 (1.0 of the mean) 940 / 909, 1,908 / 1,207; 24 x 1,024 3/1 x 256 (1.0) 174 / 171,
+//   205 / 195; 24 texts to 2,048 of them, window 512 (1.1) 141 / 136, 178 / 164; 14 x 1,024 16/2 x 256 (1.14) 432 / 479,
+//   627 / 618; 28 x 1,024 8/1 x 128 (1.14) 190 / 204, 262 / 251; 5 x 1,024 12/12 x 64 (1.2) 38 / 45, 44 / 50;
+//   18 x 1,024 3/1 x 256 (1.33) 118 / 169, 203 / 194; 3 x 4,096 16/2 x 256 (1.33) 1,211 / 1,558, 2,322 / 2,048;
+//   6 x 4,096 (1.33) 2,402 / 3,145, 3,584 / 4,667; 1 x 4,096 (4) 417 / 1,542, 925 / 1,964
 void bwd_classes(const inl_attn_desc& d, std::vector<BwdText>* texts, AttnBwdParams* p) {
   std::sort(texts->begin(), texts->end(), [](const BwdText& a, const BwdText& b) {
     return a.len != b.len ? a.len > b.len : a.start < b.start;
